@@ -8,13 +8,15 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_int32, c_int64, c_size_t, c_uint32, c_void_p
+from ctypes import c_float, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libecah_sampler.so")
 
 ABI_VERSION = 2
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
+KV_E4M3 = 3
+MAX_TOP_N = 32
 FLAG_FREQ_PRES = 0x1
 
 STATUS = {0: "ok", 1: "null pointer", 2: "dtype", 3: "shape", 4: "workspace", 5: "launch", 6: "abi"}
@@ -25,7 +27,9 @@ EXPORTS = ("ecah_sampler_abi_version", "ecah_status_string", "ecah_sampler_works
            "ecah_sampler_launch_noalloc", "ecah_sampler_noalloc_scratch_bytes",
            "ecah_vp_local", "ecah_vp_merge", "ecah_vp_exchange_bytes", "ecah_vp_step",
            "ecah_vp_ipc_alloc", "ecah_vp_ipc_open", "ecah_vp_ipc_close", "ecah_vp_ipc_free",
-           "ecah_quotient_mismatches", "ecah_vp_reset", "ecah_vp_dist_pass")
+           "ecah_quotient_mismatches", "ecah_vp_reset", "ecah_vp_dist_pass",
+           "ecah_token_logprobs_workspace_bytes", "ecah_token_logprobs", "ecah_paged_append",
+           "ecah_paged_decode_workspace_bytes", "ecah_paged_decode")
 IPC_HANDLE_BYTES = 64
 
 
@@ -64,6 +68,54 @@ class VPArgs(ctypes.Structure):
 class VPPeers(ctypes.Structure):
     """Mirror of ``struct ecah_vp_peers``."""
     _fields_ = [("rank", c_int32), ("max_batch", c_int32), ("base", c_void_p), ("timeout_us", c_uint32)]
+
+
+class LogprobArgs(ctypes.Structure):
+    """Mirror of ``struct ecah_logprob_args``."""
+    _fields_ = [
+        ("abi_version", c_int32), ("dtype", c_int32), ("rows", c_int32), ("vocab", c_int32),
+        ("row_stride", c_int64), ("logits", c_void_p), ("row_index", c_void_p), ("logit_rows", c_int32),
+        ("tokens_per_row", c_int32), ("token_ids", c_void_p), ("temperature", c_void_p), ("top_n", c_int32),
+        ("logprobs", c_void_p), ("entropy", c_void_p), ("top_ids", c_void_p), ("top_logprobs", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class KVCache(ctypes.Structure):
+    """Mirror of ``struct ecah_kv_cache``."""
+    _fields_ = [
+        ("kv_dtype", c_int32), ("num_pages", c_int32), ("page_size", c_int32), ("num_kv_heads", c_int32),
+        ("head_dim", c_int32), ("batch", c_int32), ("k_cache", c_void_p), ("v_cache", c_void_p),
+        ("k_page_stride", c_int64), ("k_slot_stride", c_int64), ("k_head_stride", c_int64),
+        ("v_page_stride", c_int64), ("v_slot_stride", c_int64), ("v_head_stride", c_int64),
+        ("k_scale", c_void_p), ("v_scale", c_void_p), ("kv_indptr", c_void_p), ("kv_indices", c_void_p),
+        ("num_indices", c_int64),
+    ]
+
+
+class AppendArgs(ctypes.Structure):
+    """Mirror of ``struct ecah_append_args``."""
+    _fields_ = [
+        ("abi_version", c_int32), ("dtype", c_int32), ("tokens", c_int32), ("num_qo_heads", c_int32),
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p),
+        ("q_token_stride", c_int64), ("q_head_stride", c_int64), ("k_token_stride", c_int64),
+        ("k_head_stride", c_int64), ("v_token_stride", c_int64), ("v_head_stride", c_int64),
+        ("q_out", c_void_p), ("qo_token_stride", c_int64), ("qo_head_stride", c_int64),
+        ("q_norm", c_void_p), ("k_norm", c_void_p), ("eps", c_float), ("interleaved", c_int32),
+        ("cos_sin", c_void_p), ("table_rows", c_int32), ("positions", c_void_p), ("batch_index", c_void_p),
+        ("cache", KVCache),
+    ]
+
+
+class DecodeArgs(ctypes.Structure):
+    """Mirror of ``struct ecah_decode_args``."""
+    _fields_ = [
+        ("abi_version", c_int32), ("dtype", c_int32), ("num_qo_heads", c_int32), ("sm_scale", c_float),
+        ("q", c_void_p), ("q_token_stride", c_int64), ("q_head_stride", c_int64),
+        ("out", c_void_p), ("out_token_stride", c_int64), ("out_head_stride", c_int64),
+        ("lse", c_void_p), ("kv_last_page_len", c_void_p), ("cache", KVCache),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
 
 
 class EcahError(RuntimeError):
@@ -121,6 +173,16 @@ def lib():
         L.ecah_vp_ipc_free.argtypes = [c_void_p]
         L.ecah_quotient_mismatches.restype = c_int32
         L.ecah_quotient_mismatches.argtypes = [c_int32, c_void_p, c_int32, c_void_p, c_void_p]
+        L.ecah_token_logprobs_workspace_bytes.restype = c_size_t
+        L.ecah_token_logprobs_workspace_bytes.argtypes = []
+        L.ecah_token_logprobs.restype = c_int32
+        L.ecah_token_logprobs.argtypes = [ctypes.POINTER(LogprobArgs), c_void_p]
+        L.ecah_paged_append.restype = c_int32
+        L.ecah_paged_append.argtypes = [ctypes.POINTER(AppendArgs), c_void_p]
+        L.ecah_paged_decode_workspace_bytes.restype = c_size_t
+        L.ecah_paged_decode_workspace_bytes.argtypes = [c_int32, c_int32, c_int32, c_int32]
+        L.ecah_paged_decode.restype = c_int32
+        L.ecah_paged_decode.argtypes = [ctypes.POINTER(DecodeArgs), c_void_p]
         if L.ecah_sampler_abi_version() != ABI_VERSION:
             raise EcahError("libecah_sampler.so ABI version mismatch")
         _lib = L

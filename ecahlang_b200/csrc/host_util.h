@@ -1,0 +1,80 @@
+// Host helpers shared by the launchers: the device's SM count and the
+// dynamic shared memory limit of a kernel, each looked up or set once.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <mutex>
+
+namespace ecah {
+
+// SM count of the current device, looked up once per device; 0 without one.
+inline int device_sms() {
+  constexpr int kMaxDev = 64;
+  static int cache[kMaxDev] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return 0;
+  if (cache[dev] > 0) return cache[dev];
+  int sms = 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  cache[dev] = sms;
+  return sms;
+}
+
+// cudaFuncSetAttribute once per (kernel, device, value): the attribute is a
+// property of the kernel on a device, so later launches skip the call.
+// forget_smem drops the remembered values (a launch that failed sets them
+// again: after cudaDeviceReset the kernels come back without them).
+struct SmemMemo {
+  static constexpr int kSlots = 128;
+  std::mutex mu;
+  const void* fn[kSlots];
+  int dev[kSlots], val[kSlots];
+  int used = 0;
+};
+
+inline SmemMemo& smem_memo() {
+  static SmemMemo m;
+  return m;
+}
+
+inline void forget_smem() {
+  SmemMemo& m = smem_memo();
+  std::lock_guard<std::mutex> lock(m.mu);
+  m.used = 0;
+}
+
+template <typename Args>
+inline cudaError_t set_smem_once(void (*kernel)(const Args), int smem) {
+  const void* fn = reinterpret_cast<const void*>(kernel);
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  SmemMemo& m = smem_memo();
+  std::lock_guard<std::mutex> lock(m.mu);
+  for (int i = 0; i < m.used; ++i)
+    if (m.fn[i] == fn && m.dev[i] == dev && m.val[i] >= smem) return cudaSuccess;
+  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  for (int i = 0; i < m.used; ++i)
+    if (m.fn[i] == fn && m.dev[i] == dev) { m.val[i] = smem; return cudaSuccess; }
+  if (m.used < SmemMemo::kSlots) {
+    m.fn[m.used] = fn; m.dev[m.used] = dev; m.val[m.used] = smem; ++m.used;
+  }
+  return cudaSuccess;
+}
+
+// Launches `fn` with `smem` bytes of dynamic shared memory, setting the limit
+// first where it is above the default; one retry with the limit set afresh.
+template <typename Args>
+inline bool launch_kernel(void (*fn)(const Args), dim3 grid, int threads, int smem, cudaStream_t s, const Args& args) {
+  for (int attempt = 0; attempt < 2; ++attempt) {
+    if (smem > 48 * 1024 && set_smem_once(fn, smem) != cudaSuccess) { cudaGetLastError(); return false; }
+    fn<<<grid, threads, smem, s>>>(args);
+    if (cudaGetLastError() == cudaSuccess) return true;
+    forget_smem();
+  }
+  return false;
+}
+
+}  // namespace ecah

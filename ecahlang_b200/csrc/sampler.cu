@@ -7,8 +7,8 @@
 #include <algorithm>
 #include <cstdio>
 #include <cstring>
-#include <mutex>
 
+#include "host_util.h"
 #include "row_kernel.cuh"
 #include "vp_kernel.cuh"
 #include "vp_dist.cuh"
@@ -94,19 +94,6 @@ struct Plan {
 static constexpr size_t kMaxDynSmem = 128 * 1024;
 // the cluster kernel's workspace: the Philox completion counter
 static constexpr size_t kMinWorkspace = 256;
-
-// SM count of the current device, looked up once per device.
-static int device_sms() {
-  constexpr int kMaxDev = 64;
-  static int cache[kMaxDev] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return 0;
-  if (cache[dev] > 0) return cache[dev];
-  int sms = 0;
-  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  cache[dev] = sms;
-  return sms;
-}
 
 // Workspace header: [0, 256) the Philox completion counter and the error
 // word; [256, 4096) one arrival counter per row split over several CTAs.
@@ -210,41 +197,6 @@ const char* ecah_status_string(int s) {
     case ECAH_ERR_ABI: return "abi_version mismatch";
     default: return "unknown status";
   }
-}
-
-// cudaFuncSetAttribute once per (kernel, device, value): the attribute is a
-// property of the kernel on a device, so later launches skip the call.
-// forget_smem drops the remembered values (a launch that failed sets them
-// again: after cudaDeviceReset the kernels come back without them).
-static std::mutex g_smem_mu;
-static constexpr int kSmemSlots = 64;
-static KernelFn g_smem_fn[kSmemSlots];
-static int g_smem_dev[kSmemSlots], g_smem_val[kSmemSlots];
-static int g_smem_used = 0;
-
-static void forget_smem() {
-  std::lock_guard<std::mutex> lock(g_smem_mu);
-  g_smem_used = 0;
-}
-
-static cudaError_t set_smem_once(KernelFn fn, int smem) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  std::lock_guard<std::mutex> lock(g_smem_mu);
-  KernelFn* fns = g_smem_fn;
-  int* devs = g_smem_dev;
-  int* vals = g_smem_val;
-  int& used = g_smem_used;
-  constexpr int kSlots = kSmemSlots;
-  for (int i = 0; i < used; ++i)
-    if (fns[i] == fn && devs[i] == dev && vals[i] >= smem) return cudaSuccess;
-  e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
-  for (int i = 0; i < used; ++i)
-    if (fns[i] == fn && devs[i] == dev) { vals[i] = smem; return cudaSuccess; }
-  if (used < kSlots) { fns[used] = fn; devs[used] = dev; vals[used] = smem; ++used; }
-  return cudaSuccess;
 }
 
 size_t ecah_sampler_workspace_bytes(int32_t batch, int32_t vocab, int32_t dtype) {

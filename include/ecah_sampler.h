@@ -321,6 +321,169 @@ ECAH_API int ecah_vp_ipc_free(void* ptr);
  * counterpart in the reference, which runs on one GPU. */
 ECAH_API int ecah_vp_reset(void* own_buffer, uint32_t epoch, void* stream);
 
+/*
+ * Token log probabilities: for every row, the log probability of given
+ * tokens, the entropy of the row's distribution and its most likely
+ * alternatives (the `logprobs` / `top_logprobs` fields of a completion).
+ * The reference has no such output (ecahlang/main.py:170 discards the logits
+ * after the draw).  With x = the row's logits, T = its temperature, m = max x:
+ *
+ *   z_i = (x_i - m) / T,  Z = sum_i exp(z_i)            float32 sums
+ *   logprob(t) = z_t - ln Z
+ *   entropy    = ln Z - (1/Z) sum_i exp(z_i) z_i        natural units
+ *   alternatives: the top_n largest x_i, by x descending, then id ascending
+ *
+ * Edges.  Entries of -inf have no mass and are never alternatives; slots past
+ * the row's last alternative hold id -1 and -inf.  A row of -inf alone has
+ * log probabilities -inf and entropy 0.  T <= 0 is the greedy distribution
+ * (all mass on the lowest id holding m).  A row with a NaN or a +inf has NaN
+ * everywhere and ids -1; a token outside [0, vocab) has NaN.
+ */
+#define ECAH_MAX_TOP_N 32
+
+typedef struct ecah_logprob_args {
+  int32_t abi_version;        /* = ECAH_SAMPLER_ABI_VERSION                      */
+  int32_t dtype;              /* enum ecah_dtype                                  */
+  int32_t rows;               /* R >= 0                                           */
+  int32_t vocab;              /* 1 <= V <= 2^31 - 65536                           */
+  int64_t row_stride;         /* elements between rows, >= vocab                  */
+  const void* logits;         /* [R or logit_rows, row_stride]                    */
+  const int32_t* row_index;   /* [R] row gather as in ecah_sampler_args, or NULL  */
+  int32_t logit_rows;         /* rows of the logits buffer (>= 1 with row_index)  */
+  int32_t tokens_per_row;     /* K >= 0                                           */
+  const int32_t* token_ids;   /* [R, K]                                           */
+  const float* temperature;   /* [R], or NULL: 1                                  */
+  int32_t top_n;              /* 0 .. ECAH_MAX_TOP_N                              */
+  float* logprobs;            /* [R, K]                                           */
+  float* entropy;             /* [R], or NULL                                     */
+  int32_t* top_ids;           /* [R, top_n]                                       */
+  float* top_logprobs;        /* [R, top_n]                                       */
+  void* workspace;            /* >= ecah_token_logprobs_workspace_bytes(),
+                                 zero-filled once; every launch leaves its
+                                 counters at zero                                 */
+  size_t workspace_bytes;
+} ecah_logprob_args;
+
+/* Workspace of any ecah_token_logprobs call on the current device (its size
+ * depends on the SM count alone; 0 when there is no device). */
+ECAH_API size_t ecah_token_logprobs_workspace_bytes(void);
+ECAH_API int ecah_token_logprobs(const ecah_logprob_args* args, void* stream);
+
+/*
+ * Paged key-value cache.  A request's keys and values lie in pages of
+ * page_size tokens, kv_indices[kv_indptr[b] .. kv_indptr[b+1]) in order, the
+ * layout the reference plans its attention with (ecahlang/main.py:341-347,
+ * manager.py:228-253).  k_cache / v_cache are [num_pages, page_size,
+ * num_kv_heads, head_dim] with any page, slot and head strides (elements,
+ * multiples of 16 bytes) and contiguous rows of head_dim, 16-byte aligned.
+ * kv_dtype is the model dtype, or ECAH_KV_E4M3: 8-bit floats (4 exponent and 3
+ * mantissa bits, largest 448) with one float32 scale per token and head,
+ * k_scale / v_scale [num_pages, num_kv_heads, page_size] contiguous; the
+ * value is code * scale.  head_dim is 64, 96, 128, 192 or 256; num_qo_heads is
+ * a multiple of num_kv_heads.  Model dtypes are f16 and bf16.
+ */
+#define ECAH_KV_E4M3 3
+
+typedef struct ecah_kv_cache {
+  int32_t kv_dtype;           /* the model dtype, or ECAH_KV_E4M3                 */
+  int32_t num_pages;
+  int32_t page_size;          /* >= 1                                             */
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t batch;              /* requests: kv_indptr has batch + 1 entries        */
+  void* k_cache;
+  void* v_cache;
+  int64_t k_page_stride, k_slot_stride, k_head_stride;
+  int64_t v_page_stride, v_slot_stride, v_head_stride;
+  float* k_scale;             /* ECAH_KV_E4M3 only, else NULL                     */
+  float* v_scale;
+  const int32_t* kv_indptr;   /* [batch + 1] device                               */
+  const int32_t* kv_indices;  /* [num_indices] device                             */
+  int64_t num_indices;
+} ecah_kv_cache;
+
+/*
+ * Append: the new tokens' queries and keys are normalised per head (RMS norm,
+ * when a weight is given) and rotated (rotary position embedding, when a table
+ * is given); queries go to q_out, keys and values into their cache slot.
+ * Replaces the append of the reference's attention hook
+ * (ecahlang/manager.py:143-185, :270-281) and the norm and rotation before it.
+ *
+ *   y = x * rsqrt(mean(x^2) + eps) * w                      (q and k, given w)
+ *   (a, b) -> (a cos - b sin, b cos + a sin)                (q and k, given a table)
+ *     pairs (i, i + head_dim/2), or (2i, 2i+1) with interleaved
+ *   slot: page kv_indices[kv_indptr[b] + pos / page_size], offset pos % page_size
+ *   E4M3: scale = max(max|y|, 448e-12) / 448, code = round(y / scale)
+ *
+ * All of it in float32, rounded once on the way out.  Tokens with batch_index
+ * outside [0, batch), or a position outside their request's pages, or a page
+ * outside the cache, are not written (padding rows of a captured batch use
+ * -1); their queries are still computed.  Positions outside the table take
+ * its first or last row.  Two tokens of one launch never share a slot.
+ */
+typedef struct ecah_append_args {
+  int32_t abi_version;
+  int32_t dtype;              /* of q, k, v and the norm weights: f16 or bf16     */
+  int32_t tokens;             /* T >= 0                                           */
+  int32_t num_qo_heads;       /* 0 with q == NULL                                 */
+  const void* q;              /* [T, num_qo_heads, head_dim], or NULL: keys and values only */
+  const void* k;              /* [T, num_kv_heads, head_dim]                      */
+  const void* v;
+  int64_t q_token_stride, q_head_stride;   /* elements; rows of head_dim are      */
+  int64_t k_token_stride, k_head_stride;   /* contiguous and 16-byte aligned      */
+  int64_t v_token_stride, v_head_stride;
+  void* q_out;                /* may be q itself                                  */
+  int64_t qo_token_stride, qo_head_stride;
+  const void* q_norm;         /* [head_dim] model dtype, or NULL                  */
+  const void* k_norm;
+  float eps;
+  int32_t interleaved;
+  const float* cos_sin;       /* [table_rows, head_dim]: cosines, then sines; or NULL */
+  int32_t table_rows;
+  const int32_t* positions;   /* [T]                                              */
+  const int32_t* batch_index; /* [T]                                              */
+  ecah_kv_cache cache;
+} ecah_append_args;
+
+ECAH_API int ecah_paged_append(const ecah_append_args* args, void* stream);
+
+/*
+ * Decode attention: one query token per request over the request's cached
+ * keys and values.  Replaces the reference's decode wrapper run
+ * (ecahlang/main.py:68, planned at :341-347).
+ *
+ *   len(b) = (pages(b) - 1) * page_size + kv_last_page_len[b], 0 without pages
+ *   s_j = sm_scale q . k_j  (j < len),  o = sum_j softmax(s)_j v_j
+ *   lse = ln sum_j exp(s_j)
+ *
+ * Query head h reads KV head h / (num_qo_heads / num_kv_heads).  Requests of
+ * length 0 (padding rows) give o = 0 and lse = -inf.  Slots past a request's
+ * length are never read.  Indices outside the cache are clamped into it.
+ * The sums are float32; softmax weights are rounded to the 16-bit operand of
+ * the tensor cores.  Results do not depend on which block finishes last.
+ */
+typedef struct ecah_decode_args {
+  int32_t abi_version;
+  int32_t dtype;              /* of q and out: f16 or bf16                        */
+  int32_t num_qo_heads;
+  float sm_scale;
+  const void* q;              /* [batch, num_qo_heads, head_dim]                  */
+  int64_t q_token_stride, q_head_stride;
+  void* out;                  /* [batch, num_qo_heads, head_dim]                  */
+  int64_t out_token_stride, out_head_stride;
+  float* lse;                 /* [batch, num_qo_heads] contiguous, or NULL        */
+  const int32_t* kv_last_page_len;   /* [batch] device                            */
+  ecah_kv_cache cache;
+  void* workspace;            /* >= ecah_paged_decode_workspace_bytes() for some
+                                 batch >= cache.batch, zero-filled once; every
+                                 launch leaves its counters at zero               */
+  size_t workspace_bytes;
+} ecah_decode_args;
+
+ECAH_API size_t ecah_paged_decode_workspace_bytes(int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
+                                                  int32_t head_dim);
+ECAH_API int ecah_paged_decode(const ecah_decode_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
