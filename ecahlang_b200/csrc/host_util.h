@@ -65,11 +65,11 @@ inline cudaError_t set_smem_once(void (*kernel)(const Args), int smem) {
 }
 
 // Launches `fn` with `smem` bytes of dynamic shared memory, setting the limit
-// first where it is above the default; one retry with the limit set afresh.
+// first where it may exceed the 48 KB default beside static shared memory; one retry with the limit set afresh.
 template <typename Args>
 inline bool launch_kernel(void (*fn)(const Args), dim3 grid, int threads, int smem, cudaStream_t s, const Args& args) {
   for (int attempt = 0; attempt < 2; ++attempt) {
-    if (smem > 48 * 1024 && set_smem_once(fn, smem) != cudaSuccess) { cudaGetLastError(); return false; }
+    if (smem > 32 * 1024 && set_smem_once(fn, smem) != cudaSuccess) { cudaGetLastError(); return false; }
     fn<<<grid, threads, smem, s>>>(args);
     if (cudaGetLastError() == cudaSuccess) return true;
     forget_smem();
