@@ -36,6 +36,7 @@ constexpr int kSlice = 16;            // keys per warp and step
 constexpr int kTile = kW * kSlice;    // keys per work unit
 constexpr int kRows = 16;             // query heads per head tile
 constexpr int kMaxGroup = 32;         // parts joined at once
+constexpr int kItemCost = 4;          // tiles of streaming that starting and joining an item takes
 constexpr float kLazy = 8.0f;         // the reference moves when a score is 2^8 above it
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -182,20 +183,13 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3>::kBlocks) decode_kernel(con
   const kv::Cache& C = P.cache;
   const int per_req = C.heads * P.tiles_h;       // (head, head tile) pairs of a request
 
-  // requests without tokens: zeros, spread over the blocks
-  for (int b = blockIdx.x; b < C.batch; b += gridDim.x) {
-    long long f;
-    if (request_len(P, b, &f) != 0) continue;
-    for (int i = tid; i < P.hq * D; i += kT)
-      static_cast<uint16_t*>(P.out)[b * P.o_tok + (i / D) * P.o_head + i % D] = 0;
-    if (P.lse)
-      for (int i = tid; i < P.hq; i += kT) P.lse[static_cast<long long>(b) * P.hq + i] = -INFINITY;
-  }
-
-  // total tiles, then this block's share [begin, end) and its first request
+  // Total cost, then this block's share [begin, end) and its first request.  An
+  // item (one head tile of one request) costs kItemCost units, then one a tile.
   auto tiles_of = [&](int b) -> long long {
     long long f;
-    return b < C.batch ? (request_len(P, b, &f) + kTile - 1) / kTile : 0;
+    if (b >= C.batch) return 0;
+    const long long len = request_len(P, b, &f);
+    return len ? (len + kTile - 1) / kTile + kItemCost : 0;
   };
   long long sum = 0;
   for (int b = tid; b < C.batch; b += kT) sum += tiles_of(b);
@@ -207,10 +201,10 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3>::kBlocks) decode_kernel(con
   for (int w = 0; w < kW; ++w) total += s_scan[w];
   total *= per_req;
   const long long blocks = min(static_cast<long long>(gridDim.x), total);
-  if (blockIdx.x >= blocks) return;
-  const long long begin = blockIdx.x * total / blocks, end = (blockIdx.x + 1ll) * total / blocks;
+  const bool busy = blockIdx.x < blocks;
+  const long long begin = busy ? blockIdx.x * total / blocks : 0, end = busy ? (blockIdx.x + 1ll) * total / blocks : 0;
   long long run = 0;
-  for (int b0 = 0; b0 < C.batch; b0 += kT) {
+  for (int b0 = 0; busy && b0 < C.batch; b0 += kT) {
     const long long mine = tiles_of(b0 + tid);
     long long inc = mine;
 #pragma unroll
@@ -231,8 +225,8 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3>::kBlocks) decode_kernel(con
     if (begin < run * per_req) break;
   }
   __syncthreads();
-  int req = s_req;
-  long long req_start = s_start * per_req;       // first unit of the request
+  int req = busy ? s_req : 0;
+  long long req_start = busy ? s_start * per_req : 0;       // first unit of the request
   long long at = begin;
 
   const uint32_t ring = smem_u32(smem) + warp * S::kWarpBytes;
@@ -242,14 +236,17 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3>::kBlocks) decode_kernel(con
     // the unit's request, head and head tile
     long long first;
     const long long len = request_len(P, req, &first);
-    const long long nt = (len + kTile - 1) / kTile;
-    if (at >= req_start + nt * per_req) { req_start += nt * per_req; ++req; continue; }
-    const int pair = static_cast<int>((at - req_start) / nt);
-    const long long item_start = req_start + pair * nt;       // units [item_start, item_start + nt)
+    const long long nt = (len + kTile - 1) / kTile, cost = len ? nt + kItemCost : 0;
+    if (at >= req_start + cost * per_req) { req_start += cost * per_req; ++req; continue; }
+    const int pair = static_cast<int>((at - req_start) / cost);
+    const long long item_start = req_start + pair * cost;
+    const long long tile0 = item_start + kItemCost;           // unit of the item's first tile
     const int h = pair / P.tiles_h, ht = pair % P.tiles_h;
-    const long long seg_end = min(end, item_start + nt);
-    const long long t0 = at - item_start;
-    const int n = static_cast<int>(seg_end - at);
+    const long long seg_end = min(end, item_start + cost);
+    const long long t0 = max(at, tile0) - tile0;
+    const int n = static_cast<int>(seg_end - tile0 - t0);
+    at = seg_end;
+    if (n <= 0) continue;                                     // only the item's first units: no tile
     const int rows = min(P.group - ht * kRows, kRows);        // query heads of this tile
     const int head0 = h * P.group + ht * kRows;
 
@@ -520,8 +517,8 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3>::kBlocks) decode_kernel(con
     }
     __syncthreads();
 
-    // parts of this item: the blocks whose shares overlap its units
-    const long long a = ((item_start + 1) * blocks - 1) / total, z = ((item_start + nt) * blocks - 1) / total;
+    // parts of this item: the blocks whose shares overlap its tiles
+    const long long a = ((tile0 + 1) * blocks - 1) / total, z = ((tile0 + nt) * blocks - 1) / total;
     const int parts = static_cast<int>(z - a) + 1, part = static_cast<int>(blockIdx.x - a);
     auto slot_of = [&](int p) -> long long { return p == 0 ? 2 * a + 1 : 2 * (a + p); };
 
@@ -583,7 +580,16 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3>::kBlocks) decode_kernel(con
       }
     }
     __syncthreads();       // the rings are free again
-    at = seg_end;
+  }
+
+  // requests without tokens: zeros, spread over the blocks
+  for (int b = blockIdx.x; b < C.batch; b += gridDim.x) {
+    long long f;
+    if (request_len(P, b, &f) != 0) continue;
+    for (int i = tid; i < P.hq * D; i += kT)
+      static_cast<uint16_t*>(P.out)[b * P.o_tok + (i / D) * P.o_head + i % D] = 0;
+    if (P.lse)
+      for (int i = tid; i < P.hq; i += kT) P.lse[static_cast<long long>(b) * P.hq + i] = -INFINITY;
   }
 }
 
@@ -666,7 +672,7 @@ int ecah_paged_decode(const ecah_decode_args* a, void* stream) {
   const decode::Variant v = f16 ? (e4m3 ? decode::variant_for<ECAH_DTYPE_F16, true>(c.head_dim) : decode::variant_for<ECAH_DTYPE_F16, false>(c.head_dim))
                                 : (e4m3 ? decode::variant_for<ECAH_DTYPE_BF16, true>(c.head_dim) : decode::variant_for<ECAH_DTYPE_BF16, false>(c.head_dim));
   // no more blocks than tiles the listed pages can hold (and one for the empty requests)
-  const double most = (static_cast<double>(c.num_indices) * c.page_size / decode::kTile + c.batch) * c.num_kv_heads * P.tiles_h + 1;
+  const double most = (static_cast<double>(c.num_indices) * c.page_size / decode::kTile + c.batch * (1.0 + decode::kItemCost)) * c.num_kv_heads * P.tiles_h + 1;
   const int blocks = static_cast<int>(std::min(most, static_cast<double>(sms * v.blocks)));
   return launch_kernel(v.fn, dim3(blocks), decode::kT, v.smem, reinterpret_cast<cudaStream_t>(stream), P) ? ECAH_OK : ECAH_ERR_LAUNCH;
 }
