@@ -375,7 +375,8 @@ ECAH_API int ecah_token_logprobs(const ecah_logprob_args* args, void* stream);
  * layout the reference plans its attention with (ecahlang/main.py:341-347,
  * manager.py:228-253).  k_cache / v_cache are [num_pages, page_size,
  * num_kv_heads, head_dim] with any page, slot and head strides (elements,
- * multiples of 16 bytes) and contiguous rows of head_dim, 16-byte aligned.
+ * multiples of 16 bytes) and contiguous rows of head_dim, 16-byte aligned, all
+ * within 64 GB of their base.
  * kv_dtype is the model dtype, or ECAH_KV_E4M3: 8-bit floats (4 exponent and 3
  * mantissa bits, largest 448) with one float32 scale per token and head,
  * k_scale / v_scale [num_pages, num_kv_heads, page_size] contiguous; the
