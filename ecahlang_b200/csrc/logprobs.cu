@@ -16,10 +16,11 @@ namespace lp {
 // and ln Z = ln z, entropy = ln z - ln 2 s / z.  The differences are taken before
 // the multiplication, so a temperature of 1e-5 loses nothing.
 //
-// The alternatives need no second pass either: entries are kept while they may
-// still be among the N largest.  Within a step (a contiguous piece of the row, so
-// later steps have larger indices and lose ties) a floor below the N-th best is
-// found from the threads' maxima; after that an entry is kept only above it.
+// The alternatives: a thread leaves the largest value of each of its steps (32 or
+// 16 entries) as a record in shared memory, nothing more while the row streams.
+// Afterwards the N-th largest of the threads' maxima is a floor that N entries
+// reach; only the steps whose record reaches it, about N of them, are read again
+// (from L2) for the entries at or above it.
 //
 // Bound: HBM for many rows (one read of the logits); 16-bit logits at 6.5 TB/s
 // bring 11.6 entries a clock to an SM, whose 16 exponentials a clock are then 70 %
@@ -34,18 +35,21 @@ constexpr int kT = 256;
 constexpr int kW = kT / 32;
 constexpr int kU = 4;                  // vectors of a thread and step
 constexpr int kStep = kT * kU;         // vectors of a step
-constexpr int kBlocks = 4;             // per SM
+constexpr int kBlocks = 3;             // per SM: 80 registers a thread, 48 KB in flight
 constexpr int kRing = 2 * kU;          // a step in flight behind the one at work
-constexpr int kC = 2048;               // kept entries
+constexpr int kC = 1024;               // entries of one selection
+constexpr int kMaxSteps = 20;          // steps with a record: 163840 16-bit logits
 constexpr int kMaxN = ECAH_MAX_TOP_N;
-constexpr int kMaxParts = kC / kMaxN;  // parts of a row: all their alternatives fit the kept entries
+constexpr int kList = 128;             // steps read again at once
+constexpr int kMaxParts = 64;          // parts of a row
+constexpr int kJoin = (kC - kMaxN) / kMaxN;   // parts whose alternatives are joined at once
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 40.0f;        // the reference moves when an exponent would pass it
 constexpr float kTiny = -150.0f;       // 2^kTiny is zero in float32
 
 struct alignas(16) Part {
   float m, z, s;
-  int flags;                           // alternatives | bad << 16
+  int flags;                           // 1: a NaN or +inf
 };
 
 struct Params {
@@ -68,9 +72,13 @@ struct Params {
 struct Smem {
   uint4 ring[kRing][kT];
   unsigned long long kept[kC];
+  uint16_t records[kMaxSteps][kT];
+  int chunks[kList];
   unsigned long long top[kMaxN];
   float red[3][kW];
-  int n, flag, count;
+  uint32_t floors[kW], tops[kW];
+  int n, flag, count, list;
+  long long end;                       // of this block's share
 };
 
 // Order of the alternatives: value descending, then index ascending, as one
@@ -115,6 +123,8 @@ __device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
 // (a NaN if it holds one), and the word that stands for entries outside the row.
 template <int DT> struct Vec {
   static constexpr int kN = DType<DT>::kVec;
+  // a value's record, in the order of the values (f32: rounded down to 16 bits)
+  static __device__ __forceinline__ uint32_t rec(float x) { return key16(DType<DT>::to_raw(x == 0.0f ? 0.0f : x)); }
   static constexpr uint32_t kOut = DT == ECAH_DTYPE_F16 ? 0xFC00FC00u : 0xFF80FF80u;   // -inf
   static __device__ __forceinline__ void pair(const uint4& v, int i, float& a, float& b) {
     const uint32_t w = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
@@ -140,6 +150,7 @@ template <int DT> struct Vec {
 };
 template <> struct Vec<ECAH_DTYPE_F32> {
   static constexpr int kN = 4;
+  static __device__ __forceinline__ uint32_t rec(float x) { return value_key(x) >> 16; }
   static constexpr uint32_t kOut = 0xFF800000u;
   static __device__ __forceinline__ void pair(const uint4& v, int i, float& a, float& b) {
     a = __uint_as_float(i == 0 ? v.x : v.z);
@@ -179,54 +190,47 @@ struct Row {
   }
 };
 
-// This block's walk over its vectors [pos, end): steps of at most kStep vectors
-// within one row.
+// This block's piece of one row: vectors [v, v_end).
 template <int DT>
-struct Walk {
-  long long pos, end, row_start;
-  int r;
+struct Piece {
   Row<DT> row;
-  __device__ __forceinline__ bool done() const { return pos >= end; }
-  __device__ __forceinline__ int length(const Params& P) const {
-    return static_cast<int>(min(static_cast<long long>(kStep), min(end, row_start + P.nv) - pos));
-  }
-  __device__ __forceinline__ void advance(const Params& P) {
-    pos += length(P);
-    if (pos >= row_start + P.nv && pos < end) {
-      row_start += P.nv;
-      row.set(P, ++r);
-    }
-  }
+  int v, v_end;
 };
 
-// Copies this thread's vectors of the step into its own ring slots.
+// Copies this thread's vectors of the step at piece.v into its own ring slots.
 template <int DT>
-__device__ __forceinline__ void fetch(const Params& P, const Walk<DT>& w, Smem& S, int parity) {
+__device__ __forceinline__ void fetch(const Piece<DT>& p, int V, Smem& S, int parity) {
   constexpr int kN = Vec<DT>::kN;
-  if (!w.done()) {
-    const int v0 = static_cast<int>(w.pos - w.row_start), len = w.length(P), tid = threadIdx.x;
+  const int tid = threadIdx.x;
+  uint4* slot = &S.ring[parity * kU][tid];
+  const int whole0 = p.row.mis ? 1 : 0, whole1 = (V + p.row.mis) / kN;   // vectors wholly inside the row
+  if (p.v >= whole0 && p.v + kStep <= min(whole1, p.v_end)) {
+    const unsigned char* src = p.row.base + static_cast<long long>(p.v + tid) * 16;
+    const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(slot));
 #pragma unroll
+    for (int u = 0; u < kU; ++u) cp16(dst + u * kT * 16, src + u * kT * 16);
+  } else {
+#pragma unroll 1
     for (int u = 0; u < kU; ++u) {
-      const int i = u * kT + tid, v = v0 + i;
-      const long long first = static_cast<long long>(v) * kN - w.row.mis;
-      uint4* slot = &S.ring[parity * kU + u][tid];
-      if (i < len && first >= 0 && first + kN <= P.V) {
-        cp16(static_cast<uint32_t>(__cvta_generic_to_shared(slot)), w.row.base + static_cast<long long>(v) * 16);
-      } else {
-        uint32_t q[4] = {Vec<DT>::kOut, Vec<DT>::kOut, Vec<DT>::kOut, Vec<DT>::kOut};
-        if (i < len) {                  // the row's edge: entry by entry
-          using Raw = typename DType<DT>::Raw;
-          const Raw* x = reinterpret_cast<const Raw*>(w.row.base) + static_cast<long long>(v) * kN;
-#pragma unroll
-          for (int j = 0; j < kN; ++j)
-            if (first + j >= 0 && first + j < P.V) {
-              const uint32_t raw = x[j];
-              if (kN == 4) q[j] = raw;
-              else q[j / 2] = (j & 1) ? (q[j / 2] & 0xFFFFu) | (raw << 16) : (q[j / 2] & 0xFFFF0000u) | raw;
-            }
-        }
-        *slot = make_uint4(q[0], q[1], q[2], q[3]);
+      const int v = p.v + u * kT + tid;
+      if (v >= whole0 && v < whole1 && v < p.v_end) {
+        cp16(static_cast<uint32_t>(__cvta_generic_to_shared(slot + u * kT)), p.row.base + static_cast<long long>(v) * 16);
+        continue;
       }
+      uint32_t q[4] = {Vec<DT>::kOut, Vec<DT>::kOut, Vec<DT>::kOut, Vec<DT>::kOut};
+      if (v < p.v_end) {                // the row's edge: entry by entry
+        using Raw = typename DType<DT>::Raw;
+        const long long first = static_cast<long long>(v) * kN - p.row.mis;
+        const Raw* x = reinterpret_cast<const Raw*>(p.row.base) + static_cast<long long>(v) * kN;
+#pragma unroll
+        for (int j = 0; j < kN; ++j)
+          if (first + j >= 0 && first + j < V) {
+            const uint32_t raw = x[j];
+            if (kN == 4) q[j] = raw;
+            else q[j / 2] = (j & 1) ? (q[j / 2] & 0xFFFFu) | (raw << 16) : (q[j / 2] & 0xFFFF0000u) | raw;
+          }
+      }
+      slot[u * kT] = make_uint4(q[0], q[1], q[2], q[3]);
     }
   }
   cp_commit();
@@ -268,7 +272,17 @@ __device__ __noinline__ int select_top(Smem& S, int n, int N) {
   }
   unsigned long long k = 0;
   int rank = N;
-  if (tid < n) {
+  if (n <= kT / 4) {                   // four threads a key
+    const int i = tid >> 2;
+    int above = 0;
+    if (i < n) {
+      k = S.kept[i];
+      for (int j = tid & 3; j < n; j += 4) above += S.kept[j] > k;
+    }
+    above += __shfl_xor_sync(0xFFFFFFFFu, above, 1);
+    above += __shfl_xor_sync(0xFFFFFFFFu, above, 2);
+    if (i < n && (tid & 3) == 0) rank = above;
+  } else if (tid < n) {
     k = S.kept[tid];
     rank = 0;
     for (int i = 0; i < n; ++i) rank += S.kept[i] > k;
@@ -279,29 +293,105 @@ __device__ __noinline__ int select_top(Smem& S, int n, int N) {
   return min(n, N);
 }
 
-// A floor for this step when its candidates are too many to keep: at least N
-// threads hold an entry at or above it, and no more than `most` threads do, by
-// value (key) or, among equal values, by the index `last` of the latest kept one.
-__device__ __noinline__ void find_floor(Smem& S, uint32_t mine, int first_of_mine, int N, int most, uint32_t* floor_key, int* last) {
-  uint32_t T = 0;
-  int cnt = kT;
-  for (int bit = 31; bit >= 0 && cnt > most; --bit) {
-    const uint32_t t = T | (1u << bit);
-    const int c = __syncthreads_count(mine >= t);
-    if (c >= N) { T = t; cnt = c; }
+// The N best of what this block has kept (`have` in S.top) and of the steps
+// recorded since, vectors [v0, v_end) of the row in steps of kStep, in S.top; returns
+// their number.  `best` is the largest record of this thread.
+template <int DT>
+__device__ __noinline__ int collect(Smem& S, Row<DT> row, int V, int v0, int v_end, uint32_t best, int have, int N) {
+  constexpr int kN = Vec<DT>::kN, kEach = kU * kN, kGroup = (kC - kMaxN) / kEach;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t none = Vec<DT>::rec(-INFINITY);
+  const int steps = (v_end - v0 + kStep - 1) / kStep;
+  // A floor that N entries reach: every warp has ceil(N / kW) lanes at or above it;
+  // then halved towards the largest record while N threads still are.
+  const int share = (N + kW - 1) / kW;
+  uint32_t v = best, floor_r = 0;
+  const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, best);
+  for (int i = 0; i < share; ++i) {
+    floor_r = __reduce_max_sync(0xFFFFFFFFu, v);
+    if (lane == __ffs(__ballot_sync(0xFFFFFFFFu, v == floor_r)) - 1) v = 0;
   }
-  *floor_key = T;
-  *last = 0x7FFFFFFF;
-  if (cnt > most) {
-    // ties at T: the N-th lowest first index among the threads at it
-    const int above = __syncthreads_count(mine > T);
-    int I = 0;
-    for (int bit = 30; bit >= 0; --bit) {
-      const int t = I | (1 << bit);
-      if (above + __syncthreads_count(mine == T && first_of_mine < t) < N) I = t;
+  if (lane == 0) { S.floors[warp] = floor_r; S.tops[warp] = most; }
+  const unsigned long long carried = have == N ? S.top[N - 1] : 0ull;
+  if (tid < have) S.kept[tid] = S.top[tid];
+  if (tid == 0) { S.n = have; S.list = 0; }
+  __syncthreads();
+  floor_r = S.floors[0];
+  uint32_t above = S.tops[0];
+#pragma unroll
+  for (int i = 1; i < kW; ++i) {
+    floor_r = min(floor_r, S.floors[i]);
+    above = max(above, S.tops[i]);
+  }
+  ++above;                                       // no thread reaches it
+  while (above - floor_r > 1) {
+    const uint32_t t = (above + floor_r) / 2;
+    const int c = __syncthreads_count(best >= t);
+    if (c >= N) floor_r = t;
+    else above = t;
+    if (c >= N && c <= N + N / 4 + 1) break;
+  }
+  floor_r = max(floor_r, none + 1u);             // entries of -inf are none
+  unsigned long long floor_k = carried;
+  if (best >= floor_r)
+    for (int i = 0; i < steps; ++i)
+      if (S.records[i][tid] >= floor_r) {
+        const int at = atomicAdd(&S.list, 1);
+        if (at < kList) S.chunks[at] = i * kT + tid;
+      }
+  __syncthreads();
+
+  // read the listed chunks again, a warp to a chunk and a lane to an entry
+  auto read_list = [&]() {
+    const int list = S.list;
+    for (int j = warp * (32 / kEach) + lane / kEach; j < list + 32; j += kW * (32 / kEach)) {
+      if (__all_sync(0xFFFFFFFFu, j >= list)) break;
+      const int l = lane % kEach, chunk = j < list ? S.chunks[j] : 0;
+      const int v = v0 + (chunk / kT) * kStep + (l / kN) * kT + chunk % kT;
+      const long long at = static_cast<long long>(v) * kN - row.mis + l % kN;
+      const float x = j < list && v < v_end && at >= 0 && at < V ? row.at(static_cast<int>(at)) : -INFINITY;
+      const unsigned long long k = order_key(x, static_cast<unsigned>(at));
+      const bool in = x > -INFINITY && Vec<DT>::rec(x) >= floor_r && k > floor_k;
+      const unsigned who = __ballot_sync(0xFFFFFFFFu, in);
+      int base = 0;
+      if (lane == 0 && who) base = atomicAdd(&S.n, __popc(who));
+      base = __shfl_sync(0xFFFFFFFFu, base, 0);
+      base += __popc(who & ((1u << lane) - 1u));
+      if (in && base < kC) S.kept[base] = k;
     }
-    *last = I;
+    __syncthreads();
+  };
+  if (S.list <= kList) {
+    read_list();
+    if (S.n <= kC) return select_top(S, S.n, N);
+    if (tid < have) S.kept[tid] = S.top[tid];
   }
+  __syncthreads();
+  if (tid == 0) S.n = have;
+  // Many: ties, or one thread's entries large in many steps.  In the row's order and
+  // in groups, the floor rising: equal values stop at the first group (where a
+  // record is the value; an f32 record stands for a range of values).
+  int n = have;
+  for (int i = 0; i < steps; ++i)
+    for (int part = 0; part < kT; part += kGroup) {
+      const int first = (v0 + i * kStep + tid) * kN - row.mis;      // the chunk's lowest index
+      const uint32_t k = S.records[i][tid];
+      const bool in = tid >= part && tid < part + kGroup && k >= floor_r &&
+                      (floor_k == 0ull || k > Vec<DT>::rec(order_value(floor_k)) ||
+                       (k == Vec<DT>::rec(order_value(floor_k)) && (kN == 4 || first <= order_index(floor_k))));
+      if (!__syncthreads_or(in)) continue;
+      if (tid == 0) S.list = 0;
+      __syncthreads();
+      if (in) S.chunks[atomicAdd(&S.list, 1)] = i * kT + tid;
+      __syncthreads();
+      read_list();
+      n = select_top(S, S.n, N);
+      if (tid < n) S.kept[tid] = S.top[tid];
+      if (tid == 0) S.n = n;
+      if (n == N) floor_k = S.top[N - 1];
+      __syncthreads();
+    }
+  return n;
 }
 
 // One row's (or part's) running state and the reading of it, by one block.
@@ -313,48 +403,50 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long total = P.nv * P.R, blocks = gridDim.x;
 
-  Walk<DT> w;
-  w.pos = blockIdx.x * total / blocks;
-  w.end = (blockIdx.x + 1ll) * total / blocks;
-  w.r = static_cast<int>(w.pos / P.nv);
-  w.row_start = w.r * P.nv;
-  w.row.set(P, w.r);
-  Walk<DT> ahead = w;
-  fetch(P, ahead, S, 0);
-  ahead.advance(P);
-  if (tid == 0) S.n = 0;
+  const long long begin = blockIdx.x * total / blocks;
+  if (tid == 0) {
+    S.end = (blockIdx.x + 1ll) * total / blocks;
+    S.n = 0;
+  }
+  __syncthreads();
+  int r = static_cast<int>(begin / P.nv);
+  Piece<DT> p;
+  p.row.set(P, r);
+  p.v = static_cast<int>(begin - r * P.nv);
+  p.v_end = static_cast<int>(min(S.end - r * P.nv, P.nv));
+  fetch(p, P.V, S, 0);
   int parity = 0;
 
-  while (!w.done()) {
-    const int r = w.r;
-    const Row<DT> row = w.row;
-    const long long row_start = w.row_start, row_end = min(w.end, row_start + P.nv);
-    const float T = P.temperature ? P.temperature[r] : 1.0f;
-    const bool greedy = T <= 0.0f;
-    const float c = greedy ? 0.0f : fminf(kLog2e / T, 3e38f);
-    const int N = max(P.N, greedy ? 1 : 0);
-    // the row's tokens, read while the row streams
-    int tok = -1;
-    float tok_x = 0.0f;
-    if (tid < P.K) {
-      tok = P.token_ids[static_cast<long long>(r) * P.K + tid];
-      if (tok >= 0 && tok < P.V) tok_x = row.at(tok);
+  for (;;) {
+    int N = P.N, have = 0;
+    float c = kLog2e;
+    if (P.temperature) {
+      const float T = P.temperature[r];
+      c = T <= 0.0f ? 0.0f : fminf(kLog2e / T, 3e38f);
+      if (T <= 0.0f) N = max(N, 1);                // greedy: the maximum's index is the answer
     }
 
-    float ref = -INFINITY, big = -INFINITY, floor_v = -INFINITY;
+    float ref = -INFINITY, big = -INFINITY;
     f2 z2 = pack(0.0f, 0.0f), s2 = pack(0.0f, 0.0f);
-    bool bad = false;
-    int n = 0;
-    for (; w.pos < row_end; w.advance(P), parity ^= 1) {
-      fetch(P, ahead, S, parity ^ 1);
-      if (!ahead.done()) ahead.advance(P);
+    while (p.v < p.v_end) {             // once, but for rows of more steps than there are records
+    const int v0 = p.v;
+    uint32_t best = 0;
+    for (int step = 0; step < kMaxSteps && p.v < p.v_end; ++step, parity ^= 1) {
+      p.v += kStep;
+      if (p.v < p.v_end) fetch(p, P.V, S, parity ^ 1);
+      else if ((r + 1) * P.nv < S.end) {
+        Piece<DT> next;                // the next row begins while this one ends
+        next.row.set(P, r + 1);
+        next.v = 0;
+        next.v_end = static_cast<int>(min(S.end - (r + 1) * P.nv, P.nv));
+        fetch(next, P.V, S, parity ^ 1);
+      } else cp_commit();
       cp_wait<1>();
       uint4 v[kU];
 #pragma unroll
       for (int u = 0; u < kU; ++u) v[u] = S.ring[parity * kU + u][tid];
       const float top = Vec<DT>::biggest(v);
-      bad |= !(top < INFINITY);
-      big = fmaxf(big, top);
+      big = max_nan(big, top);
       if ((top - ref) * c > kSlack || (ref == -INFINITY && top > ref)) {
         const float d = (ref - top) * c, f = ref == -INFINITY ? 0.0f : ex2_approx(d);
         float za, zb, sa, sb;
@@ -385,66 +477,32 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
           }
       }
       if (N > 0) {
-        const int cand = __syncthreads_count(top > floor_v);
-        if (cand) {
-          const int v0 = static_cast<int>(w.pos - row_start);
-          uint32_t floor_key = 0;
-          int last = 0x7FFFFFFF;
-          bool keep = top > floor_v;
-          const int most = (kC - n) / (kU * kN);
-          if (cand > most) {
-            const uint32_t mine = keep ? value_key(top) : 0u;
-            int first = 0x7FFFFFFF;
-#pragma unroll
-            for (int u = kU - 1; u >= 0; --u)
-#pragma unroll
-              for (int i = kN / 2 - 1; i >= 0; --i) {
-                float a, b;
-                Vec<DT>::pair(v[u], i, a, b);
-                const int at = (v0 + u * kT + tid) * kN - row.mis + 2 * i;
-                if (b == top) first = at + 1;
-                if (a == top) first = at;
-              }
-            find_floor(S, mine, first, N, most, &floor_key, &last);
-            keep = mine > floor_key || (mine == floor_key && first <= last);
-          }
-          if (keep) {
-#pragma unroll 1
-            for (int u = 0; u < kU; ++u) {
-              const uint4 q = S.ring[parity * kU + u][tid];
-              const int at = (v0 + u * kT + tid) * kN - row.mis;
-#pragma unroll
-              for (int i = 0; i < kN; ++i) {
-                float a, b;
-                Vec<DT>::pair(q, i / 2, a, b);
-                const float x = i & 1 ? b : a;
-                const uint32_t k = value_key(x);
-                if (x > floor_v && (k > floor_key || (k == floor_key && at + i <= last)))
-                  S.kept[atomicAdd(&S.n, 1)] = order_key(x, at + i);
-              }
-            }
-          }
-          __syncthreads();
-          n = S.n;
-          if (floor_key) floor_v = fmaxf(floor_v, unkey32(floor_key));
-          if (n > 3 * N + 16) {        // fewer candidates from here on
-            n = select_top(S, n, N);
-            if (tid < n) S.kept[tid] = S.top[tid];
-            if (tid == 0) S.n = n;
-            if (n == N) floor_v = order_value(S.top[N - 1]);
-            __syncthreads();
-          }
-        }
+        const uint32_t k = Vec<DT>::rec(top);
+        S.records[step][tid] = static_cast<uint16_t>(k);
+        best = max(best, k);
       }
+    }
+    if (N > 0)
+      have = collect<DT>(S, p.row, P.V, v0, min(p.v, p.v_end), best, have, N);
     }
 
     // ---- this block's triple
+    const Row<DT> row = p.row;
+    const long long row_start = r * P.nv;
+    const float T = P.temperature ? P.temperature[r] : 1.0f;
+    const bool greedy = T <= 0.0f;
+    int tok = -1;
+    float tok_x = 0.0f;
+    if (tid < P.K) {
+      tok = P.token_ids[static_cast<long long>(r) * P.K + tid];
+      if (tok >= 0 && tok < P.V) tok_x = row.at(tok);
+    }
     float M = big, z, s, zb, sb;
     unpack(z2, z, zb);
     unpack(s2, s, sb);
     z += zb;
     s += sb;
-    bad = __syncthreads_or(bad);
+    bool bad = __syncthreads_or(!(big < INFINITY));
 #pragma unroll
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
     if (lane == 0) S.red[0][warp] = M;
@@ -464,9 +522,7 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
       s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
     }
     if (lane == 0) { S.red[1][warp] = z; S.red[2][warp] = s; }
-    int have = 0;
-    if (N > 0) have = select_top(S, n, N);
-    else __syncthreads();
+    __syncthreads();
     z = s = 0.0f;
 #pragma unroll
     for (int i = 0; i < kW; ++i) { z += S.red[1][i]; s += S.red[2][i]; }
@@ -478,8 +534,8 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
     if (parts > 1) {
       auto slot_of = [&](int p) -> long long { return p == 0 ? 2 * a + 1 : 2 * (a + p); };
       const long long slot = slot_of(static_cast<int>(blockIdx.x - a));
-      if (tid < have) P.part_top[slot * kMaxN + tid] = S.top[tid];
-      if (tid == 0) P.parts[slot] = Part{M, z, s, have | (bad ? 1 << 16 : 0)};
+      if (tid < N) P.part_top[slot * kMaxN + tid] = tid < have ? S.top[tid] : 0ull;
+      if (tid == 0) P.parts[slot] = Part{M, z, s, bad ? 1 : 0};
       __syncthreads();
       if (tid == 0) {
         unsigned got;
@@ -492,16 +548,22 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
       __syncthreads();
       finish = S.flag != 0;
       if (finish) {
-        // parts <= kMaxParts < kT: one each
+        // parts <= kMaxParts < kT: one each; their alternatives in the same round of loads
+        constexpr int kEach = kMaxParts * kMaxN / kT;
+        unsigned long long key[kEach];
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+          const int i = j * kT + tid;
+          key[j] = i < parts * N ? __ldcg(P.part_top + slot_of(i / N) * kMaxN + i % N) : 0ull;
+        }
         Part q = {-INFINITY, 0.0f, 0.0f, 0};
-        unsigned long long low = 0;
+        unsigned long long low = 0;    // a part's N-th bounds the row's from below
         if (tid < parts) {
           const float4 u = __ldcg(reinterpret_cast<const float4*>(P.parts + slot_of(tid)));
           q = Part{u.x, u.y, u.z, __float_as_int(u.w)};
-          // a part with N alternatives bounds the row's N-th from below
-          if (N > 0 && (q.flags & 0xFFFF) == N) low = __ldcg(P.part_top + slot_of(tid) * kMaxN + N - 1);
+          if (N > 0) low = __ldcg(P.part_top + slot_of(tid) * kMaxN + N - 1);
         }
-        bad = __syncthreads_or(q.flags >> 16);
+        bad = __syncthreads_or(q.flags);
         M = q.m;
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
@@ -527,16 +589,34 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
           s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
         }
         if (lane == 0) { S.red[1][warp] = z; S.red[2][warp] = s; }
+        have = 0;
         if (N > 0) {
-          for (int i = tid; i < parts * N; i += kT) {
-            const long long from = slot_of(i / N);
-            if (i % N < (__ldcg(&P.parts[from].flags) & 0xFFFF)) {
-              const unsigned long long k = __ldcg(P.part_top + from * kMaxN + i % N);
-              if (k >= low) S.kept[atomicAdd(&S.n, 1)] = k;
+          // the parts' entries that reach the bound
+          low = max(low, 1ull);
+#pragma unroll
+          for (int j = 0; j < kEach; ++j)
+            if (key[j] >= low) {
+              const int at = atomicAdd(&S.n, 1);
+              if (at < kC) S.kept[at] = key[j];
+            }
+          __syncthreads();
+          if (S.n <= kC) {
+            have = select_top(S, S.n, N);
+          } else {
+            // too many for one selection: in groups of parts
+            for (int p0 = 0; p0 < parts; p0 += kJoin) {
+              __syncthreads();
+              if (tid < have) S.kept[tid] = S.top[tid];
+              if (tid == 0) S.n = have;
+              __syncthreads();
+              for (int i = tid; i < min(kJoin, parts - p0) * N; i += kT) {
+                const unsigned long long k = __ldcg(P.part_top + slot_of(p0 + i / N) * kMaxN + i % N);
+                if (k >= low) S.kept[atomicAdd(&S.n, 1)] = k;
+              }
+              __syncthreads();
+              have = select_top(S, S.n, N);
             }
           }
-          __syncthreads();
-          have = select_top(S, S.n, N);
         } else {
           __syncthreads();
         }
@@ -574,11 +654,15 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
         P.top_logprobs[at] = is ? logprob(order_value(S.top[tid]), order_index(S.top[tid])) : bad ? NAN : -INFINITY;
       }
     }
+    ++r;
+    if (r * P.nv >= S.end) break;
+    p.row.set(P, r);
+    p.v = 0;
+    p.v_end = static_cast<int>(min(S.end - r * P.nv, P.nv));
     __syncthreads();
     if (tid == 0) S.n = 0;
     __syncthreads();
   }
-  cp_wait<0>();
 }
 
 // Workspace: one slot for a part a block shares with the one before it, one for
@@ -648,6 +732,9 @@ int ecah_token_logprobs(const ecah_logprob_args* a, void* stream) {
   // alternatives are joined of at most kMaxParts
   long long blocks = std::min<long long>(static_cast<long long>(sms) * lp::kBlocks, (P.nv * P.R + lp::kT - 1) / lp::kT);
   blocks = std::min<long long>(blocks, (lp::kMaxParts - 2ll) * P.R);
+  // Few rows: whole blocks to a row, so that none starts and ends two of them.
+  // 128 rows of 151936 f16 with 20 alternatives on 444 blocks, against 384: see below.
+  if (blocks >= 2ll * P.R) blocks = blocks / P.R * P.R;
   auto fn = a->dtype == ECAH_DTYPE_F16 ? lp::token_logprobs_kernel<ECAH_DTYPE_F16>
             : a->dtype == ECAH_DTYPE_BF16 ? lp::token_logprobs_kernel<ECAH_DTYPE_BF16>
                                           : lp::token_logprobs_kernel<ECAH_DTYPE_F32>;
