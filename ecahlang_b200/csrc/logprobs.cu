@@ -31,26 +31,21 @@ namespace lp {
 // that spans several blocks is joined by the block that arrives last, in the order
 // of the parts.
 
-constexpr int kT = 256;
+constexpr int kT = 128;
 constexpr int kW = kT / 32;
-constexpr int kU = 4;                  // vectors of a thread and step
+constexpr int kU = 5;                  // vectors of a thread and step
 constexpr int kStep = kT * kU;         // vectors of a step
-constexpr int kBlocks = 3;             // per SM: 80 registers a thread, 48 KB in flight
+constexpr int kBlocks = 5;             // per SM: 96 registers a thread, 50 KB in flight
 constexpr int kRing = 2 * kU;          // a step in flight behind the one at work
-constexpr int kC = 1024;               // entries of one selection
-constexpr int kMaxSteps = 20;          // steps with a record: 163840 16-bit logits
+constexpr int kC = 512;                // entries of one selection
+constexpr int kMaxSteps = 32;          // steps with a record: 163840 16-bit logits
 constexpr int kMaxN = ECAH_MAX_TOP_N;
 constexpr int kList = 128;             // steps read again at once
-constexpr int kMaxParts = 64;          // parts of a row
+constexpr int kMaxParts = 32;          // parts of a row
 constexpr int kJoin = (kC - kMaxN) / kMaxN;   // parts whose alternatives are joined at once
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 40.0f;        // the reference moves when an exponent would pass it
 constexpr float kTiny = -150.0f;       // 2^kTiny is zero in float32
-
-struct alignas(16) Part {
-  float m, z, s;
-  int flags;                           // 1: a NaN or +inf
-};
 
 struct Params {
   const void* logits;
@@ -64,8 +59,10 @@ struct Params {
   int* top_ids;
   float* top_logprobs;
   long long nv;                        // vectors of a row, its edges included
+  long long share;                     // vectors of a block: share, and one more in the first `more`
+  int more;
   unsigned* counters;                  // [slots], zero between launches
-  Part* parts;                         // [slots]
+  float4* parts;                       // [slots] m (NaN: the row has no distribution), z, s
   unsigned long long* part_top;        // [slots][kMaxN]
 };
 
@@ -76,10 +73,12 @@ struct Smem {
   int chunks[kList];
   unsigned long long top[kMaxN];
   float red[3][kW];
-  uint32_t floors[kW], tops[kW];
-  int n, flag, count, list;
-  long long end;                       // of this block's share
+  uint32_t best[32];
+  int n, flag, list;
+  long long begin, end;                // this block's share
 };
+
+static_assert((sizeof(Smem) + 1024) * kBlocks <= 227 * 1024, "the blocks of an SM fit its shared memory");
 
 // Order of the alternatives: value descending, then index ascending, as one
 // 64-bit key (larger is earlier).  -0 counts as +0, as a comparison would.
@@ -125,6 +124,7 @@ template <int DT> struct Vec {
   static constexpr int kN = DType<DT>::kVec;
   // a value's record, in the order of the values (f32: rounded down to 16 bits)
   static __device__ __forceinline__ uint32_t rec(float x) { return key16(DType<DT>::to_raw(x == 0.0f ? 0.0f : x)); }
+  static __device__ __forceinline__ float value(uint32_t rec) { return DType<DT>::to_f32(unkey16(rec)); }
   static constexpr uint32_t kOut = DT == ECAH_DTYPE_F16 ? 0xFC00FC00u : 0xFF80FF80u;   // -inf
   static __device__ __forceinline__ void pair(const uint4& v, int i, float& a, float& b) {
     const uint32_t w = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
@@ -141,25 +141,28 @@ template <int DT> struct Vec {
     else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
   }
-  static __device__ __forceinline__ float biggest(const uint4 (&v)[kU]) {
+  template <int U>
+  static __device__ __forceinline__ float biggest(const uint4 (&v)[U]) {
     uint32_t m = v[0].x;
 #pragma unroll
-    for (int u = 0; u < kU; ++u) m = max2(max2(m, max2(v[u].x, v[u].y)), max2(v[u].z, v[u].w));
+    for (int u = 0; u < U; ++u) m = max2(max2(m, max2(v[u].x, v[u].y)), max2(v[u].z, v[u].w));
     return max_nan(DType<DT>::to_f32(m & 0xFFFFu), DType<DT>::to_f32(m >> 16));
   }
 };
 template <> struct Vec<ECAH_DTYPE_F32> {
   static constexpr int kN = 4;
   static __device__ __forceinline__ uint32_t rec(float x) { return value_key(x) >> 16; }
+  static __device__ __forceinline__ float value(uint32_t rec) { return unkey32(rec << 16); }
   static constexpr uint32_t kOut = 0xFF800000u;
   static __device__ __forceinline__ void pair(const uint4& v, int i, float& a, float& b) {
     a = __uint_as_float(i == 0 ? v.x : v.z);
     b = __uint_as_float(i == 0 ? v.y : v.w);
   }
-  static __device__ __forceinline__ float biggest(const uint4 (&v)[kU]) {
+  template <int U>
+  static __device__ __forceinline__ float biggest(const uint4 (&v)[U]) {
     float m = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < kU; ++u)
+    for (int u = 0; u < U; ++u)
       m = max_nan(max_nan(max_nan(m, __uint_as_float(v[u].x)), max_nan(__uint_as_float(v[u].y), __uint_as_float(v[u].z))),
                   __uint_as_float(v[u].w));
     return m;
@@ -197,140 +200,130 @@ struct Piece {
   int v, v_end;
 };
 
-// Copies this thread's vectors of the step at piece.v into its own ring slots.
+// A vector at the row's edge, entry by entry: -inf outside the row.
 template <int DT>
-__device__ __forceinline__ void fetch(const Piece<DT>& p, int V, Smem& S, int parity) {
+__device__ __noinline__ uint4 edge_vector(const unsigned char* base, int mis, int v, int V) {
   constexpr int kN = Vec<DT>::kN;
-  const int tid = threadIdx.x;
-  uint4* slot = &S.ring[parity * kU][tid];
-  const int whole0 = p.row.mis ? 1 : 0, whole1 = (V + p.row.mis) / kN;   // vectors wholly inside the row
-  if (p.v >= whole0 && p.v + kStep <= min(whole1, p.v_end)) {
-    const unsigned char* src = p.row.base + static_cast<long long>(p.v + tid) * 16;
+  using Raw = typename DType<DT>::Raw;
+  uint32_t q[4] = {Vec<DT>::kOut, Vec<DT>::kOut, Vec<DT>::kOut, Vec<DT>::kOut};
+  const long long first = static_cast<long long>(v) * kN - mis;
+  const Raw* x = reinterpret_cast<const Raw*>(base) + static_cast<long long>(v) * kN;
+#pragma unroll
+  for (int j = 0; j < kN; ++j)
+    if (first + j >= 0 && first + j < V) {
+      const uint32_t raw = x[j];
+      if (kN == 4) q[j] = raw;
+      else q[j / 2] = (j & 1) ? (q[j / 2] & 0xFFFFu) | (raw << 16) : (q[j / 2] & 0xFFFF0000u) | raw;
+    }
+  return make_uint4(q[0], q[1], q[2], q[3]);
+}
+
+// Copies this thread's vectors of the step at v0 into its own ring slots, where
+// the step is not wholly inside the row and the piece.
+template <int DT>
+__device__ __noinline__ void fetch_edge(const unsigned char* base, int mis, int v0, int v_end, int V, uint4* slot) {
+  const int whole0 = mis ? 1 : 0, whole1 = (V + mis) / Vec<DT>::kN;     // vectors wholly inside the row
+  for (int u = 0; u < kU; ++u) {
+    const int v = v0 + u * kT + threadIdx.x;
+    if (v >= whole0 && v < whole1 && v < v_end)
+      cp16(static_cast<uint32_t>(__cvta_generic_to_shared(slot + u * kT)), base + static_cast<long long>(v) * 16);
+    else
+      slot[u * kT] = v < v_end ? edge_vector<DT>(base, mis, v, V) : make_uint4(Vec<DT>::kOut, Vec<DT>::kOut, Vec<DT>::kOut, Vec<DT>::kOut);
+  }
+}
+
+// Steps that begin at [first, last] are wholly inside: copied without a look.
+template <int DT>
+__device__ __forceinline__ void fetch(const Piece<DT>& p, int first, int last, int V, Smem& S, int parity) {
+  uint4* slot = &S.ring[parity * kU][threadIdx.x];
+  if (p.v >= first && p.v <= last) {
+    const unsigned char* src = p.row.base + static_cast<long long>(p.v + static_cast<int>(threadIdx.x)) * 16;
     const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(slot));
 #pragma unroll
     for (int u = 0; u < kU; ++u) cp16(dst + u * kT * 16, src + u * kT * 16);
   } else {
-#pragma unroll 1
-    for (int u = 0; u < kU; ++u) {
-      const int v = p.v + u * kT + tid;
-      if (v >= whole0 && v < whole1 && v < p.v_end) {
-        cp16(static_cast<uint32_t>(__cvta_generic_to_shared(slot + u * kT)), p.row.base + static_cast<long long>(v) * 16);
-        continue;
-      }
-      uint32_t q[4] = {Vec<DT>::kOut, Vec<DT>::kOut, Vec<DT>::kOut, Vec<DT>::kOut};
-      if (v < p.v_end) {                // the row's edge: entry by entry
-        using Raw = typename DType<DT>::Raw;
-        const long long first = static_cast<long long>(v) * kN - p.row.mis;
-        const Raw* x = reinterpret_cast<const Raw*>(p.row.base) + static_cast<long long>(v) * kN;
-#pragma unroll
-        for (int j = 0; j < kN; ++j)
-          if (first + j >= 0 && first + j < V) {
-            const uint32_t raw = x[j];
-            if (kN == 4) q[j] = raw;
-            else q[j / 2] = (j & 1) ? (q[j / 2] & 0xFFFFu) | (raw << 16) : (q[j / 2] & 0xFFFF0000u) | raw;
-          }
-      }
-      slot[u * kT] = make_uint4(q[0], q[1], q[2], q[3]);
-    }
+    fetch_edge<DT>(p.row.base, p.row.mis, p.v, p.v_end, V, slot);
   }
   cp_commit();
 }
+template <int DT>
+__device__ __forceinline__ int first_whole(const Piece<DT>& p) { return p.row.mis ? 1 : 0; }
+template <int DT>
+__device__ __forceinline__ int last_whole(const Piece<DT>& p, int V) { return min((V + p.row.mis) / Vec<DT>::kN, p.v_end) - kStep; }
 
-__device__ __forceinline__ int block_sum(int v, Smem& S) {
-  __syncthreads();
-  if (threadIdx.x == 0) S.count = 0;
-  __syncthreads();
-  v = __reduce_add_sync(0xFFFFFFFFu, v);
-  if ((threadIdx.x & 31) == 0) atomicAdd(&S.count, v);
-  __syncthreads();
-  return S.count;
+// A triple (m, z, s) as seen from M >= m.
+__device__ __forceinline__ void seen_from(float M, float m, float c, float& z, float& s) {
+  const float d = (m - M) * c, f = m == -INFINITY ? 0.0f : m == M ? 1.0f : ex2_approx(d);
+  s = f > 0.0f ? f * (s + (m == M ? 0.0f : d) * z) : 0.0f;
+  z *= f;
 }
 
 // The N largest of the n kept entries, in order, in S.top; returns their number.
-// Called by the whole block; S.kept is then free to be written again.
+// Called by the whole block after a barrier; ends with one.
 __device__ __noinline__ int select_top(Smem& S, int n, int N) {
   const int tid = threadIdx.x;
-  __syncthreads();
-  if (n > kT) {
-    // more than one each: the N-th largest by bits (the keys are distinct), then only those
-    unsigned long long T = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-      const unsigned long long t = T | (1ull << bit);
-      int c = 0;
-      for (int i = tid; i < n; i += kT) c += S.kept[i] >= t;
-      if (block_sum(c, S) >= N) T = t;
-    }
-    __syncthreads();
-    if (tid == 0) S.count = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += kT)
-      if (S.kept[i] >= T) S.top[atomicAdd(&S.count, 1)] = S.kept[i];
-    __syncthreads();
-    n = N;
-    if (tid < n) S.kept[tid] = S.top[tid];
-    __syncthreads();
-  }
-  unsigned long long k = 0;
-  int rank = N;
-  if (n <= kT / 4) {                   // four threads a key
-    const int i = tid >> 2;
-    int above = 0;
+  if (n <= kT) {                       // four, two or one threads a key
+    const int shift = n <= kT / 4 ? 2 : n <= kT / 2 ? 1 : 0, i = tid >> shift, step = 1 << shift;
+    unsigned long long k = 0;
+    int rank = 0;
     if (i < n) {
       k = S.kept[i];
-      for (int j = tid & 3; j < n; j += 4) above += S.kept[j] > k;
+#pragma unroll 8
+      for (int j = tid & (step - 1); j < n; j += step) rank += S.kept[j] > k;
     }
-    above += __shfl_xor_sync(0xFFFFFFFFu, above, 1);
-    above += __shfl_xor_sync(0xFFFFFFFFu, above, 2);
-    if (i < n && (tid & 3) == 0) rank = above;
-  } else if (tid < n) {
-    k = S.kept[tid];
-    rank = 0;
-    for (int i = 0; i < n; ++i) rank += S.kept[i] > k;
+    if (shift >= 1) rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 1);
+    if (shift == 2) rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 2);
+    if (i < n && rank < N) S.top[rank] = k;      // the threads of a key agree
+  } else {                             // up to kC / kT keys a thread
+    unsigned long long key[kC / kT];
+    int above[kC / kT];
+#pragma unroll
+    for (int i = 0; i < kC / kT; ++i) {
+      key[i] = i * kT + tid < n ? S.kept[i * kT + tid] : 0ull;
+      above[i] = 0;
+    }
+    for (int j = 0; j < n; ++j) {
+      const unsigned long long q = S.kept[j];
+#pragma unroll
+      for (int i = 0; i < kC / kT; ++i) above[i] += q > key[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kC / kT; ++i)
+      if (i * kT + tid < n && above[i] < N) S.top[above[i]] = key[i];
   }
-  __syncthreads();
-  if (rank < N) S.top[rank] = k;
   __syncthreads();
   return min(n, N);
 }
 
 // The N best of what this block has kept (`have` in S.top) and of the steps
 // recorded since, vectors [v0, v_end) of the row in steps of kStep, in S.top; returns
-// their number.  `best` is the largest record of this thread.
+// their number.  `best` is the largest record of this thread; a single step is
+// still in the ring's half `parity`.
 template <int DT>
-__device__ __noinline__ int collect(Smem& S, Row<DT> row, int V, int v0, int v_end, uint32_t best, int have, int N) {
+__device__ __noinline__ int collect(Smem& S, Row<DT> row, int V, int v0, int v_end, int parity, uint32_t best, int have, int N) {
   constexpr int kN = Vec<DT>::kN, kEach = kU * kN, kGroup = (kC - kMaxN) / kEach;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t none = Vec<DT>::rec(-INFINITY);
   const int steps = (v_end - v0 + kStep - 1) / kStep;
-  // A floor that N entries reach: every warp has ceil(N / kW) lanes at or above it;
-  // then halved towards the largest record while N threads still are.
-  const int share = (N + kW - 1) / kW;
-  uint32_t v = best, floor_r = 0;
-  const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, best);
-  for (int i = 0; i < share; ++i) {
-    floor_r = __reduce_max_sync(0xFFFFFFFFu, v);
-    if (lane == __ffs(__ballot_sync(0xFFFFFFFFu, v == floor_r)) - 1) v = 0;
+  // A floor that N threads reach: the N-th largest of every warp's few best lanes.
+  const int share = (N + kW - 1) / kW, few = min(share > 1 ? share + 2 : 1, 32 / kW), all = few * kW;
+  uint32_t v = best;
+  for (int i = 0; i < few; ++i) {
+    const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, v);
+    const bool mine = lane == __ffs(__ballot_sync(0xFFFFFFFFu, v == m)) - 1;
+    if (mine) { S.best[warp * few + i] = m; v = 0; }
   }
-  if (lane == 0) { S.floors[warp] = floor_r; S.tops[warp] = most; }
   const unsigned long long carried = have == N ? S.top[N - 1] : 0ull;
   if (tid < have) S.kept[tid] = S.top[tid];
   if (tid == 0) { S.n = have; S.list = 0; }
   __syncthreads();
-  floor_r = S.floors[0];
-  uint32_t above = S.tops[0];
-#pragma unroll
-  for (int i = 1; i < kW; ++i) {
-    floor_r = min(floor_r, S.floors[i]);
-    above = max(above, S.tops[i]);
+  v = lane < all ? S.best[lane] : 0u;
+  int rank = 0;
+  for (int i = 0; i < all; ++i) {
+    const uint32_t k = S.best[i];
+    rank += k > v || (k == v && i < lane);
   }
-  ++above;                                       // no thread reaches it
-  while (above - floor_r > 1) {
-    const uint32_t t = (above + floor_r) / 2;
-    const int c = __syncthreads_count(best >= t);
-    if (c >= N) floor_r = t;
-    else above = t;
-    if (c >= N && c <= N + N / 4 + 1) break;
-  }
+  uint32_t floor_r = __shfl_sync(0xFFFFFFFFu, v, __ffs(__ballot_sync(0xFFFFFFFFu, lane < all && rank == N - 1)) - 1);
   floor_r = max(floor_r, none + 1u);             // entries of -inf are none
   unsigned long long floor_k = carried;
   if (best >= floor_r)
@@ -341,32 +334,44 @@ __device__ __noinline__ int collect(Smem& S, Row<DT> row, int V, int v0, int v_e
       }
   __syncthreads();
 
-  // read the listed chunks again, a warp to a chunk and a lane to an entry
+  // Read the listed steps again, a lane to a vector.  `low_v` is the smallest value of
+  // the floor's record; an entry at or below the carried floor leaves an empty key.
+  const float low_v = Vec<DT>::value(floor_r);
+  const int whole0 = row.mis ? 1 : 0, whole1 = (V + row.mis) / kN;
   auto read_list = [&]() {
-    const int list = S.list;
-    for (int j = warp * (32 / kEach) + lane / kEach; j < list + 32; j += kW * (32 / kEach)) {
-      if (__all_sync(0xFFFFFFFFu, j >= list)) break;
-      const int l = lane % kEach, chunk = j < list ? S.chunks[j] : 0;
-      const int v = v0 + (chunk / kT) * kStep + (l / kN) * kT + chunk % kT;
-      const long long at = static_cast<long long>(v) * kN - row.mis + l % kN;
-      const float x = j < list && v < v_end && at >= 0 && at < V ? row.at(static_cast<int>(at)) : -INFINITY;
-      const unsigned long long k = order_key(x, static_cast<unsigned>(at));
-      const bool in = x > -INFINITY && Vec<DT>::rec(x) >= floor_r && k > floor_k;
-      const unsigned who = __ballot_sync(0xFFFFFFFFu, in);
-      int base = 0;
-      if (lane == 0 && who) base = atomicAdd(&S.n, __popc(who));
-      base = __shfl_sync(0xFFFFFFFFu, base, 0);
-      base += __popc(who & ((1u << lane) - 1u));
-      if (in && base < kC) S.kept[base] = k;
+    const int vectors = S.list * kU;
+    for (int e = tid; e < vectors; e += kT) {
+      const int chunk = S.chunks[e / kU], u = e % kU, v = v0 + (chunk / kT) * kStep + u * kT + chunk % kT;
+      uint4 q = make_uint4(Vec<DT>::kOut, Vec<DT>::kOut, Vec<DT>::kOut, Vec<DT>::kOut);
+      if (steps == 1) q = S.ring[parity * kU + u][chunk % kT];
+      else if (v >= whole0 && v < min(whole1, v_end)) q = __ldg(reinterpret_cast<const uint4*>(row.base) + v);
+      else if (v < v_end) q = edge_vector<DT>(row.base, row.mis, v, V);
+      const uint4 one[1] = {q};
+      if (!(Vec<DT>::rec(Vec<DT>::biggest(one)) >= floor_r)) continue;
+      const int at = v * kN - row.mis;
+      float x[kN];
+      unsigned in = 0;
+#pragma unroll
+      for (int i = 0; i < kN / 2; ++i) Vec<DT>::pair(q, i, x[2 * i], x[2 * i + 1]);
+#pragma unroll
+      for (int i = 0; i < kN; ++i) in |= (x[i] >= low_v ? 1u : 0u) << i;
+      int to = atomicAdd(&S.n, __popc(in));
+#pragma unroll
+      for (int i = 0; i < kN; ++i)
+        if (in >> i & 1u) {
+          const unsigned long long k = order_key(x[i], static_cast<unsigned>(at + i));
+          if (to < kC) S.kept[to] = k > floor_k ? k : 0ull;
+          ++to;
+        }
     }
     __syncthreads();
   };
   if (S.list <= kList) {
     read_list();
     if (S.n <= kC) return select_top(S, S.n, N);
-    if (tid < have) S.kept[tid] = S.top[tid];
   }
   __syncthreads();
+  if (tid < have) S.kept[tid] = S.top[tid];
   if (tid == 0) S.n = have;
   // Many: ties, or one thread's entries large in many steps.  In the row's order and
   // in groups, the floor rising: equal values stop at the first group (where a
@@ -401,12 +406,10 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Smem& S = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long total = P.nv * P.R, blocks = gridDim.x;
-
-  const long long begin = blockIdx.x * total / blocks;
+  const long long begin = blockIdx.x * P.share + min(static_cast<int>(blockIdx.x), P.more);
   if (tid == 0) {
-    S.end = (blockIdx.x + 1ll) * total / blocks;
-    S.n = 0;
+    S.begin = begin;
+    S.end = begin + P.share + (static_cast<int>(blockIdx.x) < P.more);
   }
   __syncthreads();
   int r = static_cast<int>(begin / P.nv);
@@ -414,7 +417,7 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
   p.row.set(P, r);
   p.v = static_cast<int>(begin - r * P.nv);
   p.v_end = static_cast<int>(min(S.end - r * P.nv, P.nv));
-  fetch(p, P.V, S, 0);
+  fetch(p, first_whole(p), last_whole(p, P.V), P.V, S, 0);
   int parity = 0;
 
   for (;;) {
@@ -426,6 +429,13 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
       if (T <= 0.0f) N = max(N, 1);                // greedy: the maximum's index is the answer
     }
 
+    const int fast = last_whole(p, P.V);
+    int tok = -1;
+    float tok_x = 0.0f;
+    if (tid < P.K) {                   // the row's tokens, read while it streams
+      tok = P.token_ids[static_cast<long long>(r) * P.K + tid];
+      if (tok >= 0 && tok < P.V) tok_x = p.row.at(tok);
+    }
     float ref = -INFINITY, big = -INFINITY;
     f2 z2 = pack(0.0f, 0.0f), s2 = pack(0.0f, 0.0f);
     while (p.v < p.v_end) {             // once, but for rows of more steps than there are records
@@ -433,13 +443,13 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
     uint32_t best = 0;
     for (int step = 0; step < kMaxSteps && p.v < p.v_end; ++step, parity ^= 1) {
       p.v += kStep;
-      if (p.v < p.v_end) fetch(p, P.V, S, parity ^ 1);
+      if (p.v < p.v_end) fetch(p, 1, fast, P.V, S, parity ^ 1);
       else if ((r + 1) * P.nv < S.end) {
         Piece<DT> next;                // the next row begins while this one ends
         next.row.set(P, r + 1);
         next.v = 0;
         next.v_end = static_cast<int>(min(S.end - (r + 1) * P.nv, P.nv));
-        fetch(next, P.V, S, parity ^ 1);
+        fetch(next, first_whole(next), last_whole(next, P.V), P.V, S, parity ^ 1);
       } else cp_commit();
       cp_wait<1>();
       uint4 v[kU];
@@ -482,60 +492,57 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
         best = max(best, k);
       }
     }
-    if (N > 0)
-      have = collect<DT>(S, p.row, P.V, v0, min(p.v, p.v_end), best, have, N);
+    if (p.v >= p.v_end) {
+      // the warp's triple; a NaN or +inf stays in its maximum
+      float m = big, z, s, zb, sb;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+      unpack(z2, z, zb);
+      unpack(s2, s, sb);
+      z += zb;
+      s += sb;
+      seen_from(m, ref, c, z, s);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) {
+        z += __shfl_xor_sync(0xFFFFFFFFu, z, o);
+        s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+      }
+      if (lane == 0) { S.red[0][warp] = m; S.red[1][warp] = z; S.red[2][warp] = s; }
+      if (N == 0) __syncthreads();
+    }
+    if (N > 0) have = collect<DT>(S, p.row, P.V, v0, min(p.v, p.v_end), parity ^ 1, best, have, N);
     }
 
     // ---- this block's triple
     const Row<DT> row = p.row;
     const long long row_start = r * P.nv;
-    const float T = P.temperature ? P.temperature[r] : 1.0f;
-    const bool greedy = T <= 0.0f;
-    int tok = -1;
-    float tok_x = 0.0f;
-    if (tid < P.K) {
-      tok = P.token_ids[static_cast<long long>(r) * P.K + tid];
-      if (tok >= 0 && tok < P.V) tok_x = row.at(tok);
+    float M = -INFINITY, z = 0.0f, s = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < kW; ++i) {
+      bad |= !(S.red[0][i] < INFINITY);
+      M = fmaxf(M, S.red[0][i]);
     }
-    float M = big, z, s, zb, sb;
-    unpack(z2, z, zb);
-    unpack(s2, s, sb);
-    z += zb;
-    s += sb;
-    bool bad = __syncthreads_or(!(big < INFINITY));
 #pragma unroll
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
-    if (lane == 0) S.red[0][warp] = M;
-    __syncthreads();
-    M = S.red[0][0];
-#pragma unroll
-    for (int i = 1; i < kW; ++i) M = fmaxf(M, S.red[0][i]);
-    auto seen_from = [&](float m, float& zz, float& ss) {
-      const float d = (m - M) * c, f = m == -INFINITY ? 0.0f : m == M ? 1.0f : ex2_approx(d);
-      ss = f > 0.0f ? f * (ss + (m == M ? 0.0f : d) * zz) : 0.0f;
-      zz *= f;
-    };
-    seen_from(ref, z, s);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      z += __shfl_xor_sync(0xFFFFFFFFu, z, o);
-      s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+    for (int i = 0; i < kW; ++i) {
+      float zi = S.red[1][i], si = S.red[2][i];
+      seen_from(M, S.red[0][i], c, zi, si);
+      z += zi;
+      s += si;
     }
-    if (lane == 0) { S.red[1][warp] = z; S.red[2][warp] = s; }
-    __syncthreads();
-    z = s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kW; ++i) { z += S.red[1][i]; s += S.red[2][i]; }
 
     // ---- the row's parts: the blocks whose shares overlap it
-    const long long a = ((row_start + 1) * blocks - 1) / total, b = ((row_start + P.nv) * blocks - 1) / total;
-    const int parts = static_cast<int>(b - a) + 1;
-    bool finish = parts == 1;
-    if (parts > 1) {
+    bool finish = row_start >= S.begin && row_start + P.nv <= S.end;
+    if (!finish) {
+      // the block of a vector: the first `more` blocks have share + 1, the others share
+      const long long head = P.more * (P.share + 1);
+      auto block_of = [&](long long x) { return x < head ? x / (P.share + 1) : P.more + (x - head) / P.share; };
+      const long long a = block_of(row_start);
+      const int parts = static_cast<int>(block_of(row_start + P.nv - 1) - a) + 1;
       auto slot_of = [&](int p) -> long long { return p == 0 ? 2 * a + 1 : 2 * (a + p); };
       const long long slot = slot_of(static_cast<int>(blockIdx.x - a));
       if (tid < N) P.part_top[slot * kMaxN + tid] = tid < have ? S.top[tid] : 0ull;
-      if (tid == 0) P.parts[slot] = Part{M, z, s, bad ? 1 : 0};
+      if (tid == 0) P.parts[slot] = make_float4(bad ? NAN : M, z, s, 0.0f);
       __syncthreads();
       if (tid == 0) {
         unsigned got;
@@ -548,57 +555,52 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
       __syncthreads();
       finish = S.flag != 0;
       if (finish) {
-        // parts <= kMaxParts < kT: one each; their alternatives in the same round of loads
-        constexpr int kEach = kMaxParts * kMaxN / kT;
+        // parts <= 32: a lane each, in every warp; the alternatives in the same round of loads
+        constexpr int kEach = kMaxParts / kW;
         unsigned long long key[kEach];
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-          const int i = j * kT + tid;
-          key[j] = i < parts * N ? __ldcg(P.part_top + slot_of(i / N) * kMaxN + i % N) : 0ull;
+          const int i = j * kW + warp;
+          key[j] = i < parts && lane < N ? __ldcg(P.part_top + slot_of(i) * kMaxN + lane) : 0ull;
         }
-        Part q = {-INFINITY, 0.0f, 0.0f, 0};
+        float4 q = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
         unsigned long long low = 0;    // a part's N-th bounds the row's from below
-        if (tid < parts) {
-          const float4 u = __ldcg(reinterpret_cast<const float4*>(P.parts + slot_of(tid)));
-          q = Part{u.x, u.y, u.z, __float_as_int(u.w)};
-          if (N > 0) low = __ldcg(P.part_top + slot_of(tid) * kMaxN + N - 1);
+        if (lane < parts) {
+          q = __ldcg(P.parts + slot_of(lane));
+          if (N > 0) low = __ldcg(P.part_top + slot_of(lane) * kMaxN + N - 1);
         }
-        bad = __syncthreads_or(q.flags);
-        M = q.m;
+        bad = __any_sync(0xFFFFFFFFu, !(q.x < INFINITY));
+        M = q.x;
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
           M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
           const unsigned long long other = __shfl_xor_sync(0xFFFFFFFFu, low, o);
           low = other > low ? other : low;
         }
-        if (lane == 0) { S.red[0][warp] = M; S.top[warp] = low; }
-        __syncthreads();
-        M = S.red[0][0];
-        low = S.top[0];
-#pragma unroll
-        for (int i = 1; i < kW; ++i) {
-          M = fmaxf(M, S.red[0][i]);
-          low = S.top[i] > low ? S.top[i] : low;
-        }
-        z = q.z;
-        s = q.s;
-        seen_from(q.m, z, s);
+        z = q.y;
+        s = q.z;
+        seen_from(M, q.x, c, z, s);
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
           z += __shfl_xor_sync(0xFFFFFFFFu, z, o);
           s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
         }
-        if (lane == 0) { S.red[1][warp] = z; S.red[2][warp] = s; }
         have = 0;
         if (N > 0) {
           // the parts' entries that reach the bound
           low = max(low, 1ull);
+          int mine = 0;
 #pragma unroll
-          for (int j = 0; j < kEach; ++j)
-            if (key[j] >= low) {
-              const int at = atomicAdd(&S.n, 1);
-              if (at < kC) S.kept[at] = key[j];
-            }
+          for (int j = 0; j < kEach; ++j) mine += key[j] >= low;
+          if (mine) {
+            int to = atomicAdd(&S.n, mine);
+#pragma unroll
+            for (int j = 0; j < kEach; ++j)
+              if (key[j] >= low) {
+                if (to < kC) S.kept[to] = key[j];
+                ++to;
+              }
+          }
           __syncthreads();
           if (S.n <= kC) {
             have = select_top(S, S.n, N);
@@ -617,17 +619,14 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
               have = select_top(S, S.n, N);
             }
           }
-        } else {
-          __syncthreads();
         }
-        z = s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kW; ++i) { z += S.red[1][i]; s += S.red[2][i]; }
       }
     }
 
     // ---- the row's results
-    if (finish) {
+    if (finish && warp * 32 < max(max(P.K, P.N), 1)) {
+      const float T = P.temperature ? P.temperature[r] : 1.0f;
+      const bool greedy = T <= 0.0f;
       const bool empty = !bad && M == -INFINITY;
       const float lz = logf(z);
       const int arg = greedy && have > 0 ? order_index(S.top[0]) : -1;
@@ -643,7 +642,7 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
         const long long at = static_cast<long long>(r) * P.K + j;
         if (j >= kT) {
           tok = P.token_ids[at];
-          tok_x = tok >= 0 && tok < P.V ? row.at(tok) : 0.0f;
+          if (tok >= 0 && tok < P.V) tok_x = row.at(tok);
         }
         P.logprobs[at] = (tok < 0 || tok >= P.V) ? NAN : logprob(tok_x, tok);
       }
@@ -660,8 +659,6 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
     p.v = 0;
     p.v_end = static_cast<int>(min(S.end - r * P.nv, P.nv));
     __syncthreads();
-    if (tid == 0) S.n = 0;
-    __syncthreads();
   }
 }
 
@@ -675,7 +672,7 @@ static Layout layout(int sms) {
   const size_t slots = 2 * static_cast<size_t>(sms) * kBlocks + 2;
   Layout L;
   L.parts = (slots * sizeof(unsigned) + 255) / 256 * 256;
-  L.top = L.parts + slots * sizeof(Part);
+  L.top = L.parts + slots * sizeof(float4);
   L.total = L.top + slots * kMaxN * sizeof(unsigned long long);
   return L;
 }
@@ -724,7 +721,7 @@ int ecah_token_logprobs(const ecah_logprob_args* a, void* stream) {
   const lp::Layout L = lp::layout(sms);
   unsigned char* ws = static_cast<unsigned char*>(a->workspace);
   P.counters = reinterpret_cast<unsigned*>(ws);
-  P.parts = reinterpret_cast<lp::Part*>(ws + L.parts);
+  P.parts = reinterpret_cast<float4*>(ws + L.parts);
   P.part_top = reinterpret_cast<unsigned long long*>(ws + L.top);
   const int vec = a->dtype == ECAH_DTYPE_F32 ? 4 : 8;
   P.nv = (static_cast<long long>(P.V) + 2 * (vec - 1)) / vec;
@@ -732,9 +729,14 @@ int ecah_token_logprobs(const ecah_logprob_args* a, void* stream) {
   // alternatives are joined of at most kMaxParts
   long long blocks = std::min<long long>(static_cast<long long>(sms) * lp::kBlocks, (P.nv * P.R + lp::kT - 1) / lp::kT);
   blocks = std::min<long long>(blocks, (lp::kMaxParts - 2ll) * P.R);
-  // Few rows: whole blocks to a row, so that none starts and ends two of them.
-  // 128 rows of 151936 f16 with 20 alternatives on 444 blocks, against 384: see below.
-  if (blocks >= 2ll * P.R) blocks = blocks / P.R * P.R;
+  // Few rows: whole blocks to a row, so that no block ends one and begins another.
+  if (blocks >= 2ll * P.R) {
+    const long long k = blocks / P.R;
+    blocks = k * P.R;
+    P.nv = (P.nv + k - 1) / k * k;
+  }
+  P.share = P.nv * P.R / blocks;
+  P.more = static_cast<int>(P.nv * P.R % blocks);
   auto fn = a->dtype == ECAH_DTYPE_F16 ? lp::token_logprobs_kernel<ECAH_DTYPE_F16>
             : a->dtype == ECAH_DTYPE_BF16 ? lp::token_logprobs_kernel<ECAH_DTYPE_BF16>
                                           : lp::token_logprobs_kernel<ECAH_DTYPE_F32>;
