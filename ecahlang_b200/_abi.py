@@ -7,11 +7,14 @@ library is missing -- there is no CPU or torch fallback for the sampler.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 from ctypes import c_float, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libecah_sampler.so")
+BINDING_PATH = os.path.join(_HERE, "lib", "_ecah_binding.so")
 
 ABI_VERSION = 2
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
@@ -187,6 +190,27 @@ def lib():
             raise EcahError("libecah_sampler.so ABI version mismatch")
         _lib = L
     return _lib
+
+
+_binding = None
+
+
+def binding():
+    """The torch binding of the log-probability and paged-cache entry points,
+    loaded once and given the library's functions; raise if it is absent."""
+    global _binding
+    if _binding is None:
+        import torch  # noqa: F401  (the module links torch's libraries)
+        L = lib()
+        if not os.path.exists(BINDING_PATH):
+            raise EcahError(f"{BINDING_PATH} is missing: build it with `python -m ecahlang_b200.build`")
+        loader = importlib.machinery.ExtensionFileLoader("_ecah_binding", BINDING_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_ecah_binding", loader))
+        loader.exec_module(module)
+        module.bind(EcahError, *(ctypes.cast(f, c_void_p).value for f in (
+            L.ecah_token_logprobs, L.ecah_paged_append, L.ecah_paged_decode, L.ecah_status_string)))
+        _binding = module
+    return _binding
 
 
 def check(status: int, what: str) -> None:

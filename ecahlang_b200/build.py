@@ -2,14 +2,18 @@
 
 The library is plain CUDA C++ behind an ``extern "C"`` ABI
 (include/ecah_sampler.h); it links the CUDA runtime statically and has no
-torch dependency, so any FFI (ctypes here) can load it.
+torch dependency, so any FFI (ctypes here) can load it.  ``lib/_ecah_binding.so``
+is the torch side of the newer entry points: a CPython module that checks
+tensors and calls the library.
 """
 from __future__ import annotations
 
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -17,6 +21,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIB_DIR, "libecah_sampler.so")
+BINDING = os.path.join(LIB_DIR, "_ecah_binding.so")
 OBJ_DIR = os.path.join(LIB_DIR, "build")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
@@ -31,12 +36,29 @@ def _nvcc() -> str:
     raise RuntimeError("nvcc not found; the sampler is CUDA-only and has no fallback")
 
 
-def _stale() -> bool:
-    if not os.path.exists(LIB):
+def _stale(product: str) -> bool:
+    if not os.path.exists(product):
         return True
-    t = os.path.getmtime(LIB)
+    t = os.path.getmtime(product)
     deps = glob.glob(os.path.join(CSRC, "*")) + glob.glob(os.path.join(ROOT, "include", "*.h"))
+    binding = os.path.join(CSRC, "binding.cpp")
+    deps = [d for d in deps if (d == binding) == (product == BINDING) or d.endswith("ecah_sampler.h")]
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def _build_binding() -> None:
+    spec = importlib.util.find_spec("torch")     # headers and libraries, without importing it
+    torch = os.path.dirname(spec.origin)
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    include = [os.path.join(ROOT, "include"), os.path.join(torch, "include"),
+               os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    tmp = BINDING + ".tmp"
+    subprocess.run([os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
+                    *(f"-I{d}" for d in include), os.path.join(CSRC, "binding.cpp"), "-o", tmp,
+                    "-L" + os.path.join(torch, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
+                    "-lc10", "-lc10_cuda"], check=True)
+    os.replace(tmp, BINDING)
 
 
 def _object(source: str, force: bool, verbose: bool) -> str:
@@ -58,18 +80,24 @@ def _object(source: str, force: bool, verbose: bool) -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile the library if a source is newer than it; returns its path."""
-    if not force and not _stale():
+    """Compile the library and its torch binding where a source is newer; returns the library's path."""
+    lib, binding = force or _stale(LIB), force or _stale(BINDING)
+    if not lib and not binding:
         return LIB
     os.makedirs(OBJ_DIR, exist_ok=True)
-    with ThreadPoolExecutor(len(SOURCES)) as pool:
-        objects = list(pool.map(lambda s: _object(s, force, verbose), SOURCES))
-    tmp = LIB + ".tmp"
-    subprocess.run([_nvcc(), *ARCH, "-shared", "-o", tmp, *objects], check=True)
-    os.replace(tmp, LIB)
+    with ThreadPoolExecutor(len(SOURCES) + 1) as pool:
+        bound = pool.submit(_build_binding) if binding else None
+        if lib:
+            objects = list(pool.map(lambda s: _object(s, force, verbose), SOURCES))
+            tmp = LIB + ".tmp"
+            subprocess.run([_nvcc(), *ARCH, "-shared", "-o", tmp, *objects], check=True)
+            os.replace(tmp, LIB)
+        if bound:
+            bound.result()
     return LIB
 
 
 if __name__ == "__main__":
     import sys
-    print(build(force="--changed" not in sys.argv, verbose=True))
+    changed = "--changed" in sys.argv        # only what a source is newer than
+    print(build(force=not changed, verbose=True))

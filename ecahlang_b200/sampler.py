@@ -44,15 +44,6 @@ def _need(t: torch.Tensor, name: str, dtype: torch.dtype, numel: int, device: to
         raise RuntimeError(f"{name}: expected {numel} elements, got {t.numel()}")
 
 
-def on_device(dev: torch.device, entry, args) -> int:
-    """Status of ``entry(args, stream)`` on dev's current stream, with dev
-    current (a launch goes to the current device)."""
-    if dev.index == torch.cuda.current_device():
-        return entry(args, torch.cuda.current_stream().cuda_stream)
-    with torch.cuda.device(dev):
-        return entry(args, torch.cuda.current_stream().cuda_stream)
-
-
 class PenaltyState:
     """Per-slot token histories on the device.
 
