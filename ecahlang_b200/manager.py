@@ -24,6 +24,7 @@ from typing import Dict, Iterable, Optional, Sequence
 import numpy as np
 import torch
 
+from .logprobs import RowLogprobs, TokenLogprobs
 from .sampler import PenaltyState, launch, new_philox_state, new_workspace, repetition_factor, resolve_device
 
 
@@ -54,6 +55,7 @@ class SamplingManager:
         # freq_pres_in_graphs=True captures every bucket with them.
         self.freq_pres_in_graphs = freq_pres_in_graphs
         self._cg_captured_fp: Dict[int, bool] = {}
+        self._scorer: Optional[TokenLogprobs] = None
         # overflow flags of the slot histories, copied to the host after every
         # update and checked when the next step's parameters are filled (the
         # host has read the previous step's ids by then)
@@ -236,6 +238,22 @@ class SamplingManager:
                       uniforms=uniforms, philox_state=None if uniforms is not None else self.philox_state,
                       rep_factor=rep, freq_pen=freq if fp else None, pres_pen=pres if fp else None,
                       penalty=self.penalty, row_slot=slot, freq_pres=fp, row_index=row_index)
+
+    def logprobs(self, logits: torch.Tensor, ids: Optional[torch.Tensor], top_n: int = 0,
+                 bucket_size: Optional[int] = None, row_index: Optional[torch.Tensor] = None,
+                 tempered: bool = False) -> "RowLogprobs":
+        """Log probabilities of ``ids`` (int32 [B] or [B, K], e.g. ``sample``'s)
+        under the same rows of ``logits``, their entropy and ``top_n``
+        alternatives, for completions that ask for them.  Of the model's own
+        distribution, or with ``tempered`` at the filled temperatures.  Enqueued on
+        the current stream; capturable."""
+        T = None
+        if tempered:
+            B = logits.shape[0] if row_index is None else row_index.numel()
+            T = self._buffers(B, bucket_size)[0].view(-1)
+        if self._scorer is None:
+            self._scorer = TokenLogprobs(self.vocab_size, self.dtype, self.device)
+        return self._scorer(logits, ids, top_n=top_n, temperature=T, row_index=row_index)
 
     def sample_async(self, logits: torch.Tensor, bucket_size: Optional[int] = None,
                      uniforms: Optional[torch.Tensor] = None, row_index=None) -> "PendingIds":
