@@ -37,6 +37,7 @@ constexpr int kSlice = 16;            // keys per warp and step
 constexpr int kTile = kW * kSlice;    // keys per work unit
 constexpr int kMaxGroup = 32;         // parts joined at once
 constexpr int kItemCost = 4;          // tiles of streaming that starting and joining an item takes
+constexpr int kWhole = 8;             // items of up to so many tiles are not divided
 constexpr float kLazy = 8.0f;         // the reference moves when a score is 2^8 above it
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -163,12 +164,15 @@ __device__ __forceinline__ float rcp(float x) {
   return r;
 }
 
-__device__ __forceinline__ long long request_len(const Params& P, int b, long long* first) {
-  long long count;
-  kv::page_range(P.cache, b, first, &count);
-  if (count <= 0 || P.cache.num_pages <= 0) return 0;
-  const long long len = (count - 1) * P.cache.page_size + min(max(P.last_page_len[b], 0), P.cache.page_size);
-  return min(len, 0x7FFFFFFFll - kTile);
+// Tokens of request b and its first entry in the page list (the launcher has seen
+// that there are fewer than 2^31 entries and units of work).
+__device__ __forceinline__ int request_len(const Params& P, int b, int* first) {
+  const int most = static_cast<int>(P.cache.num_indices);
+  const int lo = min(max(P.cache.indptr[b], 0), most), hi = min(max(P.cache.indptr[b + 1], lo), most);
+  *first = lo;
+  if (hi <= lo || P.cache.num_pages <= 0) return 0;
+  const long long len = static_cast<long long>(hi - lo - 1) * P.cache.page_size + min(max(P.last_page_len[b], 0), P.cache.page_size);
+  return static_cast<int>(min(len, 0x7FFFFFFFll - kTile));
 }
 
 // Reads of a joined triple: from this block's shared memory, or of another
@@ -203,77 +207,94 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT>::kBlocks) decode_kernel
   constexpr int kRows = S::kRows;
   constexpr int HT = E4M3 ? static_cast<int>(ECAH_DTYPE_F16) : DT;   // operand type of the products
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ long long s_scan[kW];
-  __shared__ long long s_start;          // cost before s_req
-  __shared__ int s_req, s_flag;
+  __shared__ unsigned s_scan[kW];
+  __shared__ unsigned s_start[2];        // first unit of s_req
+  __shared__ int s_req[2], s_flag;       // requests of the share's edges
   __shared__ float2 s_ml[kMaxGroup][kRows];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   const kv::Cache& C = P.cache;
   const int per_req = C.heads * P.tiles_h;       // items of a request
 
-  // Total cost, then this block's share [begin, end) and its first request.  An
-  // item costs kItemCost units, then one a tile.
-  auto tiles_of = [&](int b) -> long long {
-    long long f;
+  // Total cost, then this block's share.  An item costs kItemCost units, then one a
+  // tile; the first `more` blocks take share + 1 units, the others share.
+  auto tiles_of = [&](int b) -> int {
+    int f;
     if (b >= C.batch) return 0;
-    const long long len = request_len(P, b, &f);
+    const int len = request_len(P, b, &f);
     return len ? (len + kTile - 1) / kTile + kItemCost : 0;
   };
-  long long sum = 0;
+  int sum = 0;
   for (int b = tid; b < C.batch; b += kT) sum += tiles_of(b);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  sum = __reduce_add_sync(0xFFFFFFFFu, sum);
   if (lane == 0) s_scan[warp] = sum;
+  if (tid < 2) s_req[tid] = -1;
   __syncthreads();
-  long long total = 0;
+  unsigned total = 0;
   for (int w = 0; w < kW; ++w) total += s_scan[w];
   total *= per_req;
-  const long long blocks = min(static_cast<long long>(gridDim.x), total);
+  const unsigned blocks = min(gridDim.x, total);
   const bool busy = blockIdx.x < blocks;
-  const long long begin = busy ? blockIdx.x * total / blocks : 0, end = busy ? (blockIdx.x + 1ll) * total / blocks : 0;
-  long long run = 0;
+  const unsigned share = busy ? total / blocks : 1, more = total - share * blocks;
+  unsigned edge[2] = {0, 0};
+  if (busy) {
+    edge[0] = blockIdx.x * share + min(blockIdx.x, more);
+    edge[1] = edge[0] + share + (blockIdx.x < more);
+  }
+  unsigned run = 0;
   for (int b0 = 0; busy && b0 < C.batch; b0 += kT) {
-    const long long mine = tiles_of(b0 + tid);
-    long long inc = mine;
+    const unsigned mine = tiles_of(b0 + tid) * per_req;
+    unsigned inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+      const unsigned v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
       if (lane >= o) inc += v;
     }
     __syncthreads();
     if (lane == 31) s_scan[warp] = inc;
     __syncthreads();
-    long long before = run;
+    unsigned before = run;
     for (int w = 0; w < kW; ++w) {
       if (w < warp) before += s_scan[w];
       run += s_scan[w];
     }
-    const long long lo = (before + inc - mine) * per_req, hi = (before + inc) * per_req;
-    if (begin >= lo && begin < hi) { s_req = b0 + tid; s_start = before + inc - mine; }
-    if (begin < run * per_req) break;
+    const unsigned lo = before + inc - mine, hi = before + inc;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (edge[e] >= lo && edge[e] < hi) { s_req[e] = b0 + tid; s_start[e] = lo; }
+    if (edge[1] < run) break;
   }
   __syncthreads();
-  int req = busy ? s_req : 0;
-  long long req_start = busy ? s_start * per_req : 0;       // first unit of the request
-  long long at = begin;
+  // A share's edge inside a short item moves to the item's nearer end: joining its
+  // parts would take longer than streaming it.
+  auto settle = [&](int e) -> unsigned {
+    if (!busy || s_req[e] < 0) return edge[e];                // the end of all
+    int f;
+    const unsigned nt = (request_len(P, s_req[e], &f) + kTile - 1) / kTile, cost = nt + kItemCost;
+    if (nt > kWhole) return edge[e];
+    const unsigned into = (edge[e] - s_start[e]) % cost;
+    return edge[e] - into + (2 * into < cost ? 0 : cost);
+  };
+  unsigned at = settle(0);
+  const unsigned end = settle(1);
+  int req = busy ? s_req[0] : 0;
+  unsigned req_start = busy ? s_start[0] : 0;                 // first unit of the request
 
   const uint32_t ring = smem_u32(smem) + warp * S::kWarpBytes;
   unsigned char* ring_p = smem + warp * S::kWarpBytes;
 
-  while (at < end) {
+  while (at < end && req < C.batch) {
     // the unit's request, head and head tile
-    long long first;
-    const long long len = request_len(P, req, &first);
-    const long long nt = (len + kTile - 1) / kTile, cost = len ? nt + kItemCost : 0;
+    int first;
+    const int len = request_len(P, req, &first);
+    const unsigned nt = (len + kTile - 1) / kTile, cost = len ? nt + kItemCost : 0;
     if (at >= req_start + cost * per_req) { req_start += cost * per_req; ++req; continue; }
-    const int pair = static_cast<int>((at - req_start) / cost);
-    const long long item_start = req_start + pair * cost;
-    const long long tile0 = item_start + kItemCost;           // unit of the item's first tile
+    const unsigned pair = (at - req_start) / cost, item_start = req_start + pair * cost;
+    const unsigned tile0 = item_start + kItemCost;            // unit of the item's first tile
     const int h = pair / P.tiles_h, ht = pair % P.tiles_h;
-    const long long seg_end = min(end, item_start + cost);
-    const long long t0 = max(at, tile0) - tile0;
-    const int n = static_cast<int>(seg_end - tile0 - t0);
+    const unsigned seg_end = min(end, item_start + cost);
+    const int t0 = static_cast<int>(max(at, tile0) - tile0);
+    const int n = static_cast<int>(seg_end) - static_cast<int>(tile0) - t0;
     at = seg_end;
     if (n <= 0) continue;                                     // only the item's first units: no tile
     const int rows = min(P.group - ht * kRows, kRows);        // query heads of this tile
@@ -288,33 +309,41 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT>::kBlocks) decode_kernel
     auto nth_page = [&](unsigned j) { return P.page_shift >= 0 ? j >> P.page_shift : j / static_cast<unsigned>(C.page_size); };
     auto page_of = [&](int i) -> int {
       const unsigned j = key0 + static_cast<unsigned>(i) * kTile;
-      return i < n && j < len ? min(max(pages[nth_page(j)], 0), C.num_pages - 1) : -1;
+      return i < n && j < static_cast<unsigned>(len) ? min(max(pages[nth_page(j)], 0), C.num_pages - 1) : -1;
     };
-    int page = page_of(0);
+    int page = page_of(0), page_after = page_of(1);           // two slices ahead: an L2 read away
     auto issue = [&](int i) {
       if (i < n) {
         const unsigned j = key0 + static_cast<unsigned>(i) * kTile;
         const int pg = page;
         const unsigned slot = j - nth_page(j) * static_cast<unsigned>(C.page_size);
-        page = page_of(i + 1);
+        page = page_after;
+        page_after = page_of(i + 2);
         const unsigned off = pg < 0 ? 0u : pg * side.page + slot * side.slot + head_off;
         const unsigned live = __ballot_sync(0xFFFFFFFFu, pg >= 0);
         const uint32_t st = ring + (i % S::kStages) * S::kStage;
+        constexpr int kCopies = kSlice * S::kChunks / 32;     // of a lane and side
+        unsigned ko[kCopies], vo[kCopies];
+#pragma unroll
+        for (int x = 0; x < kCopies; ++x) {                   // all in flight before the first copy needs one
+          const int r = (x * 32 + lane) / S::kChunks;
+          ko[x] = __shfl_sync(0xFFFFFFFFu, off, r);
+          vo[x] = __shfl_sync(0xFFFFFFFFu, off, r + kSlice);
+        }
         if (live == 0xFFFFFFFFu) {
 #pragma unroll
-          for (int c0 = 0; c0 < kSlice * S::kChunks; c0 += 32) {
-            const int c = c0 + lane, r = c / S::kChunks, col = c % S::kChunks;
-            const unsigned ko = __shfl_sync(0xFFFFFFFFu, off, r) + col, vo = __shfl_sync(0xFFFFFFFFu, off, r + kSlice) + col;
-            cp16(st + r * S::kKStride + col * 16, P.k.base + static_cast<unsigned long long>(ko) * 16);
-            cp16(st + kSlice * S::kKStride + r * S::kVStride + col * 16, P.v.base + static_cast<unsigned long long>(vo) * 16);
+          for (int x = 0; x < kCopies; ++x) {
+            const int c = x * 32 + lane, r = c / S::kChunks, col = c % S::kChunks;
+            cp16(st + r * S::kKStride + col * 16, P.k.base + (ko[x] + col) * 16ull);
+            cp16(st + kSlice * S::kKStride + r * S::kVStride + col * 16, P.v.base + (vo[x] + col) * 16ull);
           }
         } else {                                              // past the length: zeros
-          for (int c0 = 0; c0 < kSlice * S::kChunks; c0 += 32) {
-            const int c = c0 + lane, r = c / S::kChunks, col = c % S::kChunks;
-            const unsigned ko = __shfl_sync(0xFFFFFFFFu, off, r) + col, vo = __shfl_sync(0xFFFFFFFFu, off, r + kSlice) + col;
+#pragma unroll
+          for (int x = 0; x < kCopies; ++x) {
+            const int c = x * 32 + lane, r = c / S::kChunks, col = c % S::kChunks;
             const bool ok = (live >> r) & 1u;
-            cp16_or_zero(st + r * S::kKStride + col * 16, P.k.base + (ok ? ko : 0u) * 16ull, ok);
-            cp16_or_zero(st + kSlice * S::kKStride + r * S::kVStride + col * 16, P.v.base + (ok ? vo : 0u) * 16ull, ok);
+            cp16_or_zero(st + r * S::kKStride + col * 16, P.k.base + (ok ? ko[x] + col : 0u) * 16ull, ok);
+            cp16_or_zero(st + kSlice * S::kKStride + r * S::kVStride + col * 16, P.v.base + (ok ? vo[x] + col : 0u) * 16ull, ok);
           }
         }
         if (E4M3) {
@@ -393,7 +422,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT>::kBlocks) decode_kernel
       issue(i + S::kStages - 1);
       cp_wait<S::kStages - 1>();
       __syncwarp();
-      const long long base = (t0 + i) * kTile + warp * kSlice;
+      const int base = (t0 + i) * kTile + warp * kSlice;
       if (base < len) {
         const uint32_t ks = ring + (i % S::kStages) * S::kStage, vs = ks + kSlice * S::kKStride;
         const unsigned char* ks_p = ring_p + (i % S::kStages) * S::kStage;
@@ -435,7 +464,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT>::kBlocks) decode_kernel
         // scales are: weight 2^(s + log2 scale - m), and the sum takes it back out.
         float inv[2] = {1.0f, 1.0f};
         const bool tail = base + kSlice > len;
-        const int left = static_cast<int>(len - base);
+        const int left = len - base;
         if (E4M3) {
           const float* sc = reinterpret_cast<const float*>(ks_p + kSlice * (S::kKStride + S::kVStride));
           const float kx0 = sc[g], kx1 = sc[g + 8];
@@ -566,8 +595,13 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT>::kBlocks) decode_kernel
     __syncthreads();
 
     // parts of this item: the blocks whose shares overlap its tiles
-    const long long a = ((tile0 + 1) * blocks - 1) / total, z = ((tile0 + nt) * blocks - 1) / total;
-    const int parts = static_cast<int>(z - a) + 1, part = static_cast<int>(blockIdx.x - a);
+    int a = blockIdx.x, parts = 1;
+    if (nt > kWhole) {
+      auto block_of = [&](unsigned x) { return x < more * (share + 1) ? x / (share + 1) : more + (x - more * (share + 1)) / share; };
+      a = block_of(tile0);
+      parts = block_of(tile0 + nt - 1) - a + 1;
+    }
+    const int part = blockIdx.x - a;
     auto slot_of = [&](int p) -> long long { return p == 0 ? 2 * a + 1 : 2 * (a + p); };
 
     // combine `count` (m, l, o) triples into the output or a part's slot
@@ -633,7 +667,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT>::kBlocks) decode_kernel
 
   // requests without tokens: zeros, spread over the blocks
   for (int b = blockIdx.x; b < C.batch; b += gridDim.x) {
-    long long f;
+    int f;
     if (request_len(P, b, &f) != 0) continue;
     for (int i = tid; i < P.hq * D; i += kT)
       static_cast<uint16_t*>(P.out)[b * P.o_tok + (i / D) * P.o_head + i % D] = 0;
@@ -749,6 +783,7 @@ int ecah_paged_decode(const ecah_decode_args* a, void* stream) {
           : (e4m3 ? decode::variant_for<ECAH_DTYPE_BF16, true>(c.head_dim, P.group) : decode::variant_for<ECAH_DTYPE_BF16, false>(c.head_dim, P.group));
   // no more blocks than tiles the listed pages can hold (and one for the empty requests)
   const double most = (static_cast<double>(c.num_indices) * c.page_size / decode::kTile + c.batch * (1.0 + decode::kItemCost)) * c.num_kv_heads * P.tiles_h + 1;
+  if (most >= 2147483648.0 || c.num_indices > 0x7FFFFFFF) return ECAH_ERR_SHAPE;   // units are counted in 32 bits
   const int blocks = static_cast<int>(std::min(most, static_cast<double>(sms * v.blocks)));
   return launch_kernel(v.fn, dim3(blocks), decode::kT, v.smem, reinterpret_cast<cudaStream_t>(stream), P) ? ECAH_OK : ECAH_ERR_LAUNCH;
 }
