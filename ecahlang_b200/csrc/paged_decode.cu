@@ -22,22 +22,26 @@ namespace decode {
 // rows of keys staged as whole tiles and the softmax through TMEM for the same
 // memory-bound rate; plain FMAs would need 26 Tfma/s beside the conversions.
 //
-// Split: a work unit is a tile of 64 keys of one item (request, KV head, head
-// tile).  All units, in order, are divided evenly over the blocks by the lengths
+// Split: a block's 4 warps take 4, 2 or 1 KV heads of a request, with 16-key slices
+// of the same keys: an item is (request, group of KV heads, head tile), a work unit
+// 64 rows of it (16 keys of 4 heads to 64 keys of one).  Neighbouring heads of a token
+// lie side by side, so several of them make longer runs of DRAM.  All units, in order, are divided evenly over the blocks by the lengths
 // the device holds (no host read, so a captured launch serves any lengths); an
 // item that spans several blocks is joined by the block that arrives last, in the
 // order of the parts, so results do not depend on which that is.
 //
 // Inside a block each warp streams 16-key slices of its own through its own
-// cp.async ring (no block barrier while streaming).
+// ring of bulk copies (no block barrier while streaming).
 
 constexpr int kW = 4;                 // warps
 constexpr int kT = kW * 32;
 constexpr int kSlice = 16;            // keys per warp and step
-constexpr int kTile = kW * kSlice;    // keys per work unit
-constexpr int kMaxGroup = 32;         // parts joined at once
+constexpr int kTile = kW * kSlice;    // rows (keys of a head) per work unit
+constexpr int kMaxGroup = 25;         // parts joined at once: 25 * 25 blocks to an item at most
+constexpr int kMaxRows = 32;          // query heads of an item
 constexpr int kItemCost = 4;          // tiles of streaming that starting and joining an item takes
-constexpr int kWhole = 8;             // items of up to so many tiles are not divided
+constexpr int kWhole = 8;             // items of up to so many tiles are not divided, ...
+constexpr int kWholeAlone = 4;        // ... or so many where there is a block for every tile
 constexpr float kLazy = 8.0f;         // the reference moves when a score is 2^8 above it
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -55,16 +59,17 @@ struct Params {
   const int* last_page_len;
   long long q_tok, q_head, o_tok, o_head;
   int hq, group, tiles_h;    // query heads, per KV head, head tiles per KV head
+  int wh;                    // KV heads of an item: 1, 2 or 4
   int page_shift;            // log2 page_size, or -1
   float scale;               // sm_scale * log2 e
   unsigned* counters;        // [2 slots][2]: group and item arrivals, zero between launches
-  float2* part_ml;           // [slots][rows]
-  float* part_o;             // [slots][rows][D]
+  float2* part_ml;           // [slots][wh rows]
+  float* part_o;             // [slots][wh rows][D]
   Side16 k, v;
   kv::Cache cache;
 };
 
-template <int D, bool E4M3, int NT>
+template <int D, bool E4M3, int NT, bool BULK>
 struct Shape {
   static constexpr int kRows = 8 * NT;                    // query heads per head tile
   static constexpr int kElem = E4M3 ? 1 : 2;
@@ -78,19 +83,20 @@ struct Shape {
   static constexpr int kVStride = kRowBytes + 16;
   static constexpr int kScaleBytes = E4M3 ? 2 * kSlice * 4 : 0;
   static constexpr int kStage = kSlice * (kKStride + kVStride) + kScaleBytes;
-  // Blocks of an SM and stages of a warp's ring: 75 to 130 KB in flight on an SM
+  // Blocks of an SM and stages of a warp's ring: 65 to 130 KB in flight on an SM
   // (6.5 TB/s over 148 SMs at about 1 us wants 45 KB) and 8 to 16 warps.
-  static constexpr int kStages = E4M3 ? (D == 64 ? 4 : 3) : (D == 64 || D == 96 || D == 256 ? 3 : 2);
+  static constexpr int kStages = E4M3 ? (D <= 96 ? 4 : 3) : BULK ? (D == 256 ? 3 : 2) : (D == 256 ? 2 : 3);
   static constexpr int kOStride = D + 4;                  // of a warp's result: 8 heads on 8 bank quads
   static constexpr int kWarpBytes = kStages * kStage;
   static constexpr int kSmem = kW * kWarpBytes;
-  static constexpr int kStatic = kMaxGroup * kRows * 8 + 256 + 1024;
+  static constexpr int kResult = kRows * kOStride * 4 + kRows * 8;   // a warp's (m, l, o)
+  static constexpr int kStatic = 256 + kT * 8 + 1024;
   static constexpr int kFit = (227 * 1024) / (kSmem + kStatic);
   static constexpr int kRegs = 50 + D / 4 * NT + D / 8 * NT;   // about: results, queries and the rest
   static constexpr int kByRegs = kRegs <= 110 ? 4 : kRegs <= 160 ? 3 : kRegs <= 215 ? 2 : 1;
   static constexpr int kBlocks = kFit < kByRegs ? kFit : kByRegs;
   static_assert(kBlocks >= 1 && kBlocks <= 4, "");
-  static_assert(kWarpBytes >= kRows * kOStride * 4 + kRows * 8, "a warp's result fits its ring");
+  static_assert(kWarpBytes >= kResult + kMaxGroup * kMaxRows * 8, "a warp's result and the join's factors fit its ring");
   static_assert(kStage % 16 == 0, "");
 };
 
@@ -102,6 +108,28 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
+// One row of the cache to shared memory by the copy engine, counted by a barrier.
+__device__ __forceinline__ void copy_row(uint32_t dst, const void* src, int bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_init(uint32_t bar) { asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void bar_expect(uint32_t bar, int bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Waits for a phase of the barrier; false after a bounded number of tries (each may
+// itself wait), which a copy in flight cannot need.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+  for (int tries = 0; tries < 1 << 20; ++tries) {
+    uint32_t done;
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+// Orders this thread's ordinary accesses to shared memory before later copies into it.
+__device__ __forceinline__ void fence_copies() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void cp4_or_zero(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
 }
@@ -201,68 +229,94 @@ __device__ __forceinline__ bool arrive(unsigned* counter, int expect, int* flag)
   return *flag != 0;
 }
 
-template <int DT, bool E4M3, int D, int NT>
-__global__ void __launch_bounds__(kT, Shape<D, E4M3, NT>::kBlocks) decode_kernel(const Params P) {
-  using S = Shape<D, E4M3, NT>;
+template <int DT, bool E4M3, int D, int NT, bool BULK>
+__global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_kernel(const Params P) {
+  using S = Shape<D, E4M3, NT, BULK>;
   constexpr int kRows = S::kRows;
   constexpr int HT = E4M3 ? static_cast<int>(ECAH_DTYPE_F16) : DT;   // operand type of the products
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ unsigned s_scan[kW];
   __shared__ unsigned s_start[2];        // first unit of s_req
   __shared__ int s_req[2], s_flag;       // requests of the share's edges
-  __shared__ float2 s_ml[kMaxGroup][kRows];
+  __shared__ int s_len[kT], s_first[kT];
+  __shared__ unsigned long long s_bar[kW][S::kStages];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // the join's (m, l) and factors: behind the first warp's result in its ring
+  float2(*s_ml)[kMaxRows] = reinterpret_cast<float2(*)[kMaxRows]>(smem + S::kResult);
+  const int wh = P.wh, sub = warp & (wh - 1), tile = kTile / wh;   // KV heads, this warp's, keys of a unit
+  const int slice0 = (warp / wh) * kSlice;                         // this warp's keys of a unit
   const int g = lane >> 2, t = lane & 3;
   const kv::Cache& C = P.cache;
-  const int per_req = C.heads * P.tiles_h;       // items of a request
+  const int per_req = C.heads / wh * P.tiles_h;  // items of a request
 
   // Total cost, then this block's share.  An item costs kItemCost units, then one a
   // tile; the first `more` blocks take share + 1 units, the others share.
-  auto tiles_of = [&](int b) -> int {
-    int f;
-    if (b >= C.batch) return 0;
-    const int len = request_len(P, b, &f);
-    return len ? (len + kTile - 1) / kTile + kItemCost : 0;
+  // A batch of up to kT requests leaves its lengths in shared memory.
+  const bool kept = C.batch <= kT;
+  auto look = [&](int b, int* first) -> int {
+    if (!kept) return request_len(P, b, first);
+    *first = s_first[b];
+    return s_len[b];
   };
-  int sum = 0;
-  for (int b = tid; b < C.batch; b += kT) sum += tiles_of(b);
-  sum = __reduce_add_sync(0xFFFFFFFFu, sum);
-  if (lane == 0) s_scan[warp] = sum;
+  auto cost_of = [&](int len) { return len ? (len + tile - 1) / tile + kItemCost : 0; };
+  unsigned mine = 0, total = 0;                               // mine: of request tid, or of this thread's requests
+  for (int b = tid; b < C.batch; b += kT) {
+    int f;
+    const int len = request_len(P, b, &f);
+    if (kept) { s_len[b] = len; s_first[b] = f; }
+    mine += cost_of(len);
+  }
+  unsigned inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 31) s_scan[warp] = inc;
   if (tid < 2) s_req[tid] = -1;
   __syncthreads();
-  unsigned total = 0;
-  for (int w = 0; w < kW; ++w) total += s_scan[w];
+  unsigned before = 0;
+#pragma unroll
+  for (int w = 0; w < kW; ++w) {
+    if (w < warp) before += s_scan[w];
+    total += s_scan[w];
+  }
   total *= per_req;
   const unsigned blocks = min(gridDim.x, total);
   const bool busy = blockIdx.x < blocks;
   const unsigned share = busy ? total / blocks : 1, more = total - share * blocks;
+  const unsigned whole = share > 1 ? kWhole : kWholeAlone;
   unsigned edge[2] = {0, 0};
   if (busy) {
     edge[0] = blockIdx.x * share + min(blockIdx.x, more);
     edge[1] = edge[0] + share + (blockIdx.x < more);
   }
+  // the requests of the share's edges
   unsigned run = 0;
   for (int b0 = 0; busy && b0 < C.batch; b0 += kT) {
-    const unsigned mine = tiles_of(b0 + tid) * per_req;
-    unsigned inc = mine;
+    if (!kept) {                                              // the scan again, by requests in order
+      int f;
+      mine = b0 + tid < C.batch ? cost_of(request_len(P, b0 + tid, &f)) : 0;
+      inc = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-      if (lane >= o) inc += v;
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      __syncthreads();
+      if (lane == 31) s_scan[warp] = inc;
+      __syncthreads();
+      before = run;
+      for (int w = 0; w < kW; ++w) {
+        if (w < warp) before += s_scan[w];
+        run += s_scan[w];
+      }
     }
-    __syncthreads();
-    if (lane == 31) s_scan[warp] = inc;
-    __syncthreads();
-    unsigned before = run;
-    for (int w = 0; w < kW; ++w) {
-      if (w < warp) before += s_scan[w];
-      run += s_scan[w];
-    }
-    const unsigned lo = before + inc - mine, hi = before + inc;
+    const unsigned lo = (before + inc - mine) * per_req, hi = (before + inc) * per_req;
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       if (edge[e] >= lo && edge[e] < hi) { s_req[e] = b0 + tid; s_start[e] = lo; }
-    if (edge[1] < run) break;
+    if (!kept && edge[1] < run * per_req) break;
   }
   __syncthreads();
   // A share's edge inside a short item moves to the item's nearer end: joining its
@@ -270,8 +324,8 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT>::kBlocks) decode_kernel
   auto settle = [&](int e) -> unsigned {
     if (!busy || s_req[e] < 0) return edge[e];                // the end of all
     int f;
-    const unsigned nt = (request_len(P, s_req[e], &f) + kTile - 1) / kTile, cost = nt + kItemCost;
-    if (nt > kWhole) return edge[e];
+    const unsigned nt = (look(s_req[e], &f) + tile - 1) / tile, cost = nt + kItemCost;
+    if (nt > whole) return edge[e];
     const unsigned into = (edge[e] - s_start[e]) % cost;
     return edge[e] - into + (2 * into < cost ? 0 : cost);
   };
@@ -282,16 +336,23 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT>::kBlocks) decode_kernel
 
   const uint32_t ring = smem_u32(smem) + warp * S::kWarpBytes;
   unsigned char* ring_p = smem + warp * S::kWarpBytes;
+  const uint32_t bars = smem_u32(s_bar[warp]);
+  uint32_t phase = 0;                            // of each stage's barrier
+  if (BULK && lane == 0) {
+    for (int i = 0; i < S::kStages; ++i) bar_init(bars + 8 * i);
+    fence_copies();
+  }
+  __syncwarp();
 
   while (at < end && req < C.batch) {
     // the unit's request, head and head tile
     int first;
-    const int len = request_len(P, req, &first);
-    const unsigned nt = (len + kTile - 1) / kTile, cost = len ? nt + kItemCost : 0;
+    const int len = look(req, &first);
+    const unsigned nt = (len + tile - 1) / tile, cost = len ? nt + kItemCost : 0;
     if (at >= req_start + cost * per_req) { req_start += cost * per_req; ++req; continue; }
     const unsigned pair = (at - req_start) / cost, item_start = req_start + pair * cost;
     const unsigned tile0 = item_start + kItemCost;            // unit of the item's first tile
-    const int h = pair / P.tiles_h, ht = pair % P.tiles_h;
+    const int h0 = pair / P.tiles_h * wh, ht = pair % P.tiles_h, h = h0 + sub;
     const unsigned seg_end = min(end, item_start + cost);
     const int t0 = static_cast<int>(max(at, tile0) - tile0);
     const int n = static_cast<int>(seg_end) - static_cast<int>(tile0) - t0;
@@ -300,50 +361,82 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT>::kBlocks) decode_kernel
     const int rows = min(P.group - ht * kRows, kRows);        // query heads of this tile
     const int head0 = h * P.group + ht * kRows;
 
-    // ---- stream: the first slices go out before the queries are read
+    // ---- stream: the first slices
     // Lane l < 16 finds the key row of key l of a slice, lane 16 + l the value row.
     const Side16& side = lane < kSlice ? P.k : P.v;
     const unsigned head_off = h * side.head;
-    const unsigned key0 = static_cast<unsigned>(t0) * kTile + warp * kSlice + (lane & 15);
+    const unsigned key0 = static_cast<unsigned>(t0) * tile + slice0 + (lane & 15);
     const int* pages = C.indices + first;
     auto nth_page = [&](unsigned j) { return P.page_shift >= 0 ? j >> P.page_shift : j / static_cast<unsigned>(C.page_size); };
     auto page_of = [&](int i) -> int {
-      const unsigned j = key0 + static_cast<unsigned>(i) * kTile;
+      const unsigned j = key0 + static_cast<unsigned>(i) * tile;
       return i < n && j < static_cast<unsigned>(len) ? min(max(pages[nth_page(j)], 0), C.num_pages - 1) : -1;
     };
     int page = page_of(0), page_after = page_of(1);           // two slices ahead: an L2 read away
+    // ---- the queries, asked for while the pages come and before the stream fills the memory's queues: heads
+    // 8 x + g, as the products' second operand takes them (e4m3: 8 dimensions a load)
+    uint32_t qf[NT][D / 16][2];
+    uint4 qw[NT][E4M3 ? D / 32 : 1];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      const bool live = 8 * x + g < rows;
+      const uint16_t* q = static_cast<const uint16_t*>(P.q) + req * P.q_tok + (head0 + 8 * x + g) * P.q_head;
+      if (!E4M3) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          qf[x][k][0] = live ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 2 * t) : 0u;
+          qf[x][k][1] = live ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 2 * t + 8) : 0u;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k)
+          qw[x][k] = live ? *reinterpret_cast<const uint4*>(q + 32 * k + 8 * t) : uint4{0, 0, 0, 0};
+      }
+    }
+
     auto issue = [&](int i) {
       if (i < n) {
-        const unsigned j = key0 + static_cast<unsigned>(i) * kTile;
+        const unsigned j = key0 + static_cast<unsigned>(i) * tile;
         const int pg = page;
         const unsigned slot = j - nth_page(j) * static_cast<unsigned>(C.page_size);
         page = page_after;
         page_after = page_of(i + 2);
         const unsigned off = pg < 0 ? 0u : pg * side.page + slot * side.slot + head_off;
         const unsigned live = __ballot_sync(0xFFFFFFFFu, pg >= 0);
-        const uint32_t st = ring + (i % S::kStages) * S::kStage;
-        constexpr int kCopies = kSlice * S::kChunks / 32;     // of a lane and side
-        unsigned ko[kCopies], vo[kCopies];
-#pragma unroll
-        for (int x = 0; x < kCopies; ++x) {                   // all in flight before the first copy needs one
-          const int r = (x * 32 + lane) / S::kChunks;
-          ko[x] = __shfl_sync(0xFFFFFFFFu, off, r);
-          vo[x] = __shfl_sync(0xFFFFFFFFu, off, r + kSlice);
-        }
-        if (live == 0xFFFFFFFFu) {
-#pragma unroll
-          for (int x = 0; x < kCopies; ++x) {
-            const int c = x * 32 + lane, r = c / S::kChunks, col = c % S::kChunks;
-            cp16(st + r * S::kKStride + col * 16, P.k.base + (ko[x] + col) * 16ull);
-            cp16(st + kSlice * S::kKStride + r * S::kVStride + col * 16, P.v.base + (vo[x] + col) * 16ull);
+        const uint32_t st = ring + (i % S::kStages) * S::kStage, bar = bars + 8 * (i % S::kStages);
+        if (BULK) {
+          const uint32_t row = st + (lane < kSlice ? lane * S::kKStride : kSlice * S::kKStride + (lane - kSlice) * S::kVStride);
+          if (lane == 0) bar_expect(bar, __popc(live) * S::kRowBytes);
+          if (pg >= 0) {
+            copy_row(row, side.base + off * 16ull, S::kRowBytes, bar);
+          } else {                                            // past the length: zeros
+            for (int c = 0; c < S::kChunks; ++c)
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(row + c * 16), "r"(0) : "memory");
           }
-        } else {                                              // past the length: zeros
+        } else {
+          constexpr int kCopies = kSlice * S::kChunks / 32;   // of a lane and side
+          unsigned ko[kCopies], vo[kCopies];
 #pragma unroll
-          for (int x = 0; x < kCopies; ++x) {
-            const int c = x * 32 + lane, r = c / S::kChunks, col = c % S::kChunks;
-            const bool ok = (live >> r) & 1u;
-            cp16_or_zero(st + r * S::kKStride + col * 16, P.k.base + (ok ? ko[x] + col : 0u) * 16ull, ok);
-            cp16_or_zero(st + kSlice * S::kKStride + r * S::kVStride + col * 16, P.v.base + (ok ? vo[x] + col : 0u) * 16ull, ok);
+          for (int x = 0; x < kCopies; ++x) {                 // all in flight before the first copy needs one
+            const int r = (x * 32 + lane) / S::kChunks;
+            ko[x] = __shfl_sync(0xFFFFFFFFu, off, r);
+            vo[x] = __shfl_sync(0xFFFFFFFFu, off, r + kSlice);
+          }
+          if (live == 0xFFFFFFFFu) {
+#pragma unroll
+            for (int x = 0; x < kCopies; ++x) {
+              const int c = x * 32 + lane, r = c / S::kChunks, col = c % S::kChunks;
+              cp16(st + r * S::kKStride + col * 16, P.k.base + (ko[x] + col) * 16ull);
+              cp16(st + kSlice * S::kKStride + r * S::kVStride + col * 16, P.v.base + (vo[x] + col) * 16ull);
+            }
+          } else {                                            // past the length: zeros
+#pragma unroll
+            for (int x = 0; x < kCopies; ++x) {
+              const int c = x * 32 + lane, r = c / S::kChunks, col = c % S::kChunks;
+              const bool ok = (live >> r) & 1u;
+              cp16_or_zero(st + r * S::kKStride + col * 16, P.k.base + (ok ? ko[x] + col : 0u) * 16ull, ok);
+              cp16_or_zero(st + kSlice * S::kKStride + r * S::kVStride + col * 16, P.v.base + (ok ? vo[x] + col : 0u) * 16ull, ok);
+            }
           }
         }
         if (E4M3) {
@@ -352,38 +445,27 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT>::kBlocks) decode_kernel
           cp4_or_zero(st + kSlice * (S::kKStride + S::kVStride) + lane * 4, sc, pg >= 0);
         }
       }
-      cp_commit();
+      if (E4M3 || !BULK) cp_commit();
     };
 #pragma unroll
     for (int i = 0; i < S::kStages - 1; ++i) issue(i);
 
-    // ---- query fragments (the products' second operand): head 8 x + g
-    uint32_t qf[NT][D / 16][2];
-    float rs[NT][2];                                          // score scale of heads 8 x + 2 t and + 1
+    // ---- score scales of heads 8 x + 2 t and + 1
+    float rs[NT][2];
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
-      const bool live = 8 * x + g < rows;
-      const uint16_t* q = static_cast<const uint16_t*>(P.q) + req * P.q_tok + (head0 + 8 * x + g) * P.q_head;
       rs[x][0] = rs[x][1] = P.scale;
-      if (!E4M3) {
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          qf[x][k][0] = live ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 2 * t) : 0u;
-          qf[x][k][1] = live ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 2 * t + 8) : 0u;
-        }
-      } else {
+      if (E4M3) {
         // The products run in f16 (e4m3 codes are exact there).  Each query head is
         // scaled by a power of two to a largest magnitude in [1, 2), so that bf16
         // queries fit its range; the power goes into the head's score scale.
         // Dimensions are dealt so that a lane's 8 consecutive codes of a key feed
         // its operands of two products: k index 2t, 2t+1, 2t+8, 2t+9 of product 2i
         // are dimensions 32 i + 8 t + 0..3, of product 2i + 1 + 4..7.
-        uint4 w[D / 32];
         float m = 0.0f;
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) {
-          w[k] = live ? *reinterpret_cast<const uint4*>(q + 32 * k + 8 * t) : uint4{0, 0, 0, 0};
-          const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+          const uint32_t u[4] = {qw[x][k].x, qw[x][k].y, qw[x][k].z, qw[x][k].w};
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             m = fmaxf(m, fmaxf(fabsf(DType<DT>::to_f32(u[i] & 0xFFFFu)), fabsf(DType<DT>::to_f32(u[i] >> 16))));
@@ -400,10 +482,10 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT>::kBlocks) decode_kernel
         };
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) {
-          qf[x][2 * k][0] = half2of(w[k].x);
-          qf[x][2 * k][1] = half2of(w[k].y);
-          qf[x][2 * k + 1][0] = half2of(w[k].z);
-          qf[x][2 * k + 1][1] = half2of(w[k].w);
+          qf[x][2 * k][0] = half2of(qw[x][k].x);
+          qf[x][2 * k][1] = half2of(qw[x][k].y);
+          qf[x][2 * k + 1][0] = half2of(qw[x][k].z);
+          qf[x][2 * k + 1][1] = half2of(qw[x][k].w);
         }
       }
     }
@@ -420,9 +502,11 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT>::kBlocks) decode_kernel
 
     for (int i = 0; i < n; ++i) {
       issue(i + S::kStages - 1);
-      cp_wait<S::kStages - 1>();
+      if (E4M3 || !BULK) cp_wait<S::kStages - 1>();
+      if (BULK && !bar_wait(bars + 8 * (i % S::kStages), phase >> (i % S::kStages) & 1u)) l[0][0] = NAN;
+      phase ^= 1u << (i % S::kStages);
       __syncwarp();
-      const int base = (t0 + i) * kTile + warp * kSlice;
+      const int base = (t0 + i) * tile + slice0;
       if (base < len) {
         const uint32_t ks = ring + (i % S::kStages) * S::kStage, vs = ks + kSlice * S::kKStride;
         const unsigned char* ks_p = ring_p + (i % S::kStages) * S::kStage;
@@ -564,7 +648,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT>::kBlocks) decode_kernel
       }
       __syncwarp();
     }
-    cp_wait<0>();
+    if (E4M3 || !BULK) cp_wait<0>();
     __syncwarp();
 
     // ---- join the warps: each leaves (m, l, o) in its ring
@@ -596,20 +680,25 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT>::kBlocks) decode_kernel
 
     // parts of this item: the blocks whose shares overlap its tiles
     int a = blockIdx.x, parts = 1;
-    if (nt > kWhole) {
+    if (nt > whole) {
       auto block_of = [&](unsigned x) { return x < more * (share + 1) ? x / (share + 1) : more + (x - more * (share + 1)) / share; };
       a = block_of(tile0);
       parts = block_of(tile0 + nt - 1) - a + 1;
     }
     const int part = blockIdx.x - a;
-    auto slot_of = [&](int p) -> long long { return p == 0 ? 2 * a + 1 : 2 * (a + p); };
+    auto slot_of = [&](int p) { return p == 0 ? 2 * a + 1 : 2 * (a + p); };
 
-    // combine `count` (m, l, o) triples into the output or a part's slot
-    auto combine = [&](auto from, int count, auto ml_of, auto o_of, int o_stride, long long to) {
+    // Combine `count` triples (m, l, o) of each of the item's rows (head h0 + j, query
+    // head r of its tile; row j kRows + r) into the output or a part's slot.
+    const int item_rows = wh * kRows;
+    auto combine = [&](auto from, int count, auto ml_of, auto o_of, int o_stride, int to) {
       using From = decltype(from);
-      for (int i = tid; i < count * kRows; i += kT) s_ml[i / kRows][i % kRows] = From::two(ml_of(i / kRows) + i % kRows);
+      for (int i = tid; i < count * item_rows; i += kT) {
+        const int p = i / item_rows, r = i % item_rows;
+        s_ml[p][r] = From::two(ml_of(p, r / kRows) + r);
+      }
       __syncthreads();
-      if (tid < rows) {
+      if (tid < item_rows && tid % kRows < rows) {
         float mm = -INFINITY, ll = 0.0f;
         for (int p = 0; p < count; ++p) mm = fmaxf(mm, s_ml[p][tid].x);
         for (int p = 0; p < count; ++p) {
@@ -619,56 +708,68 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT>::kBlocks) decode_kernel
           s_ml[p][tid].x = f;
         }
         if (to >= 0) {
-          P.part_ml[to * kRows + tid] = make_float2(mm, ll);
+          P.part_ml[static_cast<long long>(to) * item_rows + tid] = make_float2(mm, ll);
         } else {
           // a sum of zero (no key has mass) gives zeros
           const float r = ll == 0.0f ? 0.0f : 1.0f / ll;
           for (int p = 0; p < count; ++p) s_ml[p][tid].x *= r;
-          if (P.lse) P.lse[static_cast<long long>(req) * P.hq + head0 + tid] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * kLn2;
+          if (P.lse)
+            P.lse[static_cast<long long>(req) * P.hq + (h0 + tid / kRows) * P.group + ht * kRows + tid % kRows] =
+                ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * kLn2;
         }
       }
       __syncthreads();
-      for (int e = tid * 4; e < rows * D; e += kT * 4) {
-        const int r = e / D, d = e % D;
+      for (int e = tid * 4; e < item_rows * D; e += kT * 4) {
+        const int r = e / D, d = e % D, j = r / kRows;
+        if (r % kRows >= rows) continue;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
         for (int p = 0; p < count; ++p) {
-          const float4 w = From::four(o_of(p) + r * o_stride + d);
+          const float4 w = From::four(o_of(p, j) + r * o_stride + d);
           const float f = s_ml[p][r].x;
           v.x = fmaf(w.x, f, v.x); v.y = fmaf(w.y, f, v.y); v.z = fmaf(w.z, f, v.z); v.w = fmaf(w.w, f, v.w);
         }
         if (to >= 0) {
-          *reinterpret_cast<float4*>(P.part_o + to * kRows * D + e) = v;
+          *reinterpret_cast<float4*>(P.part_o + static_cast<long long>(to) * item_rows * D + e) = v;
         } else {
           const uint2 w = make_uint2(pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w));
-          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.out) + req * P.o_tok + (head0 + r) * P.o_head + d) = w;
+          const int head = (h0 + j) * P.group + ht * kRows + r % kRows;
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.out) + req * P.o_tok + head * P.o_head + d) = w;
         }
       }
     };
-    auto warp_o = [&](int w) -> const float* { return reinterpret_cast<const float*>(smem + w * S::kWarpBytes); };
-    combine(FromShared(), kW, [&](int w) { return reinterpret_cast<const float2*>(warp_o(w) + kRows * S::kOStride); }, warp_o,
-            S::kOStride, parts == 1 ? -1 : slot_of(part));
+    // the warps of head j: j, j + wh, ...; their rows start at theirs
+    auto warp_o = [&](int p, int j) -> const float* {
+      return reinterpret_cast<const float*>(smem + (p * wh + j) * S::kWarpBytes) - j * kRows * S::kOStride;
+    };
+    auto warp_ml = [&](int p, int j) -> const float2* {
+      return reinterpret_cast<const float2*>(smem + (p * wh + j) * S::kWarpBytes + kRows * S::kOStride * 4) - j * kRows;
+    };
+    combine(FromShared(), kW / wh, warp_ml, warp_o, S::kOStride, parts == 1 ? -1 : slot_of(part));
 
     if (parts > 1) {
       // joined in one step, or in groups of about sqrt(parts) first
       int gs = parts;
       if (parts > kMaxGroup) { gs = 1; while (gs * gs < parts) ++gs; }
       const int groups = (parts + gs - 1) / gs, grp = part / gs, p0 = grp * gs, in_grp = min(gs, parts - p0);
+      auto ml_at = [&](int slot) { return P.part_ml + static_cast<long long>(slot) * item_rows; };
+      auto o_at = [&](int slot) { return P.part_o + static_cast<long long>(slot) * item_rows * D; };
       if (arrive(P.counters + 2 * slot_of(p0), in_grp, &s_flag)) {
-        combine(FromParts(), in_grp, [&](int p) { return P.part_ml + slot_of(p0 + p) * kRows; },
-                [&](int p) { return P.part_o + slot_of(p0 + p) * kRows * D; }, D, groups == 1 ? -1 : slot_of(p0));
+        combine(FromParts(), in_grp, [&](int p, int) { return ml_at(slot_of(p0 + p)); },
+                [&](int p, int) { return o_at(slot_of(p0 + p)); }, D, groups == 1 ? -1 : slot_of(p0));
         if (groups > 1 && arrive(P.counters + 2 * slot_of(0) + 1, groups, &s_flag))
-          combine(FromParts(), groups, [&](int p) { return P.part_ml + slot_of(p * gs) * kRows; },
-                  [&](int p) { return P.part_o + slot_of(p * gs) * kRows * D; }, D, -1);
+          combine(FromParts(), groups, [&](int p, int) { return ml_at(slot_of(p * gs)); },
+                  [&](int p, int) { return o_at(slot_of(p * gs)); }, D, -1);
       }
     }
+    if (BULK) fence_copies();
     __syncthreads();       // the rings are free again
   }
 
   // requests without tokens: zeros, spread over the blocks
   for (int b = blockIdx.x; b < C.batch; b += gridDim.x) {
     int f;
-    if (request_len(P, b, &f) != 0) continue;
+    if (look(b, &f) != 0) continue;
     for (int i = tid; i < P.hq * D; i += kT)
       static_cast<uint16_t*>(P.out)[b * P.o_tok + (i / D) * P.o_head + i % D] = 0;
     if (P.lse)
@@ -682,24 +783,40 @@ struct Variant {
 };
 
 // The kernel of a head layout: one head tile of 8 query heads where a KV head has
-// at most 8, else tiles of 16 (a KV row is then read once per 16 heads).
+// at most 8, else tiles of 16 (a KV row is then read once per 16 heads).  BULK: rows
+// of 256 bytes and more by the copy engine.  It starts a copy about every 10 clocks
+// an SM: at 256 bytes that is more than HBM brings, and it leaves the threads free (4
+// requests of 100 000 to 131 072 tokens in bf16: 296 us against 321); a block alone
+// waits longer for its 128 copies than for its threads' own (128 requests of up to 512
+// tokens: 18.9 us against 13.0), and shorter rows starve (128 bytes: 3.4 TB/s).
+constexpr int kBulkRow = 256;
+
+template <int DT, bool E4M3, int D, int NT>
+static Variant variant_of(bool bulk) {
+  constexpr bool kCan = D * (E4M3 ? 1 : 2) >= kBulkRow;
+  using Bulk = Shape<D, E4M3, NT, kCan>;
+  using Threads = Shape<D, E4M3, NT, false>;
+  if (kCan && bulk) return Variant{decode_kernel<DT, E4M3, D, NT, kCan>, Bulk::kSmem, Bulk::kBlocks};
+  return Variant{decode_kernel<DT, E4M3, D, NT, false>, Threads::kSmem, Threads::kBlocks};
+}
+
 template <int DT, bool E4M3, int NT>
-static Variant variant_for(int D) {
+static Variant variant_for(int D, bool bulk) {
   switch (D) {
-#define ECAH_D(N) case N: return Variant{decode_kernel<DT, E4M3, N, NT>, Shape<N, E4M3, NT>::kSmem, Shape<N, E4M3, NT>::kBlocks};
-    ECAH_D(64) ECAH_D(96) ECAH_D(128) ECAH_D(192)
-#undef ECAH_D
-    default: return Variant{decode_kernel<DT, E4M3, 256, NT>, Shape<256, E4M3, NT>::kSmem, Shape<256, E4M3, NT>::kBlocks};
+    case 64: return variant_of<DT, E4M3, 64, NT>(bulk);
+    case 96: return variant_of<DT, E4M3, 96, NT>(bulk);
+    case 128: return variant_of<DT, E4M3, 128, NT>(bulk);
+    case 192: return variant_of<DT, E4M3, 192, NT>(bulk);
+    default: return variant_of<DT, E4M3, 256, NT>(bulk);
   }
 }
 
 template <int DT, bool E4M3>
-static Variant variant_for(int D, int group) {
-  return group <= 8 ? variant_for<DT, E4M3, 1>(D) : variant_for<DT, E4M3, 2>(D);
+static Variant variant_for(int D, int group, bool bulk) {
+  return group <= 8 ? variant_for<DT, E4M3, 1>(D, bulk) : variant_for<DT, E4M3, 2>(D, bulk);
 }
 
 constexpr int kMaxBlocksPerSm = 4;
-constexpr int kMaxRows = 16;
 
 // Workspace: counters, then the parts' (m, l), then their sums.  A block has at
 // most two parts of items it shares with others, whatever the batch is.
@@ -778,12 +895,24 @@ int ecah_paged_decode(const ecah_decode_args* a, void* stream) {
   if (!decode::side16(P.cache.k, c.num_pages, c.page_size, c.num_kv_heads, e4m3 ? 1 : 2, &P.k) ||
       !decode::side16(P.cache.v, c.num_pages, c.page_size, c.num_kv_heads, e4m3 ? 1 : 2, &P.v))
     return ECAH_ERR_SHAPE;
+  // Units that the listed pages can hold with one KV head an item; `much`: 32 of them
+  // and more to each of 296 blocks.
+  const double units = static_cast<double>(c.num_indices) * c.page_size / decode::kTile * c.num_kv_heads * P.tiles_h;
+  const bool much = units > 64.0 * sms;
   const decode::Variant v =
-      f16 ? (e4m3 ? decode::variant_for<ECAH_DTYPE_F16, true>(c.head_dim, P.group) : decode::variant_for<ECAH_DTYPE_F16, false>(c.head_dim, P.group))
-          : (e4m3 ? decode::variant_for<ECAH_DTYPE_BF16, true>(c.head_dim, P.group) : decode::variant_for<ECAH_DTYPE_BF16, false>(c.head_dim, P.group));
-  // no more blocks than tiles the listed pages can hold (and one for the empty requests)
-  const double most = (static_cast<double>(c.num_indices) * c.page_size / decode::kTile + c.batch * (1.0 + decode::kItemCost)) * c.num_kv_heads * P.tiles_h + 1;
+      f16 ? (e4m3 ? decode::variant_for<ECAH_DTYPE_F16, true>(c.head_dim, P.group, much)
+                  : decode::variant_for<ECAH_DTYPE_F16, false>(c.head_dim, P.group, much))
+          : (e4m3 ? decode::variant_for<ECAH_DTYPE_BF16, true>(c.head_dim, P.group, much)
+                  : decode::variant_for<ECAH_DTYPE_BF16, false>(c.head_dim, P.group, much));
+  P.wh = 1;
+  // Runs of 256 bytes of a token where there is much to stream.
+  const int row_bytes = c.head_dim * (e4m3 ? 1 : 2);
+  if (much)
+    while (P.wh < 4 && P.wh * row_bytes < 256 && P.wh * 2 * rows <= decode::kMaxRows && c.num_kv_heads % (P.wh * 2) == 0) P.wh *= 2;
+  const double items = static_cast<double>(c.batch) * (c.num_kv_heads / P.wh) * P.tiles_h;
+  const double most = units + items * (1.0 + decode::kItemCost) + 1;
   if (most >= 2147483648.0 || c.num_indices > 0x7FFFFFFF) return ECAH_ERR_SHAPE;   // units are counted in 32 bits
+  // no more blocks than units (and one for the empty requests)
   const int blocks = static_cast<int>(std::min(most, static_cast<double>(sms * v.blocks)));
   return launch_kernel(v.fn, dim3(blocks), decode::kT, v.smem, reinterpret_cast<cudaStream_t>(stream), P) ? ECAH_OK : ECAH_ERR_LAUNCH;
 }
