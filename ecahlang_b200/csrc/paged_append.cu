@@ -19,9 +19,13 @@ namespace append {
 // interleaved.  A warp holds several heads of one token and, with many tokens, goes
 // through kMany heads a group with all their loads in flight and one reading of the
 // token's table row; with few tokens one head a group spreads over more warps.
+//
+// Measured on one B200, device time of graph replays: 8192 tokens of 32/8 heads of
+// 128 with norm and rotation into a bf16 cache 37.5 us (5.4 TB/s), 128 tokens into
+// an e4m3 cache 2.9 us, one token 2.2 us (a launch).
 
-constexpr int kT = 64;
-constexpr int kMany = 2;
+constexpr int kT = 64;               // 8192 tokens: 37.5 us, with 128 threads 37.8, with 256 39.3
+constexpr int kMany = 2;             // with 4 38.7 us, with 6 43.2
 
 struct Params {
   const void *q, *k, *v;

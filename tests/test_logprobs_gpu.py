@@ -100,6 +100,16 @@ def test_top_n_and_temperature(dtype, top_n):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_longer_than_their_records(dtype):
+    """A block's piece of the row is recorded and read again in several goes."""
+    V = 6_000_011
+    x, tok, _ = make(1, V, dtype, seed=9)
+    check(x, tok, 20)
+    check((torch.arange(V, device=DEV)[None] % 997).to(dtype), tok, 32)
+    check(torch.zeros(1, V, device=DEV, dtype=dtype), tok, 32)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_row_starts_and_strides(dtype):
     """Rows at every offset from a 16-byte boundary; nothing outside them is read."""
     for off in range(0, 9):

@@ -92,9 +92,11 @@ def decode_reference(q, lengths, indptr, indices, k, v, ks, vs, sm_scale):
     return out, lse, tol, 2e-5 + 4e-6 * smax
 
 
-def check_decode(lengths, Hq, Hk, D, page, dtype, kv=None, layout="nhd", seed=0, scale=1.5, sm_scale=None):
+def check_decode(lengths, Hq, Hk, D, page, dtype, kv=None, layout="nhd", seed=0, scale=1.5, sm_scale=None, listed=0):
     g = torch.Generator(device=DEV).manual_seed(seed)
     pages, indptr, indices, last = pages_for(lengths, page, g)
+    if listed:                               # a page list with room for more, as a captured step keeps it
+        indices = torch.cat([indices, torch.full((listed,), -1, dtype=torch.int32, device=DEV)])
     k, v, ks, vs = cache_of(pages, page, Hk, D, kv or dtype, g, layout)
     # what no request owns, or lies past its length, must not be read
     owned = torch.zeros(pages, page, dtype=torch.bool, device=DEV)
@@ -159,6 +161,21 @@ def test_decode_lengths(dtype, kv, lengths):
 def test_decode_score_ranges(dtype, kv, scale, sm_scale):
     """All weights alike, and one key that takes nearly all of it."""
     check_decode([300, 2000, 1], 8, 2, 128, 16, dtype, kv, scale=scale, sm_scale=sm_scale)
+
+
+@pytest.mark.parametrize("dtype,kv", KINDS)
+@pytest.mark.parametrize("Hq,Hk,D", [(16, 2, 128), (32, 8, 128), (32, 8, 64), (12, 6, 96), (8, 4, 256), (32, 4, 192),
+                                     (64, 4, 128), (5, 5, 64), (40, 2, 64), (34, 2, 256), (7, 1, 192)])
+@pytest.mark.parametrize("page", [5, 16])
+def test_decode_with_a_long_page_list(dtype, kv, Hq, Hk, D, page):
+    """The kernels of much work: chosen by the pages listed, whatever the lengths are."""
+    check_decode([1, 0, 15, 16, 17, 63, 64, 65, 700, 0, 1900, 5000, 129], Hq, Hk, D, page, dtype, kv, seed=D + Hq,
+                 listed=2_000_000 // (page * Hk))
+
+
+@pytest.mark.parametrize("dtype,kv", KINDS)
+def test_decode_much_work(dtype, kv):
+    check_decode([40001, 0, 1, 39000, 77, 3001], 32, 8, 128, 16, dtype, kv)
 
 
 @pytest.mark.parametrize("kv", [None, E4M3])
