@@ -118,6 +118,15 @@ __device__ __forceinline__ float row_uniform(uint64_t seed, uint64_t offset, uin
   return static_cast<float>(o.x >> 8) * 5.9604644775390625e-08f;  // 2^-24
 }
 
+// ------------------------------------------------------------------ launch
+// First statement of a kernel launched by launch_kernel(): lets the next such kernel of
+// the stream be set up while this one runs, and waits until everything before this
+// one has ended and is visible.
+__device__ __forceinline__ void grid_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // -------------------------------------------------------------- numerics
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;

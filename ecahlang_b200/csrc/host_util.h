@@ -65,13 +65,26 @@ inline cudaError_t set_smem_once(void (*kernel)(const Args), int smem) {
 }
 
 // Launches `fn` with `smem` bytes of dynamic shared memory, setting the limit
-// first where it may exceed the 48 KB default beside static shared memory; one retry with the limit set afresh.
+// first where it may exceed the 48 KB default beside static shared memory; one retry
+// with the limit set afresh.  The launch may begin while the kernel before it in the
+// stream ends (programmatic stream serialisation): `fn` calls grid_start() before its
+// first access to global memory.
 template <typename Args>
 inline bool launch_kernel(void (*fn)(const Args), dim3 grid, int threads, int smem, cudaStream_t s, const Args& args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   for (int attempt = 0; attempt < 2; ++attempt) {
     if (smem > 32 * 1024 && set_smem_once(fn, smem) != cudaSuccess) { cudaGetLastError(); return false; }
-    fn<<<grid, threads, smem, s>>>(args);
-    if (cudaGetLastError() == cudaSuccess) return true;
+    if (cudaLaunchKernelEx(&cfg, fn, args) == cudaSuccess) return true;
+    cudaGetLastError();
     forget_smem();
   }
   return false;

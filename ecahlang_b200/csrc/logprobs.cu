@@ -414,6 +414,7 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
   constexpr int kN = Vec<DT>::kN;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Smem& S = *reinterpret_cast<Smem*>(smem_raw);
+  grid_start();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long begin = blockIdx.x * P.share + min(static_cast<int>(blockIdx.x), P.more);
   if (tid == 0) {

@@ -79,6 +79,7 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], float inv) {
 
 template <int DT, bool E4M3, int D, int ITERS>
 __global__ void __launch_bounds__(kT) append_kernel(const Params P) {
+  grid_start();
   constexpr int kLanes = D / 16;                                     // of a head
   constexpr int kGroup = kLanes <= 4 ? 4 : kLanes <= 8 ? 8 : 16;     // lanes set aside for it
   constexpr int kGroups = 32 / kGroup;

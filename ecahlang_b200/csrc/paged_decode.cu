@@ -261,6 +261,8 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
   const kv::Cache& C = P.cache;
   const int per_req = C.heads / wh * P.tiles_h;  // items of a request
 
+  grid_start();
+
   // Total cost, then this block's share.  An item costs kItemCost units, then one a
   // tile; the first `more` blocks take share + 1 units, the others share.
   // A batch of up to kT requests leaves its lengths in shared memory.
