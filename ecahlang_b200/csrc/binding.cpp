@@ -65,7 +65,11 @@ struct Args {
     if (v == -1.0 && PyErr_Occurred()) { PyErr_Clear(); refuse("expected a number"); }
     return v;
   }
-  bool truth(int i) const { return PyObject_IsTrue(a[i]) == 1; }
+  bool truth(int i) const {
+    const int v = PyObject_IsTrue(a[i]);
+    if (v < 0) { PyErr_Clear(); refuse("expected a truth value"); }
+    return v != 0;
+  }
 };
 
 void need(const at::Tensor& t, const char* name, at::ScalarType type, int64_t numel, at::Device dev) {

@@ -39,14 +39,15 @@ inline SmemMemo& smem_memo() {
 }
 
 inline void forget_smem() {
-  SmemMemo& m = smem_memo();
-  std::lock_guard<std::mutex> lock(m.mu);
-  m.used = 0;
+  try {
+    SmemMemo& m = smem_memo();
+    std::lock_guard<std::mutex> lock(m.mu);
+    m.used = 0;
+  } catch (...) {                      // no exception leaves a C entry point
+  }
 }
 
-template <typename Args>
-inline cudaError_t set_smem_once(void (*kernel)(const Args), int smem) {
-  const void* fn = reinterpret_cast<const void*>(kernel);
+inline cudaError_t remember_smem(const void* fn, int smem) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -62,6 +63,15 @@ inline cudaError_t set_smem_once(void (*kernel)(const Args), int smem) {
     m.fn[m.used] = fn; m.dev[m.used] = dev; m.val[m.used] = smem; ++m.used;
   }
   return cudaSuccess;
+}
+
+template <typename Args>
+inline cudaError_t set_smem_once(void (*kernel)(const Args), int smem) {
+  try {
+    return remember_smem(reinterpret_cast<const void*>(kernel), smem);
+  } catch (...) {
+    return cudaErrorUnknown;
+  }
 }
 
 // Launches `fn` with `smem` bytes of dynamic shared memory, setting the limit

@@ -97,7 +97,7 @@ struct Shape {
   static constexpr int kStage = kSlice * (kKStride + kVStride) + kScaleBytes;
   // Blocks of an SM and stages of a warp's ring: 65 to 130 KB in flight on an SM
   // (6.5 TB/s over 148 SMs at about 1 us wants 45 KB) and 8 to 16 warps.
-  static constexpr int kStages = E4M3 ? (D <= 96 ? 4 : 3) : BULK ? (D == 256 ? 3 : 2) : (D == 256 ? 2 : 3);
+  static constexpr int kStages = E4M3 ? (D <= 96 ? 4 : 3) : BULK || D == 256 ? 2 : 3;
   static constexpr int kOStride = D + 4;                  // of a warp's result: 8 heads on 8 bank quads
   static constexpr int kWarpBytes = kStages * kStage;
   static constexpr int kSmem = kW * kWarpBytes;
@@ -421,6 +421,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
         if (BULK) {
           const uint32_t row = st + (lane < kSlice ? lane * S::kKStride : kSlice * S::kKStride + (lane - kSlice) * S::kVStride);
           if (lane == 0) bar_expect(bar, __popc(live) * S::kRowBytes);
+          fence_copies();                                     // after the reads of the slice before
           if (pg >= 0) {
             copy_row(row, side.base + off * 16ull, S::kRowBytes, bar);
           } else {                                            // past the length: zeros
@@ -797,17 +798,19 @@ struct Variant {
 };
 
 // The kernel of a head layout: one head tile of 8 query heads where a KV head has
-// at most 8, else tiles of 16 (a KV row is then read once per 16 heads).  BULK: rows
-// of 256 bytes and more by the copy engine.  It starts a copy about every 10 clocks
-// an SM: at 256 bytes that is more than HBM brings, and it leaves the threads free (4
-// requests of 100 000 to 131 072 tokens in bf16: 296 us against 321); a block alone
-// waits longer for its 128 copies than for its threads' own (128 requests of up to 512
-// tokens: 18.9 us against 13.0), and shorter rows starve (128 bytes: 3.4 TB/s).
-constexpr int kBulkRow = 256;
-
+// at most 8, else tiles of 16 (a KV row is then read once per 16 heads).
+//
+// BULK: rows by the copy engine, for 16-bit heads of 128 and 192 where there is much
+// to stream.  It starts a copy about every 10 clocks an SM, at 256 bytes more than HBM
+// brings, and leaves the threads free.  4 requests of 100 001 to 131 072 tokens, 32/8
+// heads: 300 us against 321 with heads of 128, 454 against 495 with 192.  Elsewhere
+// the threads' copies are better: shorter rows starve (128 bytes: 3.4 TB/s), rows of 256
+// in 8 bits with their conversions take 430 us against 339, heads of 256 leave room for
+// one block (711 against 657), and a block with little to do waits longer for its 128
+// copies (128 requests of up to 512 tokens: 18.9 us against 14).
 template <int DT, bool E4M3, int D, int NT>
 static Variant variant_of(bool bulk) {
-  constexpr bool kCan = D * (E4M3 ? 1 : 2) >= kBulkRow;
+  constexpr bool kCan = !E4M3 && (D == 128 || D == 192);
   using Bulk = Shape<D, E4M3, NT, kCan>;
   using Threads = Shape<D, E4M3, NT, false>;
   if (kCan && bulk) return Variant{decode_kernel<DT, E4M3, D, NT, kCan>, Bulk::kSmem, Bulk::kBlocks};

@@ -188,6 +188,14 @@ def test_workspace_serves_calls_of_any_shape_in_a_row():
         assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
+@pytest.mark.parametrize("K", [2, 33, 128, 129, 400])
+@pytest.mark.parametrize("top_n", [0, 3])
+def test_many_tokens_of_a_row(K, top_n):
+    x, _, g = make(4, 3001, torch.bfloat16)
+    tok = torch.randint(-1, 3003, (4, K), generator=g, device=DEV, dtype=torch.int32)
+    check(x, tok, top_n)
+
+
 def test_row_index_gathers_and_clamps():
     x, _, _ = make(11, 5003, torch.bfloat16)
     at = torch.tensor([10, 0, 3, 3, -5, 99], device=DEV, dtype=torch.int32)
