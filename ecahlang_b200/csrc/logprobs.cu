@@ -34,7 +34,7 @@ namespace lp {
 // Measured on one B200, device time of graph replays: 2048 rows of 128256 bf16 with
 // one alternative 107 us (4.9 TB/s; 94 us without alternatives), 128 rows of 151936
 // f16 with 20 alternatives at a temperature 20.1 us (13.4 without), one row with 5
-// alternatives 9.6 us, 37 masked rows of 32003 f32 with 8 alternatives 10.8 us.
+// alternatives 9.4 us, 37 masked rows of 32003 f32 with 8 alternatives 10.5 us.
 // What bounds them: 7.6 instructions an entry and the row's end (a row every 3 us in
 // each block) for many rows; start, row end and join, in turn, for few.
 
