@@ -414,7 +414,7 @@ typedef struct ecah_kv_cache {
  *   (a, b) -> (a cos - b sin, b cos + a sin)                (q and k, given a table)
  *     pairs (i, i + head_dim/2), or (2i, 2i+1) with interleaved
  *   slot: page kv_indices[kv_indptr[b] + pos / page_size], offset pos % page_size
- *   E4M3: scale = max(max|y|, 448e-12) / 448, code = round(y / scale)
+ *   E4M3: scale = max(max|y|, 448e-12) / 448, code = round(y * (1 / scale))
  *
  * All of it in float32, rounded once on the way out.  Tokens with batch_index
  * outside [0, batch), or a position outside their request's pages, or a page
