@@ -87,6 +87,7 @@ at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, at::Device dev) {
 const void* checked_workspace(const at::Tensor& w, at::Device dev) {
   if (w.device() != dev || w.scalar_type() != at::kByte || !w.is_contiguous())
     refuse("workspace must be a contiguous uint8 tensor on the operands' device");
+  if (reinterpret_cast<uintptr_t>(w.data_ptr()) % 16) refuse("workspace must be 16-byte aligned");
   return w.data_ptr();
 }
 

@@ -1,12 +1,15 @@
-// Host helpers shared by the launchers: the device's SM count and the
-// dynamic shared memory limit of a kernel, each looked up or set once.
+// Host helpers shared by the launchers: pointer alignment, the device's SM count
+// and the dynamic shared memory limit of a kernel, each looked up or set once.
 #pragma once
 
 #include <cuda_runtime.h>
 
+#include <cstdint>
 #include <mutex>
 
 namespace ecah {
+
+inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // SM count of the current device, looked up once per device; 0 without one.
 inline int device_sms() {

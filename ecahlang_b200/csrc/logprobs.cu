@@ -710,7 +710,8 @@ int ecah_token_logprobs(const ecah_logprob_args* a, void* stream) {
   if (!a->logits || (a->tokens_per_row && (!a->token_ids || !a->logprobs)) ||
       (a->top_n && (!a->top_ids || !a->top_logprobs)))
     return ECAH_ERR_NULL;
-  if (!a->workspace || a->workspace_bytes < ecah_token_logprobs_workspace_bytes()) return ECAH_ERR_WORKSPACE;
+  if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < ecah_token_logprobs_workspace_bytes())
+    return ECAH_ERR_WORKSPACE;
   lp::Params P = {};
   P.logits = a->logits;
   P.row_stride = a->row_stride;

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "host_util.h"
 
 namespace ecah {
 namespace kv {
@@ -30,8 +31,6 @@ __device__ __forceinline__ void page_range(const Cache& c, int b, long long* fir
   *first = lo;
   *count = hi - lo;
 }
-
-inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 inline bool head_dim_ok(int d) { return d == 64 || d == 96 || d == 128 || d == 192 || d == 256; }
 

@@ -252,7 +252,7 @@ extern "C" int ecah_paged_append(const ecah_append_args* a, void* stream) {
   if (a->q ? (!a->q_out || a->num_qo_heads < 1) : a->num_qo_heads != 0) return a->q && !a->q_out ? ECAH_ERR_NULL : ECAH_ERR_SHAPE;
   for (const void* p : {a->q, a->k, a->v, static_cast<const void*>(a->q_out), a->q_norm, a->k_norm,
                         static_cast<const void*>(a->cos_sin)})
-    if (!kv::aligned16(p)) return ECAH_ERR_SHAPE;
+    if (!aligned16(p)) return ECAH_ERR_SHAPE;
   append::Params P = {};
   P.q = a->q; P.k = a->k; P.v = a->v; P.q_out = a->q_out;
   P.q_norm = a->q_norm; P.k_norm = a->k_norm;

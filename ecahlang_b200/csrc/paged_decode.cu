@@ -888,8 +888,9 @@ int ecah_paged_decode(const ecah_decode_args* a, void* stream) {
     if (s < 0 || s % 8) return ECAH_ERR_SHAPE;
   if (c.batch == 0) return ECAH_OK;
   if (!a->q || !a->out || !a->kv_last_page_len) return ECAH_ERR_NULL;
-  if (!kv::aligned16(a->q) || !kv::aligned16(a->out)) return ECAH_ERR_SHAPE;
-  if (!a->workspace || a->workspace_bytes < ecah_paged_decode_workspace_bytes(c.batch, a->num_qo_heads, c.num_kv_heads, c.head_dim))
+  if (!aligned16(a->q) || !aligned16(a->out)) return ECAH_ERR_SHAPE;
+  if (!a->workspace || !aligned16(a->workspace) ||
+      a->workspace_bytes < ecah_paged_decode_workspace_bytes(c.batch, a->num_qo_heads, c.num_kv_heads, c.head_dim))
     return ECAH_ERR_WORKSPACE;
   const int sms = device_sms();
   if (sms <= 0) return ECAH_ERR_LAUNCH;

@@ -68,7 +68,8 @@ def decode(q: torch.Tensor, kv_indptr: torch.Tensor, kv_indices: torch.Tensor, k
     without pages gets zeros.  ``sm_scale`` defaults to ``1 / sqrt(D)``.
     ``lse`` float32 [batch, Hq], when given, receives the natural logarithm of
     the softmax denominators (to join partial attentions; -inf without
-    tokens).  ``workspace``: zero-filled uint8, one per concurrent stream."""
+    tokens).  ``workspace``: zero-filled uint8, 16-byte aligned,
+    one per concurrent stream."""
     got = binding().decode(q, kv_indptr, kv_indices, kv_last_page_len, k_cache, v_cache, workspace, k_scale, v_scale,
                            sm_scale, out, lse, None)
     return got if lse is None else got[0]

@@ -48,7 +48,8 @@ enum ecah_status {
   ECAH_ERR_NULL = 1,       /* a required pointer is NULL                         */
   ECAH_ERR_DTYPE = 2,      /* dtype is not one of enum ecah_dtype                */
   ECAH_ERR_SHAPE = 3,      /* batch/vocab/stride out of range (vocab too large)  */
-  ECAH_ERR_WORKSPACE = 4,  /* workspace NULL or smaller than _workspace_bytes()  */
+  ECAH_ERR_WORKSPACE = 4,  /* workspace NULL, smaller than _workspace_bytes() or
+                              not aligned as its argument struct says           */
   ECAH_ERR_LAUNCH = 5,     /* the CUDA launch itself failed                      */
   ECAH_ERR_ABI = 6         /* args.abi_version does not match this library       */
 };
@@ -359,8 +360,8 @@ typedef struct ecah_logprob_args {
   int32_t* top_ids;           /* [R, top_n]                                       */
   float* top_logprobs;        /* [R, top_n]                                       */
   void* workspace;            /* >= ecah_token_logprobs_workspace_bytes(),
-                                 zero-filled once; every launch leaves its
-                                 counters at zero                                 */
+                                 16-byte aligned, zero-filled once; every launch
+                                 leaves its counters at zero                      */
   size_t workspace_bytes;
 } ecah_logprob_args;
 
@@ -476,8 +477,8 @@ typedef struct ecah_decode_args {
   const int32_t* kv_last_page_len;   /* [batch] device                            */
   ecah_kv_cache cache;
   void* workspace;            /* >= ecah_paged_decode_workspace_bytes() for some
-                                 batch >= cache.batch, zero-filled once; every
-                                 launch leaves its counters at zero               */
+                                 batch >= cache.batch, 16-byte aligned, zero-filled
+                                 once; every launch leaves its counters at zero   */
   size_t workspace_bytes;
 } ecah_decode_args;
 

@@ -134,3 +134,13 @@ def test_cpu_tensors_are_rejected():
         paged.append(k, k, k, ids[:1], ids[:1], ids, ids[:1], c, c)
     with pytest.raises(RuntimeError, match="CUDA"):
         paged.decode(k, ids, ids[:1], ids[:1], c, c, torch.zeros(256, dtype=torch.uint8))
+
+
+def test_misaligned_workspaces_are_refused_without_a_device(L):
+    """The kernels read and write their workspaces 16 bytes at a time."""
+    lp = dict(abi_version=_abi.ABI_VERSION, dtype=0, rows=2, vocab=10, row_stride=10, logits=16, workspace_bytes=1 << 30)
+    dec = dict(abi_version=_abi.ABI_VERSION, dtype=1, num_qo_heads=8, sm_scale=0.1, q=64, out=64, kv_last_page_len=64,
+               cache=_cache(), workspace_bytes=1 << 30)
+    for off in (1, 2, 4, 8, 24):
+        assert L.ecah_token_logprobs(_set(_abi.LogprobArgs(), dict(lp, workspace=4096 + off)), None) == 4
+        assert L.ecah_paged_decode(_set(_abi.DecodeArgs(), dict(dec, workspace=4096 + off)), None) == 4
