@@ -4,12 +4,14 @@
 
 #include <cuda_runtime.h>
 
+#include <cstddef>
 #include <cstdint>
 #include <mutex>
 
 namespace ecah {
 
-inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+inline bool aligned16(const void* p) { return aligned_to(p, 16); }
 
 // SM count of the current device, looked up once per device; 0 without one.
 inline int device_sms() {

@@ -222,7 +222,7 @@ int ecah_sampler_launch(const ecah_sampler_args* a, void* stream) {
   if (!a->logits || !a->temperature || !a->top_k || !a->top_p || !a->out) return ECAH_ERR_NULL;
   if (!a->uniforms && !a->philox_state) return ECAH_ERR_NULL;
   if (a->row_slot && (!a->slot_len || !a->hist_tok || !a->hist_cnt || a->hist_cap < 0)) return ECAH_ERR_NULL;
-  if (!a->workspace || a->workspace_bytes < kMinWorkspace) return ECAH_ERR_WORKSPACE;
+  if (!a->workspace || a->workspace_bytes < kMinWorkspace || !aligned_to(a->workspace, alignof(unsigned))) return ECAH_ERR_WORKSPACE;
   if (a->row_index && a->logit_rows < 1) return ECAH_ERR_SHAPE;
 
   KParams P = {};
@@ -261,6 +261,7 @@ int ecah_sampler_launch(const ecah_sampler_args* a, void* stream) {
   RowLayout L;
   const bool k16 = k16_dtype(a->dtype);   // additive penalties keep the logits in the model dtype
   if (k16 && row_layout(a->batch, a->vocab, &L) && a->workspace_bytes >= L.total) {
+    if (!aligned_to(a->workspace, alignof(unsigned long long))) return ECAH_ERR_WORKSPACE;   // candidates
     unsigned char* ws = static_cast<unsigned char*>(a->workspace);
     P.NC = L.NC;
     P.ws_fin = ws + L.fin;
@@ -527,7 +528,7 @@ int ecah_vp_merge(const ecah_vp_args* a, void* stream) {
   if (a->batch == 0) return ECAH_OK;
   if (!a->all_cand || !a->all_count || !a->out) return ECAH_ERR_NULL;
   if (!a->uniforms && !a->philox_state) return ECAH_ERR_NULL;
-  if (!a->workspace || a->workspace_bytes < kMinWorkspace) return ECAH_ERR_WORKSPACE;
+  if (!a->workspace || a->workspace_bytes < kMinWorkspace || !aligned_to(a->workspace, alignof(unsigned))) return ECAH_ERR_WORKSPACE;
   vp::VParams P = {};
   P.B = a->batch; P.V = a->vocab; P.Bs = a->batch;
   P.temperature = a->temperature; P.top_k = a->top_k; P.top_p = a->top_p;

@@ -113,7 +113,8 @@ typedef struct ecah_sampler_args {
   float* probs_out;           /* [B, vocab] renormalised probabilities of the final
                                  set (0 elsewhere); greedy rows get a one-hot row */
   void* workspace;            /* >= ecah_sampler_workspace_bytes(B, vocab, dtype) for
-                                 some B >= batch, zero-filled once before first use.
+                                 some B >= batch, 8-byte aligned, zero-filled once
+                                 before first use.
                                  Its first 4096 bytes hold counters that every launch
                                  leaves at zero; the rest is scratch.               */
   size_t workspace_bytes;
@@ -237,7 +238,7 @@ typedef struct ecah_vp_args {
   uint64_t* philox_state;     /* [2], advanced by 1 after the merge               */
   int32_t* out;               /* [batch] sampled ids (the same on every rank)     */
   float* row_stats;           /* [batch, 4] optional, as in ecah_sampler_args     */
-  void* workspace;            /* >= 256 bytes, zero-filled once                   */
+  void* workspace;            /* >= 256 bytes, 4-byte aligned, zero-filled once   */
   size_t workspace_bytes;
 } ecah_vp_args;
 

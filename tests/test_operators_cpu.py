@@ -144,3 +144,16 @@ def test_misaligned_workspaces_are_refused_without_a_device(L):
     for off in (1, 2, 4, 8, 24):
         assert L.ecah_token_logprobs(_set(_abi.LogprobArgs(), dict(lp, workspace=4096 + off)), None) == 4
         assert L.ecah_paged_decode(_set(_abi.DecodeArgs(), dict(dec, workspace=4096 + off)), None) == 4
+
+
+def test_misaligned_sampler_workspaces_are_refused_without_a_device(L):
+    """Counters are 32-bit; the row kernel's candidates 64-bit."""
+    a = dict(abi_version=_abi.ABI_VERSION, dtype=0, batch=2, vocab=1000, row_stride=1000, logits=4096, temperature=4096,
+             top_k=4096, top_p=4096, out=4096, uniforms=4096, workspace_bytes=1 << 30)
+    for off in (1, 2, 4, 6):
+        assert L.ecah_sampler_launch(_set(_abi.SamplerArgs(), dict(a, workspace=4096 + off)), None) == 4
+    vp = dict(abi_version=_abi.ABI_VERSION, dtype=0, batch=1, vocab=1000, row_stride=1000, logits=4096, world=1,
+              vocab_local=1000, cand_cap=64, temperature=4096, top_k=4096, top_p=4096, out=4096, uniforms=4096, all_cand=4096,
+              all_count=4096, workspace_bytes=256)
+    for off in (1, 2):
+        assert L.ecah_vp_merge(_set(_abi.VPArgs(), dict(vp, workspace=4096 + off)), None) == 4
