@@ -32,7 +32,7 @@ EXPORTS = ("ecah_sampler_abi_version", "ecah_status_string", "ecah_sampler_works
            "ecah_vp_ipc_alloc", "ecah_vp_ipc_open", "ecah_vp_ipc_close", "ecah_vp_ipc_free",
            "ecah_quotient_mismatches", "ecah_vp_reset", "ecah_vp_dist_pass",
            "ecah_token_logprobs_workspace_bytes", "ecah_token_logprobs", "ecah_paged_append",
-           "ecah_paged_decode_workspace_bytes", "ecah_paged_decode")
+           "ecah_paged_decode_workspace_bytes", "ecah_paged_decode", "ecah_paged_decode_bounded")
 IPC_HANDLE_BYTES = 64
 
 
@@ -186,6 +186,8 @@ def lib():
         L.ecah_paged_decode_workspace_bytes.argtypes = [c_int32, c_int32, c_int32, c_int32]
         L.ecah_paged_decode.restype = c_int32
         L.ecah_paged_decode.argtypes = [ctypes.POINTER(DecodeArgs), c_void_p]
+        L.ecah_paged_decode_bounded.restype = c_int32
+        L.ecah_paged_decode_bounded.argtypes = [ctypes.POINTER(DecodeArgs), c_int32, c_void_p]
         if L.ecah_sampler_abi_version() != ABI_VERSION:
             raise EcahError("libecah_sampler.so ABI version mismatch")
         _lib = L

@@ -54,6 +54,7 @@ constexpr int kItemCost = 4;
 constexpr int kWhole = 8;             // items of up to so many tiles are not divided, ...
 constexpr int kWholeAlone = 4;        // ... or so many where there is a block for every tile (one
                                       // request of 512: 8.8 us divided, 10.4 whole; 128: 18.0, 13.2)
+constexpr int kTries = 1 << 20;       // of a wait for copies: more than one in flight can need
 constexpr float kLazy = 8.0f;         // the reference moves when a score is 2^8 above it
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -73,6 +74,7 @@ struct Params {
   int hq, group, tiles_h;    // query heads, per KV head, head tiles per KV head
   int wh;                    // KV heads of an item: 1, 2 or 4
   int page_shift;            // log2 page_size, or -1
+  int tries;                 // of a wait for the copy engine
   float scale;               // sm_scale * log2 e
   unsigned* counters;        // [2 slots][2]: group and item arrivals, zero between launches
   float2* part_ml;           // [slots][wh rows]
@@ -129,10 +131,9 @@ __device__ __forceinline__ void bar_init(uint32_t bar) { asm volatile("mbarrier.
 __device__ __forceinline__ void bar_expect(uint32_t bar, int bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// Waits for a phase of the barrier; false after a bounded number of tries (each may
-// itself wait), which a copy in flight cannot need.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
-  for (int tries = 0; tries < 1 << 20; ++tries) {
+// Waits for a phase of the barrier; false after `most` tries (each may itself wait).
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, int most) {
+  for (int tries = 0; tries < most; ++tries) {
     uint32_t done;
     asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
                  : "=r"(done) : "r"(bar), "r"(parity) : "memory");
@@ -252,6 +253,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
   __shared__ int s_req[2], s_flag;       // requests of the share's edges
   __shared__ int s_len[kT], s_first[kT];
   __shared__ unsigned long long s_bar[kW][S::kStages];
+  __shared__ int s_failed;               // a wait for copies ran out: this block's results are NaN from then on
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // the join's (m, l) and factors: behind the first warp's result in its ring
   float2(*s_ml)[kMaxRows] = reinterpret_cast<float2(*)[kMaxRows]>(smem + S::kResult);
@@ -288,6 +290,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
   }
   if (lane == 31) s_scan[warp] = inc;
   if (tid < 2) s_req[tid] = -1;
+  if (BULK && tid == 0) s_failed = 0;
   __syncthreads();
   unsigned before = 0;
 #pragma unroll
@@ -352,6 +355,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
   unsigned char* ring_p = smem + warp * S::kWarpBytes;
   const uint32_t bars = smem_u32(s_bar[warp]);
   uint32_t phase = 0;                            // of each stage's barrier
+  bool failed = false;                           // this warp's wait ran out: it copies nothing more
   if (BULK && lane == 0) {
     for (int i = 0; i < S::kStages; ++i) bar_init(bars + 8 * i);
     fence_copies();
@@ -372,6 +376,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
     const int n = static_cast<int>(seg_end) - static_cast<int>(tile0) - t0;
     at = seg_end;
     if (n <= 0) continue;                                     // only the item's first units: no tile
+    const int steps = BULK && failed ? 0 : n;
     const int rows = min(P.group - ht * kRows, kRows);        // query heads of this tile
     const int head0 = h * P.group + ht * kRows;
 
@@ -384,7 +389,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
     auto nth_page = [&](unsigned j) { return P.page_shift >= 0 ? j >> P.page_shift : j / static_cast<unsigned>(C.page_size); };
     auto page_of = [&](int i) -> int {
       const unsigned j = key0 + static_cast<unsigned>(i) * tile;
-      return i < n && j < static_cast<unsigned>(len) ? min(max(pages[nth_page(j)], 0), C.num_pages - 1) : -1;
+      return i < steps && j < static_cast<unsigned>(len) ? min(max(pages[nth_page(j)], 0), C.num_pages - 1) : -1;
     };
     int page = page_of(0), page_after = page_of(1);           // two slices ahead: an L2 read away
     // ---- the queries, asked for while the pages come and before the stream fills the memory's queues: heads
@@ -409,7 +414,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
     }
 
     auto issue = [&](int i) {
-      if (i < n) {
+      if (i < steps) {
         const unsigned j = key0 + static_cast<unsigned>(i) * tile;
         const int pg = page;
         const unsigned slot = j - nth_page(j) * static_cast<unsigned>(C.page_size);
@@ -515,11 +520,21 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
       l[x][0] = l[x][1] = 0.0f;
     }
 
-    for (int i = 0; i < n; ++i) {
+    for (int i = 0; i < steps; ++i) {
       issue(i + S::kStages - 1);
       if (E4M3 || !BULK) cp_wait<S::kStages - 1>();
-      if (BULK && !bar_wait(bars + 8 * (i % S::kStages), phase >> (i % S::kStages) & 1u)) l[0][0] = NAN;
-      phase ^= 1u << (i % S::kStages);
+      if (BULK) {
+        if (!__all_sync(0xFFFFFFFFu, bar_wait(bars + 8 * (i % S::kStages), phase >> (i % S::kStages) & 1u, P.tries))) {
+          // Give up: wait again for the copies in flight, so that none lands in the
+          // results or after the block has ended.
+          for (int k = i; k < min(steps, i + S::kStages); ++k)
+            bar_wait(bars + 8 * (k % S::kStages), phase >> (k % S::kStages) & 1u, kTries);
+          failed = true;
+          if (lane == 0) s_failed = 1;
+          break;
+        }
+        phase ^= 1u << (i % S::kStages);
+      }
       __syncwarp();
       const int base = (t0 + i) * tile + slice0;
       if (base < len) {
@@ -708,6 +723,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
     // Combine `count` triples (m, l, o) of each of the item's rows (head h0 + j, query
     // head r of its tile; row j kRows + r) into the output or a part's slot.
     const int item_rows = wh * kRows;
+    const bool bad = BULK && s_failed;
     auto combine = [&](auto from, int count, auto ml_of, auto o_of, int o_stride, int to) {
       using From = decltype(from);
       for (int i = tid; i < count * item_rows; i += kT) {
@@ -724,6 +740,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
           ll = fmaf(v.y, f, ll);
           s_ml[p][tid].x = f;
         }
+        if (bad) ll = NAN;
         if (to >= 0) {
           P.part_ml[static_cast<long long>(to) * item_rows + tid] = make_float2(mm, ll);
         } else {
@@ -746,6 +763,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
           const float f = s_ml[p][r].x;
           v.x = fmaf(w.x, f, v.x); v.y = fmaf(w.y, f, v.y); v.z = fmaf(w.z, f, v.z); v.w = fmaf(w.w, f, v.w);
         }
+        if (bad) v = make_float4(NAN, NAN, NAN, NAN);
         if (to >= 0) {
           *reinterpret_cast<float4*>(P.part_o + static_cast<long long>(to) * item_rows * D + e) = v;
         } else {
@@ -877,7 +895,9 @@ size_t ecah_paged_decode_workspace_bytes(int32_t batch, int32_t num_qo_heads, in
   return decode::layout(device_sms(), head_dim).total;
 }
 
-int ecah_paged_decode(const ecah_decode_args* a, void* stream) {
+int ecah_paged_decode(const ecah_decode_args* a, void* stream) { return ecah_paged_decode_bounded(a, decode::kTries, stream); }
+
+int ecah_paged_decode_bounded(const ecah_decode_args* a, int32_t tries, void* stream) {
   if (!a) return ECAH_ERR_NULL;
   if (a->abi_version != ECAH_SAMPLER_ABI_VERSION) return ECAH_ERR_ABI;
   const int st = kv::check_cache(a->cache, a->dtype);
@@ -904,6 +924,7 @@ int ecah_paged_decode(const ecah_decode_args* a, void* stream) {
   P.page_shift = -1;
   for (int i = 0; i < 31; ++i)
     if (c.page_size == 1 << i) P.page_shift = i;
+  P.tries = tries;
   P.scale = a->sm_scale * kLog2e;
   P.cache = kv::make_cache(c);
   const decode::Layout L = decode::layout(sms, c.head_dim);

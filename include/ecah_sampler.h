@@ -487,6 +487,13 @@ ECAH_API size_t ecah_paged_decode_workspace_bytes(int32_t batch, int32_t num_qo_
                                                   int32_t head_dim);
 ECAH_API int ecah_paged_decode(const ecah_decode_args* args, void* stream);
 
+/* ecah_paged_decode with a limit of its own on the waits for the copy engine
+ * (where the launch uses it, at much work and 16-bit heads of 128 or 192): a
+ * block whose wait runs out copies nothing more and gives NaN for every row
+ * that it still has a part in.  0 makes every wait run out; a launch that
+ * does not use the copy engine is not affected. */
+ECAH_API int ecah_paged_decode_bounded(const ecah_decode_args* args, int32_t tries, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

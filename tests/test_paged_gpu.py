@@ -11,12 +11,13 @@ its 10):
     for f16 2^-25 of the row's largest), so |error| <= u |o| + u sum p|v| +
     2^-24 max(p) sum|v| + float32's 2^-16 sum p|v|.
 """
+import ctypes
 import math
 
 import pytest
 import torch
 
-from ecahlang_b200 import paged
+from ecahlang_b200 import _abi, paged
 from ecahlang_b200.paged import PagedAttention
 
 pytestmark = pytest.mark.gpu
@@ -252,6 +253,40 @@ def test_decode_many_shapes_on_one_workspace_streams_and_graph():
         graph.replay()
         want, _, tol, _ = decode_reference(q, n, indptr, indices, k, v, None, None, 128 ** -0.5)
         assert ((out.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("Hq,Hk,D", [(32, 8, 128), (64, 4, 128), (8, 8, 192), (32, 2, 192)])
+def test_decode_wait_that_runs_out_gives_nan_in_every_row(dtype, Hq, Hk, D):
+    """With no tries for the copy engine's waits (its copies still land) nothing finite is left of a
+    request with tokens; the launch after it finds its workspace as it should be."""
+    g = torch.Generator(device=DEV).manual_seed(9)
+    lengths = [20000, 0, 3, 700, 64]
+    pages, indptr, indices, last = pages_for(lengths, 16, g)
+    indices = torch.cat([indices, torch.full((2_000_000 // (16 * Hk),), -1, dtype=torch.int32, device=DEV)])
+    k, v, _, _ = cache_of(pages, 16, Hk, D, dtype, g)
+    q = torch.randn(len(lengths), Hq, D, generator=g, device=DEV).to(dtype)
+    att = PagedAttention(Hq, Hk, D, 16, dtype, max_batch=len(lengths))
+    out, lse = torch.zeros_like(q), torch.zeros(len(lengths), Hq, device=DEV)
+    page, slot, head, _ = k.stride()
+    cache = _abi.KVCache(kv_dtype=paged._DTYPES[dtype], num_pages=pages, page_size=16, num_kv_heads=Hk, head_dim=D,
+                         batch=len(lengths), k_cache=k.data_ptr(), v_cache=v.data_ptr(), k_page_stride=page,
+                         k_slot_stride=slot, k_head_stride=head, v_page_stride=page, v_slot_stride=slot,
+                         v_head_stride=head, kv_indptr=indptr.data_ptr(), kv_indices=indices.data_ptr(),
+                         num_indices=indices.numel())
+    a = _abi.DecodeArgs(abi_version=_abi.ABI_VERSION, dtype=paged._DTYPES[dtype], num_qo_heads=Hq, sm_scale=D ** -0.5,
+                        q=q.data_ptr(), q_token_stride=Hq * D, q_head_stride=D, out=out.data_ptr(),
+                        out_token_stride=Hq * D, out_head_stride=D, lse=lse.data_ptr(),
+                        kv_last_page_len=last.data_ptr(), cache=cache, workspace=att.workspace.data_ptr(),
+                        workspace_bytes=att.workspace.numel())
+    stream = torch.cuda.current_stream().cuda_stream
+    assert _abi.lib().ecah_paged_decode_bounded(ctypes.byref(a), 0, stream) == 0
+    some = torch.tensor(lengths, device=DEV) > 0
+    assert torch.isnan(out[some]).all() and torch.isnan(lse[some]).all()
+    assert (out[~some] == 0).all() and (lse[~some] == -math.inf).all()
+    assert _abi.lib().ecah_paged_decode_bounded(ctypes.byref(a), 1 << 20, stream) == 0
+    want, wlse = att.decode(q, indptr, indices, last, k, v, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, wlse) and torch.isfinite(want).all()
 
 
 # ------------------------------------------------------------------- append
