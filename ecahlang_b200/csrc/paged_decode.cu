@@ -55,7 +55,12 @@ constexpr int kWhole = 8;             // items of up to so many tiles are not di
 constexpr int kWholeAlone = 4;        // ... or so many where there is a block for every tile (one
                                       // request of 512: 8.8 us divided, 10.4 whole; 128: 18.0, 13.2)
 constexpr int kTries = 1 << 20;       // of a wait for copies: more than one in flight can need
-constexpr float kLazy = 8.0f;         // the reference moves when a score is 2^8 above it
+// The reference moves when a score passes its last place by 2^kLazy.  Where the weights
+// are f16 operands it then lies 2^kLift below the largest: weights reach 2^15, and one is
+// lost to f16's smallest only at 2^-32 of the largest (2^-25 without the lift: a long tail
+// of such weights is in the denominator, so it has to be in the sum).
+constexpr float kLazy = 8.0f;
+constexpr float kLift = 7.0f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // One side of the cache in 16-byte units from its base.
@@ -247,6 +252,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
   using S = Shape<D, E4M3, NT, BULK>;
   constexpr int kRows = S::kRows;
   constexpr int HT = E4M3 ? static_cast<int>(ECAH_DTYPE_F16) : DT;   // operand type of the products
+  constexpr float lift = HT == ECAH_DTYPE_F16 ? kLift : 0.0f;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ unsigned s_scan[kW];
   __shared__ unsigned s_start[2];        // first unit of s_req
@@ -574,7 +580,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
           }
         }
         // Scores in log2 units.  An e4m3 value's scale goes into its weight through
-        // the exponent, so that the f16 weights stay at or below 2^8 whatever the
+        // the exponent, so that the f16 weights stay at or below 2^15 whatever the
         // scales are: weight 2^(s + log2 scale - m), and the sum takes it back out.
         float inv[2] = {1.0f, 1.0f};
         const bool tail = base + kSlice > len;
@@ -612,7 +618,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
         for (int x = 0; x < NT; ++x) {
           top[x][0] = fmaxf(s[x][0], s[x][2]);
           top[x][1] = fmaxf(s[x][1], s[x][3]);
-          above |= top[x][0] > m[x][0] + kLazy || top[x][1] > m[x][1] + kLazy;
+          above |= top[x][0] > m[x][0] + (kLazy + lift) || top[x][1] > m[x][1] + (kLazy + lift);
         }
         if (__any_sync(0xFFFFFFFFu, above)) {
 #pragma unroll
@@ -622,7 +628,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
               float v = top[x][y];
 #pragma unroll
               for (int z = 4; z < 32; z <<= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, z));
-              v = fmaxf(v, m[x][y]);
+              v = fmaxf(v - lift, m[x][y]);
               const float f = m[x][y] == v ? 1.0f : ex2_approx(m[x][y] - v);
               m[x][y] = v;
               l[x][y] *= f;
