@@ -61,14 +61,15 @@ def launch(logits: torch.Tensor, token_ids: Optional[torch.Tensor], workspace: t
 
 class TokenLogprobs:
     """Owns the workspace of one stream, so repeated calls (and CUDA-graph
-    replays) of any number of rows allocate nothing but their outputs."""
+    replays) of any number of rows allocate nothing but their outputs.
+    ``workspace``: one that ``new_workspace`` made before (default: a new one)."""
 
-    def __init__(self, vocab: int, dtype: torch.dtype, device="cuda"):
+    def __init__(self, vocab: int, dtype: torch.dtype, device="cuda", workspace: Optional[torch.Tensor] = None):
         if dtype not in _DTYPES:
             raise RuntimeError(f"unsupported logits dtype {dtype}")
         self.vocab, self.dtype = vocab, dtype
         self.device = resolve_device(device)
-        self.workspace = new_workspace(self.device)
+        self.workspace = new_workspace(self.device) if workspace is None else workspace
         self._launch = binding().logprobs
 
     def __call__(self, logits: torch.Tensor, token_ids: Optional[torch.Tensor] = None, *, top_n: int = 0,

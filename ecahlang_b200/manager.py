@@ -24,6 +24,7 @@ from typing import Dict, Iterable, Optional, Sequence
 import numpy as np
 import torch
 
+from . import logprobs as token_logprobs
 from .logprobs import RowLogprobs, TokenLogprobs
 from .sampler import PenaltyState, launch, new_philox_state, new_workspace, repetition_factor, resolve_device
 
@@ -55,7 +56,9 @@ class SamplingManager:
         # freq_pres_in_graphs=True captures every bucket with them.
         self.freq_pres_in_graphs = freq_pres_in_graphs
         self._cg_captured_fp: Dict[int, bool] = {}
+        self._workspace: Optional[torch.Tensor] = None
         self._scorer: Optional[TokenLogprobs] = None
+        self._scorer_workspace: Optional[torch.Tensor] = None
         # overflow flags of the slot histories, copied to the host after every
         # update and checked when the next step's parameters are filled (the
         # host has read the previous step's ids by then)
@@ -93,8 +96,10 @@ class SamplingManager:
     # ------------------------------------------------------- eager buffers
     def init_sampling_buffers(self, max_batch_size: int) -> None:
         """Pinned host buffers with numpy views and persistent device buffers
-        (manager.py:74-88), plus the penalty columns and the sampler's own
-        workspace and output."""
+        (manager.py:74-88), plus the penalty columns, the sampler's output and
+        the workspaces of ``sample`` and ``logprobs``: made here, because one
+        made inside a CUDA-graph capture would be zero-filled by that graph's
+        replays alone."""
         B, V, dev = max_batch_size, self.vocab_size, self.device
         self.max_batch_size = B
         self.sampling_temperature_cpu = _pinned(torch.ones(B, 1, dtype=torch.float32))
@@ -119,7 +124,27 @@ class SamplingManager:
         self.sampling_pres_gpu = torch.zeros(B, dtype=torch.float32, device=dev)
         self.sampling_slot_gpu = torch.full((B,), -1, dtype=torch.int32, device=dev)
         self.sampling_out = torch.zeros(B, dtype=torch.int32, device=dev)
-        self._workspace = None
+        self._workspace = self._scorer = self._scorer_workspace = None
+        if dev.type == "cuda":
+            self._sample_workspace()
+            self._logprob_workspace()
+
+    def _outside_capture(self, what: str) -> None:
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"the workspace of {what} cannot be made inside a CUDA-graph capture: "
+                               "call init_sampling_buffers before it")
+
+    def _sample_workspace(self) -> torch.Tensor:
+        if self._workspace is None:
+            self._outside_capture("sample")
+            self._workspace = new_workspace(self.max_batch_size, self.vocab_size, self.dtype, self.device)
+        return self._workspace
+
+    def _logprob_workspace(self) -> torch.Tensor:
+        if self._scorer_workspace is None:
+            self._outside_capture("logprobs")
+            self._scorer_workspace = token_logprobs.new_workspace(self.device)
+        return self._scorer_workspace
 
     def _write_host(self, n, temperatures, top_ks, top_ps, rep_pens, freq_pens, pres_pens, batch_ids) -> bool:
         self.sampling_temperature_np[:n, 0] = temperatures
@@ -232,9 +257,7 @@ class SamplingManager:
             fp = fp or self.freq_pres_in_graphs
             if torch.cuda.is_current_stream_capturing():
                 self._cg_captured_fp[bucket_size] = fp
-        if self._workspace is None:
-            self._workspace = new_workspace(self.max_batch_size, self.vocab_size, self.dtype, self.device)
-        return launch(logits, T.view(-1), K, P, out, self._workspace,
+        return launch(logits, T.view(-1), K, P, out, self._sample_workspace(),
                       uniforms=uniforms, philox_state=None if uniforms is not None else self.philox_state,
                       rep_factor=rep, freq_pen=freq if fp else None, pres_pen=pres if fp else None,
                       penalty=self.penalty, row_slot=slot, freq_pres=fp, row_index=row_index)
@@ -252,7 +275,7 @@ class SamplingManager:
             B = logits.shape[0] if row_index is None else row_index.numel()
             T = self._buffers(B, bucket_size)[0].view(-1)
         if self._scorer is None:
-            self._scorer = TokenLogprobs(self.vocab_size, self.dtype, self.device)
+            self._scorer = TokenLogprobs(self.vocab_size, self.dtype, self.device, self._logprob_workspace())
         return self._scorer(logits, ids, top_n=top_n, temperature=T, row_index=row_index)
 
     def sample_async(self, logits: torch.Tensor, bucket_size: Optional[int] = None,

@@ -157,3 +157,15 @@ def test_misaligned_sampler_workspaces_are_refused_without_a_device(L):
               all_count=4096, workspace_bytes=256)
     for off in (1, 2):
         assert L.ecah_vp_merge(_set(_abi.VPArgs(), dict(vp, workspace=4096 + off)), None) == 4
+
+
+def test_manager_makes_no_workspace_inside_a_capture(monkeypatch):
+    from ecahlang_b200.manager import SamplingManager
+    m = SamplingManager(100, seq_lens=8, dtype=torch.float16, device="cpu", history_capacity=16)
+    m.init_sampling_buffers(2)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    x = torch.zeros(2, 100, dtype=torch.float16)
+    for call in (lambda: m.sample(x), lambda: m.logprobs(x, None)):
+        with pytest.raises(RuntimeError, match="inside a CUDA-graph capture"):
+            call()

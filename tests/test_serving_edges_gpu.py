@@ -5,6 +5,8 @@ import math
 import pytest
 import torch
 
+from ecahlang_b200.logprobs import TokenLogprobs
+from ecahlang_b200.manager import SamplingManager
 from ecahlang_b200.paged import PagedAttention
 
 pytestmark = pytest.mark.gpu
@@ -49,3 +51,48 @@ def test_decode_long_tail_of_small_weights(dtype, kv, D):
     tol = (UNIT[dtype] + weight + 2.0 ** -16) * want + n * 2.0 ** -32 / 4 + 2.0 ** -25
     assert float((out.double() - want).abs().max()) <= tol
     assert float((lse.double() - (gap + math.log(4 + tail))).abs().max()) <= 2e-5 + 4e-6 * gap
+
+
+def _garbage_pool():
+    """A graph whose memory pool holds freed blocks of a log-probability workspace's size, none of them zero."""
+    graph = torch.cuda.CUDAGraph()
+    n = TokenLogprobs(8, torch.float16).workspace.numel()
+    with torch.cuda.graph(graph):
+        kept = [torch.empty(n, dtype=torch.uint8, device=DEV).fill_(0x5A) for _ in range(12)]
+    graph.replay()
+    del kept
+    return graph
+
+
+def test_manager_calls_first_made_inside_a_capture():
+    """The first `sample` and `logprobs` of a manager are captured; an eager call and another bucket
+    run before that graph is replayed."""
+    V = 151936
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(4, V, generator=g, device=DEV).half()
+    m = SamplingManager(V, seq_lens=8, dtype=torch.float16, seed=1)
+    m.init_sampling_buffers(8)
+    m.init_cuda_graph_buffers([2, 4])
+    for bs in (2, 4):
+        m.fill_cuda_graph_sampling_params(bs, bs, [0.7] * bs, [V] * bs, [0.9] * bs)
+    m.fill_sampling_params(4, [0.7] * 4, [V] * 4, [0.9] * 4)
+    pool = _garbage_pool()
+    got, graphs = {}, {}
+    for bs in (2, 4):
+        graphs[bs] = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graphs[bs], pool=pool.pool()):
+            ids = m.sample(x[:bs], bucket_size=bs, uniforms=torch.full((bs,), 0.5, device=DEV))
+            got[bs] = m.logprobs(x[:bs], ids, 5, bucket_size=bs), ids
+    want = TokenLogprobs(V, torch.float16)
+
+    def same(rows, a, ids):
+        b = want(x[:rows], ids, top_n=5)
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+    u = torch.full((4,), 0.5, device=DEV)
+    ids = m.sample(x, uniforms=u)
+    same(4, m.logprobs(x, ids, 5), ids)
+    for bs in (4, 2):
+        graphs[bs].replay()
+        same(bs, *got[bs])
+        assert torch.equal(got[bs][1], ids[:bs])
