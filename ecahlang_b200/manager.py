@@ -228,6 +228,18 @@ class SamplingManager:
                 self.sampling_rep_gpu[:B], self.sampling_freq_gpu[:B], self.sampling_pres_gpu[:B],
                 self.sampling_slot_gpu[:B], self.sampling_out[:B], self._fp_eager)
 
+    def _rows(self, logits: torch.Tensor, row_index):
+        """``row_index`` as a device tensor, a host sequence range-checked, and the number of rows."""
+        if row_index is None:
+            return None, logits.shape[0]
+        if not torch.is_tensor(row_index) or not row_index.is_cuda:
+            idx = np.asarray(torch.as_tensor(row_index).cpu() if torch.is_tensor(row_index) else row_index,
+                             dtype=np.int64).reshape(-1)
+            if idx.size and (idx.min() < 0 or idx.max() >= logits.shape[0]):
+                raise IndexError(f"row_index outside [0, {logits.shape[0]})")
+            row_index = torch.as_tensor(idx.astype(np.int32)).to(self.device, non_blocking=True)
+        return row_index, row_index.numel()
+
     def sample(self, logits: torch.Tensor, bucket_size: Optional[int] = None,
                uniforms: Optional[torch.Tensor] = None, row_index=None) -> torch.Tensor:
         """One token per row of ``logits`` [B, V] (B = bucket_size for the
@@ -240,16 +252,7 @@ class SamplingManager:
         ``append_indptr[1:] - 1`` (ecahlang/main.py:476), read in place.  A
         host sequence is range-checked here and copied to the device; a
         device int32 tensor is used as it is."""
-        if row_index is not None:
-            if not torch.is_tensor(row_index) or not row_index.is_cuda:
-                idx = np.asarray(torch.as_tensor(row_index).cpu() if torch.is_tensor(row_index) else row_index,
-                                 dtype=np.int64).reshape(-1)
-                if idx.size and (idx.min() < 0 or idx.max() >= logits.shape[0]):
-                    raise IndexError(f"row_index outside [0, {logits.shape[0]})")
-                row_index = torch.as_tensor(idx.astype(np.int32)).to(self.device, non_blocking=True)
-            B = row_index.numel()
-        else:
-            B = logits.shape[0]
+        row_index, B = self._rows(logits, row_index)
         if bucket_size is not None and B != bucket_size:
             raise RuntimeError(f"bucket {bucket_size} needs {bucket_size} logits rows, got {B}")
         T, K, P, rep, freq, pres, slot, out, fp = self._buffers(B, bucket_size)
@@ -263,16 +266,16 @@ class SamplingManager:
                       penalty=self.penalty, row_slot=slot, freq_pres=fp, row_index=row_index)
 
     def logprobs(self, logits: torch.Tensor, ids: Optional[torch.Tensor], top_n: int = 0,
-                 bucket_size: Optional[int] = None, row_index: Optional[torch.Tensor] = None,
-                 tempered: bool = False) -> "RowLogprobs":
+                 bucket_size: Optional[int] = None, row_index=None, tempered: bool = False) -> "RowLogprobs":
         """Log probabilities of ``ids`` (int32 [B] or [B, K], e.g. ``sample``'s)
         under the same rows of ``logits``, their entropy and ``top_n``
         alternatives, for completions that ask for them.  Of the model's own
-        distribution, or with ``tempered`` at the filled temperatures.  Enqueued on
-        the current stream; capturable."""
+        distribution, or with ``tempered`` at the filled temperatures.
+        ``row_index`` as ``sample`` takes it.  Enqueued on the current stream;
+        capturable."""
+        row_index, B = self._rows(logits, row_index)
         T = None
         if tempered:
-            B = logits.shape[0] if row_index is None else row_index.numel()
             T = self._buffers(B, bucket_size)[0].view(-1)
         if self._scorer is None:
             self._scorer = TokenLogprobs(self.vocab_size, self.dtype, self.device, self._logprob_workspace())

@@ -169,3 +169,13 @@ def test_manager_makes_no_workspace_inside_a_capture(monkeypatch):
     for call in (lambda: m.sample(x), lambda: m.logprobs(x, None)):
         with pytest.raises(RuntimeError, match="inside a CUDA-graph capture"):
             call()
+
+
+def test_manager_logprobs_checks_a_host_row_index():
+    from ecahlang_b200.manager import SamplingManager
+    m = SamplingManager(100, seq_lens=8, dtype=torch.float16, device="cpu", history_capacity=16)
+    m.init_sampling_buffers(2)
+    x = torch.zeros(5, 100, dtype=torch.float16)
+    for bad in ([0, 5], [-1], torch.tensor([7]), range(4, 6)):
+        with pytest.raises(IndexError, match="row_index"):
+            m.logprobs(x, None, row_index=bad, tempered=True)

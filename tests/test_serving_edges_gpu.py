@@ -96,3 +96,17 @@ def test_manager_calls_first_made_inside_a_capture():
         graphs[bs].replay()
         same(bs, *got[bs])
         assert torch.equal(got[bs][1], ids[:bs])
+
+
+def test_manager_logprobs_takes_the_row_index_that_sample_takes():
+    V = 5000
+    x = torch.randn(9, V, generator=torch.Generator(device=DEV).manual_seed(4), device=DEV).half()
+    m = SamplingManager(V, seq_lens=8, dtype=torch.float16, seed=1)
+    m.init_sampling_buffers(8)
+    m.fill_sampling_params(3, [0.5, 1.0, 2.0], [V] * 3, [0.9] * 3)
+    at = torch.tensor([8, 0, 8], dtype=torch.int32, device=DEV)
+    ids = m.sample(x, row_index=[8, 0, 8])
+    want = TokenLogprobs(V, torch.float16)(x[at.long()], ids, top_n=3, temperature=torch.tensor([0.5, 1.0, 2.0], device=DEV))
+    for rows in ([8, 0, 8], at, at.cpu(), (8, 0, 8)):
+        got = m.logprobs(x, ids, 3, row_index=rows, tempered=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
