@@ -644,8 +644,9 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
         if (bad) return NAN;
         if (empty || x == -INFINITY) return -INFINITY;
         if (greedy) return i == arg ? 0.0f : -INFINITY;
-        // halved, so that the difference of two values of opposite sign near the type's largest stays finite
-        return (0.5f * x - 0.5f * M) / (0.5f * T) - lz;
+        // halved, so that the difference of two values of opposite sign near the type's largest stays
+        // finite; doubled afterwards, since half of the smallest T is zero
+        return 2.0f * ((0.5f * x - 0.5f * M) / T) - lz;
       };
       if (tid == 0 && P.entropy) P.entropy[r] = bad ? NAN : (empty || greedy) ? 0.0f : lz - s / z * kLn2;
       for (int j = tid; j < P.K; j += kT) {

@@ -25,7 +25,7 @@ MAX_TOP_N = _abi.MAX_TOP_N
 
 class RowLogprobs(NamedTuple):
     """One launch's results.  ``top_ids`` is -1 (and ``top_logprobs`` -inf)
-    past a row's last entry with mass."""
+    past a row's last entry above -inf."""
     logprobs: torch.Tensor       # float32, the shape of token_ids
     entropy: torch.Tensor        # float32 [R], natural units
     top_ids: torch.Tensor        # int32 [R, top_n]

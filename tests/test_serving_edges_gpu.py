@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from ecahlang_b200.logprobs import TokenLogprobs
+from ecahlang_b200.logprobs import TokenLogprobs, launch, new_workspace
 from ecahlang_b200.manager import SamplingManager
 from ecahlang_b200.paged import PagedAttention
 
@@ -110,3 +110,19 @@ def test_manager_logprobs_takes_the_row_index_that_sample_takes():
     for rows in ([8, 0, 8], at, at.cpu(), (8, 0, 8)):
         got = m.logprobs(x, ids, 3, row_index=rows, tempered=True)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [7, 5000, 151936])
+def test_logprobs_with_the_smallest_temperatures(dtype, V):
+    """All mass is on the largest logits, evenly."""
+    x = torch.zeros(3, V, dtype=dtype, device=DEV)
+    x[:, 1], x[:, 3] = 2.0, 2.0
+    T = torch.tensor([2.0 ** -149, 2.0 ** -148, 2.0 ** -126], device=DEV)
+    tok = torch.tensor([[1, 0]] * 3, dtype=torch.int32, device=DEV)
+    got = launch(x, tok, new_workspace(), top_n=3, temperature=T)
+    for r in range(3):
+        assert abs(float(got.logprobs[r, 0]) + math.log(2)) <= 1e-6 and float(got.logprobs[r, 1]) < -1e37
+        assert abs(float(got.entropy[r]) - math.log(2)) <= 1e-6
+        assert got.top_ids[r].tolist() == [1, 3, 0]
+        assert (got.top_logprobs[r, :2] + math.log(2)).abs().max() <= 1e-6 and float(got.top_logprobs[r, 2]) < -1e37
