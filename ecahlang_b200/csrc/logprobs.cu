@@ -637,6 +637,7 @@ __global__ void __launch_bounds__(kT, kBlocks) token_logprobs_kernel(const Param
     if (finish && warp * 32 < max(max(P.K, P.N), 1)) {
       const float T = P.temperature ? P.temperature[r] : 1.0f;
       const bool greedy = T <= 0.0f;
+      bad |= T != T;
       const bool empty = !bad && M == -INFINITY;
       const float lz = logf(z);
       const int arg = greedy && have > 0 ? order_index(S.top[0]) : -1;

@@ -339,7 +339,7 @@ ECAH_API int ecah_vp_reset(void* own_buffer, uint32_t epoch, void* stream);
  * the row's last alternative hold id -1 and -inf.  A row of -inf alone has
  * log probabilities -inf and entropy 0.  T <= 0 is the greedy distribution
  * (all mass on the lowest id holding m; the alternatives are listed all the
- * same).  A row with a NaN or a +inf has NaN
+ * same).  A row with a NaN or a +inf, or whose temperature is NaN, has NaN
  * everywhere and ids -1; a token outside [0, vocab) has NaN.
  */
 #define ECAH_MAX_TOP_N 32

@@ -126,3 +126,17 @@ def test_logprobs_with_the_smallest_temperatures(dtype, V):
         assert abs(float(got.entropy[r]) - math.log(2)) <= 1e-6
         assert got.top_ids[r].tolist() == [1, 3, 0]
         assert (got.top_logprobs[r, :2] + math.log(2)).abs().max() <= 1e-6 and float(got.top_logprobs[r, 2]) < -1e37
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [7, 5000, 151936])
+def test_logprobs_without_a_temperature(dtype, V):
+    """A NaN is no temperature: its row has no distribution, the row beside it has one."""
+    x = torch.zeros(2, V, dtype=dtype, device=DEV)
+    x[:, 1], x[:, 3] = 2.0, 2.0
+    T = torch.tensor([float("nan"), 1.0], device=DEV)
+    tok = torch.tensor([[1, 0]] * 2, dtype=torch.int32, device=DEV)
+    got = launch(x, tok, new_workspace(), top_n=3, temperature=T)
+    assert torch.isnan(got.logprobs[0]).all() and torch.isnan(got.entropy[0]) and torch.isnan(got.top_logprobs[0]).all()
+    assert got.top_ids[0].tolist() == [-1] * 3
+    assert got.top_ids[1].tolist() == [1, 3, 0] and torch.isfinite(got.logprobs[1]).all()
