@@ -4,7 +4,7 @@ The library is plain CUDA C++ behind an ``extern "C"`` ABI
 (include/ecah_sampler.h); it links the CUDA runtime statically and has no
 torch dependency, so any FFI (ctypes here) can load it.  ``lib/_ecah_binding.so``
 is the torch side of the newer entry points: a CPython module that checks
-tensors and calls the library.
+tensors and calls the library; it is left out where there is no torch with CUDA.
 """
 from __future__ import annotations
 
@@ -46,9 +46,15 @@ def _stale(product: str) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def _build_binding() -> None:
-    spec = importlib.util.find_spec("torch")     # headers and libraries, without importing it
-    torch = os.path.dirname(spec.origin)
+def _torch():
+    """Directory of a torch with CUDA (headers and libraries, without importing
+    it), or None: the library needs none, its torch binding does."""
+    spec = importlib.util.find_spec("torch")
+    where = os.path.dirname(spec.origin) if spec and spec.origin else None
+    return where if where and os.path.exists(os.path.join(where, "lib", "libtorch_cuda.so")) else None
+
+
+def _build_binding(torch: str) -> None:
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
     include = [os.path.join(ROOT, "include"), os.path.join(torch, "include"),
                os.path.join(torch, "include", "torch", "csrc", "api", "include"),
@@ -80,13 +86,15 @@ def _object(source: str, force: bool, verbose: bool) -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile the library and its torch binding where a source is newer; returns the library's path."""
-    lib, binding = force or _stale(LIB), force or _stale(BINDING)
+    """Compile the library and, beside a torch with CUDA, its torch binding, where a source is newer; returns the
+    library's path."""
+    torch = _torch()
+    lib, binding = force or _stale(LIB), torch is not None and (force or _stale(BINDING))
     if not lib and not binding:
         return LIB
     os.makedirs(OBJ_DIR, exist_ok=True)
     with ThreadPoolExecutor(len(SOURCES) + 1) as pool:
-        bound = pool.submit(_build_binding) if binding else None
+        bound = pool.submit(_build_binding, torch) if binding else None
         if lib:
             objects = list(pool.map(lambda s: _object(s, force, verbose), SOURCES))
             tmp = LIB + ".tmp"
