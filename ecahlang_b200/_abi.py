@@ -14,7 +14,6 @@ from ctypes import c_float, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libecah_sampler.so")
-BINDING_PATH = os.path.join(_HERE, "lib", "_ecah_binding.so")
 
 ABI_VERSION = 2
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
@@ -203,10 +202,11 @@ def binding():
     global _binding
     if _binding is None:
         import torch  # noqa: F401  (the module links torch's libraries)
-        L = lib()
-        if not os.path.exists(BINDING_PATH):
-            raise EcahError(f"{BINDING_PATH} is missing: build it with `python -m ecahlang_b200.build`")
-        loader = importlib.machinery.ExtensionFileLoader("_ecah_binding", BINDING_PATH)
+        from .build import binding_path
+        L, path = lib(), binding_path()
+        if not os.path.exists(path):
+            raise EcahError(f"{path} is missing: build it with `python -m ecahlang_b200.build`")
+        loader = importlib.machinery.ExtensionFileLoader("_ecah_binding", path)
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_ecah_binding", loader))
         loader.exec_module(module)
         module.bind(EcahError, *(ctypes.cast(f, c_void_p).value for f in (

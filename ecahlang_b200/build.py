@@ -2,13 +2,14 @@
 
 The library is plain CUDA C++ behind an ``extern "C"`` ABI
 (include/ecah_sampler.h); it links the CUDA runtime statically and has no
-torch dependency, so any FFI (ctypes here) can load it.  ``lib/_ecah_binding.so``
+torch dependency, so any FFI (ctypes here) can load it.  ``lib/_ecah_binding.*.so``
 is the torch side of the newer entry points: a CPython module that checks
 tensors and calls the library; it is left out where there is no torch with CUDA.
 """
 from __future__ import annotations
 
 import glob
+import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -21,7 +22,19 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIB_DIR, "libecah_sampler.so")
-BINDING = os.path.join(LIB_DIR, "_ecah_binding.so")
+
+
+def binding_path() -> str:
+    """The torch binding's file.  It depends on the ABIs of the interpreter and
+    of torch, so it carries both names, and one built for others is not taken."""
+    try:
+        torch = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        torch = "unknown"
+    return os.path.join(LIB_DIR, f"_ecah_binding.{sysconfig.get_config_var('SOABI')}.torch-{torch}.so")
+
+
+BINDING = binding_path()
 OBJ_DIR = os.path.join(LIB_DIR, "build")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",

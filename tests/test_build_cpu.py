@@ -49,3 +49,19 @@ def test_the_binding_builds_beside_a_cuda_torch(monkeypatch, tmp_path, steps):
     _torch_at(monkeypatch, str(tmp_path / "torch" / "__init__.py"))
     B.build(force=True)
     assert sorted(steps) == sorted([*B.SOURCES, "library", "binding"])
+
+
+def test_a_binding_of_another_torch_or_interpreter_is_not_taken(monkeypatch):
+    """Its file name holds both versions, and loading looks for the one that building makes."""
+    import torch
+    from ecahlang_b200 import _abi
+    B.build()
+    assert B.BINDING == B.binding_path() and not B._stale(B.BINDING)
+    here = os.path.basename(B.BINDING)
+    assert B.sysconfig.get_config_var("SOABI") in here and torch.__version__ in here
+    monkeypatch.setattr(B.importlib.metadata, "version", lambda name: "9.9.9")
+    other = B.binding_path()
+    assert other != B.BINDING and B._stale(other)
+    monkeypatch.setattr(_abi, "_binding", None)
+    with pytest.raises(_abi.EcahError, match="torch-9.9.9.so is missing"):
+        _abi.binding()
