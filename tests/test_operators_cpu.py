@@ -179,3 +179,18 @@ def test_manager_logprobs_checks_a_host_row_index():
     for bad in ([0, 5], [-1], torch.tensor([7]), range(4, 6)):
         with pytest.raises(IndexError, match="row_index"):
             m.logprobs(x, None, row_index=bad, tempered=True)
+
+
+@pytest.mark.parametrize("dtype,kv,run", [(torch.float16, False, 16), (torch.bfloat16, False, 64),
+                                          (torch.bfloat16, True, 16)])
+def test_long_decode_tolerance_sees_a_lost_run_of_keys(dtype, kv, run):
+    """Values of `run` neighbouring keys left out of the oracle's sum exceed the tolerance, wherever they lie."""
+    from decode_util import long_cache, long_reference
+    g = torch.Generator().manual_seed(1)
+    n = 20000
+    q = (torch.randn(4, 64, generator=g) * 1.5).to(dtype)
+    cache = long_cache(n, 16, 2, 64, dtype, kv, g, "cpu")
+    want, _, tol = long_reference(q, n, *cache, dtype)
+    for at in (0, 7000, 12345, n - run):
+        got, _, _ = long_reference(q, n, *cache, dtype, lost=slice(at, at + run))
+        assert (((got - want).abs() / tol).amax(-1) > 1).all(), at

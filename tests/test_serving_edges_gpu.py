@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from decode_util import long_cache, long_reference
 from ecahlang_b200.logprobs import TokenLogprobs, launch, new_workspace
 from ecahlang_b200.manager import SamplingManager
 from ecahlang_b200.paged import PagedAttention
@@ -140,3 +141,40 @@ def test_logprobs_without_a_temperature(dtype, V):
     assert torch.isnan(got.logprobs[0]).all() and torch.isnan(got.entropy[0]) and torch.isnan(got.top_logprobs[0]).all()
     assert got.top_ids[0].tolist() == [-1] * 3
     assert got.top_ids[1].tolist() == [1, 3, 0] and torch.isfinite(got.logprobs[1]).all()
+
+
+@pytest.mark.parametrize("dtype,kv", KINDS)
+@pytest.mark.parametrize("Hq,Hk,D,lengths,listed", [
+    (16, 2, 128, [40000], 0), (16, 2, 128, [5, 70001, 1, 0], 0), (32, 8, 128, [40001, 33, 39000, 3001], 0),
+    (40, 2, 64, [30011, 700], 0), (8, 4, 192, [25000, 9], 100_000), (34, 2, 256, [20001, 64], 100_000),
+    (12, 6, 96, [1500, 35000], 100_000)])
+def test_decode_long_contexts(dtype, kv, Hq, Hk, D, lengths, listed):
+    """Work divided over the blocks and joined, at a tolerance that a lost run of keys exceeds."""
+    g = torch.Generator(device=DEV).manual_seed(D + Hq)
+    page = 16
+    parts = [long_cache(n, page, Hk, D, dtype, kv is not None, g, DEV) for n in lengths if n]
+    q = (torch.randn(len(lengths), Hq, D, generator=g, device=DEV) * 1.5).to(dtype)
+    cat = lambda ts: torch.cat([t.view(torch.uint8) for t in ts]).view(ts[0].dtype) if ts[0] is not None else None   # noqa: E731
+    k, v, ks, vs = (cat([p[i] for p in parts]) for i in range(4))
+    # pages in a scattered order
+    order = torch.randperm(k.shape[0], generator=g, device=DEV)
+    place = torch.empty_like(order)
+    place[order] = torch.arange(len(order), device=DEV)
+    k, v = (c.view(torch.uint8)[order].view(c.dtype) for c in (k, v))
+    if ks is not None:
+        ks, vs = ks[order].contiguous(), vs[order].contiguous()
+    counts = [-(-n // page) for n in lengths]
+    indptr = torch.tensor([0] + counts).cumsum(0).to(torch.int32).to(DEV)
+    indices = torch.cat([place.to(torch.int32), torch.zeros(listed, dtype=torch.int32, device=DEV)])
+    last = torch.tensor([(n - 1) % page + 1 if n else 0 for n in lengths], dtype=torch.int32, device=DEV)
+    out, lse = PagedAttention(Hq, Hk, D, page, dtype, kv_dtype=kv).decode(
+        q, indptr, indices, last, k, v, k_scale=ks, v_scale=vs, return_lse=True)
+    at = 0
+    for b, n in enumerate(lengths):
+        if not n:
+            assert (out[b] == 0).all() and (lse[b] == -math.inf).all()
+            continue
+        want, wlse, tol = long_reference(q[b], n, *parts[at], dtype)
+        at += 1
+        assert ((out[b].double() - want).abs() <= tol).all(), float(((out[b].double() - want).abs() / tol).max())
+        assert ((lse[b].double() - wlse).abs() <= 2e-5 + 4e-6 * 16).all()
