@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
   unsigned char* ring_p = smem + warp * S::kWarpBytes;
   const uint32_t bars = smem_u32(s_bar[warp]);
   uint32_t phase = 0;                            // of each stage's barrier
-  bool failed = false;                           // this warp's wait ran out: it copies nothing more
+  bool failed = false;                           // a wait ran out: the warp copies nothing more
   if (BULK && lane == 0) {
     for (int i = 0; i < S::kStages; ++i) bar_init(bars + 8 * i);
     fence_copies();
@@ -526,18 +526,18 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
       l[x][0] = l[x][1] = 0.0f;
     }
 
-    for (int i = 0; i < steps; ++i) {
+    bool stop = false;
+    for (int i = 0; i < steps && !stop; ++i) {
       issue(i + S::kStages - 1);
       if (E4M3 || !BULK) cp_wait<S::kStages - 1>();
       if (BULK) {
-        if (!__all_sync(0xFFFFFFFFu, bar_wait(bars + 8 * (i % S::kStages), phase >> (i % S::kStages) & 1u, P.tries))) {
+        if (!bar_wait(bars + 8 * (i % S::kStages), phase >> (i % S::kStages) & 1u, P.tries)) {
           // Give up: wait again for the copies in flight, so that none lands in the
           // results or after the block has ended.
           for (int k = i; k < min(steps, i + S::kStages); ++k)
             bar_wait(bars + 8 * (k % S::kStages), phase >> (k % S::kStages) & 1u, kTries);
           failed = true;
-          if (lane == 0) s_failed = 1;
-          break;
+          s_failed = 1;
         }
         phase ^= 1u << (i % S::kStages);
       }
@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
           }
         }
         float top[NT][2];
-        bool above = false;
+        bool above = BULK && failed;                          // of one lane: told to all by the vote below
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
           top[x][0] = fmaxf(s[x][0], s[x][2]);
@@ -621,6 +621,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
           above |= top[x][0] > m[x][0] + (kLazy + lift) || top[x][1] > m[x][1] + (kLazy + lift);
         }
         if (__any_sync(0xFFFFFFFFu, above)) {
+          if (BULK) stop = __any_sync(0xFFFFFFFFu, failed);
 #pragma unroll
           for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -687,6 +688,7 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
       __syncwarp();
     }
     if (E4M3 || !BULK) cp_wait<0>();
+    if (BULK) failed = __any_sync(0xFFFFFFFFu, failed);       // also where the last slice had no key
     __syncwarp();
 
     // ---- join the warps: each leaves (m, l, o) in its ring
