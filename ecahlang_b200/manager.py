@@ -124,7 +124,7 @@ class SamplingManager:
         self.sampling_pres_gpu = torch.zeros(B, dtype=torch.float32, device=dev)
         self.sampling_slot_gpu = torch.full((B,), -1, dtype=torch.int32, device=dev)
         self.sampling_out = torch.zeros(B, dtype=torch.int32, device=dev)
-        self._workspace = self._scorer = self._scorer_workspace = None
+        self._workspace = None
         if dev.type == "cuda":
             self._sample_workspace()
             self._logprob_workspace()
