@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -217,6 +218,12 @@ void rows(const at::Tensor& t, const char* name, int64_t tokens, int64_t heads, 
     refuse(std::string(name) + ": rows of head_dim must be contiguous and 16-byte aligned");
 }
 
+// Blocks write rows in no order: none may lie on another.
+void need_apart(const at::Tensor& t, const char* name) {
+  if (t.numel() && at::has_internal_overlap(t) == at::MemOverlap::Yes)
+    refuse(std::string(name) + ": rows to be written share memory (an expanded tensor)");
+}
+
 // What a PagedAttention was made for: (num_qo_heads, num_kv_heads, head_dim,
 // page_size, e4m3, max_batch, dtype code), or None.
 struct Made {
@@ -309,6 +316,8 @@ PyObject* append(PyObject*, PyObject* const* raw, Py_ssize_t n) {
     const Made made = made_for(raw[17]);
     fill_cache(a.cache, type, dev, *in.tensor(7, "k_cache"), *in.tensor(8, "v_cache"), in.tensor(9, "k_scale", true),
                in.tensor(10, "v_scale", true), *in.tensor(5, "kv_indptr"), *in.tensor(6, "kv_indices"), made);
+    need_apart(*in.tensor(7, "k_cache"), "k_cache");
+    need_apart(*in.tensor(8, "v_cache"), "v_cache");
     const int64_t heads = a.cache.num_kv_heads, D = a.cache.head_dim;
     if (k.dim() != 3) refuse("k must be [T, num_kv_heads, head_dim], got " + shape_of(k));
     const int64_t T = k.size(0);
@@ -324,6 +333,7 @@ PyObject* append(PyObject*, PyObject* const* raw, Py_ssize_t n) {
       rows(*q, "q", T, hq, D, type, dev, &a.q_token_stride, &a.q_head_stride);
       out = given ? *given : empty({T, hq, D}, type, dev);
       rows(out, "q_out", T, hq, D, type, dev, &a.qo_token_stride, &a.qo_head_stride);
+      need_apart(out, "q_out");
       a.q = q->data_ptr();
       a.q_out = out.data_ptr();
       a.num_qo_heads = static_cast<int32_t>(hq);
@@ -383,6 +393,7 @@ PyObject* decode(PyObject*, PyObject* const* raw, Py_ssize_t n) {
     const at::Tensor* given = in.tensor(10, "out", true);
     at::Tensor out = given ? *given : empty({B, hq, D}, type, dev);
     rows(out, "out", B, hq, D, type, dev, &a.out_token_stride, &a.out_head_stride);
+    need_apart(out, "out");
     at::Tensor lse;
     const bool new_lse = raw[11] == Py_True;
     if (new_lse) lse = empty({B, hq}, at::kFloat, dev);

@@ -178,3 +178,27 @@ def test_decode_long_contexts(dtype, kv, Hq, Hk, D, lengths, listed):
         at += 1
         assert ((out[b].double() - want).abs() <= tol).all(), float(((out[b].double() - want).abs() / tol).max())
         assert ((lse[b].double() - wlse).abs() <= 2e-5 + 4e-6 * 16).all()
+
+
+def test_expanded_tensors_are_read_but_not_written():
+    """Rows that share memory serve as inputs; as outputs, whose rows are written in no order, they are refused."""
+    att = PagedAttention(8, 2, 64, 16, torch.float16, max_batch=4)
+    k, v, _, _ = att.new_cache(3)
+    t = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)   # noqa: E731
+    one = torch.randn(1, 1, 64, device=DEV).half()
+    q, new = one.expand(4, 8, 64), one.expand(4, 2, 64)
+    place = (t(0, 1, 2, 3), t(0, 0, 0, 0), t(0, 1, 1, 1, 1), t(2))
+    got = att.append(q, new, new, *place, k, v)
+    assert torch.equal(got, q) and torch.equal(k[2, :4], new) and torch.equal(v[2, :4], new)
+    for bad in (dict(q_out=torch.empty_like(one).expand(4, 8, 64)), dict(q_out=torch.empty(4, 1, 64, device=DEV).half().expand(4, 8, 64))):
+        with pytest.raises(RuntimeError, match="share memory"):
+            att.append(q, new, new, *place, k, v, **bad)
+    for bad in ((k[:1].expand(3, 16, 2, 64), v), (k, v[:, :, :1].expand(3, 16, 2, 64)), (k[:, :1].expand(3, 16, 2, 64), v)):
+        with pytest.raises(RuntimeError, match="share memory"):
+            att.append(q, new, new, *place, *bad)
+    last = t(4, 0, 0, 0)
+    out = att.decode(q, place[2], place[3], last, k, v)
+    shared = att.decode(q, place[2], place[3], last, k[:, :, :1].expand(3, 16, 2, 64), v[:, :, :1].expand(3, 16, 2, 64))
+    assert torch.equal(out, shared)
+    with pytest.raises(RuntimeError, match="share memory"):
+        att.decode(q, place[2], place[3], last, k, v, out=torch.empty_like(one).expand(4, 8, 64))
