@@ -7,7 +7,6 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -220,8 +219,8 @@ void rows(const at::Tensor& t, const char* name, int64_t tokens, int64_t heads, 
 
 // Blocks write rows in no order: none may lie on another.
 void need_apart(const at::Tensor& t, const char* name) {
-  if (t.numel() && at::has_internal_overlap(t) == at::MemOverlap::Yes)
-    refuse(std::string(name) + ": rows to be written share memory (an expanded tensor)");
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) == 0) refuse(std::string(name) + ": rows to be written share memory (an expanded tensor)");
 }
 
 // What a PagedAttention was made for: (num_qo_heads, num_kv_heads, head_dim,
