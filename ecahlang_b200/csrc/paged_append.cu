@@ -21,8 +21,8 @@ namespace append {
 // token's table row; with few tokens one head a group spreads over more warps.
 //
 // Measured on one B200, device time of graph replays: 8192 tokens of 32/8 heads of
-// 128 with norm and rotation into a bf16 cache 37.5 us (5.4 TB/s), 128 tokens into
-// an e4m3 cache 2.9 us, one token 2.2 us (a launch).
+// 128 with norm and rotation into a bf16 cache 37.8 us (5.4 TB/s), into an e4m3 cache
+// 42.9 us (4.3 TB/s), 128 tokens into an e4m3 cache 3.4 us, one token 2.1 us (a launch).
 
 constexpr int kT = 64;               // 8192 tokens: 37.5 us, with 128 threads 37.8, with 256 39.3
 constexpr int kMany = 2;             // with 4 38.7 us, with 6 43.2

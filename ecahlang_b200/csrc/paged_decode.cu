@@ -36,9 +36,10 @@ namespace decode {
 // while streaming).
 //
 // Measured on one B200, device time of graph replays: 4 requests of 100 001 to 131 072
-// tokens, 32/8 heads of 128, bf16 300 us (6.5 TB/s), the same over an e4m3 cache 172 us
-// (5.9 TB/s); 64 requests of 1 to 16 384 tokens over an e4m3 cache 57 us (4.7 TB/s); 128
-// requests of 128 to 512 tokens, 16/2 heads, f16 14.0 us; one request of 512 9.1 us.
+// tokens, 32/8 heads of 128, bf16 302 us (6.5 TB/s), the same over an e4m3 cache 178 us
+// (5.7 TB/s), with heads of 64 and 96 in bf16 174 and 258 us (5.6 TB/s); 64 requests of 1 to
+// 16 384 tokens over an e4m3 cache 57 us (4.7 TB/s); 128 requests of 128 to 512 tokens,
+// 16/2 heads, f16 13.7 us; one request of 512 9.2 us.
 // What bounds the last three: finding the share (1.3 us), the first pages and rows (2
 // us), and joining (1.5 us a block, 5 us where the item was divided).
 
@@ -831,11 +832,13 @@ struct Variant {
 // BULK: rows by the copy engine, for 16-bit heads of 128 and 192 where there is much
 // to stream.  It starts a copy about every 10 clocks an SM, at 256 bytes more than HBM
 // brings, and leaves the threads free.  4 requests of 100 001 to 131 072 tokens, 32/8
-// heads: 300 us against 321 with heads of 128, 454 against 495 with 192.  Elsewhere
+// heads: 302 us against 321 with heads of 128, 454 against 495 with 192.  Elsewhere
 // the threads' copies are better: shorter rows starve (128 bytes: 3.4 TB/s), rows of 256
 // in 8 bits with their conversions take 430 us against 339, heads of 256 leave room for
-// one block (711 against 657), and a block with little to do waits longer for its 128
-// copies (128 requests of up to 512 tokens: 18.9 us against 14).
+// one block (711 against 638), and a block with little to do waits longer for its 128
+// copies (128 requests of up to 512 tokens: 18.6 us against 13.7).  The rule goes by the
+// pages listed, which is all that the host knows: a list with room for much more than the
+// requests hold, as a captured step keeps one, takes the copy engine for short requests too.
 template <int DT, bool E4M3, int D, int NT>
 static Variant variant_of(bool bulk) {
   constexpr bool kCan = !E4M3 && (D == 128 || D == 192);

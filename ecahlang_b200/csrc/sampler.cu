@@ -192,7 +192,7 @@ const char* ecah_status_string(int s) {
     case ECAH_ERR_NULL: return "a required pointer is NULL";
     case ECAH_ERR_DTYPE: return "unsupported dtype";
     case ECAH_ERR_SHAPE: return "batch/vocab/row_stride out of range";
-    case ECAH_ERR_WORKSPACE: return "workspace missing or too small";
+    case ECAH_ERR_WORKSPACE: return "workspace missing, too small or misaligned";
     case ECAH_ERR_LAUNCH: return "CUDA launch failed";
     case ECAH_ERR_ABI: return "abi_version mismatch";
     default: return "unknown status";
