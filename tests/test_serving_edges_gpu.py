@@ -202,3 +202,22 @@ def test_expanded_tensors_are_read_but_not_written():
     assert torch.equal(out, shared)
     with pytest.raises(RuntimeError, match="share memory"):
         att.decode(q, place[2], place[3], last, k, v, out=torch.empty_like(one).expand(4, 8, 64))
+
+
+def test_manager_keeps_the_workspace_that_a_captured_bucket_uses():
+    """The sampling buffers are made again, larger, between the capture and a replay."""
+    V = 151936
+    x = torch.randn(2, V, generator=torch.Generator(device=DEV).manual_seed(5), device=DEV).half()
+    ids = torch.tensor([7, 9], dtype=torch.int32, device=DEV)
+    m = SamplingManager(V, seq_lens=8, dtype=torch.float16, seed=1)
+    m.init_sampling_buffers(2)
+    m.logprobs(x, ids, 5)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = m.logprobs(x, ids, 5)
+    m.init_sampling_buffers(16)
+    n = TokenLogprobs(8, torch.float16).workspace.numel()
+    kept = [torch.empty(n, dtype=torch.uint8, device=DEV).fill_(0x5A) for _ in range(8)]
+    graph.replay()
+    want = TokenLogprobs(V, torch.float16)(x, ids, top_n=5)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and all((t == 0x5A).all() for t in kept)
