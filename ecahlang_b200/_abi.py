@@ -31,7 +31,9 @@ EXPORTS = ("ecah_sampler_abi_version", "ecah_status_string", "ecah_sampler_works
            "ecah_vp_ipc_alloc", "ecah_vp_ipc_open", "ecah_vp_ipc_close", "ecah_vp_ipc_free",
            "ecah_quotient_mismatches", "ecah_vp_reset", "ecah_vp_dist_pass",
            "ecah_token_logprobs_workspace_bytes", "ecah_token_logprobs", "ecah_paged_append",
-           "ecah_paged_decode_workspace_bytes", "ecah_paged_decode", "ecah_paged_decode_bounded")
+           "ecah_paged_decode_workspace_bytes", "ecah_paged_decode", "ecah_paged_decode_bounded",
+           "ecah_paged_prefill_workspace_bytes", "ecah_paged_prefill", "ecah_paged_copy",
+           "ecah_verify_drafts_workspace_bytes", "ecah_verify_drafts")
 IPC_HANDLE_BYTES = 64
 
 
@@ -120,6 +122,41 @@ class DecodeArgs(ctypes.Structure):
     ]
 
 
+class PrefillArgs(ctypes.Structure):
+    """Mirror of ``struct ecah_prefill_args``."""
+    _fields_ = [
+        ("abi_version", c_int32), ("dtype", c_int32), ("tokens", c_int32), ("num_qo_heads", c_int32),
+        ("sm_scale", c_float), ("causal", c_int32),
+        ("q", c_void_p), ("q_token_stride", c_int64), ("q_head_stride", c_int64),
+        ("out", c_void_p), ("out_token_stride", c_int64), ("out_head_stride", c_int64),
+        ("lse", c_void_p), ("qo_indptr", c_void_p), ("kv_last_page_len", c_void_p), ("cache", KVCache),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class CopyArgs(ctypes.Structure):
+    """Mirror of ``struct ecah_copy_args``."""
+    _fields_ = [
+        ("abi_version", c_int32), ("kv_dtype", c_int32), ("num_pages", c_int32), ("page_size", c_int32),
+        ("num_kv_heads", c_int32), ("head_dim", c_int32), ("layers", c_int32), ("pairs", c_int32),
+        ("k_page_stride", c_int64), ("k_slot_stride", c_int64), ("k_head_stride", c_int64),
+        ("v_page_stride", c_int64), ("v_slot_stride", c_int64), ("v_head_stride", c_int64),
+        ("k_caches", c_void_p), ("v_caches", c_void_p), ("k_scales", c_void_p), ("v_scales", c_void_p),
+        ("src", c_void_p), ("dst", c_void_p), ("tokens", c_void_p),
+    ]
+
+
+class VerifyArgs(ctypes.Structure):
+    """Mirror of ``struct ecah_verify_args``."""
+    _fields_ = [
+        ("abi_version", c_int32), ("dtype", c_int32), ("batch", c_int32), ("drafts", c_int32), ("vocab", c_int32),
+        ("target", c_void_p), ("target_batch_stride", c_int64), ("target_row_stride", c_int64),
+        ("draft", c_void_p), ("draft_batch_stride", c_int64), ("draft_row_stride", c_int64),
+        ("draft_ids", c_void_p), ("num_drafts", c_void_p), ("uniforms", c_void_p),
+        ("tokens", c_void_p), ("accepted", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
 class EcahError(RuntimeError):
     pass
 
@@ -187,6 +224,16 @@ def lib():
         L.ecah_paged_decode.argtypes = [ctypes.POINTER(DecodeArgs), c_void_p]
         L.ecah_paged_decode_bounded.restype = c_int32
         L.ecah_paged_decode_bounded.argtypes = [ctypes.POINTER(DecodeArgs), c_int32, c_void_p]
+        L.ecah_paged_prefill_workspace_bytes.restype = c_size_t
+        L.ecah_paged_prefill_workspace_bytes.argtypes = [c_int32]
+        L.ecah_paged_prefill.restype = c_int32
+        L.ecah_paged_prefill.argtypes = [ctypes.POINTER(PrefillArgs), c_void_p]
+        L.ecah_paged_copy.restype = c_int32
+        L.ecah_paged_copy.argtypes = [ctypes.POINTER(CopyArgs), c_void_p]
+        L.ecah_verify_drafts_workspace_bytes.restype = c_size_t
+        L.ecah_verify_drafts_workspace_bytes.argtypes = [c_int32]
+        L.ecah_verify_drafts.restype = c_int32
+        L.ecah_verify_drafts.argtypes = [ctypes.POINTER(VerifyArgs), c_void_p]
         if L.ecah_sampler_abi_version() != ABI_VERSION:
             raise EcahError("libecah_sampler.so ABI version mismatch")
         _lib = L
@@ -197,7 +244,7 @@ _binding = None
 
 
 def binding():
-    """The torch binding of the log-probability and paged-cache entry points,
+    """The torch binding of the log-probability, paged-cache and draft entry points,
     loaded once and given the library's functions; raise if it is absent."""
     global _binding
     if _binding is None:
@@ -210,7 +257,8 @@ def binding():
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_ecah_binding", loader))
         loader.exec_module(module)
         module.bind(EcahError, *(ctypes.cast(f, c_void_p).value for f in (
-            L.ecah_token_logprobs, L.ecah_paged_append, L.ecah_paged_decode, L.ecah_status_string)))
+            L.ecah_token_logprobs, L.ecah_paged_append, L.ecah_paged_decode, L.ecah_paged_prefill, L.ecah_paged_copy,
+            L.ecah_verify_drafts, L.ecah_status_string)))
         _binding = module
     return _binding
 

@@ -39,7 +39,8 @@ OBJ_DIR = os.path.join(LIB_DIR, "build")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
          "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr"]
-SOURCES = ["sampler.cu", "noalloc.cu", "diag.cu", "logprobs.cu", "paged_append.cu", "paged_decode.cu"]
+SOURCES = ["sampler.cu", "noalloc.cu", "diag.cu", "logprobs.cu", "paged_append.cu", "paged_decode.cu",
+           "paged_prefill.cu", "paged_copy.cu", "drafts.cu"]
 
 
 def _nvcc() -> str:

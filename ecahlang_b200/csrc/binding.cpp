@@ -1,4 +1,4 @@
-// Python binding of the log-probability and paged-cache entry points
+// Python binding of the log-probability, paged-cache and draft entry points
 // (include/ecah_sampler.h): checks torch tensors, allocates outputs, fills the
 // argument structs and launches on the current torch stream.  A call costs a few
 // microseconds of host time, where the same checks in Python cost more than the
@@ -15,6 +15,7 @@
 #include <cmath>
 #include <stdexcept>
 #include <string>
+#include <vector>
 
 #include "ecah_sampler.h"
 
@@ -25,6 +26,9 @@ PyObject* g_error = nullptr;
 decltype(&ecah_token_logprobs) g_logprobs = nullptr;
 decltype(&ecah_paged_append) g_append = nullptr;
 decltype(&ecah_paged_decode) g_decode = nullptr;
+decltype(&ecah_paged_prefill) g_prefill = nullptr;
+decltype(&ecah_paged_copy) g_copy = nullptr;
+decltype(&ecah_verify_drafts) g_verify = nullptr;
 decltype(&ecah_status_string) g_status_string = nullptr;
 
 [[noreturn]] void refuse(const std::string& why) { throw std::runtime_error(why); }
@@ -238,8 +242,9 @@ Made made_for(PyObject* o) {
   return Made{v[0], v[1], v[2], v[3], v[4], v[5], v[6]};
 }
 
-void fill_cache(ecah_kv_cache& c, at::ScalarType type, at::Device dev, const at::Tensor& k, const at::Tensor& v,
-                const at::Tensor* ks, const at::Tensor* vs, const at::Tensor& indptr, const at::Tensor& indices, const Made& made) {
+// One layer's cache, without page lists.
+void fill_layer(ecah_kv_cache& c, at::ScalarType type, at::Device dev, const at::Tensor& k, const at::Tensor& v,
+                const at::Tensor* ks, const at::Tensor* vs, const Made& made) {
   if (k.dim() != 4 || v.sizes() != k.sizes()) refuse("k_cache and v_cache must be [num_pages, page_size, num_kv_heads, head_dim]");
   const at::ScalarType kv = k.scalar_type();
   const bool e4m3 = kv == at::kFloat8_e4m3fn;
@@ -277,17 +282,22 @@ void fill_cache(ecah_kv_cache& c, at::ScalarType type, at::Device dev, const at:
     if (ks || vs) refuse("a cache in the model dtype takes no scales");
     c.kv_dtype = kv == at::kHalf ? ECAH_DTYPE_F16 : ECAH_DTYPE_BF16;
   }
-  const int64_t n = indptr.numel();
-  if (n < 1 || n > INT32_MAX) refuse("kv_indptr must have batch + 1 entries");
-  need(indptr, "kv_indptr", at::kInt, n, dev);
-  need(indices, "kv_indices", at::kInt, indices.numel(), dev);
   c.num_pages = static_cast<int32_t>(pages);
   c.page_size = static_cast<int32_t>(page);
   c.num_kv_heads = static_cast<int32_t>(heads);
   c.head_dim = static_cast<int32_t>(D);
-  c.batch = static_cast<int32_t>(n - 1);
   c.k_cache = k.data_ptr();
   c.v_cache = v.data_ptr();
+}
+
+void fill_cache(ecah_kv_cache& c, at::ScalarType type, at::Device dev, const at::Tensor& k, const at::Tensor& v,
+                const at::Tensor* ks, const at::Tensor* vs, const at::Tensor& indptr, const at::Tensor& indices, const Made& made) {
+  fill_layer(c, type, dev, k, v, ks, vs, made);
+  const int64_t n = indptr.numel();
+  if (n < 1 || n > INT32_MAX) refuse("kv_indptr must have batch + 1 entries");
+  need(indptr, "kv_indptr", at::kInt, n, dev);
+  need(indices, "kv_indices", at::kInt, indices.numel(), dev);
+  c.batch = static_cast<int32_t>(n - 1);
   c.kv_indptr = indptr.data_ptr<int32_t>();
   c.kv_indices = indices.data_ptr<int32_t>();
   c.num_indices = indices.numel();
@@ -420,12 +430,205 @@ PyObject* decode(PyObject*, PyObject* const* raw, Py_ssize_t n) {
   });
 }
 
-// bind(error class, addresses of ecah_token_logprobs, ecah_paged_append,
-// ecah_paged_decode and ecah_status_string)
-PyObject* bind(PyObject*, PyObject* const* raw, Py_ssize_t n) {
+// q, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, k_cache, v_cache, workspace,
+// k_scale, v_scale, causal, sm_scale (None: 1 / sqrt(head_dim)), out, lse (True: allocate), layout
+PyObject* prefill(PyObject*, PyObject* const* raw, Py_ssize_t n) {
+  if (!count_is(n, 15)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const Args in{raw, n};
+    const at::Tensor& q = *in.tensor(0, "q");
+    const at::ScalarType type = q.scalar_type();
+    ecah_prefill_args a = {};
+    a.dtype = half_dtype(type, "prefill");
+    if (!q.is_cuda()) refuse("prefill needs CUDA tensors (there is no CPU path)");
+    const at::Device dev = q.device();
+    const Made made = made_for(raw[14]);
+    fill_cache(a.cache, type, dev, *in.tensor(5, "k_cache"), *in.tensor(6, "v_cache"), in.tensor(8, "k_scale", true),
+               in.tensor(9, "v_scale", true), *in.tensor(2, "kv_indptr"), *in.tensor(3, "kv_indices"), made);
+    const int64_t heads = a.cache.num_kv_heads, D = a.cache.head_dim, B = a.cache.batch;
+    check_query(q, made, a.dtype);
+    if (q.dim() != 3 || q.size(1) < 1 || q.size(1) % heads || q.size(1) > INT32_MAX)
+      refuse("q must be [T, num_qo_heads, " + std::to_string(D) + "] with num_qo_heads a multiple of " + std::to_string(heads) + ", got " + shape_of(q));
+    if (made.hq >= 0 && B > made.batch) refuse(std::to_string(B) + " requests, max_batch is " + std::to_string(made.batch));
+    const int64_t T = q.size(0), hq = q.size(1);
+    if (T > INT32_MAX) refuse("too many tokens");
+    rows(q, "q", T, hq, D, type, dev, &a.q_token_stride, &a.q_head_stride);
+    const at::Tensor* given = in.tensor(12, "out", true);
+    at::Tensor out = given ? *given : empty({T, hq, D}, type, dev);
+    rows(out, "out", T, hq, D, type, dev, &a.out_token_stride, &a.out_head_stride);
+    need_apart(out, "out");
+    at::Tensor lse;
+    const bool new_lse = raw[13] == Py_True;
+    if (new_lse) lse = empty({T, hq}, at::kFloat, dev);
+    else if (const at::Tensor* t = in.tensor(13, "lse", true)) lse = *t;
+    if (lse.defined()) {
+      need(lse, "lse", at::kFloat, T * hq, dev);
+      a.lse = lse.data_ptr<float>();
+    }
+    const at::Tensor &qptr = *in.tensor(1, "qo_indptr"), &last = *in.tensor(4, "kv_last_page_len");
+    need(qptr, "qo_indptr", at::kInt, B + 1, dev);
+    need(last, "kv_last_page_len", at::kInt, B, dev);
+    const at::Tensor& ws = *in.tensor(7, "workspace");
+    a.workspace = const_cast<void*>(checked_workspace(ws, dev));
+    a.workspace_bytes = static_cast<size_t>(ws.numel());
+    a.causal = in.truth(10);
+    a.sm_scale = raw[11] == Py_None ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(D))) : static_cast<float>(in.real(11));
+    if (!(a.sm_scale > 0.0f) || std::isinf(a.sm_scale)) refuse("sm_scale must be positive and finite");
+    a.abi_version = ECAH_SAMPLER_ABI_VERSION;
+    a.tokens = static_cast<int32_t>(T);
+    a.num_qo_heads = static_cast<int32_t>(hq);
+    a.q = q.data_ptr();
+    a.out = out.data_ptr();
+    a.qo_indptr = qptr.data_ptr<int32_t>();
+    a.kv_last_page_len = last.data_ptr<int32_t>();
+    run(g_prefill, a, dev, "ecah_paged_prefill");
+    PyObject* o = given ? Py_NewRef(raw[12]) : THPVariable_Wrap(out);
+    if (raw[13] == Py_None) return o;
+    return Py_BuildValue("(NN)", o, new_lse ? THPVariable_Wrap(lse) : Py_NewRef(raw[13]));
+  });
+}
+
+// src, dst, tokens (or None), caches: a sequence of (k_cache, v_cache, k_scale, v_scale), layout
+PyObject* copy_pages(PyObject*, PyObject* const* raw, Py_ssize_t n) {
   if (!count_is(n, 5)) return nullptr;
-  void* at[4];
-  for (int i = 0; i < 4; ++i) {
+  return guarded([&]() -> PyObject* {
+    const Args in{raw, n};
+    const at::Tensor &src = *in.tensor(0, "src"), &dst = *in.tensor(1, "dst");
+    if (!src.is_cuda()) refuse("copy_pages needs CUDA tensors (there is no CPU path)");
+    const at::Device dev = src.device();
+    const int64_t pairs = src.numel();
+    if (pairs > INT32_MAX) refuse("too many pairs");
+    need(src, "src", at::kInt, pairs, dev);
+    need(dst, "dst", at::kInt, pairs, dev);
+    ecah_copy_args a = {};
+    if (const at::Tensor* t = in.tensor(2, "tokens", true)) {
+      need(*t, "tokens", at::kInt, pairs, dev);
+      a.tokens = t->data_ptr<int32_t>();
+    }
+    struct Ref {                                             // a new reference, dropped on every way out
+      PyObject* o;
+      ~Ref() { Py_XDECREF(o); }
+    } seq{PySequence_Fast(raw[3], "caches: expected a sequence of (k_cache, v_cache, k_scale, v_scale)")};
+    if (!seq.o) { PyErr_Clear(); refuse("caches: expected a sequence of (k_cache, v_cache, k_scale, v_scale)"); }
+    const Py_ssize_t layers = PySequence_Fast_GET_SIZE(seq.o);
+    const Made made = made_for(raw[4]);
+    std::vector<void*> k(layers), v(layers);
+    std::vector<float*> ks(layers), vs(layers);
+    ecah_kv_cache first = {};
+    for (Py_ssize_t i = 0; i < layers; ++i) {
+      const std::string who = "caches[" + std::to_string(i) + "]";
+      PyObject* item = PySequence_Fast_GET_ITEM(seq.o, i);
+      if (!(PyTuple_Check(item) || PyList_Check(item)) || PySequence_Fast_GET_SIZE(item) != 4)
+        refuse(who + ": expected (k_cache, v_cache, k_scale, v_scale)");
+      const Args c{PySequence_Fast_ITEMS(item), 4};
+      const at::Tensor &kc = *c.tensor(0, "k_cache"), &vc = *c.tensor(1, "v_cache");
+      if (kc.scalar_type() != at::kHalf && kc.scalar_type() != at::kBFloat16 && kc.scalar_type() != at::kFloat8_e4m3fn)
+        refuse(who + ": unsupported cache dtype " + type_name(kc.scalar_type()));
+      need_apart(kc, "k_cache");
+      need_apart(vc, "v_cache");
+      ecah_kv_cache one = {};
+      fill_layer(one, kc.scalar_type(), dev, kc, vc, c.tensor(2, "k_scale", true), c.tensor(3, "v_scale", true), made);
+      if (i == 0) {
+        first = one;
+      } else if (one.kv_dtype != first.kv_dtype || one.num_pages != first.num_pages || one.page_size != first.page_size ||
+                 one.num_kv_heads != first.num_kv_heads || one.head_dim != first.head_dim || one.k_page_stride != first.k_page_stride ||
+                 one.k_slot_stride != first.k_slot_stride || one.k_head_stride != first.k_head_stride ||
+                 one.v_page_stride != first.v_page_stride || one.v_slot_stride != first.v_slot_stride || one.v_head_stride != first.v_head_stride) {
+        refuse(who + ": all layers must have one shape, dtype and set of strides");
+      }
+      k[i] = one.k_cache; v[i] = one.v_cache; ks[i] = one.k_scale; vs[i] = one.v_scale;
+    }
+    if (layers == 0) Py_RETURN_NONE;
+    if (layers > INT32_MAX) refuse("too many layers");
+    a.abi_version = ECAH_SAMPLER_ABI_VERSION;
+    a.kv_dtype = first.kv_dtype;
+    a.num_pages = first.num_pages; a.page_size = first.page_size;
+    a.num_kv_heads = first.num_kv_heads; a.head_dim = first.head_dim;
+    a.layers = static_cast<int32_t>(layers);
+    a.pairs = static_cast<int32_t>(pairs);
+    a.k_page_stride = first.k_page_stride; a.k_slot_stride = first.k_slot_stride; a.k_head_stride = first.k_head_stride;
+    a.v_page_stride = first.v_page_stride; a.v_slot_stride = first.v_slot_stride; a.v_head_stride = first.v_head_stride;
+    a.k_caches = k.data(); a.v_caches = v.data();
+    if (first.kv_dtype == ECAH_KV_E4M3) { a.k_scales = ks.data(); a.v_scales = vs.data(); }
+    a.src = src.data_ptr<int32_t>();
+    a.dst = dst.data_ptr<int32_t>();
+    run(g_copy, a, dev, "ecah_paged_copy");
+    Py_RETURN_NONE;
+  });
+}
+
+// target, draft_ids, uniforms, workspace, draft (or None), num_drafts, tokens, accepted,
+// vocab (-1: any), max_batch (-1: any)
+PyObject* verify(PyObject*, PyObject* const* raw, Py_ssize_t n) {
+  if (!count_is(n, 10)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const Args in{raw, n};
+    const at::Tensor& p = *in.tensor(0, "target_probs");
+    if (p.dim() != 3) refuse("target_probs must be [B, N + 1, V], got " + shape_of(p));
+    ecah_verify_args a = {};
+    switch (p.scalar_type()) {
+      case at::kHalf: a.dtype = ECAH_DTYPE_F16; break;
+      case at::kBFloat16: a.dtype = ECAH_DTYPE_BF16; break;
+      case at::kFloat: a.dtype = ECAH_DTYPE_F32; break;
+      default: refuse("unsupported dtype of probabilities " + type_name(p.scalar_type()));
+    }
+    if (!p.is_cuda()) refuse("target_probs must be a CUDA tensor (there is no CPU path)");
+    const at::Device dev = p.device();
+    const int64_t B = p.size(0), V = p.size(2);
+    if (p.size(1) < 1) refuse("target_probs must have a row after the last draft, got " + shape_of(p));
+    const int64_t N = p.size(1) - 1;
+    const long vocab = in.integer(8), most = in.integer(9);
+    if (vocab >= 0 && V != vocab) refuse("target_probs must be [B, N + 1, " + std::to_string(vocab) + "], got " + shape_of(p));
+    if (most >= 0 && B > most) refuse(std::to_string(B) + " requests, max_batch is " + std::to_string(most));
+    if (V < 1 || V > INT32_MAX || B > INT32_MAX || N > INT32_MAX - 1) refuse("target_probs too large or empty: " + shape_of(p));
+    auto strides = [&](const at::Tensor& t, const char* name, int64_t* b, int64_t* r) {
+      if (t.size(2) > 1 && t.stride(2) != 1) refuse(std::string(name) + ": rows of probabilities must be contiguous");
+      *b = t.size(0) > 1 ? t.stride(0) : 0;
+      *r = t.size(1) > 1 ? t.stride(1) : 0;
+    };
+    strides(p, "target_probs", &a.target_batch_stride, &a.target_row_stride);
+    if (const at::Tensor* q = in.tensor(4, "draft_probs", true)) {
+      if (q->scalar_type() != p.scalar_type() || q->device() != dev)
+        refuse("draft_probs: expected " + type_name(p.scalar_type()) + " on " + dev.str() + ", got " + type_name(q->scalar_type()) + " on " + q->device().str());
+      if (q->dim() != 3 || q->size(0) != B || q->size(1) != N || q->size(2) != V)
+        refuse("draft_probs: expected shape [" + std::to_string(B) + ", " + std::to_string(N) + ", " + std::to_string(V) + "], got " + shape_of(*q));
+      strides(*q, "draft_probs", &a.draft_batch_stride, &a.draft_row_stride);
+      a.draft = N ? q->data_ptr() : nullptr;
+    }
+    const at::Tensor &ids = *in.tensor(1, "draft_ids"), &u = *in.tensor(2, "uniforms");
+    need(ids, "draft_ids", at::kInt, B * N, dev);
+    need(u, "uniforms", at::kFloat, B * (N + 1), dev);
+    if (const at::Tensor* t = in.tensor(5, "num_drafts", true)) {
+      need(*t, "num_drafts", at::kInt, B, dev);
+      a.num_drafts = t->data_ptr<int32_t>();
+    }
+    const at::Tensor& ws = *in.tensor(3, "workspace");
+    a.workspace = const_cast<void*>(checked_workspace(ws, dev));
+    a.workspace_bytes = static_cast<size_t>(ws.numel());
+    at::Tensor tokens = output(in.tensor(6, "tokens", true), "tokens", {B, N + 1}, at::kInt, dev);
+    at::Tensor accepted = output(in.tensor(7, "accepted", true), "accepted", {B}, at::kInt, dev);
+    a.abi_version = ECAH_SAMPLER_ABI_VERSION;
+    a.batch = static_cast<int32_t>(B);
+    a.drafts = static_cast<int32_t>(N);
+    a.vocab = static_cast<int32_t>(V);
+    a.target = p.data_ptr();
+    a.draft_ids = ids.data_ptr<int32_t>();
+    a.uniforms = u.data_ptr<float>();
+    a.tokens = tokens.data_ptr<int32_t>();
+    a.accepted = accepted.data_ptr<int32_t>();
+    run(g_verify, a, dev, "ecah_verify_drafts");
+    return Py_BuildValue("(NN)", THPVariable_Wrap(tokens), THPVariable_Wrap(accepted));
+  });
+}
+
+// bind(error class, addresses of ecah_token_logprobs, ecah_paged_append,
+// ecah_paged_decode, ecah_paged_prefill, ecah_paged_copy, ecah_verify_drafts and
+// ecah_status_string)
+PyObject* bind(PyObject*, PyObject* const* raw, Py_ssize_t n) {
+  constexpr int kEntries = 7;
+  if (!count_is(n, 1 + kEntries)) return nullptr;
+  void* at[kEntries];
+  for (int i = 0; i < kEntries; ++i) {
     at[i] = PyLong_AsVoidPtr(raw[i + 1]);
     if (!at[i]) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "an entry point's address is null");
@@ -437,7 +640,10 @@ PyObject* bind(PyObject*, PyObject* const* raw, Py_ssize_t n) {
   g_logprobs = reinterpret_cast<decltype(g_logprobs)>(at[0]);
   g_append = reinterpret_cast<decltype(g_append)>(at[1]);
   g_decode = reinterpret_cast<decltype(g_decode)>(at[2]);
-  g_status_string = reinterpret_cast<decltype(g_status_string)>(at[3]);
+  g_prefill = reinterpret_cast<decltype(g_prefill)>(at[3]);
+  g_copy = reinterpret_cast<decltype(g_copy)>(at[4]);
+  g_verify = reinterpret_cast<decltype(g_verify)>(at[5]);
+  g_status_string = reinterpret_cast<decltype(g_status_string)>(at[6]);
   Py_RETURN_NONE;
 }
 
@@ -445,6 +651,9 @@ PyMethodDef methods[] = {
     {"logprobs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(logprobs)), METH_FASTCALL, nullptr},
     {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(append)), METH_FASTCALL, nullptr},
     {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(decode)), METH_FASTCALL, nullptr},
+    {"prefill", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefill)), METH_FASTCALL, nullptr},
+    {"copy_pages", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(copy_pages)), METH_FASTCALL, nullptr},
+    {"verify", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(verify)), METH_FASTCALL, nullptr},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

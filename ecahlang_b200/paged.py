@@ -1,13 +1,15 @@
-"""The decode step's paged key-value cache: ``PagedAttention`` (and the
-functions ``append`` and ``decode`` it calls, and the torch custom ops
-``torch.ops.ecah.paged_append`` / ``paged_decode``).
+"""The paged key-value cache: ``PagedAttention`` (and the functions ``append``,
+``decode``, ``prefill`` and ``copy_pages`` it calls, and the torch custom ops
+``torch.ops.ecah.paged_append`` / ``paged_decode`` / ``paged_prefill`` /
+``paged_copy``).
 
 ``append`` normalises and rotates the new tokens' queries and keys and writes
 keys and values into their cache pages -- as they are, or as 8-bit floats with
 a scale per token and head; ``decode`` attends one new token per request over
-the pages.  Pages are listed per request as the reference lists them for its
+the pages, ``prefill`` several (a prompt, a chunk of one, drafted tokens);
+``copy_pages`` copies pages in all layers, to fork requests.  Pages are listed per request as the reference lists them for its
 attention (``kv_indptr`` / ``kv_indices`` / ``kv_last_page_len``,
-ecahlang/manager.py:228-253), so its page allocator feeds both calls
+ecahlang/manager.py:228-253), so its page allocator feeds all calls
 (manager.py:143-185 and main.py:68 are the calls they replace).
 
 The arithmetic lives in ``libecah_sampler.so``; its torch binding
@@ -75,12 +77,90 @@ def decode(q: torch.Tensor, kv_indptr: torch.Tensor, kv_indices: torch.Tensor, k
     return got if lse is None else got[0]
 
 
+def prefill_workspace_bytes(head_dim: int) -> int:
+    """Workspace of any ``prefill`` launch with heads of `head_dim` on the
+    current device."""
+    return int(lib().ecah_paged_prefill_workspace_bytes(head_dim))
+
+
+def prefill(q: torch.Tensor, qo_indptr: torch.Tensor, kv_indptr: torch.Tensor, kv_indices: torch.Tensor,
+            kv_last_page_len: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, workspace: torch.Tensor, *,
+            k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None, causal: bool = True,
+            sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+            lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Enqueue the attention of ``q`` [T, Hq, D], the requests' new tokens one
+    request behind another, over the requests' cached keys and values (the new
+    tokens' own among them: ``append`` comes first); returns ``out`` [T, Hq, D]
+    (allocated unless given).
+
+    Request b's tokens are ``q[qo_indptr[b]:qo_indptr[b + 1]]`` (``qo_indptr``
+    int32 [batch + 1], not decreasing), the last of its cached ones; token i of
+    n sees the first ``len - n + i + 1`` keys if ``causal``, else all ``len``.
+    A token that sees no key gets zeros.  Rows outside every request (padding
+    behind the last one) are neither read nor written.  ``lse`` float32
+    [T, Hq], ``sm_scale``, the page lists and the cache as ``decode`` takes
+    them.  ``workspace``: zero-filled uint8, 16-byte aligned, one per
+    concurrent stream."""
+    got = binding().prefill(q, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, k_cache, v_cache, workspace, k_scale,
+                            v_scale, causal, sm_scale, out, lse, None)
+    return got if lse is None else got[0]
+
+
+def _pages(src, dst, tokens, num_pages: int, page_size: int, device):
+    """``copy_pages``'s lists as device tensors; host sequences are checked first."""
+    on_device = [torch.is_tensor(t) and t.is_cuda for t in (src, dst)]
+    if all(on_device):
+        return src, dst, tokens
+    if any(on_device) or (torch.is_tensor(tokens) and tokens.is_cuda):
+        raise RuntimeError("src, dst and tokens must all be device tensors, or all host sequences")
+    src, dst = ([int(p) for p in t] for t in (src, dst))
+    if len(src) != len(dst):
+        raise RuntimeError(f"{len(src)} source and {len(dst)} destination pages")
+    if any(not 0 <= p < num_pages for p in src + dst):
+        raise IndexError(f"page outside [0, {num_pages})")
+    if len(set(dst)) != len(dst) or set(dst) & set(src):
+        raise RuntimeError("destination pages must differ from each other and from every source")
+    if tokens is not None:
+        tokens = [int(n) for n in tokens]
+        if len(tokens) != len(src) or any(not 0 <= n <= page_size for n in tokens):
+            raise RuntimeError(f"tokens must be {len(src)} numbers in [0, {page_size}]")
+        tokens = torch.tensor(tokens, dtype=torch.int32).to(device, non_blocking=True)
+    return (*(torch.tensor(t, dtype=torch.int32).to(device, non_blocking=True) for t in (src, dst)), tokens)
+
+
+def _copy(caches, src, dst, tokens, layout) -> None:
+    caches = list(caches)
+    if not caches:
+        return
+    k = caches[0][0]
+    if not torch.is_tensor(k) or k.dim() != 4:
+        raise RuntimeError("caches must be (k_cache, v_cache, k_scale, v_scale) of each layer")
+    src, dst, tokens = _pages(src, dst, tokens, k.shape[0], k.shape[1], k.device)
+    binding().copy_pages(src, dst, tokens, caches, layout)
+
+
+def copy_pages(src, dst, caches, *, tokens=None) -> None:
+    """Enqueue the copy of pages ``src[i]`` to ``dst[i]`` in every layer of
+    ``caches``, a sequence of ``(k_cache, v_cache, k_scale, v_scale)`` of one
+    shape (as ``PagedAttention.new_cache`` gives them); one launch for up to 64
+    layers.
+
+    ``tokens``: copy the first ``tokens[i]`` slots of the page alone (None:
+    all).  To fork a request, list its whole pages in the child's page list and
+    copy its last page, ``kv_last_page_len`` tokens of it.  Destinations must
+    differ from each other and from every source.  ``src``, ``dst`` and
+    ``tokens`` are int32 tensors on the device, used as they are (pairs with a
+    page outside the cache, such as -1, are skipped; for captured calls), or
+    host sequences, which are checked and copied to it."""
+    _copy(caches, src, dst, tokens, None)
+
+
 class PagedAttention:
     """One model's paged attention on one stream: its head layout and the
-    decode workspace, shared by all layers.
+    workspaces, shared by all layers.
 
     ``kv_dtype`` is the model dtype (default) or ``torch.float8_e4m3fn``;
-    ``max_batch`` bounds the requests of one ``decode``."""
+    ``max_batch`` bounds the requests of one ``decode`` or ``prefill``."""
 
     def __init__(self, num_qo_heads: int, num_kv_heads: int, head_dim: int, page_size: int, dtype: torch.dtype,
                  kv_dtype: Optional[torch.dtype] = None, max_batch: int = 128, device="cuda"):
@@ -100,10 +180,12 @@ class PagedAttention:
         self.device = resolve_device(device)
         with torch.cuda.device(self.device):
             n = decode_workspace_bytes(max_batch, num_qo_heads, num_kv_heads, head_dim)
+            m = prefill_workspace_bytes(head_dim)
         self.workspace = torch.zeros(n, dtype=torch.uint8, device=self.device)
+        self.prefill_workspace = torch.zeros(m, dtype=torch.uint8, device=self.device)
         self._layout = (num_qo_heads, num_kv_heads, head_dim, page_size, int(kv_dtype == E4M3), max_batch,
                         _DTYPES[dtype])
-        self._append, self._decode = binding().append, binding().decode
+        self._append, self._decode, self._prefill = binding().append, binding().decode, binding().prefill
 
     def new_cache(self, num_pages: int):
         """(k_cache, v_cache, k_scale, v_scale) of one layer, zero-filled; the
@@ -133,6 +215,20 @@ class PagedAttention:
                            v_scale, sm_scale, out, lse, self._layout)
         return got[0] if lse is not None and not return_lse else got
 
+    def prefill(self, q, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, k_cache, v_cache, *, k_scale=None,
+                v_scale=None, causal: bool = True, sm_scale=None, out=None, lse=None, return_lse: bool = False):
+        """``prefill`` with this model's layout checked and its workspace;
+        ``(out, lse)`` with ``return_lse``."""
+        if lse is None and return_lse:
+            lse = True
+        got = self._prefill(q, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, k_cache, v_cache,
+                            self.prefill_workspace, k_scale, v_scale, causal, sm_scale, out, lse, self._layout)
+        return got[0] if lse is not None and not return_lse else got
+
+    def copy_pages(self, src, dst, caches, *, tokens=None) -> None:
+        """``copy_pages`` with this model's layout checked."""
+        _copy(caches, src, dst, tokens, self._layout)
+
 
 # ----------------------------------------------------------- torch custom ops
 _LIB.define(
@@ -143,6 +239,13 @@ _LIB.define(
     "paged_decode(Tensor q, Tensor kv_indptr, Tensor kv_indices, Tensor kv_last_page_len, Tensor k_cache, "
     "Tensor v_cache, Tensor? k_scale, Tensor? v_scale, float sm_scale, Tensor(a!) out, Tensor(b!)? lse, "
     "Tensor(c!) workspace) -> ()")
+_LIB.define(
+    "paged_prefill(Tensor q, Tensor qo_indptr, Tensor kv_indptr, Tensor kv_indices, Tensor kv_last_page_len, "
+    "Tensor k_cache, Tensor v_cache, Tensor? k_scale, Tensor? v_scale, bool causal, float sm_scale, Tensor(a!) out, "
+    "Tensor(b!)? lse, Tensor(c!) workspace) -> ()")
+_LIB.define(
+    "paged_copy(Tensor src, Tensor dst, Tensor? tokens, Tensor(a!)[] k_caches, Tensor(b!)[] v_caches, "
+    "Tensor(c!)[] k_scales, Tensor(d!)[] v_scales) -> ()")
 
 
 def _append_op_cuda(q, k, v, positions, batch_index, kv_indptr, kv_indices, k_cache, v_cache, k_scale, v_scale,
@@ -160,8 +263,25 @@ def _decode_op_cuda(q, kv_indptr, kv_indices, kv_last_page_len, k_cache, v_cache
            v_scale=v_scale, sm_scale=sm_scale, out=out, lse=lse)
 
 
+def _prefill_op_cuda(q, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, k_cache, v_cache, k_scale, v_scale, causal,
+                     sm_scale, out, lse, workspace):
+    prefill(q, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, k_cache, v_cache, workspace, k_scale=k_scale,
+            v_scale=v_scale, causal=causal, sm_scale=sm_scale, out=out, lse=lse)
+
+
+def _copy_op_cuda(src, dst, tokens, k_caches, v_caches, k_scales, v_scales):
+    """Empty lists of scales for caches in the model dtype."""
+    none = [None] * len(k_caches)
+    for name, t in (("v_caches", v_caches), ("k_scales", k_scales or none), ("v_scales", v_scales or none)):
+        if len(t) != len(k_caches):
+            raise RuntimeError(f"{name}: expected {len(k_caches)} layers, got {len(t)}")
+    copy_pages(src, dst, list(zip(k_caches, v_caches, k_scales or none, v_scales or none)), tokens=tokens)
+
+
 _LIB.impl("paged_append", _append_op_cuda, "CUDA")
 _LIB.impl("paged_decode", _decode_op_cuda, "CUDA")
+_LIB.impl("paged_prefill", _prefill_op_cuda, "CUDA")
+_LIB.impl("paged_copy", _copy_op_cuda, "CUDA")
 
 
 @torch.library.register_fake("ecah::paged_append")
@@ -173,4 +293,15 @@ def _append_op_fake(q, k, v, positions, batch_index, kv_indptr, kv_indices, k_ca
 @torch.library.register_fake("ecah::paged_decode")
 def _decode_op_fake(q, kv_indptr, kv_indices, kv_last_page_len, k_cache, v_cache, k_scale, v_scale, sm_scale, out,
                     lse, workspace):
+    return None
+
+
+@torch.library.register_fake("ecah::paged_prefill")
+def _prefill_op_fake(q, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, k_cache, v_cache, k_scale, v_scale, causal,
+                     sm_scale, out, lse, workspace):
+    return None
+
+
+@torch.library.register_fake("ecah::paged_copy")
+def _copy_op_fake(src, dst, tokens, k_caches, v_caches, k_scales, v_scales):
     return None

@@ -495,6 +495,133 @@ ECAH_API int ecah_paged_decode(const ecah_decode_args* args, void* stream);
  * does not use the copy engine is not affected. */
 ECAH_API int ecah_paged_decode_bounded(const ecah_decode_args* args, int32_t tries, void* stream);
 
+/*
+ * Prefill attention: the new tokens of every request, several each, over the
+ * request's cached keys and values, their own among them (append them first).
+ * Serves whole prompts, chunks of prompts behind a context, and drafted
+ * tokens.  Replaces the reference's prefill wrapper run (ecahlang/main.py:68,
+ * planned at :432-455).
+ *
+ *   request b: tokens qo_indptr[b] .. qo_indptr[b+1) of q, n of them;
+ *   len(b) as in ecah_decode_args; its token i stands at len - n + i
+ *   s_ij = sm_scale q_i . k_j  (j <= len - n + i if causal, else j < len)
+ *   o_i = sum_j softmax(s_i)_j v_j,  lse_i = ln sum_j exp(s_ij)
+ *
+ * A token that sees no key (len == 0, or n > len and i < n - len) gives o = 0
+ * and lse = -inf.  Rows of q outside every request (padding rows behind the
+ * last one) are neither read nor written.  qo_indptr must not decrease; its
+ * entries are clamped into [0, tokens].  Sums, rounding and
+ * clamped indices as in decode attention; results do not depend on which
+ * block finishes last.
+ */
+typedef struct ecah_prefill_args {
+  int32_t abi_version;
+  int32_t dtype;              /* of q and out: f16 or bf16                        */
+  int32_t tokens;             /* T: rows of q                                     */
+  int32_t num_qo_heads;
+  float sm_scale;
+  int32_t causal;
+  const void* q;              /* [T, num_qo_heads, head_dim]                      */
+  int64_t q_token_stride, q_head_stride;
+  void* out;                  /* [T, num_qo_heads, head_dim]                      */
+  int64_t out_token_stride, out_head_stride;
+  float* lse;                 /* [T, num_qo_heads] contiguous, or NULL            */
+  const int32_t* qo_indptr;   /* [batch + 1] device                               */
+  const int32_t* kv_last_page_len;   /* [batch] device                            */
+  ecah_kv_cache cache;
+  void* workspace;            /* >= ecah_paged_prefill_workspace_bytes(), 16-byte
+                                 aligned, zero-filled once; every launch leaves its
+                                 counters at zero                                 */
+  size_t workspace_bytes;
+} ecah_prefill_args;
+
+/* Workspace of any ecah_paged_prefill call with heads of `head_dim` on the
+ * current device (0 when there is no device, or for another head_dim). */
+ECAH_API size_t ecah_paged_prefill_workspace_bytes(int32_t head_dim);
+ECAH_API int ecah_paged_prefill(const ecah_prefill_args* args, void* stream);
+
+/*
+ * Page copies: for every pair i and every layer, the first tokens[i] slots of
+ * page src[i] go to page dst[i], keys, values and (e4m3) scales.  For forking
+ * a request (its whole pages are shared by the page lists; the last, partly
+ * filled one is copied) and for compacting a pool.  The reference has no
+ * such call: its requests never share pages (ecahlang/manager.py:99-120).
+ *
+ * A pair with a page outside the cache, or with src == dst, is skipped; pairs
+ * of a captured batch that are not used are set to -1.  Destinations differ
+ * from each other and from every source (pairs are copied in no order: the
+ * contents of a page that breaks this are unspecified); a source may repeat.
+ * All layers have one shape and one set of strides.
+ */
+typedef struct ecah_copy_args {
+  int32_t abi_version;
+  int32_t kv_dtype;           /* ECAH_DTYPE_F16, _BF16 or ECAH_KV_E4M3            */
+  int32_t num_pages;
+  int32_t page_size;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t layers;             /* L >= 0                                           */
+  int32_t pairs;              /* P >= 0                                           */
+  int64_t k_page_stride, k_slot_stride, k_head_stride;
+  int64_t v_page_stride, v_slot_stride, v_head_stride;
+  void* const* k_caches;      /* host arrays [L] of device pointers, layouts as   */
+  void* const* v_caches;      /* in ecah_kv_cache; read during the call           */
+  float* const* k_scales;     /* ECAH_KV_E4M3 only, else NULL                     */
+  float* const* v_scales;
+  const int32_t* src;         /* [P] device                                       */
+  const int32_t* dst;         /* [P] device                                       */
+  const int32_t* tokens;      /* [P] device, clamped into [0, page_size]; NULL:
+                                 whole pages                                      */
+} ecah_copy_args;
+
+ECAH_API int ecah_paged_copy(const ecah_copy_args* args, void* stream);
+
+/*
+ * Verification of drafted tokens: which of a request's drafted tokens are kept,
+ * and the token that follows them, so that what comes out is distributed as
+ * the target's own samples are.  With p_j the target's probabilities at the
+ * request's place j, q_j the draft's, x_j the drafted token, u the request's
+ * uniforms and n its number of drafts:
+ *
+ *   draft j is kept while u_j q_j(x_j) < p_j(x_j)   (in order; float64 products)
+ *   k = the first refused draft, or n
+ *   r = max(p_k - q_k, 0) in float32 after a refusal, p_k when all are kept
+ *   token = the smallest i whose sum_{i' <= i} r_i' > u_N sum r   (float64 sums)
+ *   tokens[b] = x_0 .. x_{k-1}, token, then -1;  accepted[b] = k
+ *
+ * Without draft probabilities the drafts are taken as certain (looked up, not
+ * drawn): q_j is 1 at x_j and r is p_k without its entry x_k.  Where r has no
+ * mass the token is drawn from p_k; where p_k has none either, or has a NaN or
+ * an infinity (or q_k a NaN after a refusal), it is -1.  A draft outside [0, vocab) is refused.
+ * num_drafts[b] < 0 marks a padding row: tokens -1 and accepted 0, nothing
+ * read.  Uniforms are in [0, 1).  `probs_out` of ecah_sampler_launch is a target or draft row.
+ * The reference decodes one token a step (ecahlang/main.py:334-422) and has
+ * no such call.
+ */
+typedef struct ecah_verify_args {
+  int32_t abi_version;
+  int32_t dtype;              /* of both probabilities: enum ecah_dtype           */
+  int32_t batch;              /* B >= 0                                           */
+  int32_t drafts;             /* N >= 0                                           */
+  int32_t vocab;              /* 1 <= V <= 2^31 - 65536                           */
+  const void* target;         /* [B, N + 1, V]: rows contiguous                   */
+  int64_t target_batch_stride, target_row_stride;   /* elements                   */
+  const void* draft;          /* [B, N, V], or NULL                               */
+  int64_t draft_batch_stride, draft_row_stride;
+  const int32_t* draft_ids;   /* [B, N]                                           */
+  const int32_t* num_drafts;  /* [B], clamped to N; NULL: N                       */
+  const float* uniforms;      /* [B, N + 1]                                       */
+  int32_t* tokens;            /* [B, N + 1]                                       */
+  int32_t* accepted;          /* [B]                                              */
+  void* workspace;            /* >= ecah_verify_drafts_workspace_bytes() for some
+                                 batch >= this one, 16-byte aligned, zero-filled
+                                 once; every launch leaves its counters at zero   */
+  size_t workspace_bytes;
+} ecah_verify_args;
+
+ECAH_API size_t ecah_verify_drafts_workspace_bytes(int32_t batch);
+ECAH_API int ecah_verify_drafts(const ecah_verify_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
