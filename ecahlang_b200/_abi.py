@@ -32,7 +32,8 @@ EXPORTS = ("ecah_sampler_abi_version", "ecah_status_string", "ecah_sampler_works
            "ecah_quotient_mismatches", "ecah_vp_reset", "ecah_vp_dist_pass",
            "ecah_token_logprobs_workspace_bytes", "ecah_token_logprobs", "ecah_paged_append",
            "ecah_paged_decode_workspace_bytes", "ecah_paged_decode", "ecah_paged_decode_bounded",
-           "ecah_paged_prefill_workspace_bytes", "ecah_paged_prefill", "ecah_paged_copy",
+           "ecah_paged_prefill_workspace_bytes", "ecah_paged_prefill",
+           "ecah_paged_prefill_bounded", "ecah_paged_copy",
            "ecah_verify_drafts_workspace_bytes", "ecah_verify_drafts")
 IPC_HANDLE_BYTES = 64
 
@@ -228,6 +229,8 @@ def lib():
         L.ecah_paged_prefill_workspace_bytes.argtypes = [c_int32]
         L.ecah_paged_prefill.restype = c_int32
         L.ecah_paged_prefill.argtypes = [ctypes.POINTER(PrefillArgs), c_void_p]
+        L.ecah_paged_prefill_bounded.restype = c_int32
+        L.ecah_paged_prefill_bounded.argtypes = [ctypes.POINTER(PrefillArgs), c_int32, c_void_p]
         L.ecah_paged_copy.restype = c_int32
         L.ecah_paged_copy.argtypes = [ctypes.POINTER(CopyArgs), c_void_p]
         L.ecah_verify_drafts_workspace_bytes.restype = c_size_t

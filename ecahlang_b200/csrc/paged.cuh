@@ -2,6 +2,8 @@
 // the host checks its launchers share.
 #pragma once
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "host_util.h"
 
@@ -31,6 +33,13 @@ __device__ __forceinline__ void page_range(const Cache& c, int b, long long* fir
   *first = lo;
   *count = hi - lo;
 }
+
+// One side of the cache in 16-byte units from its base.
+struct Side16 {
+  const unsigned char* base;
+  unsigned page, slot, head;
+  const float* scale;
+};
 
 inline bool head_dim_ok(int d) { return d == 64 || d == 96 || d == 128 || d == 192 || d == 256; }
 
@@ -64,6 +73,24 @@ inline Cache make_cache(const ecah_kv_cache& c) {
   r.heads = c.num_kv_heads;
   r.batch = c.batch;
   return r;
+}
+
+// A side of the cache in 16-byte units; false where a row lies past 2^32 of them
+// (64 GB from the base).
+inline bool side16(const Side& s, int pages, int page_size, int heads, int elem, Side16* r) {
+  const long long unit = 16 / elem;
+  const long long most = (std::max(pages, 1) - 1ll) * (s.page / unit) + (page_size - 1ll) * (s.slot / unit) + (heads - 1ll) * (s.head / unit);
+  if (s.page / unit > 0xFFFFFFFFll || s.slot / unit > 0xFFFFFFFFll || s.head / unit > 0xFFFFFFFFll || most + 64 > 0xFFFFFFFFll) return false;
+  *r = Side16{static_cast<const unsigned char*>(s.base), static_cast<unsigned>(s.page / unit), static_cast<unsigned>(s.slot / unit),
+              static_cast<unsigned>(s.head / unit), s.scale};
+  return true;
+}
+
+// log2 of a page size that is a power of two, or -1.
+inline int page_shift(int page_size) {
+  for (int i = 0; i < 31; ++i)
+    if (page_size == 1 << i) return i;
+  return -1;
 }
 
 }  // namespace kv

@@ -64,12 +64,7 @@ constexpr float kLazy = 8.0f;
 constexpr float kLift = 7.0f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// One side of the cache in 16-byte units from its base.
-struct Side16 {
-  const unsigned char* base;
-  unsigned page, slot, head;
-  const float* scale;
-};
+using kv::Side16;
 
 struct Params {
   const void* q;
@@ -881,17 +876,6 @@ static Layout layout(int sms, int D) {
   return L;
 }
 
-// A side of the cache in 16-byte units; false where a row lies past 2^32 of them
-// (64 GB from the base).
-static bool side16(const kv::Side& s, int pages, int page_size, int heads, int elem, Side16* r) {
-  const long long unit = 16 / elem;
-  const long long most = (std::max(pages, 1) - 1ll) * (s.page / unit) + (page_size - 1ll) * (s.slot / unit) + (heads - 1ll) * (s.head / unit);
-  if (s.page / unit > 0xFFFFFFFFll || s.slot / unit > 0xFFFFFFFFll || s.head / unit > 0xFFFFFFFFll || most + 64 > 0xFFFFFFFFll) return false;
-  *r = Side16{static_cast<const unsigned char*>(s.base), static_cast<unsigned>(s.page / unit), static_cast<unsigned>(s.slot / unit),
-              static_cast<unsigned>(s.head / unit), s.scale};
-  return true;
-}
-
 }  // namespace decode
 }  // namespace ecah
 
@@ -932,9 +916,7 @@ int ecah_paged_decode_bounded(const ecah_decode_args* a, int32_t tries, void* st
   P.hq = a->num_qo_heads; P.group = a->num_qo_heads / c.num_kv_heads;
   const int rows = P.group <= 8 ? 8 : 16;
   P.tiles_h = (P.group + rows - 1) / rows;
-  P.page_shift = -1;
-  for (int i = 0; i < 31; ++i)
-    if (c.page_size == 1 << i) P.page_shift = i;
+  P.page_shift = kv::page_shift(c.page_size);
   P.tries = tries;
   P.scale = a->sm_scale * kLog2e;
   P.cache = kv::make_cache(c);
@@ -944,8 +926,8 @@ int ecah_paged_decode_bounded(const ecah_decode_args* a, int32_t tries, void* st
   P.part_ml = reinterpret_cast<float2*>(ws + L.ml);
   P.part_o = reinterpret_cast<float*>(ws + L.o);
   const bool e4m3 = c.kv_dtype == ECAH_KV_E4M3, f16 = a->dtype == ECAH_DTYPE_F16;
-  if (!decode::side16(P.cache.k, c.num_pages, c.page_size, c.num_kv_heads, e4m3 ? 1 : 2, &P.k) ||
-      !decode::side16(P.cache.v, c.num_pages, c.page_size, c.num_kv_heads, e4m3 ? 1 : 2, &P.v))
+  if (!kv::side16(P.cache.k, c.num_pages, c.page_size, c.num_kv_heads, e4m3 ? 1 : 2, &P.k) ||
+      !kv::side16(P.cache.v, c.num_pages, c.page_size, c.num_kv_heads, e4m3 ? 1 : 2, &P.v))
     return ECAH_ERR_SHAPE;
   // Units that the listed pages can hold with one KV head an item; `much`: 64 of them to
   // an SM, where streaming outweighs starting and joining.

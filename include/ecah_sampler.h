@@ -540,6 +540,11 @@ typedef struct ecah_prefill_args {
 ECAH_API size_t ecah_paged_prefill_workspace_bytes(int32_t head_dim);
 ECAH_API int ecah_paged_prefill(const ecah_prefill_args* args, void* stream);
 
+/* ecah_paged_prefill with a limit of its own on the waits of a block's warps for
+ * one another: where one runs out, the block ends early and every row that it
+ * still has a part in becomes NaN.  0 makes every wait run out. */
+ECAH_API int ecah_paged_prefill_bounded(const ecah_prefill_args* args, int32_t tries, void* stream);
+
 /*
  * Page copies: for every pair i and every layer, the first tokens[i] slots of
  * page src[i] go to page dst[i], keys, values and (e4m3) scales.  For forking

@@ -5,12 +5,13 @@ operand type (u of itself, 2^-8 for bf16, 2^-11 for f16 and e4m3 caches, which
 the model dtype's own u bounds; for f16 2^-25 of the row's largest at most),
 the output once: |error| <= u |o| + u sum p|v| + 2^-24 max(p) sum|v| +
 float32's 2^-16 sum p|v|.  A row without keys is exactly zero."""
+import ctypes
 import math
 
 import pytest
 import torch
 
-from ecahlang_b200 import paged
+from ecahlang_b200 import _abi, paged
 from ecahlang_b200.paged import PagedAttention
 from test_paged_gpu import E4M3, HALF, KINDS, cache_of, pages_for, values
 
@@ -365,3 +366,34 @@ def test_refusals():
                                  0.125, out, lse, att.prefill_workspace)
     compare(s, out, lse)
     assert call(att, dict(s, q=s["q"][:0])).shape == (0, 8, 64)           # no tokens: qo_indptr is clamped
+
+
+@pytest.mark.parametrize("dtype,kv", KINDS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_a_wait_that_runs_out_gives_nan_and_ends(dtype, kv, D):
+    """No wait between a block's warps is given any time: every row with keys is NaN, rows without are
+    zeros or NaN, no other row is written, and the next launch on the same workspace is right."""
+    Hq, Hk, page = 8, 2, 16
+    s = setup([300, 5, 40], [0, 6000, 2000], Hq, Hk, D, page, dtype, kv, behind=3)
+    att = PagedAttention(Hq, Hk, D, page, dtype, kv_dtype=kv, max_batch=3)
+    T = s["q"].shape[0]
+    out, lse = torch.full((T, Hq, D), 7.0, dtype=dtype, device=DEV), torch.full((T, Hq), 7.0, device=DEV)
+    q, k, v = s["q"], s["k"], s["v"]
+    ptr = lambda t: None if t is None else t.data_ptr()   # noqa: E731
+    a = _abi.PrefillArgs(abi_version=_abi.ABI_VERSION, dtype=0 if dtype == torch.float16 else 1, tokens=T, num_qo_heads=Hq,
+                         sm_scale=D ** -0.5, causal=1, q=ptr(q), q_token_stride=q.stride(0), q_head_stride=q.stride(1), out=ptr(out),
+                         out_token_stride=out.stride(0), out_head_stride=out.stride(1), lse=ptr(lse), qo_indptr=ptr(s["qo_indptr"]),
+                         kv_last_page_len=ptr(s["last"]), workspace=ptr(att.prefill_workspace), workspace_bytes=att.prefill_workspace.numel())
+    a.cache = _abi.KVCache(kv_dtype=_abi.KV_E4M3 if kv else a.dtype, num_pages=k.shape[0], page_size=page, num_kv_heads=Hk, head_dim=D,
+                           batch=3, k_cache=ptr(k), v_cache=ptr(v), k_page_stride=k.stride(0), k_slot_stride=k.stride(1),
+                           k_head_stride=k.stride(2), v_page_stride=v.stride(0), v_slot_stride=v.stride(1), v_head_stride=v.stride(2),
+                           k_scale=ptr(s["ks"]), v_scale=ptr(s["vs"]), kv_indptr=ptr(s["indptr"]), kv_indices=ptr(s["indices"]),
+                           num_indices=s["indices"].numel())
+    stream = torch.cuda.current_stream().cuda_stream
+    assert _abi.lib().ecah_paged_prefill_bounded(ctypes.byref(a), 0, stream) == 0
+    torch.cuda.synchronize()
+    hi = s["ptr"][-1]
+    assert torch.isnan(out[:hi]).all() and torch.isnan(lse[:hi]).all()
+    assert bool((out[hi:] == 7.0).all()) and bool((lse[hi:] == 7.0).all())
+    assert _abi.lib().ecah_paged_prefill_bounded(ctypes.byref(a), 1 << 20, stream) == 0
+    compare(s, out, lse)
