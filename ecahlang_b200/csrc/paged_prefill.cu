@@ -1,7 +1,10 @@
 // Attention of several new tokens per request over the paged key-value cache:
 // ecah_paged_prefill (contract in include/ecah_sampler.h).
 
+#include <cuda.h>
+
 #include <algorithm>
+#include <cstring>
 
 #include "host_util.h"
 #include "paged.cuh"
@@ -52,7 +55,9 @@ constexpr float kLazy = 8.0f;          // as in decode attention: a reference mo
 constexpr float kLift = 7.0f;          // f16 weights reach 2^15, so that small ones are not lost
 constexpr float kLn2 = 0.6931471805599453f;
 
-struct Params {
+struct alignas(64) Params {
+  CUtensorMap k_map, v_map;            // [pages][heads][slots][head_dim], boxes of 64 elements by the slots of a page in a tile
+  int boxes;                           // whether the copy engine brings whole tiles
   const void* q;
   void* out;
   float* lse;
@@ -135,36 +140,47 @@ __device__ __forceinline__ int tiles_of(const Params& P, const Request& r) {
 
 struct Edge { int req, head, tile; long long start; int iters; };
 
-// The items of this block's share, in order.  Every role of warps walks them alike.
+// The items of this block's share, in order.  Every warp that works on them walks them
+// alike, with its own walk in shared memory: only what a loop uses is held in registers.
 template <int D, bool E4M3>
 struct Walk {
   using S = Shape<D, E4M3>;
-  const Params& P;
   long long lo, hi, at, share, more;
-  int req, head, tile, tiles;
   Request r;
+  int req, head, tile, tiles, iters;
   // the present item's part
   int row0, rows, keys, jb, je, je0;   // key tiles [jb, je); of the first slot of two halves [jb, je0)
-  bool few, whole;
   int first_block, parts;
+  bool fresh, few, whole;
 
-  __device__ __forceinline__ Walk(const Params& p, const Edge* edge, const long long* bounds) : P(p) {
-    lo = bounds[0]; hi = bounds[1]; share = bounds[2]; more = bounds[3];
-    req = edge[0].req; head = edge[0].head; tile = edge[0].tile; at = edge[0].start;
-    if (req < P.cache.batch) {
-      r = request<S::kKeys>(P, req);
-      tiles = tiles_of<D, E4M3>(P, r);
+  __device__ __forceinline__ void begin(const Params& P, const Edge& edge, const long long* bounds) {
+    if ((threadIdx.x & 31) == 0) {
+      lo = bounds[0]; hi = bounds[1]; share = bounds[2]; more = bounds[3];
+      req = edge.req; head = edge.head; tile = edge.tile; at = edge.start;
+      fresh = true;
+      if (req < P.cache.batch) {
+        r = request<S::kKeys>(P, req);
+        tiles = tiles_of<D, E4M3>(P, r);
+      }
     }
+    __syncwarp();
   }
+  // The next item with work for this block; false behind the last.  Called by whole warps.
+  __device__ __forceinline__ bool next(const Params& P) {
+    __syncwarp();
+    bool found = false;
+    if ((threadIdx.x & 31) == 0) found = advance(P);
+    return __shfl_sync(0xFFFFFFFFu, found, 0);               // and orders what lane 0 wrote
+  }
+
+ private:
   __device__ __forceinline__ int block_of(long long x) const {
     return static_cast<int>(x < more * (share + 1) ? x / (share + 1) : more + (x - more * (share + 1)) / share);
   }
-  // The next item with work for this block; false behind the last.
-  __device__ __forceinline__ bool next(bool fresh) {
-    bool step = !fresh;
+  __device__ __forceinline__ bool advance(const Params& P) {
     while (true) {
-      if (step) {
-        at += iters_ + kItemCost;
+      if (!fresh) {
+        at += iters + kItemCost;
         if (++tile >= tiles) {
           tile = 0;
           if (++head >= P.cache.heads) {
@@ -177,13 +193,18 @@ struct Walk {
           }
         }
       }
-      step = true;
-      if (req >= P.cache.batch || at >= hi) return false;
+      fresh = false;
+      if (req >= P.cache.batch || at >= hi) {
+        fresh = true;                                         // stays behind the last
+        return false;
+      }
       const Tile<D, E4M3> t(P, r, tile);
-      iters_ = t.iters;
+      iters = t.iters;
       const long long begin = at + kItemCost;
       int i0 = 0, i1 = t.iters;
       whole = t.iters <= kWhole;
+      first_block = blockIdx.x;
+      parts = 1;
       if (whole) {
         if (at < lo) continue;
       } else {
@@ -203,7 +224,6 @@ struct Walk {
       return true;
     }
   }
-  int iters_ = 0;
 };
 
 template <int HT>
@@ -230,6 +250,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ float lg2(float x) {
   float r;
   asm("lg2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -240,8 +265,6 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void sync_some(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 // The block's barriers.
@@ -253,7 +276,7 @@ struct Bars {
 };
 
 template <int DT, bool E4M3, int D>
-__global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
+__global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ Params P) {
   using S = Shape<D, E4M3>;
   constexpr int HT = E4M3 ? static_cast<int>(ECAH_DTYPE_F16) : DT;   // operand type of the products
   constexpr float lift = HT == ECAH_DTYPE_F16 ? kLift : 0.0f;
@@ -264,6 +287,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
   __shared__ long long s_bounds[4];
   __shared__ uint32_t s_tmem;
   __shared__ int s_failed, s_flag;
+  __shared__ Walk<D, E4M3> s_walk[kIssuer + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* base_p = smem_raw + (base - tc::smem_u32(smem_raw));
@@ -419,11 +443,11 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
     return ok;
   };
 
-  Walk<D, E4M3> w(P, s_edge, s_bounds);
+  Walk<D, E4M3>& w = s_walk[min(warp, kIssuer)];
+  if (warp <= kIssuer) w.begin(P, s_edge[0], s_bounds);
 
   if (warp < 4 * kSlots) {
     // =============================================================== softmax
-    regs_up<176>();
     const int slot = warp >> 2, row = tid & 127;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
     const uint32_t sum_at = lanes + S::kSum + slot * D;
@@ -439,7 +463,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
       tc::fence_after();
       return there;
     };
-    for (bool more_items = w.next(true); more_items; more_items = w.next(false)) {
+    while (w.next(P)) {
       const bool own_rows = kSlots == 2 && !w.few;            // slots are halves of the rows
       const int my = (own_rows ? slot * 128 : 0) + row;       // row of the item
       const bool live = my < w.rows;
@@ -490,48 +514,54 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
 
       float m = -INFINITY, l = 0.0f;
       bool any = false;                                       // the sum holds something
-      const int step = own_rows || kSlots == 1 ? 1 : 2;
+      const int step = own_rows || kSlots == 1 ? 1 : 2, jb = w.jb, je = own_rows && slot == 0 ? w.je0 : w.je;
       int buf = kSlots == 2 ? slot : 0;
-      for (int j = w.jb + (own_rows || kSlots == 1 ? 0 : slot); j < (own_rows && slot == 0 ? w.je0 : w.je) && ok; j += step) {
+      for (int j = jb + (own_rows || kSlots == 1 ? 0 : slot); j < je && ok; j += step) {
         ok = wait(&s_bars.s_full[buf], s_phase >> buf & 1);
         if (!ok) break;
         s_phase ^= 1u << buf;
         tc::fence_after();
         const uint32_t s_at = lanes + buf * S::kBuffer;
-        uint32_t r[kKeys / 32][32];
-#pragma unroll
-        for (int i = 0; i < kKeys / 32; ++i) tc::load32(r[i], s_at + 32 * i);
-        tc::load_wait();
-#pragma unroll
-        for (int i = 0; i < kKeys / 32; ++i) tc::pin32(r[i]);
         // Scores in log2 units; an e4m3 value's scale goes into its weight through the
-        // exponent (weight 2^(s + log2 scale - m)), and the sum takes it back out.
-        const float* sc = reinterpret_cast<const float*>(base_p + (s_scales - base) + ((before + j - w.jb) % S::kScaleRing) * S::kScales);
-        if (E4M3) {
+        // exponent (weight 2^(s + log2 scale - m)), and the sum takes it back out.  They are
+        // read twice, 32 at a time: a row's 128 do not fit beside the rest in the registers.
+        const float* sc = reinterpret_cast<const float*>(base_p + (s_scales - base) + ((before + j - jb) % S::kScaleRing) * S::kScales);
+        const bool masked = (j + 1) * kKeys > least;
+        const int left = lim - j * kKeys;
+        auto ready = [&](uint32_t (&r)[32], int i) {
+          if (E4M3) {
 #pragma unroll
-          for (int c = 0; c < kKeys; c += 4) {
-            const float4 kx = *reinterpret_cast<const float4*>(sc + c), lv = *reinterpret_cast<const float4*>(sc + kKeys + c);
-            const float a[4] = {kx.x, kx.y, kx.z, kx.w}, b[4] = {lv.x, lv.y, lv.z, lv.w};
+            for (int c = 0; c < 32; c += 4) {
+              const float4 kx = *reinterpret_cast<const float4*>(sc + 32 * i + c), lv = *reinterpret_cast<const float4*>(sc + kKeys + 32 * i + c);
+              const float x[4] = {kx.x, kx.y, kx.z, kx.w}, y[4] = {lv.x, lv.y, lv.z, lv.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t& x = r[(c + i) / 32][(c + i) % 32];
-              x = __float_as_uint(fmaf(__uint_as_float(x) * a[i], scale, b[i]));
+              for (int e = 0; e < 4; ++e) r[c + e] = __float_as_uint(fmaf(__uint_as_float(r[c + e]) * x[e], scale, y[e]));
             }
           }
-        }
-        if ((j + 1) * kKeys > least) {
-          const int left = lim - j * kKeys;
+          if (masked) {
 #pragma unroll
-          for (int c = 0; c < kKeys; ++c)
-            if (c >= left) r[c / 32][c % 32] = 0xFF800000u;
-        }
+            for (int c = 0; c < 32; ++c)
+              if (32 * i + c >= left) r[c] = 0xFF800000u;
+          }
+        };
+        uint32_t ra[32], rb[32];
         float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < kKeys; c += 4) {
-          t0 = fmaxf(t0, __uint_as_float(r[c / 32][c % 32]));
-          t1 = fmaxf(t1, __uint_as_float(r[c / 32][c % 32 + 1]));
-          t2 = fmaxf(t2, __uint_as_float(r[c / 32][c % 32 + 2]));
-          t3 = fmaxf(t3, __uint_as_float(r[c / 32][c % 32 + 3]));
+        for (int i = 0; i < kKeys / 32; i += 2) {
+          tc::load32(ra, s_at + 32 * i);
+          tc::load32(rb, s_at + 32 * i + 32);
+          tc::load_wait();
+          tc::pin32(ra);
+          tc::pin32(rb);
+          ready(ra, i);
+          ready(rb, i + 1);
+#pragma unroll
+          for (int c = 0; c < 32; c += 4) {
+            t0 = max3(t0, __uint_as_float(ra[c]), __uint_as_float(rb[c]));
+            t1 = max3(t1, __uint_as_float(ra[c + 1]), __uint_as_float(rb[c + 1]));
+            t2 = max3(t2, __uint_as_float(ra[c + 2]), __uint_as_float(rb[c + 2]));
+            t3 = max3(t3, __uint_as_float(ra[c + 3]), __uint_as_float(rb[c + 3]));
+          }
         }
         float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
         if (!E4M3) top *= P.scale;
@@ -554,31 +584,47 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
             }
           }
         }
+        tc::load32(ra, s_at);
         const float ref = m == -INFINITY ? 0.0f : m;
-        float l0 = 0.0f, l1 = 0.0f, l2 = 0.0f, l3 = 0.0f;
+        const uint64_t scale2 = tc::two(P.scale, P.scale), ref2 = tc::two(-ref, -ref);
+        uint64_t sum0 = 0, sum1 = 0;                          // four chains
 #pragma unroll
         for (int i = 0; i < kKeys / 32; ++i) {
+          uint32_t (&r)[32] = i & 1 ? rb : ra;
+          tc::load_wait();
+          tc::pin32(r);
+          if (i + 1 < kKeys / 32) tc::load32(i & 1 ? ra : rb, s_at + 32 * i + 32);
+          ready(r, i);
           // A weight is off by at most 2^-9 of itself in bf16 (2^-12 in f16), at random over the
           // keys; the sum takes it as it was.
           uint32_t w16[16];
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
+            const uint64_t a = tc::two(__uint_as_float(r[c]), __uint_as_float(r[c + 1]));
+            const uint64_t b = tc::two(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3]));
             float p[4];
+            tc::apart(E4M3 ? tc::add2(a, ref2) : tc::fma2(a, scale2, ref2), p[0], p[1]);
+            tc::apart(E4M3 ? tc::add2(b, ref2) : tc::fma2(b, scale2, ref2), p[2], p[3]);
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              p[x] = ex2_approx(E4M3 ? __uint_as_float(r[i][c + x]) - ref : fmaf(__uint_as_float(r[i][c + x]), P.scale, -ref));
+            for (int x = 0; x < 4; ++x) p[x] = ex2_approx(p[x]);
             if (E4M3) {
               const float4 inv = *reinterpret_cast<const float4*>(sc + 2 * kKeys + 32 * i + c);
-              l0 = fmaf(p[0], inv.x, l0); l1 = fmaf(p[1], inv.y, l1); l2 = fmaf(p[2], inv.z, l2); l3 = fmaf(p[3], inv.w, l3);
+              sum0 = tc::fma2(tc::two(p[0], p[1]), tc::two(inv.x, inv.y), sum0);
+              sum1 = tc::fma2(tc::two(p[2], p[3]), tc::two(inv.z, inv.w), sum1);
             } else {
-              l0 += p[0]; l1 += p[1]; l2 += p[2]; l3 += p[3];
+              sum0 = tc::add2(tc::two(p[0], p[1]), sum0);
+              sum1 = tc::add2(tc::two(p[2], p[3]), sum1);
             }
             w16[c / 2] = pack2<HT>(p[0], p[1]);
             w16[c / 2 + 1] = pack2<HT>(p[2], p[3]);
           }
           tc::store16(s_at + 16 * i, w16);
         }
-        l += (l0 + l1) + (l2 + l3);
+        {
+          float l0, l1;
+          tc::apart(tc::add2(sum0, sum1), l0, l1);
+          l += l0 + l1;
+        }
         tc::store_wait();
         tc::fence_before();
         __syncwarp();
@@ -587,14 +633,14 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
         ++pv;
         if (kSlots == 1) buf ^= 1;
       }
-      before += max(w.je - w.jb, 0);
+      before += max(w.je - jb, 0);
       if (any && ok) ok = wait_sum();
       if (!ok) l = NAN;
 
       // ---- the item's rows, or this part of them
       const bool joined = !w.whole || w.few;                  // more than one sum to a row
-      const int part = w.whole ? 0 : static_cast<int>(blockIdx.x) - w.first_block;
-      auto part_slot = [&](int p) { return w.whole || p == 0 ? 2 * (w.whole ? static_cast<int>(blockIdx.x) : w.first_block) + 1 : 2 * (w.first_block + p); };
+      const int first_block = w.first_block, part = static_cast<int>(blockIdx.x) - first_block;
+      auto part_slot = [&](int p) { return p == 0 ? 2 * first_block + 1 : 2 * (first_block + p); };
       if (!joined) {
         // a sum of zero (no key has mass) gives zeros
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -636,12 +682,12 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
         }
         tc::fence_before();
         // the last part's block joins them all; a whole item's two sums are joined here
-        const int parts = w.whole ? 1 : w.parts;
+        const int parts = w.parts;
         sync_some(1, 128 * kSlots);
         if (tid == 0) {
           bool last = true;
           if (parts > 1) {
-            unsigned* counter = P.counters + w.first_block;
+            unsigned* counter = P.counters + first_block;
             unsigned n;
             asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(n) : "l"(counter) : "memory");
             last = n + 1u == static_cast<unsigned>(parts);
@@ -705,28 +751,32 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
     }
   } else if (warp >= kLoaders && warp < kLoaders + 4) {
     // ================================================ keys and values to the ring
-    regs_down<96>();
     constexpr int kMine = kKeys / 4;                          // rows of a warp
     const int wl = warp - kLoaders;
     unsigned n = 0, tiles = 0;                                // loads, key tiles so far
     uint32_t q_phase = 0;
     bool ok = true;
-    constexpr int kLag = 2;
-    unsigned told = 0;                                        // loads that the products know of
-    auto tell = [&]() {
+    constexpr unsigned kLag = 2;
+    unsigned long long waiting = 0;                           // ring slots filled by threads' copies that the products do not
+    unsigned told_late = 0;                                   // know of yet, oldest in the low byte; how many
+    auto tell = [&](unsigned at) {
       tc::fence_smem();
       __syncwarp();
-      if (lane == 0) tc::bar_arrive(tc::smem_u32(&s_bars.kv_full[told % kRing]));
-      ++told;
+      if (lane == 0) tc::bar_arrive(tc::smem_u32(&s_bars.kv_full[at]));
+    };
+    auto tell_oldest = [&]() {
+      tell(static_cast<unsigned>(waiting & 255));
+      waiting >>= 8;
+      --told_late;
     };
     auto free_slot = [&]() { return wait(&s_bars.kv_empty[n % kRing], ((n / kRing) & 1) ^ 1); };
 
-    for (bool more_items = w.next(true); more_items && ok; more_items = w.next(false)) {
+    while (ok && w.next(P)) {
       if (w.jb >= w.je) continue;
       const bool shared = kSlots == 2 && !w.few;
       if (!E4M3) {                                            // the item's queries
         cp_wait<0>();
-        while (told < n) tell();
+        while (told_late) tell_oldest();
         ok = wait(&s_bars.q_empty, q_phase ^ 1);
         q_phase ^= 1;
         if (!ok) break;
@@ -755,19 +805,19 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
       }
 
       const int* pages = C.indices + w.r.first;
-      const int len = w.r.len;
+      const int len = w.r.len, head = w.head, je = w.je;
       auto nth_page = [&](int key) { return P.page_shift >= 0 ? key >> P.page_shift : key / C.page_size; };
       const int ahead = shared ? 1 : 2;
       int page_next = 0;
       auto page_of = [&](int j) -> int {
         const int key = j * kKeys + wl * kMine + lane;
-        return lane < kMine && j < w.je && key < len ? min(max(pages[nth_page(key)], 0), C.num_pages - 1) : -1;
+        return lane < kMine && j < je && key < len ? min(max(pages[nth_page(key)], 0), C.num_pages - 1) : -1;
       };
       // the next loads in order: K jb .. (ahead of them), then V j, K j + ahead
       int jk = w.jb, jv = w.jb;
       page_next = page_of(jk);
       auto next_load = [&](bool* is_v, int* j, int* page) {
-        *is_v = jk >= w.je || jk - jv >= ahead;
+        *is_v = jk >= je || jk - jv >= ahead;
         *j = *is_v ? jv++ : jk++;
         if (*is_v) {
           *page = page_of(*j);                                // read a while ago: in L1
@@ -776,16 +826,46 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
           page_next = page_of(jk);
         }
       };
-      const int loads = 2 * (w.je - w.jb);
+      const int loads = 2 * (je - w.jb);
       if (!E4M3) {
+        // pages of a tile that the copy engine brings, a lane to a page
+        const int in_tile = P.boxes ? max(1, kKeys >> P.page_shift) : 0, slots = kKeys / max(1, in_tile);
+        auto listed = [&](int j) { return lane < in_tile && (j + 1) * kKeys <= len ? pages[((j * kKeys) >> P.page_shift) + lane] : 0; };
+        int box_next = listed(jk);
         for (int i = 0; i < loads; ++i) {
           bool is_v;
           int j, page;
+          const bool v_next = jk >= je || jk - jv >= ahead;
+          if (P.boxes && ((v_next ? jv : jk) + 1) * kKeys <= len) {
+            // a whole tile: boxes of 64 elements by a page's slots, dealt to the warps
+            is_v = v_next;
+            j = is_v ? jv++ : jk++;
+            int at = is_v ? listed(j) : box_next;             // values' pages were read a while ago: in L1
+            if (!is_v) {
+              box_next = listed(jk);
+              if (jk < je && (jk + 1) * kKeys > len) page_next = page_of(jk);
+            }
+            at = min(max(at, 0), C.num_pages - 1);
+            ok = free_slot();
+            if (!ok) break;
+            const uint32_t dst = s_ring + (n % kRing) * S::kTile, bar = tc::smem_u32(&s_bars.kv_full[n % kRing]);
+            const void* map = is_v ? &P.v_map : &P.k_map;
+            const int boxes = in_tile * S::kBlocks, mine = (boxes - wl + 3) / 4;
+            const int slot = (j * kKeys) & (C.page_size - 1);
+            if (tc::elect()) tc::bar_expect(bar, mine * slots * 128);
+            for (int x = wl; x < boxes; x += 4) {
+              const int nth = x / S::kBlocks, block = x - nth * S::kBlocks;
+              const int pg = __shfl_sync(0xFFFFFFFFu, at, nth);
+              if (tc::elect()) tc::copy_box(dst + block * (kKeys * 128) + nth * slots * 128, map, block * 64, slot, head, pg, bar);
+            }
+            ++n;
+            continue;
+          }
           next_load(&is_v, &j, &page);
           const kv::Side16& side = is_v ? P.v : P.k;
           const int key = j * kKeys + wl * kMine + lane;
           unsigned off = 0;
-          if (page >= 0) off = page * side.page + static_cast<unsigned>(key - nth_page(key) * C.page_size) * side.slot + w.head * side.head;
+          if (page >= 0) off = page * side.page + static_cast<unsigned>(key - nth_page(key) * C.page_size) * side.slot + head * side.head;
           const unsigned live = __ballot_sync(0xFFFFFFFFu, page >= 0);
           ok = free_slot();
           if (!ok) break;
@@ -799,10 +879,12 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
             cp16(dst + (col / 8) * (kKeys * 128) + r * 128 + ((col % 8) ^ (r & 7)) * 16, side.base + (there ? o + col : 0u) * 16ull, there);
           }
           cp_commit();
+          waiting |= static_cast<unsigned long long>(n % kRing) << (8 * told_late);
+          ++told_late;
           ++n;
-          if (n - told > kLag) {
+          if (told_late > kLag) {
             cp_wait<kLag>();
-            tell();
+            tell_oldest();
           }
         }
       } else {
@@ -822,9 +904,9 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
           ks_then = vs_then = 0.0f;
           if (on_then) {
             const int slot = key - nth_page(key) * C.page_size;
-            off = page * side.page + static_cast<unsigned>(slot) * side.slot + w.head * side.head;
+            off = page * side.page + static_cast<unsigned>(slot) * side.slot + head * side.head;
             if (!is_v_then) {
-              const long long at = (static_cast<long long>(page) * C.heads + w.head) * C.page_size + slot;
+              const long long at = (static_cast<long long>(page) * C.heads + head) * C.page_size + slot;
               ks_then = P.k.scale[at];
               vs_then = P.v.scale[at];
             }
@@ -868,22 +950,21 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
             sc[2 * kKeys] = on ? rcp(v) : 0.0f;
           }
           if (!is_v) ++tiles;
+          tell(n % kRing);
           ++n;
-          tell();
         }
       }
     }
     cp_wait<0>();
-    while (ok && told < n) tell();
+    while (ok && told_late) tell_oldest();
   } else if (warp == kIssuer) {
     // ================================================================ products
-    regs_down<64>();
     unsigned n = 0, products = 0;                             // loads taken, products O += P V
     uint32_t q_phase = 0, p_phase = 0;                        // a bit a buffer
     bool ok = true;
     constexpr uint32_t score = tc::product(HT == ECAH_DTYPE_BF16, kKeys, false), sum = tc::product(HT == ECAH_DTYPE_BF16, D, true);
     auto scores = [&](int buf, int q_tile, unsigned at) {
-      if (lane == 0) {
+      if (tc::elect()) {
         const uint64_t a = tc::tile_desc(s_q + q_tile * S::kQ, 0), b = tc::tile_desc(s_ring + (at % kRing) * S::kTile, 0);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
@@ -893,7 +974,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
       __syncwarp();
     };
     auto weigh = [&](int slot, int buf, unsigned at, bool add) {
-      if (lane == 0) {
+      if (tc::elect()) {
         const uint64_t b = tc::tile_desc(s_ring + (at % kRing) * S::kTile, kKeys * 128);
 #pragma unroll
         for (int k = 0; k < kKeys / 16; ++k)
@@ -904,7 +985,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
       __syncwarp();
     };
     auto release = [&](unsigned at) {
-      if (lane == 0) tc::commit(tc::smem_u32(&s_bars.kv_empty[at % kRing]));
+      if (tc::elect()) tc::commit(tc::smem_u32(&s_bars.kv_empty[at % kRing]));
       __syncwarp();
     };
     auto arrived = [&](unsigned at) {
@@ -918,15 +999,15 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
       tc::fence_after();
       return there;
     };
-    for (bool more_items = w.next(true); more_items && ok; more_items = w.next(false)) {
-      const int count = w.je - w.jb;
+    while (ok && w.next(P)) {
+      const int count = w.je - w.jb, first = w.je0 - w.jb;    // first: tiles of the first half
       if (count <= 0) continue;
+      const bool few = w.few;
       ok = wait(&s_bars.q_full, q_phase);
       q_phase ^= 1;
       if (!ok) break;
       tc::fence_after();
-      if (kSlots == 2 && !w.few) {
-        const int first = w.je0 - w.jb;                       // tiles of the first half
+      if (kSlots == 2 && !few) {
         if (!(ok = arrived(n))) break;
         if (first > 0) scores(0, 0, n);
         scores(1, 1, n);
@@ -972,15 +1053,13 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const Params P) {
         }
       }
       if (!ok) break;
-      if (lane == 0) tc::commit(tc::smem_u32(&s_bars.q_empty));
+      if (tc::elect()) tc::commit(tc::smem_u32(&s_bars.q_empty));
       __syncwarp();
     }
     // nothing is in flight when the tensor memory is given back
-    if (lane == 0) tc::commit(tc::smem_u32(&s_bars.done));
+    if (tc::elect()) tc::commit(tc::smem_u32(&s_bars.done));
     __syncwarp();
     for (int i = 0; i < kTries && !tc::bar_test(tc::smem_u32(&s_bars.done), 0); ++i) {}
-  } else {
-    regs_down<64>();
   }
 
   tc::fence_before();
@@ -1004,6 +1083,35 @@ static Variant variant_for(int D) {
     case 192: return {prefill_kernel<DT, E4M3, 192>, Shape<192, E4M3>::kSmem};
     default: return {prefill_kernel<DT, E4M3, 256>, Shape<256, E4M3>::kSmem};
   }
+}
+
+// A side of the cache as the copy engine reads it; false where it cannot (a stride of
+// zero, a driver that has no such call): threads copy the rows then.
+static bool box_map(CUtensorMap* map, const kv::Side& s, const ecah_kv_cache& c, int slots) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      f = nullptr;
+    }
+    return reinterpret_cast<Encode>(f);
+  }();
+  if (!encode) return false;
+  const cuuint64_t row = static_cast<cuuint64_t>(c.head_dim) * 2;
+  const cuuint64_t sizes[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.page_size), static_cast<cuuint64_t>(c.num_kv_heads),
+                               static_cast<cuuint64_t>(c.num_pages)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(s.slot) * 2, static_cast<cuuint64_t>(s.head) * 2, static_cast<cuuint64_t>(s.page) * 2};
+  for (int i = 0; i < 3; ++i) {
+    if (sizes[i + 1] == 1) strides[i] = row;                  // of a dimension of one the stride may be anything
+    if (strides[i] == 0 || strides[i] >= 1ull << 40) return false;
+  }
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(slots), 1, 1}, steps[4] = {1, 1, 1, 1};
+  return encode(map, c.kv_dtype == ECAH_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, s.base, sizes, strides,
+                box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Workspace: counters, the parts' (m, l), their sums.  A block has at most two parts of
@@ -1076,6 +1184,11 @@ int ecah_paged_prefill_bounded(const ecah_prefill_args* a, int32_t tries, void* 
   const prefill::Variant v =
       a->dtype == ECAH_DTYPE_F16 ? (e4m3 ? prefill::variant_for<ECAH_DTYPE_F16, true>(c.head_dim) : prefill::variant_for<ECAH_DTYPE_F16, false>(c.head_dim))
                                  : (e4m3 ? prefill::variant_for<ECAH_DTYPE_BF16, true>(c.head_dim) : prefill::variant_for<ECAH_DTYPE_BF16, false>(c.head_dim));
+  // Whole tiles by the copy engine where a page is a power of two of 8 slots or more (the
+  // swizzle goes by 8 rows); smaller or odd pages and 8-bit rows go through threads.
+  const int keys = c.head_dim <= 128 ? 128 : 64;
+  P.boxes = !e4m3 && P.page_shift >= 3 && prefill::box_map(&P.k_map, P.cache.k, c, std::min(c.page_size, keys)) &&
+            prefill::box_map(&P.v_map, P.cache.v, c, std::min(c.page_size, keys));
   return launch_kernel(v.fn, dim3(sms), prefill::kT, v.smem, reinterpret_cast<cudaStream_t>(stream), P) ? ECAH_OK : ECAH_ERR_LAUNCH;
 }
 

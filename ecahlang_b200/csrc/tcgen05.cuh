@@ -23,6 +23,15 @@ __device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
                : "=r"(done) : "r"(bar), "r"(parity) : "memory");
   return done != 0;
 }
+// An arrival that announces bytes to come by the copy engine.
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// A box of a tensor to shared memory by the copy engine, counted by a barrier.
+__device__ __forceinline__ void copy_box(uint32_t dst, const void* map, int x, int y, int z, int w, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
+}
 // Orders this thread's ordinary accesses to shared memory before the tensor cores'.
 __device__ __forceinline__ void fence_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -66,6 +75,29 @@ __device__ __forceinline__ void store16(uint32_t at, const uint32_t (&r)[16]) {
 }
 __device__ __forceinline__ void store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// --------------------------------------------------- pairs of float32 values
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void apart(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // ----------------------------------------------------------------- products
 // A tile in shared memory in rows of 128 bytes whose 16-byte chunks are swizzled by
 // the row's place among 8.  `lead`: bytes between neighbouring blocks of 64 elements
@@ -74,6 +106,14 @@ __device__ __forceinline__ void store_wait() { asm volatile("tcgen05.wait::st.sy
 __device__ __forceinline__ uint64_t tile_desc(uint32_t at, uint32_t lead) {
   return static_cast<uint64_t>((at & 0x3FFFFu) >> 4) | static_cast<uint64_t>(lead >> 4) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 |
          1ull << 46 | 2ull << 61;
+}
+// One thread of the warp, the same for all its calls.  The instructions below take their
+// operands from the warp's uniform registers: behind this choice the compiler needs no
+// loop over the active threads to bring them there, as behind `lane == 0`.
+__device__ __forceinline__ bool elect() {
+  uint32_t one;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xFFFFFFFF; selp.u32 %0, 1, 0, p; }" : "=r"(one));
+  return one != 0;
 }
 // 128 x n results in float32 of 16-bit operands; rows_summed: B's rows are the summed dimension.
 constexpr uint32_t product(bool bf16, int n, bool rows_summed) {
