@@ -43,9 +43,10 @@ namespace prefill {
 // lengths).  An item that spans several blocks is joined by the block that arrives
 // last, in the order of the parts, so results do not depend on which that is.
 
-constexpr int kT = 512;
-constexpr int kLoaders = 8;            // first warp of those that bring keys and values
-constexpr int kIssuer = 12;            // the warp that issues the products
+constexpr int kLoaders = 16;           // first of the warps that bring keys and values, and how many
+constexpr int kLoadWarps = 3;
+constexpr int kIssuer = 19;            // the warp that issues the products
+constexpr int kT = 32 * (kIssuer + 1);
 constexpr int kItemCost = 3;           // iterations that starting and finishing an item takes
 constexpr int kWhole = 6;              // items of up to so many iterations are not divided
 constexpr int kLeast = 4;              // iterations to a block at the least
@@ -53,6 +54,11 @@ constexpr int kKeep = 128;             // requests looked at together
 constexpr int kTries = 1 << 20;        // of a wait: more than one between warps of a block can need
 constexpr float kLazy = 8.0f;          // as in decode attention: a reference moves when a score passes it by 2^kLazy;
 constexpr float kLift = 7.0f;          // f16 weights reach 2^15, so that small ones are not lost
+// One pair of scores in kShare / 2 is raised by multiplications (exp2_pair).
+#ifndef KSHARE
+#define KSHARE 8
+#endif
+constexpr int kShare = KSHARE;
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct alignas(64) Params {
@@ -82,15 +88,19 @@ struct Shape {
   static constexpr int kQ = 128 * kBlocks * 128;           // bytes of a slot's queries
   static constexpr int kTile = kKeys * kBlocks * 128;      // bytes of a tile
   static constexpr int kScales = E4M3 ? kKeys * 12 : 0;    // of a tile: key scale, log2 and reciprocal of the value scale
-  static constexpr int kRoom = 227 * 1024 - 1024 - 512;    // alignment, barriers
-  static constexpr int ring(int n) { return kSlots * kQ + n * kTile + (n / 2 + 2) * kScales <= kRoom ? n : ring(n - 1); }
+  static constexpr int kRaw = E4M3 ? kKeys * (D + 8) : 0;  // of a tile as it is cached: codes, key and value scales
+  static constexpr int kRaws = 3;
+  static constexpr int kRoom = 227 * 1024 - 3072;          // beside the block's Notes
+  static constexpr int bytes(int n) { return kSlots * kQ + n * kTile + (n / 2 + 2) * kScales + kRaws * kRaw; }
+  static constexpr int ring(int n) { return n == 3 || bytes(n) <= kRoom ? n : ring(n - 1); }
   static constexpr int kRing = ring(8);
   static constexpr int kScaleRing = kRing / 2 + 2;
-  static constexpr int kSmem = kSlots * kQ + kRing * kTile + kScaleRing * kScales + 1024;
+  static constexpr int kSmem = bytes(kRing) + 3072;
+  static constexpr int kHalf = kKeys / 2;                  // columns of a thread
   static constexpr int kBuffer = kKeys;                    // tensor-memory columns of one of the two score buffers
   static constexpr int kSum = 2 * kKeys;                   // first column of the sums
   static constexpr int kColumns = 512;
-  static_assert(kRing >= 4 && kSum + kSlots * D <= kColumns, "");
+  static_assert(bytes(kRing) <= kRoom && kSum + kSlots * D <= kColumns, "");
 };
 
 // Device-wide facts of a request.
@@ -140,44 +150,47 @@ __device__ __forceinline__ int tiles_of(const Params& P, const Request& r) {
 
 struct Edge { int req, head, tile; long long start; int iters; };
 
-// The items of this block's share, in order.  Every warp that works on them walks them
-// alike, with its own walk in shared memory: only what a loop uses is held in registers.
+// A block's share of the order, and everybody's.
+struct Share {
+  long long lo, hi, size, more;        // the first `more` blocks have size + 1, the others size
+  __device__ __forceinline__ int block_of(long long x) const {
+    return static_cast<int>(x < more * (size + 1) ? x / (size + 1) : more + (x - more * (size + 1)) / size);
+  }
+};
+
+// The items of this block's share, in order.  Every role of warps walks them alike, with
+// walks in shared memory: only what a loop uses is held in registers.
 template <int D, bool E4M3>
 struct Walk {
   using S = Shape<D, E4M3>;
-  long long lo, hi, at, share, more;
+  long long at;                        // place of the item in the order
   Request r;
   int req, head, tile, tiles, iters;
   // the present item's part
   int row0, rows, keys, jb, je, je0;   // key tiles [jb, je); of the first slot of two halves [jb, je0)
   int first_block, parts;
-  bool fresh, few, whole;
+  bool fresh, few, whole, found;
 
-  __device__ __forceinline__ void begin(const Params& P, const Edge& edge, const long long* bounds) {
-    if ((threadIdx.x & 31) == 0) {
-      lo = bounds[0]; hi = bounds[1]; share = bounds[2]; more = bounds[3];
-      req = edge.req; head = edge.head; tile = edge.tile; at = edge.start;
-      fresh = true;
-      if (req < P.cache.batch) {
-        r = request<S::kKeys>(P, req);
-        tiles = tiles_of<D, E4M3>(P, r);
-      }
+  // By one thread.
+  __device__ __forceinline__ void begin(const Params& P, const Edge& edge) {
+    req = edge.req; head = edge.head; tile = edge.tile; at = edge.start;
+    fresh = true;
+    if (req < P.cache.batch) {
+      r = request<S::kKeys>(P, req);
+      tiles = tiles_of<D, E4M3>(P, r);
     }
+  }
+  // The next item with work for this block; false behind the last.  For a warp with a walk
+  // of its own.
+  __device__ __forceinline__ bool next(const Params& P, const Share& share) {
     __syncwarp();
-  }
-  // The next item with work for this block; false behind the last.  Called by whole warps.
-  __device__ __forceinline__ bool next(const Params& P) {
+    if ((threadIdx.x & 31) == 0) found = advance(P, share);
     __syncwarp();
-    bool found = false;
-    if ((threadIdx.x & 31) == 0) found = advance(P);
-    return __shfl_sync(0xFFFFFFFFu, found, 0);               // and orders what lane 0 wrote
+    return found;
   }
-
- private:
-  __device__ __forceinline__ int block_of(long long x) const {
-    return static_cast<int>(x < more * (share + 1) ? x / (share + 1) : more + (x - more * (share + 1)) / share);
-  }
-  __device__ __forceinline__ bool advance(const Params& P) {
+  // By one thread.
+  __device__ __forceinline__ bool advance(const Params& P, const Share& share) {
+    const long long lo = share.lo, hi = share.hi;
     while (true) {
       if (!fresh) {
         at += iters + kItemCost;
@@ -211,9 +224,11 @@ struct Walk {
         i0 = static_cast<int>(min(max(lo - begin, 0ll), static_cast<long long>(t.iters)));
         i1 = static_cast<int>(min(max(hi - begin, 0ll), static_cast<long long>(t.iters)));
         if (i0 >= i1) continue;
-        first_block = block_of(begin);
-        parts = block_of(begin + t.iters - 1) - first_block + 1;
-        whole = parts == 1;
+        whole = i0 == 0 && i1 == t.iters;
+        if (!whole) {
+          first_block = share.block_of(begin);
+          parts = share.block_of(begin + t.iters - 1) - first_block + 1;
+        }
       }
       row0 = t.row0; rows = t.rows; keys = t.keys; few = t.few;
       jb = few ? 2 * i0 : i0;
@@ -236,6 +251,9 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void st16(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -250,10 +268,32 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// keeps a NaN
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+// 2^a and 2^b for arguments below 128, -127 and less to zero, by multiplications: 2^n 2^f with
+// n = round(x) and a polynomial of degree 4 for 2^f on [-1/2, 1/2] that is 1 at zero (its
+// relative error, minimised in the maximum, is at most 2.9e-6); n comes out of the sum x + 1.5 2^23
+// in its low bits, and goes into the exponent.  The exponential's unit does 16 a clock
+// on an SM, which is as long as the products take.
+__device__ __forceinline__ void exp2_pair(float& a, float& b) {
+  constexpr float kMagic = 12582912.0f;
+  a = fmaxf(a, -127.0f);
+  b = fmaxf(b, -127.0f);
+  const uint64_t x = tc::two(a, b), t = tc::add2(x, tc::two(kMagic, kMagic));
+  const uint64_t f = tc::fma2(tc::add2(t, tc::two(-kMagic, -kMagic)), tc::two(-1.0f, -1.0f), x);
+  uint64_t p = tc::fma2(f, tc::two(0x1.3a02ccp-7f, 0x1.3a02ccp-7f), tc::two(0x1.c9fc46p-5f, 0x1.c9fc46p-5f));
+  p = tc::fma2(f, p, tc::two(0x1.ec0378p-3f, 0x1.ec0378p-3f));
+  p = tc::fma2(f, p, tc::two(0x1.62e12cp-1f, 0x1.62e12cp-1f));
+  p = tc::fma2(f, p, tc::two(1.0f, 1.0f));
+  float pa, pb, ta, tb;
+  tc::apart(p, pa, pb);
+  tc::apart(t, ta, tb);
+  a = __uint_as_float(__float_as_uint(pa) + (__float_as_uint(ta) << 23));
+  b = __uint_as_float(__float_as_uint(pb) + (__float_as_uint(tb) << 23));
 }
 __device__ __forceinline__ float lg2(float x) {
   float r;
@@ -265,6 +305,15 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// A barrier of `threads` threads that tells all of them whether one said so.
+__device__ __forceinline__ bool any_of(int id, int threads, bool said) {
+  uint32_t r;
+  asm volatile("{ .reg .pred p, q; setp.ne.u32 q, %3, 0; barrier.cta.red.or.pred p, %1, %2, q; selp.u32 %0, 1, 0, p; }"
+               : "=r"(r) : "r"(id), "r"(threads), "r"(static_cast<uint32_t>(said)) : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ void sync_some(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 // The block's barriers.
@@ -275,23 +324,32 @@ struct Bars {
   unsigned long long s_full[2], p_full[2], pv_done[2];
 };
 
+// What the block keeps beside tiles.
+template <int D, bool E4M3>
+struct Notes {
+  Bars<D, E4M3> bars;
+  Edge edge[2];
+  Share share;
+  uint32_t tmem;
+  int failed, flag;
+  Walk<D, E4M3> walk[2 + kLoadWarps + 1];                     // of the softmax slots, the loaders, the issuer
+  float other[2][2][128];                                     // between the two threads of a row
+};
+
 template <int DT, bool E4M3, int D>
 __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ Params P) {
   using S = Shape<D, E4M3>;
   constexpr int HT = E4M3 ? static_cast<int>(ECAH_DTYPE_F16) : DT;   // operand type of the products
   constexpr float lift = HT == ECAH_DTYPE_F16 ? kLift : 0.0f;
   constexpr int kKeys = S::kKeys, kRing = S::kRing, kSlots = S::kSlots;
-  extern __shared__ unsigned char smem_raw[];
-  __shared__ Bars<D, E4M3> s_bars;
-  __shared__ Edge s_edge[2];
-  __shared__ long long s_bounds[4];
-  __shared__ uint32_t s_tmem;
-  __shared__ int s_failed, s_flag;
-  __shared__ Walk<D, E4M3> s_walk[kIssuer + 1];
+  extern __shared__ __align__(1024) unsigned char base_p[];   // the swizzle goes by addresses
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
-  unsigned char* base_p = smem_raw + (base - tc::smem_u32(smem_raw));
-  const uint32_t s_q = base, s_ring = base + kSlots * S::kQ, s_scales = s_ring + kRing * S::kTile;
+  const uint32_t base = tc::smem_u32(base_p);
+  Notes<D, E4M3>& notes = *reinterpret_cast<Notes<D, E4M3>*>(base_p + S::bytes(kRing));
+  static_assert(sizeof(Notes<D, E4M3>) <= 3072 && S::bytes(kRing) % 16 == 0, "");
+  Bars<D, E4M3>& s_bars = notes.bars;
+  const uint32_t s_q = base, s_ring = base + kSlots * S::kQ, s_scales = s_ring + kRing * S::kTile,
+                 s_raw = s_scales + S::kScaleRing * S::kScales;
   const kv::Cache& C = P.cache;
 
   grid_start();
@@ -299,17 +357,17 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
   // ---- barriers, tensor memory
   if (tid == 0) {
     auto init = [&](unsigned long long* b, int n) { tc::bar_init(tc::smem_u32(b), n); };
-    init(&s_bars.q_full, E4M3 ? 4 * kSlots : 4);
+    init(&s_bars.q_full, E4M3 ? 8 * kSlots : kLoadWarps);
     init(&s_bars.q_empty, 1);
     init(&s_bars.done, 1);
-    for (int i = 0; i < kRing; ++i) { init(&s_bars.kv_full[i], 4); init(&s_bars.kv_empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { init(&s_bars.s_full[i], 1); init(&s_bars.p_full[i], 4); init(&s_bars.pv_done[i], 1); }
+    for (int i = 0; i < kRing; ++i) { init(&s_bars.kv_full[i], kLoadWarps); init(&s_bars.kv_empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { init(&s_bars.s_full[i], 1); init(&s_bars.p_full[i], 8); init(&s_bars.pv_done[i], 1); }
     tc::fence_smem();
-    s_failed = 0;
-    s_edge[0].req = s_edge[1].req = C.batch;
-    s_edge[0].start = s_edge[1].start = 0;
+    notes.failed = 0;
+    notes.edge[0].req = notes.edge[1].req = C.batch;
+    notes.edge[0].start = notes.edge[1].start = 0;
   }
-  if (warp == kIssuer) tc::tmem_alloc(tc::smem_u32(&s_tmem), S::kColumns);
+  if (warp == kIssuer) tc::tmem_alloc(tc::smem_u32(&notes.tmem), S::kColumns);
 
   // ---- this block's share.  An item costs kItemCost units, then one an iteration; the
   // first `more` blocks take share + 1 units, the others share.
@@ -399,7 +457,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
               const int l = __ffs(past) - 1;
               p += __shfl_sync(0xFFFFFFFFu, inc - c, l);
               iters = __shfl_sync(0xFFFFFFFFu, iters, l);
-              if (lane == 0) s_edge[warp] = Edge{b0 + i, head, t0 + l, p, iters};
+              if (lane == 0) notes.edge[warp] = Edge{b0 + i, head, t0 + l, p, iters};
               break;
             }
             p += __shfl_sync(0xFFFFFFFFu, inc, 31);
@@ -413,21 +471,21 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
     if (tid == 0) {
       // an edge inside an item that is not divided moves to the item's nearer end
       for (int e = 0; e < 2; ++e) {
-        const Edge& g = s_edge[e];
+        const Edge& g = notes.edge[e];
         if (busy && g.req < C.batch && g.iters <= kWhole) {
           const long long cost = g.iters + kItemCost, into = edge[e] - g.start;
           edge[e] = g.start + (2 * into < cost ? 0 : cost);
         }
-        s_bounds[e] = edge[e];
       }
-      s_bounds[2] = share;
-      s_bounds[3] = more;
+      notes.share = Share{edge[0], edge[1], share, more};
+      notes.walk[0].begin(P, notes.edge[0]);
+      for (auto& w : notes.walk) w = notes.walk[0];
     }
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
   }
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = notes.tmem;
 
   // Waits for a phase of a barrier; false when it ran out, here or in another warp: the
   // block then ends as fast as it can, and its results are NaN.
@@ -436,99 +494,108 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
     bool ok = false;
     for (int i = 0; i < P.tries && !ok; ++i) {
       ok = tc::bar_test(bar, parity);
-      if (!ok && *static_cast<volatile int*>(&s_failed)) break;
+      if (!ok && *static_cast<volatile int*>(&notes.failed)) break;
     }
     ok = __all_sync(0xFFFFFFFFu, ok);
-    if (!ok) *static_cast<volatile int*>(&s_failed) = 1;
+    if (!ok) *static_cast<volatile int*>(&notes.failed) = 1;
     return ok;
   };
 
-  Walk<D, E4M3>& w = s_walk[min(warp, kIssuer)];
-  if (warp <= kIssuer) w.begin(P, s_edge[0], s_bounds);
+  // a slot's 8 warps share a walk
+  Walk<D, E4M3>& w = notes.walk[warp < kLoaders ? warp >> 3 : warp - kLoaders + 2];
 
-  if (warp < 4 * kSlots) {
+  if (warp < 8 * kSlots) {
     // =============================================================== softmax
-    const int slot = warp >> 2, row = tid & 127;
+    regs_up<kSlots == 2 ? 104 : 136>();
+    const int slot = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
+    const int pair = 1 + slot * 4 + (warp & 3);               // the barrier of the two warps of these rows
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
-    const uint32_t sum_at = lanes + S::kSum + slot * D;
+    const uint32_t sum_at = lanes + S::kSum + slot * D + half * (D / 2);   // this thread's half of its row of O
+    constexpr int kC = S::kHalf / 32;
     uint32_t s_phase = 0, q_phase = 0;                        // a bit a buffer
     int before = 0;                                           // key tiles of the items before
     unsigned pv = 0;                                          // products O += P V of this slot so far
+    // A wait that ran out: the warp goes through the motions (its barriers are awaited by
+    // others), and its rows become NaN.
     bool ok = true;
     // The last product so far.  A slot's scores come after its product before, so at most
     // one is outstanding on a barrier; with one slot two are, on barriers in turn.
     auto wait_sum = [&]() {
       const unsigned x = pv - 1;
-      const bool there = kSlots == 2 ? wait(&s_bars.pv_done[slot], x & 1) : wait(&s_bars.pv_done[x & 1], x >> 1 & 1);
+      ok = ok && (kSlots == 2 ? wait(&s_bars.pv_done[slot], x & 1) : wait(&s_bars.pv_done[x & 1], x >> 1 & 1));
       tc::fence_after();
-      return there;
     };
-    while (w.next(P)) {
+    while (true) {
+      sync_some(10 + slot, 256);                              // nobody looks at the item before any more
+      if ((tid & 255) == 0) w.found = w.advance(P, notes.share);
+      sync_some(10 + slot, 256);
+      if (!w.found) break;
       const bool own_rows = kSlots == 2 && !w.few;            // slots are halves of the rows
       const int my = (own_rows ? slot * 128 : 0) + row;       // row of the item
       const bool live = my < w.rows;
       const int packed = w.row0 + my;
       const int token = live ? packed / P.group : 0, head = w.head * P.group + packed - token * P.group;
-      const int lim = live ? sees(P, w.r, token) : w.keys;   // other rows' scores are zeros, and not used
+      const int lim = live ? sees(P, w.r, token) : w.keys;    // other rows' scores are zeros, and not used
       const int least = __reduce_min_sync(0xFFFFFFFFu, lim);
       float scale = P.scale;
 
-      if (E4M3 && w.jb < w.je && ok) {
-        // This thread's row of queries, scaled by a power of two to a largest magnitude in
-        // [1, 2) so that bf16 queries fit f16's range; the power goes into the score scale.
-        if (ok) ok = wait(&s_bars.q_empty, q_phase ^ 1);
+      if (E4M3 && w.jb < w.je) {
+        // A row of queries, scaled by a power of two to a largest magnitude in [1, 2) so
+        // that bf16 queries fit f16's range; the power goes into the score scale.
+        ok = ok && wait(&s_bars.q_empty, q_phase ^ 1);
         q_phase ^= 1;
-        if (ok) {
-          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.q) + (w.r.q0 + token) * P.q_tok + head * P.q_head);
-          float big = 0.0f;
-          if (live) {
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.q) + (w.r.q0 + token) * P.q_tok + head * P.q_head);
+        float big = 0.0f;
+        if (live) {
 #pragma unroll 8
-            for (int c = 0; c < D / 8; ++c) {
-              const uint4 v = src[c];
-              const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+          for (int c = 0; c < D / 8; ++c) {
+            const uint4 v = src[c];
+            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                big = fmaxf(big, fmaxf(fabsf(DType<DT>::to_f32(u[i] & 0xFFFFu)), fabsf(DType<DT>::to_f32(u[i] >> 16))));
-            }
+            for (int i = 0; i < 4; ++i)
+              big = fmaxf(big, fmaxf(fabsf(DType<DT>::to_f32(u[i] & 0xFFFFu)), fabsf(DType<DT>::to_f32(u[i] >> 16))));
           }
-          const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100), 100);
-          const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-          scale = P.scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-          if (own_rows || slot == 0) {
-            const uint32_t dst = s_q + (own_rows ? slot : 0) * S::kQ + row * 128;
-#pragma unroll 8
-            for (int c = 0; c < D / 8; ++c) {
-              const uint4 v = live ? src[c] : make_uint4(0, 0, 0, 0);
-              const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-              uint32_t h[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) h[i] = pack2<HT>(DType<DT>::to_f32(u[i] & 0xFFFFu) * down, DType<DT>::to_f32(u[i] >> 16) * down);
-              st16(dst + (c / 8) * (128 * 128) + ((c % 8) ^ (row & 7)) * 16, h[0], h[1], h[2], h[3]);
-            }
-          }
-          tc::fence_smem();
-          __syncwarp();
-          if (lane == 0) tc::bar_arrive(tc::smem_u32(&s_bars.q_full));
         }
+        const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23) - 127, -100), 100);
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        scale = P.scale * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        if ((own_rows || slot == 0) && ok) {
+          const uint32_t dst = s_q + (own_rows ? slot : 0) * S::kQ + row * 128;
+#pragma unroll 4
+          for (int c = half; c < D / 8; c += 2) {
+            const uint4 v = live ? src[c] : make_uint4(0, 0, 0, 0);
+            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+            uint32_t h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = pack2<HT>(DType<DT>::to_f32(u[i] & 0xFFFFu) * down, DType<DT>::to_f32(u[i] >> 16) * down);
+            st16(dst + (c / 8) * (128 * 128) + ((c % 8) ^ (row & 7)) * 16, h[0], h[1], h[2], h[3]);
+          }
+        }
+        tc::fence_smem();
+        __syncwarp();
+        if (lane == 0) tc::bar_arrive(tc::smem_u32(&s_bars.q_full));
       }
 
-      float m = -INFINITY, l = 0.0f;
+      float m = -INFINITY, l = 0.0f;                          // l: of this thread's columns
       bool any = false;                                       // the sum holds something
       const int step = own_rows || kSlots == 1 ? 1 : 2, jb = w.jb, je = own_rows && slot == 0 ? w.je0 : w.je;
       int buf = kSlots == 2 ? slot : 0;
-      for (int j = jb + (own_rows || kSlots == 1 ? 0 : slot); j < je && ok; j += step) {
-        ok = wait(&s_bars.s_full[buf], s_phase >> buf & 1);
-        if (!ok) break;
+      for (int j = jb + (own_rows || kSlots == 1 ? 0 : slot); j < je; j += step) {
+        ok = ok && wait(&s_bars.s_full[buf], s_phase >> buf & 1);
         s_phase ^= 1u << buf;
         tc::fence_after();
         const uint32_t s_at = lanes + buf * S::kBuffer;
-        // Scores in log2 units; an e4m3 value's scale goes into its weight through the
-        // exponent (weight 2^(s + log2 scale - m)), and the sum takes it back out.  They are
-        // read twice, 32 at a time: a row's 128 do not fit beside the rest in the registers.
-        const float* sc = reinterpret_cast<const float*>(base_p + (s_scales - base) + ((before + j - jb) % S::kScaleRing) * S::kScales);
+        const int c0 = half * S::kHalf;
+        const float* sc = reinterpret_cast<const float*>(base_p + (s_scales - base) + ((before + j - jb) % S::kScaleRing) * S::kScales) + c0;
         const bool masked = (j + 1) * kKeys > least;
-        const int left = lim - j * kKeys;
-        auto ready = [&](uint32_t (&r)[32], int i) {
+        const int left = lim - j * kKeys - c0;
+        // 32 scores in log2 units (16-bit rows: without their scale); an e4m3 value's scale goes
+        // into its weight through the exponent (weight 2^(s + log2 scale - m)), and the sum
+        // takes it back out.
+        auto read = [&](uint32_t (&r)[32], int i) {
+          tc::load32(r, s_at + c0 + 32 * i);
+          tc::load_wait();
+          tc::pin32(r);
           if (E4M3) {
 #pragma unroll
             for (int c = 0; c < 32; c += 4) {
@@ -544,60 +611,23 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
               if (32 * i + c >= left) r[c] = 0xFF800000u;
           }
         };
-        uint32_t ra[32], rb[32];
-        float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
+        auto largest = [&](const uint32_t (&r)[32], float top) {
+          float t0 = top, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kKeys / 32; i += 2) {
-          tc::load32(ra, s_at + 32 * i);
-          tc::load32(rb, s_at + 32 * i + 32);
-          tc::load_wait();
-          tc::pin32(ra);
-          tc::pin32(rb);
-          ready(ra, i);
-          ready(rb, i + 1);
-#pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            t0 = max3(t0, __uint_as_float(ra[c]), __uint_as_float(rb[c]));
-            t1 = max3(t1, __uint_as_float(ra[c + 1]), __uint_as_float(rb[c + 1]));
-            t2 = max3(t2, __uint_as_float(ra[c + 2]), __uint_as_float(rb[c + 2]));
-            t3 = max3(t3, __uint_as_float(ra[c + 3]), __uint_as_float(rb[c + 3]));
+          for (int c = 0; c < 32; c += 8) {
+            t0 = max3(t0, __uint_as_float(r[c]), __uint_as_float(r[c + 1]));
+            t1 = max3(t1, __uint_as_float(r[c + 2]), __uint_as_float(r[c + 3]));
+            t2 = max3(t2, __uint_as_float(r[c + 4]), __uint_as_float(r[c + 5]));
+            t3 = max3(t3, __uint_as_float(r[c + 6]), __uint_as_float(r[c + 7]));
           }
-        }
-        float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
-        if (!E4M3) top *= P.scale;
-        if (__any_sync(0xFFFFFFFFu, top > m + (kLazy + lift))) {
-          const float v = fmaxf(top - lift, m), f = m == v ? 1.0f : ex2_approx(m - v);
-          m = v;
-          l *= f;
-          if (any) {                                          // the row of O, once the product before is in it
-            ok = wait_sum();
-            if (!ok) break;
-#pragma unroll 1
-            for (int d = 0; d < D; d += 32) {
-              uint32_t o[32];
-              tc::load32(o, sum_at + d);
-              tc::load_wait();
-              tc::pin32(o);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tc::store32(sum_at + d, o);
-            }
-          }
-        }
-        tc::load32(ra, s_at);
-        const float ref = m == -INFINITY ? 0.0f : m;
-        const uint64_t scale2 = tc::two(P.scale, P.scale), ref2 = tc::two(-ref, -ref);
-        uint64_t sum0 = 0, sum1 = 0;                          // four chains
-#pragma unroll
-        for (int i = 0; i < kKeys / 32; ++i) {
-          uint32_t (&r)[32] = i & 1 ? rb : ra;
-          tc::load_wait();
-          tc::pin32(r);
-          if (i + 1 < kKeys / 32) tc::load32(i & 1 ? ra : rb, s_at + 32 * i + 32);
-          ready(r, i);
+          return max3(max_nan(t0, t1), t2, t3);
+        };
+        uint32_t w16[kC][16];
+        uint64_t sum0, sum1;                                  // four chains
+        auto weigh = [&](const uint32_t (&r)[32], int i, float ref) {
           // A weight is off by at most 2^-9 of itself in bf16 (2^-12 in f16), at random over the
           // keys; the sum takes it as it was.
-          uint32_t w16[16];
+          const uint64_t scale2 = tc::two(P.scale, P.scale), ref2 = tc::two(-ref, -ref);
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
             const uint64_t a = tc::two(__uint_as_float(r[c]), __uint_as_float(r[c + 1]));
@@ -605,8 +635,14 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
             float p[4];
             tc::apart(E4M3 ? tc::add2(a, ref2) : tc::fma2(a, scale2, ref2), p[0], p[1]);
             tc::apart(E4M3 ? tc::add2(b, ref2) : tc::fma2(b, scale2, ref2), p[2], p[3]);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) p[x] = ex2_approx(p[x]);
+            p[0] = ex2_approx(p[0]);
+            p[1] = ex2_approx(p[1]);
+            if (c % kShare < 4) {                             // of some pairs by multiplications
+              exp2_pair(p[2], p[3]);
+            } else {
+              p[2] = ex2_approx(p[2]);
+              p[3] = ex2_approx(p[3]);
+            }
             if (E4M3) {
               const float4 inv = *reinterpret_cast<const float4*>(sc + 2 * kKeys + 32 * i + c);
               sum0 = tc::fma2(tc::two(p[0], p[1]), tc::two(inv.x, inv.y), sum0);
@@ -615,11 +651,59 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
               sum0 = tc::add2(tc::two(p[0], p[1]), sum0);
               sum1 = tc::add2(tc::two(p[2], p[3]), sum1);
             }
-            w16[c / 2] = pack2<HT>(p[0], p[1]);
-            w16[c / 2 + 1] = pack2<HT>(p[2], p[3]);
+            w16[i][c / 2] = pack2<HT>(p[0], p[1]);
+            w16[i][c / 2 + 1] = pack2<HT>(p[2], p[3]);
           }
-          tc::store16(s_at + 16 * i, w16);
+        };
+        // The reference of the tiles before nearly always serves (scores pass it by less than
+        // 2^kLazy): weights are computed with it while the largest score is found, and again
+        // where it did not.
+        float top = -INFINITY;
+        sum0 = sum1 = 0;
+        {
+          const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+          for (int i = 0; i < kC; ++i) {
+            uint32_t r[32];
+            read(r, i);
+            top = largest(r, top);
+            if (any) weigh(r, i, ref);
+          }
         }
+        if (!E4M3) top *= P.scale;
+        if (any_of(pair, 64, !any || !(top <= m + (kLazy + lift)))) {
+          notes.other[slot][half][row] = top;
+          sync_some(pair, 64);
+          top = max_nan(top, notes.other[slot][half ^ 1][row]);
+          const float v = fmaxf(top - lift, m), f = m == v ? 1.0f : ex2_approx(m - v);
+          m = v;
+          l *= f;
+          if (any) {                                          // the row of O, once the product before is in it
+            wait_sum();
+#pragma unroll 1
+            for (int d = 0; d < D / 2; d += 16) {
+              uint32_t o[16];
+              tc::load16(o, sum_at + d);
+              tc::load_wait();
+              tc::pin16(o);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tc::store16(sum_at + d, o);
+            }
+          }
+          // a NaN or an infinite score makes the row NaN, whichever way its weight is computed
+          const float ref = !(top < INFINITY) ? NAN : m == -INFINITY ? 0.0f : m;
+          sum0 = sum1 = 0;
+#pragma unroll
+          for (int i = 0; i < kC; ++i) {
+            uint32_t r[32];
+            read(r, i);
+            weigh(r, i, ref);
+          }
+          sync_some(pair, 64);                                // both have read the scores that the weights lie over
+        }
+#pragma unroll
+        for (int i = 0; i < kC; ++i) tc::store16(s_at + c0 / 2 + 16 * i, w16[i]);
         {
           float l0, l1;
           tc::apart(tc::add2(sum0, sum1), l0, l1);
@@ -634,8 +718,11 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         if (kSlots == 1) buf ^= 1;
       }
       before += max(w.je - jb, 0);
-      if (any && ok) ok = wait_sum();
+      if (any) wait_sum();
       if (!ok) l = NAN;
+      notes.other[slot][half][row] = l;
+      sync_some(pair, 64);
+      l += notes.other[slot][half ^ 1][row];
 
       // ---- the item's rows, or this part of them
       const bool joined = !w.whole || w.few;                  // more than one sum to a row
@@ -644,46 +731,45 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
       if (!joined) {
         // a sum of zero (no key has mass) gives zeros
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        uint16_t* o = static_cast<uint16_t*>(P.out) + (w.r.q0 + token) * P.o_tok + head * P.o_head;
-        if (live && P.lse) P.lse[static_cast<long long>(w.r.q0 + token) * P.hq + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+        uint16_t* o = static_cast<uint16_t*>(P.out) + (w.r.q0 + token) * P.o_tok + head * P.o_head + half * (D / 2);
+        if (live && half == 0 && P.lse)
+          P.lse[static_cast<long long>(w.r.q0 + token) * P.hq + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 #pragma unroll 1
-        for (int d = 0; d < D; d += 32) {
-          uint32_t x[32];
-          if (any && ok) {
-            tc::load32(x, sum_at + d);
+        for (int d = 0; d < D / 2; d += 16) {
+          uint32_t x[16] = {};
+          if (any) {
+            tc::load16(x, sum_at + d);
             tc::load_wait();
-            tc::pin32(x);
+            tc::pin16(x);
           }
-          const bool none = !any || l == 0.0f;
-          uint32_t h[16];
+          uint32_t h[8];
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            h[i] = !ok ? pack2<DT>(NAN, NAN) : none ? 0u : pack2<DT>(__uint_as_float(x[2 * i]) * inv, __uint_as_float(x[2 * i + 1]) * inv);
+          for (int i = 0; i < 8; ++i) h[i] = l == 0.0f ? 0u : pack2<DT>(__uint_as_float(x[2 * i]) * inv, __uint_as_float(x[2 * i + 1]) * inv);
           if (live) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(o + d + 8 * i) = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+            *reinterpret_cast<uint4*>(o + d) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(o + d + 8) = make_uint4(h[4], h[5], h[6], h[7]);
           }
         }
         tc::fence_before();
       } else {
         const long long at = static_cast<long long>(part_slot(part)) * S::kRows + slot * 128 + row;
-        if (live) P.part_ml[at] = make_float2(any || !ok ? m : -INFINITY, l);
-        float* o = P.part_o + at * D;
+        if (live && half == 0) P.part_ml[at] = make_float2(m, l);
+        float* o = P.part_o + at * D + half * (D / 2);
 #pragma unroll 1
-        for (int d = 0; d < D && any && ok; d += 32) {
-          uint32_t x[32];
-          tc::load32(x, sum_at + d);
+        for (int d = 0; d < D / 2 && any; d += 16) {
+          uint32_t x[16];
+          tc::load16(x, sum_at + d);
           tc::load_wait();
-          tc::pin32(x);
+          tc::pin16(x);
           if (live) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(o + d + 4 * i) = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(o + d + 4 * i) = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
           }
         }
         tc::fence_before();
         // the last part's block joins them all; a whole item's two sums are joined here
         const int parts = w.parts;
-        sync_some(1, 128 * kSlots);
+        sync_some(9, 256 * kSlots);
         if (tid == 0) {
           bool last = true;
           if (parts > 1) {
@@ -693,14 +779,14 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
             last = n + 1u == static_cast<unsigned>(parts);
             if (last) *counter = 0u;
           }
-          s_flag = last;
+          notes.flag = last;
         }
-        sync_some(1, 128 * kSlots);
-        const bool mine = *static_cast<volatile int*>(&s_flag) != 0;
+        sync_some(9, 256 * kSlots);
+        const bool mine = *static_cast<volatile int*>(&notes.flag) != 0;
         if (mine) {
           // A warp to a row; triple x of a row is part x, or of few rows part x / 2, slot x % 2.
           const int sums = w.few ? 2 * parts : parts;
-          for (int rr = warp; rr < w.rows; rr += 4 * kSlots) {
+          for (int rr = warp; rr < w.rows; rr += 8 * kSlots) {
             auto where = [&](int x) {
               const int p = w.few ? x >> 1 : x;
               return static_cast<long long>(part_slot(p)) * S::kRows + (w.few ? (x & 1) * 128 : 0) + rr;
@@ -746,12 +832,12 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
             if (P.lse && lane == 0) P.lse[static_cast<long long>(w.r.q0 + tok) * P.hq + hd] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * kLn2;
           }
         }
-        sync_some(1, 128 * kSlots);                           // the flag and the part's room are free again
+        sync_some(9, 256 * kSlots);                           // the flag and the part's room are free again
       }
     }
-  } else if (warp >= kLoaders && warp < kLoaders + 4) {
+  } else if (warp >= kLoaders && warp < kLoaders + kLoadWarps) {
     // ================================================ keys and values to the ring
-    constexpr int kMine = kKeys / 4;                          // rows of a warp
+    regs_down<64>();
     const int wl = warp - kLoaders;
     unsigned n = 0, tiles = 0;                                // loads, key tiles so far
     uint32_t q_phase = 0;
@@ -771,7 +857,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
     };
     auto free_slot = [&]() { return wait(&s_bars.kv_empty[n % kRing], ((n / kRing) & 1) ^ 1); };
 
-    while (ok && w.next(P)) {
+    while (ok && w.next(P, notes.share)) {
       if (w.jb >= w.je) continue;
       const bool shared = kSlots == 2 && !w.few;
       if (!E4M3) {                                            // the item's queries
@@ -780,7 +866,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         ok = wait(&s_bars.q_empty, q_phase ^ 1);
         q_phase ^= 1;
         if (!ok) break;
-        for (int g = wl; g < (shared ? 8 : 4); g += 4) {      // 32 rows at a time
+        for (int g = wl; g < (shared ? 8 : 4); g += kLoadWarps) {   // 32 rows at a time
           const int my = 32 * g + lane;
           long long off = -1;
           if (my < w.rows) {
@@ -807,26 +893,48 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
       const int* pages = C.indices + w.r.first;
       const int len = w.r.len, head = w.head, je = w.je;
       auto nth_page = [&](int key) { return P.page_shift >= 0 ? key >> P.page_shift : key / C.page_size; };
-      const int ahead = shared ? 1 : 2;
-      int page_next = 0;
-      auto page_of = [&](int j) -> int {
-        const int key = j * kKeys + wl * kMine + lane;
-        return lane < kMine && j < je && key < len ? min(max(pages[nth_page(key)], 0), C.num_pages - 1) : -1;
-      };
-      // the next loads in order: K jb .. (ahead of them), then V j, K j + ahead
+      const int ahead = shared ? 1 : 2, loads = 2 * (je - w.jb);
+      // the loads in order: K jb .. (ahead of them), then V j, K j + ahead
       int jk = w.jb, jv = w.jb;
-      page_next = page_of(jk);
-      auto next_load = [&](bool* is_v, int* j, int* page) {
+      auto turn = [&](bool* is_v) {
         *is_v = jk >= je || jk - jv >= ahead;
-        *j = *is_v ? jv++ : jk++;
-        if (*is_v) {
-          *page = page_of(*j);                                // read a while ago: in L1
-        } else {
-          *page = page_next;
-          page_next = page_of(jk);
+        return *is_v ? jv : jk;
+      };
+      // Rows by threads' copies, 16 at a time: groups wl, wl + 3, wl + 6 of a tile.  Lanes find
+      // the rows' places, of two groups at once; past the length there are none, and zeros are
+      // written.
+      constexpr int kGroups = kKeys / 16;
+      struct Places { unsigned off[2]; unsigned live[2]; };
+      auto page_of = [&](int j, int x) -> int {
+        const int g = wl + kLoadWarps * (2 * x + (lane >> 4)), key = j * kKeys + g * 16 + (lane & 15);
+        return g < kGroups && j < je && key < len ? min(max(pages[nth_page(key)], 0), C.num_pages - 1) : -1;
+      };
+      auto place = [&](int j, const int (&page)[2], const kv::Side16& side) {
+        Places p;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int key = j * kKeys + (wl + kLoadWarps * (2 * x + (lane >> 4))) * 16 + (lane & 15);
+          p.off[x] = page[x] < 0 ? 0 : page[x] * side.page + static_cast<unsigned>(key - nth_page(key) * C.page_size) * side.slot + head * side.head;
+          p.live[x] = __ballot_sync(0xFFFFFFFFu, page[x] >= 0);
+        }
+        return p;
+      };
+      constexpr int kChunks = D * (E4M3 ? 1 : 2) / 16, kEach = 16 * kChunks / 32;   // 16-byte chunks of a row; of a lane and group
+      auto copy_rows = [&](const Places& p, const kv::Side16& side, auto to) {
+#pragma unroll
+        for (int gi = 0; gi < (kGroups + kLoadWarps - 1) / kLoadWarps; ++gi) {
+          const int g = wl + kLoadWarps * gi;
+          if (g >= kGroups) break;
+#pragma unroll
+          for (int x = 0; x < kEach; ++x) {
+            const int c = x * 32 + lane, r = c / kChunks, col = c % kChunks, from = (gi & 1) * 16 + r;
+            const unsigned o = __shfl_sync(0xFFFFFFFFu, p.off[gi >> 1], from);
+            const bool there = (p.live[gi >> 1] >> from) & 1u;
+            cp16(to(g * 16 + r, col), side.base + (there ? o + col : 0u) * 16ull, there);
+          }
         }
       };
-      const int loads = 2 * (je - w.jb);
+      int page_next[2] = {page_of(jk, 0), page_of(jk, 1)};    // of the next keys: an L2 read away
       if (!E4M3) {
         // pages of a tile that the copy engine brings, a lane to a page
         const int in_tile = P.boxes ? max(1, kKeys >> P.page_shift) : 0, slots = kKeys / max(1, in_tile);
@@ -834,26 +942,30 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         int box_next = listed(jk);
         for (int i = 0; i < loads; ++i) {
           bool is_v;
-          int j, page;
-          const bool v_next = jk >= je || jk - jv >= ahead;
-          if (P.boxes && ((v_next ? jv : jk) + 1) * kKeys <= len) {
+          const int j = turn(&is_v);
+          const bool boxes_now = P.boxes && (j + 1) * kKeys <= len;
+          int page[2] = {page_next[0], page_next[1]}, at = box_next;
+          if (is_v) {                                         // values' pages were read a while ago: in L1
+            ++jv;
+            if (boxes_now) at = listed(j);
+            else { page[0] = page_of(j, 0); page[1] = page_of(j, 1); }
+          } else {
+            ++jk;
+            box_next = listed(jk);
+            if (!P.boxes || (jk + 1) * kKeys > len) { page_next[0] = page_of(jk, 0); page_next[1] = page_of(jk, 1); }
+          }
+          const uint32_t dst = s_ring + (n % kRing) * S::kTile;
+          if (boxes_now) {
             // a whole tile: boxes of 64 elements by a page's slots, dealt to the warps
-            is_v = v_next;
-            j = is_v ? jv++ : jk++;
-            int at = is_v ? listed(j) : box_next;             // values' pages were read a while ago: in L1
-            if (!is_v) {
-              box_next = listed(jk);
-              if (jk < je && (jk + 1) * kKeys > len) page_next = page_of(jk);
-            }
             at = min(max(at, 0), C.num_pages - 1);
             ok = free_slot();
             if (!ok) break;
-            const uint32_t dst = s_ring + (n % kRing) * S::kTile, bar = tc::smem_u32(&s_bars.kv_full[n % kRing]);
+            const uint32_t bar = tc::smem_u32(&s_bars.kv_full[n % kRing]);
             const void* map = is_v ? &P.v_map : &P.k_map;
-            const int boxes = in_tile * S::kBlocks, mine = (boxes - wl + 3) / 4;
+            const int boxes = in_tile * S::kBlocks, mine = (boxes - wl + kLoadWarps - 1) / kLoadWarps;
             const int slot = (j * kKeys) & (C.page_size - 1);
             if (tc::elect()) tc::bar_expect(bar, mine * slots * 128);
-            for (int x = wl; x < boxes; x += 4) {
+            for (int x = wl; x < boxes; x += kLoadWarps) {
               const int nth = x / S::kBlocks, block = x - nth * S::kBlocks;
               const int pg = __shfl_sync(0xFFFFFFFFu, at, nth);
               if (tc::elect()) tc::copy_box(dst + block * (kKeys * 128) + nth * slots * 128, map, block * 64, slot, head, pg, bar);
@@ -861,23 +973,11 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
             ++n;
             continue;
           }
-          next_load(&is_v, &j, &page);
           const kv::Side16& side = is_v ? P.v : P.k;
-          const int key = j * kKeys + wl * kMine + lane;
-          unsigned off = 0;
-          if (page >= 0) off = page * side.page + static_cast<unsigned>(key - nth_page(key) * C.page_size) * side.slot + head * side.head;
-          const unsigned live = __ballot_sync(0xFFFFFFFFu, page >= 0);
+          const Places p = place(j, page, side);
           ok = free_slot();
           if (!ok) break;
-          const uint32_t dst = s_ring + (n % kRing) * S::kTile + wl * kMine * 128;
-          constexpr int kChunks = D / 8;
-#pragma unroll
-          for (int x = 0; x < kMine * kChunks / 32; ++x) {
-            const int c = x * 32 + lane, r = c / kChunks, col = c % kChunks;
-            const unsigned o = __shfl_sync(0xFFFFFFFFu, off, r);
-            const bool there = (live >> r) & 1u;              // past the length: zeros
-            cp16(dst + (col / 8) * (kKeys * 128) + r * 128 + ((col % 8) ^ (r & 7)) * 16, side.base + (there ? o + col : 0u) * 16ull, there);
-          }
+          copy_rows(p, side, [&](int r, int col) { return dst + (col / 8) * (kKeys * 128) + r * 128 + ((col % 8) ^ (r & 7)) * 16; });
           cp_commit();
           waiting |= static_cast<unsigned long long>(n % kRing) << (8 * told_late);
           ++told_late;
@@ -888,68 +988,87 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
           }
         }
       } else {
-        constexpr int kChunks = D / 16, kEach = kMine * kChunks / 32;
-        uint4 now[kEach], then[kEach];
-        float ks = 0.0f, vs = 0.0f, ks_then = 0.0f, vs_then = 0.0f;
-        bool is_v = false, is_v_then = false;
-        int j_then = 0;
-        bool on = false, on_then = false;
-        auto fetch = [&]() {
-          int page;
-          next_load(&is_v_then, &j_then, &page);
-          const kv::Side16& side = is_v_then ? P.v : P.k;
-          const int key = j_then * kKeys + wl * kMine + lane;
-          unsigned off = 0;
-          on_then = page >= 0;
-          ks_then = vs_then = 0.0f;
-          if (on_then) {
-            const int slot = key - nth_page(key) * C.page_size;
-            off = page * side.page + static_cast<unsigned>(slot) * side.slot + head * side.head;
-            if (!is_v_then) {
-              const long long at = (static_cast<long long>(page) * C.heads + head) * C.page_size + slot;
-              ks_then = P.k.scale[at];
-              vs_then = P.v.scale[at];
+        // Codes and scales as they are cached go to a ring of their own, kRaws - 1 tiles ahead; each
+        // warp converts the rows that it copied.
+        int asked = 0;
+        const unsigned n0 = n;
+        auto ask = [&]() {
+          if (asked < loads) {
+            bool is_v;
+            const int j = turn(&is_v);
+            int page[2] = {page_next[0], page_next[1]};
+            if (is_v) {
+              ++jv;
+              page[0] = page_of(j, 0); page[1] = page_of(j, 1);
+            } else {
+              ++jk;
+              page_next[0] = page_of(jk, 0); page_next[1] = page_of(jk, 1);
+            }
+            const kv::Side16& side = is_v ? P.v : P.k;
+            const uint32_t dst = s_raw + ((n0 + asked) % S::kRaws) * S::kRaw;
+            copy_rows(place(j, page, side), side, [&](int r, int col) { return dst + r * D + col * 16; });
+            if (!is_v) {
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const int g = wl + kLoadWarps * (2 * x + (lane >> 4));
+                if (g >= kGroups) continue;
+                const int key = j * kKeys + g * 16 + (lane & 15);
+                const long long at = page[x] < 0 ? 0 : (static_cast<long long>(page[x]) * C.heads + head) * C.page_size + key - nth_page(key) * C.page_size;
+                const uint32_t to = dst + kKeys * D + (g * 16 + (lane & 15)) * 4;
+                cp4(to, P.k.scale + at, page[x] >= 0);
+                cp4(to + kKeys * 4, P.v.scale + at, page[x] >= 0);
+              }
             }
           }
-          const unsigned live = __ballot_sync(0xFFFFFFFFu, on_then);
-#pragma unroll
-          for (int x = 0; x < kEach; ++x) {
-            const int c = x * 32 + lane, r = c / kChunks, col = c % kChunks;
-            const unsigned o = __shfl_sync(0xFFFFFFFFu, off, r);
-            then[x] = make_uint4(0, 0, 0, 0);
-            if ((live >> r) & 1u) then[x] = __ldcg(reinterpret_cast<const uint4*>(side.base + (static_cast<unsigned long long>(o) + col) * 16ull));
-          }
+          ++asked;
+          cp_commit();
         };
-        fetch();
-        for (int i = 0; i < loads; ++i) {
+        int kk = w.jb, vv = w.jb;                             // the same order again, for what is converted
 #pragma unroll
-          for (int x = 0; x < kEach; ++x) now[x] = then[x];
-          ks = ks_then; vs = vs_then; is_v = is_v_then; on = on_then;
-          if (i + 1 < loads) fetch();
+        for (int x = 0; x < S::kRaws - 1; ++x) ask();
+        for (int i = 0; i < loads; ++i) {
+          const bool is_v = kk >= je || kk - vv >= ahead;
+          if (is_v) ++vv; else ++kk;
+          ask();
+          cp_wait<S::kRaws - 1>();
+          __syncwarp();
           ok = free_slot();
           if (!ok) break;
-          const uint32_t dst = s_ring + (n % kRing) * S::kTile + wl * kMine * 128;
+          const uint32_t dst = s_ring + (n % kRing) * S::kTile;
+          const unsigned char* raw = base_p + (s_raw - base) + (n % S::kRaws) * S::kRaw;
 #pragma unroll
-          for (int x = 0; x < kEach; ++x) {
-            const int c = x * 32 + lane, r = c / kChunks, col = c % kChunks;
-            uint32_t h[8];
-            e4m3x4(now[x].x, h[0], h[1]);
-            e4m3x4(now[x].y, h[2], h[3]);
-            e4m3x4(now[x].z, h[4], h[5]);
-            e4m3x4(now[x].w, h[6], h[7]);
-            const uint32_t row = dst + (col / 4) * (kKeys * 128) + r * 128;
-            const int c0 = (col % 4) * 2;
-            st16(row + (c0 ^ (r & 7)) * 16, h[0], h[1], h[2], h[3]);
-            st16(row + ((c0 + 1) ^ (r & 7)) * 16, h[4], h[5], h[6], h[7]);
+          for (int gi = 0; gi < (kGroups + kLoadWarps - 1) / kLoadWarps; ++gi) {
+            const int g = wl + kLoadWarps * gi;
+            if (g >= kGroups) break;
+#pragma unroll
+            for (int x = 0; x < kEach; ++x) {
+              const int c = x * 32 + lane, r = g * 16 + c / kChunks, col = c % kChunks;
+              const uint4 v = *reinterpret_cast<const uint4*>(raw + r * D + col * 16);
+              uint32_t h[8];
+              e4m3x4(v.x, h[0], h[1]);
+              e4m3x4(v.y, h[2], h[3]);
+              e4m3x4(v.z, h[4], h[5]);
+              e4m3x4(v.w, h[6], h[7]);
+              const uint32_t at = dst + (col / 4) * (kKeys * 128) + r * 128;
+              const int c0 = (col % 4) * 2;
+              st16(at + (c0 ^ (r & 7)) * 16, h[0], h[1], h[2], h[3]);
+              st16(at + ((c0 + 1) ^ (r & 7)) * 16, h[4], h[5], h[6], h[7]);
+            }
           }
-          if (!is_v && lane < kMine) {
-            float* sc = reinterpret_cast<float*>(base_p + (s_scales - base) + (tiles % S::kScaleRing) * S::kScales) + wl * kMine + lane;
-            const float v = max_nan(vs, 8e-28f);              // 2^-90
-            sc[0] = on ? ks : 0.0f;
-            sc[kKeys] = on ? lg2(v) : 0.0f;
-            sc[2 * kKeys] = on ? rcp(v) : 0.0f;
+          if (!is_v) {
+            float* sc = reinterpret_cast<float*>(base_p + (s_scales - base) + (tiles % S::kScaleRing) * S::kScales);
+            const float* cached = reinterpret_cast<const float*>(raw + kKeys * D);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int g = wl + kLoadWarps * (2 * x + (lane >> 4)), r = g * 16 + (lane & 15);
+              if (g >= kGroups) continue;
+              const float v = max_nan(cached[kKeys + r], 8e-28f);   // 2^-90
+              sc[r] = cached[r];
+              sc[kKeys + r] = lg2(v);
+              sc[2 * kKeys + r] = rcp(v);
+            }
+            ++tiles;
           }
-          if (!is_v) ++tiles;
           tell(n % kRing);
           ++n;
         }
@@ -959,6 +1078,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
     while (ok && told_late) tell_oldest();
   } else if (warp == kIssuer) {
     // ================================================================ products
+    regs_down<64>();
     unsigned n = 0, products = 0;                             // loads taken, products O += P V
     uint32_t q_phase = 0, p_phase = 0;                        // a bit a buffer
     bool ok = true;
@@ -999,7 +1119,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
       tc::fence_after();
       return there;
     };
-    while (ok && w.next(P)) {
+    while (ok && w.next(P, notes.share)) {
       const int count = w.je - w.jb, first = w.je0 - w.jb;    // first: tiles of the first half
       if (count <= 0) continue;
       const bool few = w.few;
@@ -1060,6 +1180,8 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
     if (tc::elect()) tc::commit(tc::smem_u32(&s_bars.done));
     __syncwarp();
     for (int i = 0; i < kTries && !tc::bar_test(tc::smem_u32(&s_bars.done), 0); ++i) {}
+  } else {
+    regs_down<64>();
   }
 
   tc::fence_before();
