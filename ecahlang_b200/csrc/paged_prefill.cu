@@ -74,7 +74,7 @@ struct alignas(64) Params {
   float scale;                         // sm_scale * log2 e
   unsigned* counters;                  // [blocks] arrivals, zero between launches
   float2* part_ml;                     // [2 blocks][256]
-  float* part_o;                       // [2 blocks][256][D] (rows of 128 with one slot)
+  float* part_o;                       // [2 blocks][slots][D / 4][128][4]
   kv::Side16 k, v;
   kv::Cache cache;
 };
@@ -305,8 +305,6 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 // A barrier of `threads` threads that tells all of them whether one said so.
 __device__ __forceinline__ bool any_of(int id, int threads, bool said) {
   uint32_t r;
@@ -506,7 +504,6 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
 
   if (warp < 8 * kSlots) {
     // =============================================================== softmax
-    regs_up<kSlots == 2 ? 104 : 136>();
     const int slot = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
     const int pair = 1 + slot * 4 + (warp & 3);               // the barrier of the two warps of these rows
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
@@ -728,6 +725,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
       const bool joined = !w.whole || w.few;                  // more than one sum to a row
       const int first_block = w.first_block, part = static_cast<int>(blockIdx.x) - first_block;
       auto part_slot = [&](int p) { return p == 0 ? 2 * first_block + 1 : 2 * (first_block + p); };
+      auto part_at = [&](int at, int tile) { return reinterpret_cast<uint4*>(P.part_o) + (static_cast<long long>(at) * kSlots + tile) * (D / 4) * 128; };
       if (!joined) {
         // a sum of zero (no key has mass) gives zeros
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -754,7 +752,8 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
       } else {
         const long long at = static_cast<long long>(part_slot(part)) * S::kRows + slot * 128 + row;
         if (live && half == 0) P.part_ml[at] = make_float2(m, l);
-        float* o = P.part_o + at * D + half * (D / 2);
+        // [128 rows' part][D / 4][128][4]: neighbouring rows side by side
+        uint4* o = part_at(part_slot(part), slot) + half * (D / 8) * 128 + row;
 #pragma unroll 1
         for (int d = 0; d < D / 2 && any; d += 16) {
           uint32_t x[16];
@@ -763,7 +762,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
           tc::pin16(x);
           if (live) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(o + d + 4 * i) = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            for (int i = 0; i < 4; ++i) o[(d / 4 + i) * 128] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
           }
         }
         tc::fence_before();
@@ -784,52 +783,52 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         sync_some(9, 256 * kSlots);
         const bool mine = *static_cast<volatile int*>(&notes.flag) != 0;
         if (mine) {
-          // A warp to a row; triple x of a row is part x, or of few rows part x / 2, slot x % 2.
-          const int sums = w.few ? 2 * parts : parts;
-          for (int rr = warp; rr < w.rows; rr += 8 * kSlots) {
-            auto where = [&](int x) {
-              const int p = w.few ? x >> 1 : x;
-              return static_cast<long long>(part_slot(p)) * S::kRows + (w.few ? (x & 1) * 128 : 0) + rr;
-            };
-            float mm = -INFINITY, ll = 0.0f, acc[D / 32];
-            bool bad = false;
-            for (int x = lane; x < sums; x += 32) {
-              const float2 v = __ldcg(P.part_ml + where(x));
-              mm = fmaxf(mm, v.x);
-              bad |= v.y != v.y;
+          // Triple x of a row is part x, or of few rows part x / 2, slot x % 2.  Several threads to a
+          // row, each with some of its columns.
+          const bool fewer = w.few;
+          const int sums = fewer ? 2 * parts : parts;
+          const int spread = fewer ? 4 : 2;                   // threads of a row (with one slot: 256 threads of 128 rows)
+          const int tile = spread == 2 && kSlots == 2 ? tid >> 8 : 0, rr = tid & 127, nth = spread == 4 ? tid >> 7 : tid >> 7 & 1;
+          const int mine_row = tile * 128 + rr;
+          if (mine_row < w.rows) {
+            auto slot_at = [&](int x) { return part_slot(fewer ? x >> 1 : x); };
+            auto half_at = [&](int x) { return fewer ? x & 1 : tile; };
+            auto ml_at = [&](int x) { return __ldcg(P.part_ml + static_cast<long long>(slot_at(x)) * S::kRows + half_at(x) * 128 + rr); };
+            float mm = -INFINITY, ll = 0.0f;
+            for (int x = 0; x < sums; ++x) mm = fmaxf(mm, ml_at(x).x);
+            for (int x = 0; x < sums; ++x) {
+              const float2 v = ml_at(x);
+              ll += v.x == -INFINITY ? (v.y != v.y ? v.y : 0.0f) : v.y * ex2_approx(v.x - mm);
             }
+            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+            const int packed_r = w.row0 + mine_row, tok = packed_r / P.group, hd = w.head * P.group + packed_r - tok * P.group;
+            uint16_t* dst = static_cast<uint16_t*>(P.out) + (w.r.q0 + tok) * P.o_tok + hd * P.o_head;
+            if (P.lse && nth == 0) P.lse[static_cast<long long>(w.r.q0 + tok) * P.hq + hd] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * kLn2;
+            // 16 columns at a time
+            for (int d = nth * 16; d < D; d += spread * 16) {
+              float acc[16];
 #pragma unroll
-            for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, o));
-            bad = __any_sync(0xFFFFFFFFu, bad);
+              for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+#pragma unroll 2
+              for (int x = 0; x < sums; ++x) {
+                const float v = ml_at(x).x, f = v == -INFINITY ? 0.0f : ex2_approx(v - mm);
+                if (f == 0.0f) continue;                      // a sum of nothing was not written
+                const uint4* src = part_at(slot_at(x), half_at(x)) + d / 4 * 128 + rr;
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
-            for (int x0 = 0; x0 < sums; x0 += 32) {
-              float f = 0.0f;
-              if (x0 + lane < sums) {
-                const float2 v = __ldcg(P.part_ml + where(x0 + lane));
-                f = v.x == -INFINITY ? 0.0f : ex2_approx(v.x - mm);
-                ll = fmaf(v.y, f, ll);
-              }
-              const int n = min(32, sums - x0);
-#pragma unroll 4
-              for (int x = 0; x < n; ++x) {
-                const float g = __shfl_sync(0xFFFFFFFFu, f, x);
-                if (g != 0.0f) {                              // a sum of nothing was not written
-                  const float* src = P.part_o + where(x0 + x) * D + lane;
-#pragma unroll
-                  for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(g, __ldcg(src + 32 * i), acc[i]);
+                for (int i = 0; i < 4; ++i) {
+                  const uint4 o = __ldcg(src + i * 128);
+                  acc[4 * i] = fmaf(f, __uint_as_float(o.x), acc[4 * i]);
+                  acc[4 * i + 1] = fmaf(f, __uint_as_float(o.y), acc[4 * i + 1]);
+                  acc[4 * i + 2] = fmaf(f, __uint_as_float(o.z), acc[4 * i + 2]);
+                  acc[4 * i + 3] = fmaf(f, __uint_as_float(o.w), acc[4 * i + 3]);
                 }
               }
+              uint32_t h[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) h[i] = pack2<DT>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+              *reinterpret_cast<uint4*>(dst + d) = make_uint4(h[0], h[1], h[2], h[3]);
+              *reinterpret_cast<uint4*>(dst + d + 8) = make_uint4(h[4], h[5], h[6], h[7]);
             }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) ll += __shfl_xor_sync(0xFFFFFFFFu, ll, o);
-            if (bad) ll = NAN;
-            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-            const int packed_r = w.row0 + rr, tok = packed_r / P.group, hd = w.head * P.group + packed_r - tok * P.group;
-            uint16_t* dst = static_cast<uint16_t*>(P.out) + (w.r.q0 + tok) * P.o_tok + hd * P.o_head + lane;
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) dst[32 * i] = static_cast<uint16_t>(DType<DT>::to_raw(acc[i] * inv));
-            if (P.lse && lane == 0) P.lse[static_cast<long long>(w.r.q0 + tok) * P.hq + hd] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * kLn2;
           }
         }
         sync_some(9, 256 * kSlots);                           // the flag and the part's room are free again
@@ -837,7 +836,6 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
     }
   } else if (warp >= kLoaders && warp < kLoaders + kLoadWarps) {
     // ================================================ keys and values to the ring
-    regs_down<64>();
     const int wl = warp - kLoaders;
     unsigned n = 0, tiles = 0;                                // loads, key tiles so far
     uint32_t q_phase = 0;
@@ -1078,110 +1076,112 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
     while (ok && told_late) tell_oldest();
   } else if (warp == kIssuer) {
     // ================================================================ products
-    regs_down<64>();
-    unsigned n = 0, products = 0;                             // loads taken, products O += P V
-    uint32_t q_phase = 0, p_phase = 0;                        // a bit a buffer
-    bool ok = true;
-    constexpr uint32_t score = tc::product(HT == ECAH_DTYPE_BF16, kKeys, false), sum = tc::product(HT == ECAH_DTYPE_BF16, D, true);
-    auto scores = [&](int buf, int q_tile, unsigned at) {
-      if (tc::elect()) {
-        const uint64_t a = tc::tile_desc(s_q + q_tile * S::kQ, 0), b = tc::tile_desc(s_ring + (at % kRing) * S::kTile, 0);
+    // One thread does all of it: what a product waits for is looked at in a few instructions.
+    if (tc::elect()) {
+      struct Place {                                          // in the ring
+        int slot;
+        uint32_t parity;
+        __device__ __forceinline__ Place after() const { return slot + 1 == kRing ? Place{0, parity ^ 1} : Place{slot + 1, parity}; }
+      };
+      Place n = {0, 0};                                       // the next load to take
+      unsigned products = 0;                                  // O += P V
+      uint32_t q_phase = 0, p_phase = 0;                      // a bit a buffer
+      bool ok = true;
+      constexpr uint32_t score = tc::product(HT == ECAH_DTYPE_BF16, kKeys, false), sum = tc::product(HT == ECAH_DTYPE_BF16, D, true);
+      const uint64_t q_desc = tc::tile_desc(s_q, 0), k_desc = tc::tile_desc(s_ring, 0), v_desc = tc::tile_desc(s_ring, kKeys * 128);
+      auto await = [&](unsigned long long* b, uint32_t parity) -> bool {
+        const uint32_t bar = tc::smem_u32(b);
+        for (int i = 0; i < P.tries; ++i) {
+          if (tc::bar_test(bar, parity)) {
+            tc::fence_after();
+            return true;
+          }
+          if (*static_cast<volatile int*>(&notes.failed)) break;
+        }
+        *static_cast<volatile int*>(&notes.failed) = 1;
+        return false;
+      };
+      auto scores = [&](int buf, int q_tile, Place at) {
+        const uint64_t a = q_desc + q_tile * (S::kQ >> 4), b = k_desc + at.slot * (S::kTile >> 4);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
           tc::mma(tmem + buf * S::kBuffer, a + (k / 4) * (128 * 128 >> 4) + (k % 4) * 2, b + (k / 4) * (kKeys * 128 >> 4) + (k % 4) * 2, score, k > 0);
         tc::commit(tc::smem_u32(&s_bars.s_full[buf]));
-      }
-      __syncwarp();
-    };
-    auto weigh = [&](int slot, int buf, unsigned at, bool add) {
-      if (tc::elect()) {
-        const uint64_t b = tc::tile_desc(s_ring + (at % kRing) * S::kTile, kKeys * 128);
+      };
+      auto weigh = [&](int slot, int buf, Place at, bool add) {
+        const uint64_t b = v_desc + at.slot * (S::kTile >> 4);
 #pragma unroll
         for (int k = 0; k < kKeys / 16; ++k)
           tc::mma_ts(tmem + S::kSum + slot * D, tmem + buf * S::kBuffer + k * 8, b + k * (2048 >> 4), sum, add || k > 0);
         tc::commit(tc::smem_u32(&s_bars.pv_done[kSlots == 2 ? slot : products & 1]));
-      }
-      ++products;
-      __syncwarp();
-    };
-    auto release = [&](unsigned at) {
-      if (tc::elect()) tc::commit(tc::smem_u32(&s_bars.kv_empty[at % kRing]));
-      __syncwarp();
-    };
-    auto arrived = [&](unsigned at) {
-      const bool there = wait(&s_bars.kv_full[at % kRing], (at / kRing) & 1);
-      tc::fence_after();
-      return there;
-    };
-    auto weights = [&](int buf) {
-      const bool there = wait(&s_bars.p_full[buf], p_phase >> buf & 1);
-      p_phase ^= 1u << buf;
-      tc::fence_after();
-      return there;
-    };
-    while (ok && w.next(P, notes.share)) {
-      const int count = w.je - w.jb, first = w.je0 - w.jb;    // first: tiles of the first half
-      if (count <= 0) continue;
-      const bool few = w.few;
-      ok = wait(&s_bars.q_full, q_phase);
-      q_phase ^= 1;
-      if (!ok) break;
-      tc::fence_after();
-      if (kSlots == 2 && !few) {
-        if (!(ok = arrived(n))) break;
-        if (first > 0) scores(0, 0, n);
-        scores(1, 1, n);
-        release(n);
-        ++n;
-        for (int x = 0; x < count && ok; ++x) {               // load n: V x; n + 1: K x + 1
-          const bool again = x + 1 < count;
+        ++products;
+      };
+      auto release = [&](Place at) { tc::commit(tc::smem_u32(&s_bars.kv_empty[at.slot])); };
+      auto arrived = [&](Place at) { return await(&s_bars.kv_full[at.slot], at.parity); };
+      auto weights = [&](int buf) {
+        const bool there = await(&s_bars.p_full[buf], p_phase >> buf & 1);
+        p_phase ^= 1u << buf;
+        return there;
+      };
+      while (ok && w.advance(P, notes.share)) {
+        const int count = w.je - w.jb, first = w.je0 - w.jb;  // first: tiles of the first half
+        if (count <= 0) continue;
+        const bool few = w.few;
+        if (!(ok = await(&s_bars.q_full, q_phase))) break;
+        q_phase ^= 1;
+        if (kSlots == 2 && !few) {
           if (!(ok = arrived(n))) break;
-          if (x < first) {
-            if (!(ok = weights(0))) break;
-            weigh(0, 0, n, x > 0);
-          }
-          if (again && !(ok = arrived(n + 1))) break;
-          if (x + 1 < first) scores(0, 0, n + 1);
-          if (!(ok = weights(1))) break;
-          weigh(1, 1, n, x > 0);
+          if (first > 0) scores(0, 0, n);
+          scores(1, 1, n);
           release(n);
-          if (again) {
-            scores(1, 1, n + 1);
-            release(n + 1);
-          }
-          n += again ? 2 : 1;
-        }
-      } else {
-        const int lead = min(2, count);
-        for (int x = 0; x < lead && ok; ++x) {
-          if (!(ok = arrived(n))) break;
-          scores(x, 0, n);
-          release(n);
-          ++n;
-        }
-        for (int x = 0; x < count && ok; ++x) {               // load n: V x; n + 1: K x + 2
-          if (!(ok = arrived(n)) || !(ok = weights(x & 1))) break;
-          weigh(kSlots == 2 ? x & 1 : 0, x & 1, n, x >= kSlots);
-          release(n);
-          ++n;
-          if (x + 2 < count) {
+          n = n.after();
+          for (int x = 0; x < count && ok; ++x) {             // load n: V x; the one after: K x + 1
+            const bool again = x + 1 < count;
+            const Place next = n.after();
             if (!(ok = arrived(n))) break;
-            scores(x & 1, 0, n);
+            if (again && !(ok = arrived(next))) break;
+            if (x < first) {
+              if (!(ok = weights(0))) break;
+              weigh(0, 0, n, x > 0);
+              if (x + 1 < first) scores(0, 0, next);
+            }
+            if (!(ok = weights(1))) break;
+            weigh(1, 1, n, x > 0);
             release(n);
-            ++n;
+            if (again) {
+              scores(1, 1, next);
+              release(next);
+            }
+            n = again ? next.after() : next;
+          }
+        } else {
+          const int lead = min(2, count);
+          for (int x = 0; x < lead && ok; ++x) {
+            if (!(ok = arrived(n))) break;
+            scores(x, 0, n);
+            release(n);
+            n = n.after();
+          }
+          for (int x = 0; x < count && ok; ++x) {             // load n: V x; the one after: K x + 2
+            if (!(ok = arrived(n)) || !(ok = weights(x & 1))) break;
+            weigh(kSlots == 2 ? x & 1 : 0, x & 1, n, x >= kSlots);
+            release(n);
+            n = n.after();
+            if (x + 2 < count) {
+              if (!(ok = arrived(n))) break;
+              scores(x & 1, 0, n);
+              release(n);
+              n = n.after();
+            }
           }
         }
+        if (ok) tc::commit(tc::smem_u32(&s_bars.q_empty));
       }
-      if (!ok) break;
-      if (tc::elect()) tc::commit(tc::smem_u32(&s_bars.q_empty));
-      __syncwarp();
+      // nothing is in flight when the tensor memory is given back
+      tc::commit(tc::smem_u32(&s_bars.done));
+      for (int i = 0; i < kTries && !tc::bar_test(tc::smem_u32(&s_bars.done), 0); ++i) {}
     }
-    // nothing is in flight when the tensor memory is given back
-    if (tc::elect()) tc::commit(tc::smem_u32(&s_bars.done));
     __syncwarp();
-    for (int i = 0; i < kTries && !tc::bar_test(tc::smem_u32(&s_bars.done), 0); ++i) {}
-  } else {
-    regs_down<64>();
   }
 
   tc::fence_before();
