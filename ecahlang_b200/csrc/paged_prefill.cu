@@ -339,6 +339,8 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
   using S = Shape<D, E4M3>;
   constexpr int HT = E4M3 ? static_cast<int>(ECAH_DTYPE_F16) : DT;   // operand type of the products
   constexpr float lift = HT == ECAH_DTYPE_F16 ? kLift : 0.0f;
+  // of a tile's weights in a thread: 2^15, the largest f16 weight; 64 of 2^kLazy in bf16
+  constexpr float kMost = HT == ECAH_DTYPE_F16 ? 32768.0f : 16384.0f;
   constexpr int kKeys = S::kKeys, kRing = S::kRing, kSlots = S::kSlots;
   extern __shared__ __align__(1024) unsigned char base_p[];   // the swizzle goes by addresses
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -653,8 +655,9 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
           }
         };
         // The reference of the tiles before nearly always serves (scores pass it by less than
-        // 2^kLazy): weights are computed with it while the largest score is found, and again
-        // where it did not.
+        // 2^kLazy): weights are computed with it, and again with the largest score's where it did
+        // not.  A 16-bit row's sum of 64 weights tells; an e4m3 row's weights carry scales, so
+        // its largest score is found beside them.
         float top = -INFINITY;
         sum0 = sum1 = 0;
         {
@@ -662,13 +665,28 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
 #pragma unroll
           for (int i = 0; i < kC; ++i) {
             uint32_t r[32];
+            if (!E4M3 && !any) break;
             read(r, i);
-            top = largest(r, top);
+            if (E4M3) top = largest(r, top);
             if (any) weigh(r, i, ref);
           }
         }
-        if (!E4M3) top *= P.scale;
-        if (any_of(pair, 64, !any || !(top <= m + (kLazy + lift)))) {
+        bool passed = !any || !(top <= m + (kLazy + lift));
+        if (!E4M3) {
+          float l0, l1;
+          tc::apart(tc::add2(sum0, sum1), l0, l1);
+          passed = !any || !(l0 + l1 <= kMost);
+        }
+        if (any_of(pair, 64, passed)) {
+          if (!E4M3) {
+#pragma unroll
+            for (int i = 0; i < kC; ++i) {
+              uint32_t r[32];
+              read(r, i);
+              top = largest(r, top);
+            }
+            top *= P.scale;
+          }
           notes.other[slot][half][row] = top;
           sync_some(pair, 64);
           top = max_nan(top, notes.other[slot][half ^ 1][row]);
@@ -934,40 +952,45 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
       };
       int page_next[2] = {page_of(jk, 0), page_of(jk, 1)};    // of the next keys: an L2 read away
       if (!E4M3) {
-        // pages of a tile that the copy engine brings, a lane to a page
+        // whole tiles come as boxes of 64 elements by a page's slots, dealt to the warps
         const int in_tile = P.boxes ? max(1, kKeys >> P.page_shift) : 0, slots = kKeys / max(1, in_tile);
-        auto listed = [&](int j) { return lane < in_tile && (j + 1) * kKeys <= len ? pages[((j * kKeys) >> P.page_shift) + lane] : 0; };
-        int box_next = listed(jk);
+        const int boxes = in_tile * S::kBlocks, mine = (boxes - wl + kLoadWarps - 1) / kLoadWarps;
+        auto soon = [&](int j) {                              // its part of the page list into L1
+          if (lane == 0 && P.boxes && j < je && (j + 1) * kKeys <= len)
+            asm volatile("prefetch.global.L1 [%0];" ::"l"(pages + ((j * kKeys) >> P.page_shift)));
+        };
+        soon(jk);
         for (int i = 0; i < loads; ++i) {
           bool is_v;
           const int j = turn(&is_v);
           const bool boxes_now = P.boxes && (j + 1) * kKeys <= len;
-          int page[2] = {page_next[0], page_next[1]}, at = box_next;
+          int page[2] = {page_next[0], page_next[1]};
           if (is_v) {                                         // values' pages were read a while ago: in L1
             ++jv;
-            if (boxes_now) at = listed(j);
-            else { page[0] = page_of(j, 0); page[1] = page_of(j, 1); }
+            if (!boxes_now) { page[0] = page_of(j, 0); page[1] = page_of(j, 1); }
           } else {
             ++jk;
-            box_next = listed(jk);
+            soon(jk + 1);
             if (!P.boxes || (jk + 1) * kKeys > len) { page_next[0] = page_of(jk, 0); page_next[1] = page_of(jk, 1); }
           }
           const uint32_t dst = s_ring + (n % kRing) * S::kTile;
           if (boxes_now) {
-            // a whole tile: boxes of 64 elements by a page's slots, dealt to the warps
-            at = min(max(at, 0), C.num_pages - 1);
             ok = free_slot();
             if (!ok) break;
-            const uint32_t bar = tc::smem_u32(&s_bars.kv_full[n % kRing]);
-            const void* map = is_v ? &P.v_map : &P.k_map;
-            const int boxes = in_tile * S::kBlocks, mine = (boxes - wl + kLoadWarps - 1) / kLoadWarps;
-            const int slot = (j * kKeys) & (C.page_size - 1);
-            if (tc::elect()) tc::bar_expect(bar, mine * slots * 128);
-            for (int x = wl; x < boxes; x += kLoadWarps) {
-              const int nth = x / S::kBlocks, block = x - nth * S::kBlocks;
-              const int pg = __shfl_sync(0xFFFFFFFFu, at, nth);
-              if (tc::elect()) tc::copy_box(dst + block * (kKeys * 128) + nth * slots * 128, map, block * 64, slot, head, pg, bar);
+            if (tc::elect()) {
+              const uint32_t bar = tc::smem_u32(&s_bars.kv_full[n % kRing]);
+              const void* map = is_v ? &P.v_map : &P.k_map;
+              const int slot = (j * kKeys) & (C.page_size - 1);
+              const int* listed = pages + ((j * kKeys) >> P.page_shift);
+              tc::bar_expect(bar, mine * slots * 128);
+#pragma unroll 4
+              for (int x = wl; x < boxes; x += kLoadWarps) {
+                const int nth = x / S::kBlocks, block = x - nth * S::kBlocks;
+                tc::copy_box(dst + block * (kKeys * 128) + nth * slots * 128, map, block * 64, slot, head,
+                             min(max(listed[nth], 0), C.num_pages - 1), bar);
+              }
             }
+            __syncwarp();
             ++n;
             continue;
           }
