@@ -47,9 +47,16 @@ constexpr int kLoaders = 16;           // first of the warps that bring keys and
 constexpr int kLoadWarps = 3;
 constexpr int kIssuer = 19;            // the warp that issues the products
 constexpr int kT = 32 * (kIssuer + 1);
-constexpr int kItemCost = 3;           // iterations that starting and finishing an item takes
-constexpr int kWhole = 6;              // items of up to so many iterations are not divided
-constexpr int kLeast = 4;              // iterations to a block at the least
+// Units of work: of an iteration (both halves of the rows against a key tile; few rows
+// against two), and of starting and finishing an item.
+#ifndef KCOSTS
+#define KCOSTS 2, 3, 6, 6, 8
+#endif
+constexpr int kCosts[5] = {KCOSTS};
+constexpr unsigned kCost = kCosts[0], kFewCost = kCosts[1], kItemCost = kCosts[2];
+constexpr int kWhole = kCosts[3];      // items of up to so many iterations are not divided
+constexpr unsigned kLeast = kCosts[4]; // units to a block at the least
+constexpr int kWalks = 2 + kLoadWarps + 1;   // of the softmax slots, the loaders, the issuer
 constexpr int kKeep = 128;             // requests looked at together
 constexpr int kTries = 1 << 20;        // of a wait: more than one between warps of a block can need
 constexpr float kLazy = 8.0f;          // as in decode attention: a reference moves when a score passes it by 2^kLazy;
@@ -141,6 +148,9 @@ struct Tile {                          // a tile of rows of a request
     few = S::kSlots == 2 && rows <= 128;
     iters = few ? (tiles + 1) / 2 : tiles;
   }
+  // Units of the order: an iteration's, and what starting and finishing the item takes.
+  __device__ __forceinline__ unsigned unit() const { return few ? kFewCost : kCost; }
+  __device__ __forceinline__ unsigned cost() const { return kItemCost + iters * unit(); }
 };
 
 template <int D, bool E4M3>
@@ -148,12 +158,10 @@ __device__ __forceinline__ int tiles_of(const Params& P, const Request& r) {
   return (r.n * P.group + Shape<D, E4M3>::kRows - 1) / Shape<D, E4M3>::kRows;
 }
 
-struct Edge { int req, head, tile; long long start; int iters; };
-
 // A block's share of the order, and everybody's.
 struct Share {
-  long long lo, hi, size, more;        // the first `more` blocks have size + 1, the others size
-  __device__ __forceinline__ int block_of(long long x) const {
+  unsigned lo, hi, size, more;         // the first `more` blocks have size + 1, the others size
+  __device__ __forceinline__ int block_of(unsigned x) const {
     return static_cast<int>(x < more * (size + 1) ? x / (size + 1) : more + (x - more * (size + 1)) / size);
   }
 };
@@ -163,23 +171,14 @@ struct Share {
 template <int D, bool E4M3>
 struct Walk {
   using S = Shape<D, E4M3>;
-  long long at;                        // place of the item in the order
+  unsigned at, cost;                   // place of the item in the order, and its units
   Request r;
-  int req, head, tile, tiles, iters;
+  int req, head, tile, tiles;
   // the present item's part
   int row0, rows, keys, jb, je, je0;   // key tiles [jb, je); of the first slot of two halves [jb, je0)
   int first_block, parts;
   bool fresh, few, whole, found;
 
-  // By one thread.
-  __device__ __forceinline__ void begin(const Params& P, const Edge& edge) {
-    req = edge.req; head = edge.head; tile = edge.tile; at = edge.start;
-    fresh = true;
-    if (req < P.cache.batch) {
-      r = request<S::kKeys>(P, req);
-      tiles = tiles_of<D, E4M3>(P, r);
-    }
-  }
   // The next item with work for this block; false behind the last.  For a warp with a walk
   // of its own.
   __device__ __forceinline__ bool next(const Params& P, const Share& share) {
@@ -190,10 +189,10 @@ struct Walk {
   }
   // By one thread.
   __device__ __forceinline__ bool advance(const Params& P, const Share& share) {
-    const long long lo = share.lo, hi = share.hi;
+    const unsigned lo = share.lo, hi = share.hi;
     while (true) {
       if (!fresh) {
-        at += iters + kItemCost;
+        at += cost;
         if (++tile >= tiles) {
           tile = 0;
           if (++head >= P.cache.heads) {
@@ -212,22 +211,22 @@ struct Walk {
         return false;
       }
       const Tile<D, E4M3> t(P, r, tile);
-      iters = t.iters;
-      const long long begin = at + kItemCost;
+      cost = t.cost();
+      const unsigned begin = at + kItemCost, unit = t.unit();
       int i0 = 0, i1 = t.iters;
       whole = t.iters <= kWhole;
       first_block = blockIdx.x;
       parts = 1;
       if (whole) {
         if (at < lo) continue;
-      } else {
-        i0 = static_cast<int>(min(max(lo - begin, 0ll), static_cast<long long>(t.iters)));
-        i1 = static_cast<int>(min(max(hi - begin, 0ll), static_cast<long long>(t.iters)));
+      } else {                         // iteration i is the block's that holds place begin + i unit
+        i0 = lo <= begin ? 0 : min((lo - begin + unit - 1) / unit, static_cast<unsigned>(t.iters));
+        i1 = hi <= begin ? 0 : min((hi - begin + unit - 1) / unit, static_cast<unsigned>(t.iters));
         if (i0 >= i1) continue;
         whole = i0 == 0 && i1 == t.iters;
         if (!whole) {
           first_block = share.block_of(begin);
-          parts = share.block_of(begin + t.iters - 1) - first_block + 1;
+          parts = share.block_of(begin + (t.iters - 1) * unit) - first_block + 1;
         }
       }
       row0 = t.row0; rows = t.rows; keys = t.keys; few = t.few;
@@ -326,12 +325,11 @@ struct Bars {
 template <int D, bool E4M3>
 struct Notes {
   Bars<D, E4M3> bars;
-  Edge edge[2];
   Share share;
   uint32_t tmem;
   int failed, flag;
-  Walk<D, E4M3> walk[2 + kLoadWarps + 1];                     // of the softmax slots, the loaders, the issuer
-  float other[2][2][128];                                     // between the two threads of a row
+  Walk<D, E4M3> walk[kWalks];
+  float other[2][2][128];                                     // between the threads of a row
 };
 
 template <int DT, bool E4M3, int D>
@@ -364,122 +362,113 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
     for (int i = 0; i < 2; ++i) { init(&s_bars.s_full[i], 1); init(&s_bars.p_full[i], 8); init(&s_bars.pv_done[i], 1); }
     tc::fence_smem();
     notes.failed = 0;
-    notes.edge[0].req = notes.edge[1].req = C.batch;
-    notes.edge[0].start = notes.edge[1].start = 0;
+  }
+  if (tid < kWalks) {
+    notes.walk[tid].req = C.batch;                            // none, unless one is found below
+    notes.walk[tid].fresh = true;
   }
   if (warp == kIssuer) tc::tmem_alloc(tc::smem_u32(&notes.tmem), S::kColumns);
 
-  // ---- this block's share.  An item costs kItemCost units, then one an iteration; the
-  // first `more` blocks take share + 1 units, the others share.
+  // ---- this block's share of the order.  The first `more` blocks take size + 1 units, the
+  // others size.
   {
-    Request* s_req = reinterpret_cast<Request*>(base_p + kSlots * S::kQ);            // the ring is not in use yet
-    long long* s_cost = reinterpret_cast<long long*>(base_p + kSlots * S::kQ + kKeep * 32);
-    auto look = [&](int b0) {          // cost of a head of each of kKeep requests
-      __syncthreads();
-      if (tid < kKeep) {
-        if (b0 + tid < C.batch) s_req[tid] = request<kKeys>(P, b0 + tid);
-        else s_req[tid].n = 0;
+    struct Seen { Request r; int tiles; unsigned cost; };      // of a request; cost: of one head
+    Seen* seen = reinterpret_cast<Seen*>(base_p + kSlots * S::kQ);   // the ring is not in use yet
+    auto look = [&](int b0) {
+      if (tid < kKeep && b0 + tid < C.batch) {
+        seen[tid].r = request<kKeys>(P, b0 + tid);
+        seen[tid].tiles = tiles_of<D, E4M3>(P, seen[tid].r);
       }
       __syncthreads();
-      for (int i = warp; i < kKeep; i += kT / 32) {
-        const Request r = s_req[i];
-        long long sum = 0;
-        for (int t = lane; t < tiles_of<D, E4M3>(P, r); t += 32) sum += Tile<D, E4M3>(P, r, t).iters + kItemCost;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-        if (lane == 0) s_cost[i] = sum;
+      for (int i = warp; i < min(kKeep, C.batch - b0); i += kT / 32) {
+        const Request r = seen[i].r;
+        unsigned sum = 0;
+        for (int t = lane; t < seen[i].tiles; t += 32) sum += Tile<D, E4M3>(P, r, t).cost();
+        sum = __reduce_add_sync(0xFFFFFFFFu, sum);
+        if (lane == 0) seen[i].cost = sum;
       }
       __syncthreads();
     };
-    auto chunk_sum = [&]() {
-      long long sum = 0;
-      for (int i = lane; i < kKeep; i += 32) sum += s_cost[i];
-#pragma unroll
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-      return sum * C.heads;
+    auto all = [&](int b0) {
+      unsigned sum = 0;
+      for (int i = lane; i < min(kKeep, C.batch - b0); i += 32) sum += seen[i].cost;
+      return __reduce_add_sync(0xFFFFFFFFu, sum) * C.heads;
     };
-    long long total = 0;
+    auto before = [&](unsigned v) {                           // sum of the lanes before
+      unsigned inc = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned w = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+        if (lane >= o) inc += w;
+      }
+      return inc - v;
+    };
+    unsigned total = 0;
     for (int b0 = 0; b0 < C.batch; b0 += kKeep) {
+      if (b0) __syncthreads();
       look(b0);
-      total += chunk_sum();
+      total += all(b0);
     }
-    const long long blocks = min(static_cast<long long>(gridDim.x), max(1ll, total / kLeast));
+    const unsigned blocks = min(gridDim.x, max(1u, total / kLeast)), size = max(1u, total / blocks), more = total - size * blocks;
     const bool busy = blockIdx.x < blocks && total > 0;
-    const long long share = max(1ll, total / blocks), more = total - share * blocks;
-    long long edge[2] = {0, 0};
-    if (busy) {
-      edge[0] = blockIdx.x * share + min(static_cast<long long>(blockIdx.x), more);
-      edge[1] = edge[0] + share + (blockIdx.x < more);
-    }
-    long long run = 0;
-    for (int b0 = 0; busy && b0 < C.batch; b0 += kKeep) {
-      if (C.batch > kKeep) look(b0);
-      const long long sum = chunk_sum();
-      if (warp < 2) {
-        const long long x = edge[warp];
-        if (x >= run && x < run + sum) {
-          long long p = run;
-          int i = 0;                                          // the request
-          for (int i0 = 0;; i0 += 32) {
-            const long long c = s_cost[i0 + lane] * C.heads;
-            long long inc = c;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const long long v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-              if (lane >= o) inc += v;
-            }
-            const unsigned past = __ballot_sync(0xFFFFFFFFu, p + inc > x);
-            if (past) {
-              const int l = __ffs(past) - 1;
-              p += __shfl_sync(0xFFFFFFFFu, inc - c, l);
-              i = i0 + l;
-              break;
-            }
-            p += __shfl_sync(0xFFFFFFFFu, inc, 31);
+    const unsigned lo = blockIdx.x * size + min(blockIdx.x, more), hi = lo + size + (blockIdx.x < more);
+    if (warp < 2 && lane == 0) (warp == 0 ? notes.share.lo : notes.share.hi) = !busy ? 0 : warp == 0 ? lo : hi;
+    if (tid == 64) { notes.share.size = size; notes.share.more = more; }
+    unsigned run = 0;
+    for (int b0 = 0; busy && b0 < C.batch && run < hi; b0 += kKeep) {
+      if (C.batch > kKeep) {
+        __syncthreads();
+        look(b0);
+      }
+      const unsigned sum = all(b0), x = warp == 0 ? lo : hi;
+      if (warp < 2 && x >= run && x < run + sum) {            // the item at an edge of the share
+        unsigned p = run;
+        int i = 0, t = 0;
+        for (int i0 = 0;; i0 += 32) {                         // its request,
+          const unsigned c = i0 + lane < min(kKeep, C.batch - b0) ? seen[i0 + lane].cost * C.heads : 0, at = p + before(c);
+          const unsigned here = __ballot_sync(0xFFFFFFFFu, x >= at && x < at + c);
+          if (here) {
+            i = i0 + __ffs(here) - 1;
+            p = __shfl_sync(0xFFFFFFFFu, at, __ffs(here) - 1);
+            break;
           }
-          const long long one = s_cost[i];
-          const int head = static_cast<int>((x - p) / one);
-          p += head * one;
-          const Request r = s_req[i];
-          const int tiles = tiles_of<D, E4M3>(P, r);
-          for (int t0 = 0;; t0 += 32) {                       // the tile
-            int iters = 0;
-            long long c = 0;
-            if (t0 + lane < tiles) { iters = Tile<D, E4M3>(P, r, t0 + lane).iters; c = iters + kItemCost; }
-            long long inc = c;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const long long v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-              if (lane >= o) inc += v;
-            }
-            const unsigned past = __ballot_sync(0xFFFFFFFFu, p + inc > x);
-            if (past) {
-              const int l = __ffs(past) - 1;
-              p += __shfl_sync(0xFFFFFFFFu, inc - c, l);
-              iters = __shfl_sync(0xFFFFFFFFu, iters, l);
-              if (lane == 0) notes.edge[warp] = Edge{b0 + i, head, t0 + l, p, iters};
-              break;
-            }
-            p += __shfl_sync(0xFFFFFFFFu, inc, 31);
+          p = __shfl_sync(0xFFFFFFFFu, at + c, 31);
+        }
+        const Request r = seen[i].r;
+        const int head = static_cast<int>((x - p) / seen[i].cost);
+        p += head * seen[i].cost;
+        unsigned cost = 0;
+        int iters = 0;
+        for (int t0 = 0;; t0 += 32) {                         // tile
+          unsigned c = 0;
+          if (t0 + lane < seen[i].tiles) {
+            const Tile<D, E4M3> tile(P, r, t0 + lane);
+            c = tile.cost();
+            iters = tile.iters;
           }
+          const unsigned at = p + before(c), here = __ballot_sync(0xFFFFFFFFu, x >= at && x < at + c);
+          if (here) {
+            const int l = __ffs(here) - 1;
+            t = t0 + l;
+            p = __shfl_sync(0xFFFFFFFFu, at, l);
+            cost = __shfl_sync(0xFFFFFFFFu, c, l);
+            iters = __shfl_sync(0xFFFFFFFFu, iters, l);
+            break;
+          }
+          p = __shfl_sync(0xFFFFFFFFu, at + c, 31);
+        }
+        if (lane == 0 && iters <= kWhole) {
+          // an edge inside an item that is not divided moves to the item's nearer end
+          (warp == 0 ? notes.share.lo : notes.share.hi) = 2 * (x - p) < cost ? p : p + cost;
+        }
+        if (warp == 0 && lane < kWalks) {
+          Walk<D, E4M3>& w = notes.walk[lane];
+          w.at = p;
+          w.r = r;
+          w.req = b0 + i; w.head = head; w.tile = t; w.tiles = seen[i].tiles;
         }
       }
       run += sum;
-      if (edge[1] < run) break;
-    }
-    __syncthreads();
-    if (tid == 0) {
-      // an edge inside an item that is not divided moves to the item's nearer end
-      for (int e = 0; e < 2; ++e) {
-        const Edge& g = notes.edge[e];
-        if (busy && g.req < C.batch && g.iters <= kWhole) {
-          const long long cost = g.iters + kItemCost, into = edge[e] - g.start;
-          edge[e] = g.start + (2 * into < cost ? 0 : cost);
-        }
-      }
-      notes.share = Share{edge[0], edge[1], share, more};
-      notes.walk[0].begin(P, notes.edge[0]);
-      for (auto& w : notes.walk) w = notes.walk[0];
     }
     tc::fence_before();
     __syncthreads();
@@ -739,82 +728,111 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
       sync_some(pair, 64);
       l += notes.other[slot][half ^ 1][row];
 
+      // ---- Few rows: both slots' sums of a row lie in its tensor-memory lane.  Each of its four
+      // threads joins a quarter of their columns, in the first slot's place.
+      constexpr int kQuarter = D / 4;
+      const bool two_sums = kSlots == 2 && !own_rows;
+      if (two_sums) {
+        sync_some(pair, 64);                                  // both have read the other's sum
+        notes.other[slot][half][row] = half == 0 ? m : l;
+        tc::fence_before();
+        sync_some(9, 512);
+        tc::fence_after();
+        const float2 a = make_float2(notes.other[0][0][row], notes.other[0][1][row]);
+        const float2 b = make_float2(notes.other[1][0][row], notes.other[1][1][row]);
+        m = fmaxf(a.x, b.x);
+        const float fa = a.x == -INFINITY ? 0.0f : ex2_approx(a.x - m), fb = b.x == -INFINITY ? 0.0f : ex2_approx(b.x - m);
+        l = a.y * fa + b.y * fb;
+        if (a.y != a.y || b.y != b.y) l = NAN;
+        const bool in_a = jb < w.je, in_b = jb + 1 < w.je;    // whether the slot had a tile
+        any = in_a;
+        if (in_b) {
+          const uint32_t at = lanes + S::kSum + (2 * slot + half) * kQuarter;
+#pragma unroll 1
+          for (int d = 0; d < kQuarter; d += 8) {
+            uint32_t x[8], y[8];
+            tc::load8(x, at + d);
+            tc::load8(y, at + D + d);
+            tc::load_wait();
+            tc::pin8(x);
+            tc::pin8(y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = __float_as_uint(fmaf(fa, __uint_as_float(x[i]), fb * __uint_as_float(y[i])));
+            tc::store8(at + d, x);
+          }
+          tc::store_wait();
+        }
+      }
+      // where this thread's columns of the row's sum lie, and how many they are
+      const int my_first = two_sums ? (2 * slot + half) * kQuarter : half * (D / 2), my_columns = two_sums ? kQuarter : D / 2;
+      const uint32_t my_at = lanes + S::kSum + (two_sums ? 0 : slot * D) + my_first;
+      const int tile = own_rows ? slot : 0;
+      const bool speaks = half == 0 && (own_rows || slot == 0);   // for the row
+
       // ---- the item's rows, or this part of them
-      const bool joined = !w.whole || w.few;                  // more than one sum to a row
+      const bool joined = !w.whole;
       const int first_block = w.first_block, part = static_cast<int>(blockIdx.x) - first_block;
       auto part_slot = [&](int p) { return p == 0 ? 2 * first_block + 1 : 2 * (first_block + p); };
       auto part_at = [&](int at, int tile) { return reinterpret_cast<uint4*>(P.part_o) + (static_cast<long long>(at) * kSlots + tile) * (D / 4) * 128; };
       if (!joined) {
         // a sum of zero (no key has mass) gives zeros
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        uint16_t* o = static_cast<uint16_t*>(P.out) + (w.r.q0 + token) * P.o_tok + head * P.o_head + half * (D / 2);
-        if (live && half == 0 && P.lse)
+        uint16_t* o = static_cast<uint16_t*>(P.out) + (w.r.q0 + token) * P.o_tok + head * P.o_head + my_first;
+        if (live && speaks && P.lse)
           P.lse[static_cast<long long>(w.r.q0 + token) * P.hq + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 #pragma unroll 1
-        for (int d = 0; d < D / 2; d += 16) {
-          uint32_t x[16] = {};
+        for (int d = 0; d < my_columns; d += 8) {
+          uint32_t x[8] = {};
           if (any) {
-            tc::load16(x, sum_at + d);
+            tc::load8(x, my_at + d);
             tc::load_wait();
-            tc::pin16(x);
+            tc::pin8(x);
           }
-          uint32_t h[8];
+          uint32_t h[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) h[i] = l == 0.0f ? 0u : pack2<DT>(__uint_as_float(x[2 * i]) * inv, __uint_as_float(x[2 * i + 1]) * inv);
-          if (live) {
-            *reinterpret_cast<uint4*>(o + d) = make_uint4(h[0], h[1], h[2], h[3]);
-            *reinterpret_cast<uint4*>(o + d + 8) = make_uint4(h[4], h[5], h[6], h[7]);
-          }
+          for (int i = 0; i < 4; ++i) h[i] = l == 0.0f ? 0u : pack2<DT>(__uint_as_float(x[2 * i]) * inv, __uint_as_float(x[2 * i + 1]) * inv);
+          if (live) *reinterpret_cast<uint4*>(o + d) = make_uint4(h[0], h[1], h[2], h[3]);
         }
         tc::fence_before();
       } else {
-        const long long at = static_cast<long long>(part_slot(part)) * S::kRows + slot * 128 + row;
-        if (live && half == 0) P.part_ml[at] = make_float2(m, l);
+        if (live && speaks) P.part_ml[static_cast<long long>(part_slot(part)) * S::kRows + tile * 128 + row] = make_float2(m, l);
         // [128 rows' part][D / 4][128][4]: neighbouring rows side by side
-        uint4* o = part_at(part_slot(part), slot) + half * (D / 8) * 128 + row;
+        uint4* o = part_at(part_slot(part), tile) + my_first / 4 * 128 + row;
 #pragma unroll 1
-        for (int d = 0; d < D / 2 && any; d += 16) {
-          uint32_t x[16];
-          tc::load16(x, sum_at + d);
+        for (int d = 0; d < my_columns && any; d += 8) {
+          uint32_t x[8];
+          tc::load8(x, my_at + d);
           tc::load_wait();
-          tc::pin16(x);
+          tc::pin8(x);
           if (live) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[(d / 4 + i) * 128] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            for (int i = 0; i < 2; ++i) o[(d / 4 + i) * 128] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
           }
         }
         tc::fence_before();
-        // the last part's block joins them all; a whole item's two sums are joined here
+        // the last part's block joins them all
         const int parts = w.parts;
         sync_some(9, 256 * kSlots);
         if (tid == 0) {
-          bool last = true;
-          if (parts > 1) {
-            unsigned* counter = P.counters + first_block;
-            unsigned n;
-            asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(n) : "l"(counter) : "memory");
-            last = n + 1u == static_cast<unsigned>(parts);
-            if (last) *counter = 0u;
-          }
+          unsigned* counter = P.counters + first_block;
+          unsigned n;
+          asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(n) : "l"(counter) : "memory");
+          const bool last = n + 1u == static_cast<unsigned>(parts);
+          if (last) *counter = 0u;
           notes.flag = last;
         }
         sync_some(9, 256 * kSlots);
         const bool mine = *static_cast<volatile int*>(&notes.flag) != 0;
         if (mine) {
-          // Triple x of a row is part x, or of few rows part x / 2, slot x % 2.  Several threads to a
-          // row, each with some of its columns.
-          const bool fewer = w.few;
-          const int sums = fewer ? 2 * parts : parts;
-          const int spread = fewer ? 4 : 2;                   // threads of a row (with one slot: 256 threads of 128 rows)
-          const int tile = spread == 2 && kSlots == 2 ? tid >> 8 : 0, rr = tid & 127, nth = spread == 4 ? tid >> 7 : tid >> 7 & 1;
+          // several threads to a row, each with some of its columns
+          const int spread = two_sums ? 4 : 2;                // threads of a row (with one slot: 256 threads of 128 rows)
+          const int tile = own_rows ? tid >> 8 : 0, rr = tid & 127, nth = two_sums ? tid >> 7 : tid >> 7 & 1;
           const int mine_row = tile * 128 + rr;
           if (mine_row < w.rows) {
-            auto slot_at = [&](int x) { return part_slot(fewer ? x >> 1 : x); };
-            auto half_at = [&](int x) { return fewer ? x & 1 : tile; };
-            auto ml_at = [&](int x) { return __ldcg(P.part_ml + static_cast<long long>(slot_at(x)) * S::kRows + half_at(x) * 128 + rr); };
+            auto ml_at = [&](int x) { return __ldcg(P.part_ml + static_cast<long long>(part_slot(x)) * S::kRows + mine_row); };
             float mm = -INFINITY, ll = 0.0f;
-            for (int x = 0; x < sums; ++x) mm = fmaxf(mm, ml_at(x).x);
-            for (int x = 0; x < sums; ++x) {
+            for (int x = 0; x < parts; ++x) mm = fmaxf(mm, ml_at(x).x);
+            for (int x = 0; x < parts; ++x) {
               const float2 v = ml_at(x);
               ll += v.x == -INFINITY ? (v.y != v.y ? v.y : 0.0f) : v.y * ex2_approx(v.x - mm);
             }
@@ -828,10 +846,10 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
 #pragma unroll
               for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
 #pragma unroll 2
-              for (int x = 0; x < sums; ++x) {
+              for (int x = 0; x < parts; ++x) {
                 const float v = ml_at(x).x, f = v == -INFINITY ? 0.0f : ex2_approx(v - mm);
                 if (f == 0.0f) continue;                      // a sum of nothing was not written
-                const uint4* src = part_at(slot_at(x), half_at(x)) + d / 4 * 128 + rr;
+                const uint4* src = part_at(part_slot(x), tile) + d / 4 * 128 + rr;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   const uint4 o = __ldcg(src + i * 128);
@@ -851,6 +869,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         }
         sync_some(9, 256 * kSlots);                           // the flag and the part's room are free again
       }
+      if (two_sums && !joined) sync_some(9, 512);             // and the first slot's sum, which four warps read
     }
   } else if (warp >= kLoaders && warp < kLoaders + kLoadWarps) {
     // ================================================ keys and values to the ring
@@ -1321,6 +1340,11 @@ int ecah_paged_prefill_bounded(const ecah_prefill_args* a, int32_t tries, void* 
   if (!kv::side16(P.cache.k, c.num_pages, c.page_size, c.num_kv_heads, e4m3 ? 1 : 2, &P.k) ||
       !kv::side16(P.cache.v, c.num_pages, c.page_size, c.num_kv_heads, e4m3 ? 1 : 2, &P.v))
     return ECAH_ERR_SHAPE;
+  // units of work are counted in 32 bits
+  const int keys = c.head_dim <= 128 ? 128 : 64, item = c.head_dim <= 128 ? 256 : 128;
+  const double items = (static_cast<double>(a->tokens) * group / item + c.batch) * c.num_kv_heads;
+  if (items * (prefill::kItemCost + prefill::kCost * (static_cast<double>(c.num_indices) * c.page_size / keys + 2.0)) >= 2147483648.0)
+    return ECAH_ERR_SHAPE;
   const prefill::Layout L = prefill::layout(sms, c.head_dim);
   unsigned char* ws = static_cast<unsigned char*>(a->workspace);
   P.counters = reinterpret_cast<unsigned*>(ws);
@@ -1331,7 +1355,6 @@ int ecah_paged_prefill_bounded(const ecah_prefill_args* a, int32_t tries, void* 
                                  : (e4m3 ? prefill::variant_for<ECAH_DTYPE_BF16, true>(c.head_dim) : prefill::variant_for<ECAH_DTYPE_BF16, false>(c.head_dim));
   // Whole tiles by the copy engine where a page is a power of two of 8 slots or more (the
   // swizzle goes by 8 rows); smaller or odd pages and 8-bit rows go through threads.
-  const int keys = c.head_dim <= 128 ? 128 : 64;
   P.boxes = !e4m3 && P.page_shift >= 3 && prefill::box_map(&P.k_map, P.cache.k, c, std::min(c.page_size, keys)) &&
             prefill::box_map(&P.v_map, P.cache.v, c, std::min(c.page_size, keys));
   return launch_kernel(v.fn, dim3(sms), prefill::kT, v.smem, reinterpret_cast<cudaStream_t>(stream), P) ? ECAH_OK : ECAH_ERR_LAUNCH;

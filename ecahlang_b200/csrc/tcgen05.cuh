@@ -62,10 +62,17 @@ __device__ __forceinline__ void load16(uint32_t (&r)[16], uint32_t at) {
                "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                : ECAH_W8(r, 0), ECAH_W8(r, 8) : "r"(at));
 }
+__device__ __forceinline__ void load8(uint32_t (&r)[8], uint32_t at) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : ECAH_W8(r, 0) : "r"(at));
+}
 __device__ __forceinline__ void load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // Nothing that uses the values is moved before this.
 __device__ __forceinline__ void pin32(uint32_t (&r)[32]) {
   asm volatile("" : ECAH_R8(r, 0), ECAH_R8(r, 8), ECAH_R8(r, 16), ECAH_R8(r, 24));
+}
+__device__ __forceinline__ void pin8(uint32_t (&r)[8]) { asm volatile("" : ECAH_R8(r, 0)); }
+__device__ __forceinline__ void store8(uint32_t at, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), ECAH_I8(r, 0) : "memory");
 }
 __device__ __forceinline__ void pin16(uint32_t (&r)[16]) { asm volatile("" : ECAH_R8(r, 0), ECAH_R8(r, 8)); }
 __device__ __forceinline__ void store32(uint32_t at, const uint32_t (&r)[32]) {
