@@ -50,10 +50,10 @@ constexpr int kT = 32 * (kIssuer + 1);
 // Units of work: of an iteration (both halves of the rows against a key tile; few rows
 // against two), and of starting and finishing an item.
 #ifndef KCOSTS
-#define KCOSTS 2, 3, 6, 6, 8
+#define KCOSTS 2, 4, 9, 6, 8, 4
 #endif
-constexpr int kCosts[5] = {KCOSTS};
-constexpr unsigned kCost = kCosts[0], kFewCost = kCosts[1], kItemCost = kCosts[2];
+constexpr int kCosts[6] = {KCOSTS};
+constexpr unsigned kCost = kCosts[0], kFewCost = kCosts[1], kItemCost = kCosts[2], kFewItemCost = kCosts[5];
 constexpr int kWhole = kCosts[3];      // items of up to so many iterations are not divided
 constexpr unsigned kLeast = kCosts[4]; // units to a block at the least
 constexpr int kWalks = 2 + kLoadWarps + 1;   // of the softmax slots, the loaders, the issuer
@@ -150,7 +150,8 @@ struct Tile {                          // a tile of rows of a request
   }
   // Units of the order: an iteration's, and what starting and finishing the item takes.
   __device__ __forceinline__ unsigned unit() const { return few ? kFewCost : kCost; }
-  __device__ __forceinline__ unsigned cost() const { return kItemCost + iters * unit(); }
+  __device__ __forceinline__ unsigned start() const { return few ? kFewItemCost : kItemCost; }
+  __device__ __forceinline__ unsigned cost() const { return start() + iters * unit(); }
 };
 
 template <int D, bool E4M3>
@@ -212,7 +213,7 @@ struct Walk {
       }
       const Tile<D, E4M3> t(P, r, tile);
       cost = t.cost();
-      const unsigned begin = at + kItemCost, unit = t.unit();
+      const unsigned begin = at + t.start(), unit = t.unit();
       int i0 = 0, i1 = t.iters;
       whole = t.iters <= kWhole;
       first_block = blockIdx.x;
@@ -328,7 +329,7 @@ struct Notes {
   Share share;
   uint32_t tmem;
   int failed, flag;
-  Walk<D, E4M3> walk[kWalks];
+  Walk<D, E4M3> walk[kWalks + 2];      // the softmax slots have two, in turn
   float other[2][2][128];                                     // between the threads of a row
 };
 
@@ -513,10 +514,10 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
       ok = ok && (kSlots == 2 ? wait(&s_bars.pv_done[slot], x & 1) : wait(&s_bars.pv_done[x & 1], x >> 1 & 1));
       tc::fence_after();
     };
-    while (true) {
+    if ((tid & 255) == 0) notes.walk[slot].found = notes.walk[slot].advance(P, notes.share);
+    for (int turn = 0;; turn ^= 1) {
       sync_some(10 + slot, 256);                              // nobody looks at the item before any more
-      if ((tid & 255) == 0) w.found = w.advance(P, notes.share);
-      sync_some(10 + slot, 256);
+      Walk<D, E4M3>& w = notes.walk[turn ? kWalks + slot : slot];
       if (!w.found) break;
       const bool own_rows = kSlots == 2 && !w.few;            // slots are halves of the rows
       const int my = (own_rows ? slot * 128 : 0) + row;       // row of the item
@@ -722,6 +723,12 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         if (kSlots == 1) buf ^= 1;
       }
       before += max(w.je - jb, 0);
+      if ((tid & 255) == 0) {                                 // the item after this, while the last product runs
+        Walk<D, E4M3>& then = notes.walk[turn ? slot : kWalks + slot];
+        then = w;
+        then.found = then.advance(P, notes.share);
+      }
+      __syncwarp();
       if (any) wait_sum();
       if (!ok) l = NAN;
       notes.other[slot][half][row] = l;
@@ -877,30 +884,22 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
     unsigned n = 0, tiles = 0;                                // loads, key tiles so far
     uint32_t q_phase = 0;
     bool ok = true;
-    constexpr unsigned kLag = 2;
-    unsigned long long waiting = 0;                           // ring slots filled by threads' copies that the products do not
-    unsigned told_late = 0;                                   // know of yet, oldest in the low byte; how many
-    auto tell = [&](unsigned at) {
-      tc::fence_smem();
+    // An arrival of the warp once all its threads' copies so far are there; nobody waits here.
+    auto arrive_copied = [&](unsigned long long* b) {
+      const uint32_t bar = tc::smem_u32(b);
+      asm volatile("cp.async.mbarrier.arrive.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
       __syncwarp();
-      if (lane == 0) tc::bar_arrive(tc::smem_u32(&s_bars.kv_full[at]));
-    };
-    auto tell_oldest = [&]() {
-      tell(static_cast<unsigned>(waiting & 255));
-      waiting >>= 8;
-      --told_late;
+      if (lane == 0) tc::bar_arrive(bar);
     };
     auto free_slot = [&]() { return wait(&s_bars.kv_empty[n % kRing], ((n / kRing) & 1) ^ 1); };
 
     while (ok && w.next(P, notes.share)) {
       if (w.jb >= w.je) continue;
       const bool shared = kSlots == 2 && !w.few;
-      if (!E4M3) {                                            // the item's queries
-        cp_wait<0>();
-        while (told_late) tell_oldest();
+      auto queries = [&]() -> bool {
         ok = wait(&s_bars.q_empty, q_phase ^ 1);
         q_phase ^= 1;
-        if (!ok) break;
+        if (!ok) return false;
         for (int g = wl; g < (shared ? 8 : 4); g += kLoadWarps) {   // 32 rows at a time
           const int my = 32 * g + lane;
           long long off = -1;
@@ -918,13 +917,9 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
                  static_cast<const uint16_t*>(P.q) + (o < 0 ? 0 : o + col * 8), o >= 0);
           }
         }
-        cp_commit();
-        cp_wait<0>();
-        tc::fence_smem();
-        __syncwarp();
-        if (lane == 0) tc::bar_arrive(tc::smem_u32(&s_bars.q_full));
-      }
-
+        arrive_copied(&s_bars.q_full);
+        return true;
+      };
       const int* pages = C.indices + w.r.first;
       const int len = w.r.len, head = w.head, je = w.je;
       auto nth_page = [&](int key) { return P.page_shift >= 0 ? key >> P.page_shift : key / C.page_size; };
@@ -980,6 +975,8 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         };
         soon(jk);
         for (int i = 0; i < loads; ++i) {
+          // the item's queries behind its first two loads, which wait for nothing of this item
+          if (i == 2 && !queries()) break;
           bool is_v;
           const int j = turn(&is_v);
           const bool boxes_now = P.boxes && (j + 1) * kKeys <= len;
@@ -1018,15 +1015,10 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
           ok = free_slot();
           if (!ok) break;
           copy_rows(p, side, [&](int r, int col) { return dst + (col / 8) * (kKeys * 128) + r * 128 + ((col % 8) ^ (r & 7)) * 16; });
-          cp_commit();
-          waiting |= static_cast<unsigned long long>(n % kRing) << (8 * told_late);
-          ++told_late;
+          arrive_copied(&s_bars.kv_full[n % kRing]);
           ++n;
-          if (told_late > kLag) {
-            cp_wait<kLag>();
-            tell_oldest();
-          }
         }
+        if (ok && loads == 2) queries();
       } else {
         // Codes and scales as they are cached go to a ring of their own, kRaws - 1 tiles ahead; each
         // warp converts the rows that it copied.
@@ -1109,13 +1101,14 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
             }
             ++tiles;
           }
-          tell(n % kRing);
+          tc::fence_smem();
+          __syncwarp();
+          if (lane == 0) tc::bar_arrive(tc::smem_u32(&s_bars.kv_full[n % kRing]));
           ++n;
         }
       }
     }
-    cp_wait<0>();
-    while (ok && told_late) tell_oldest();
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == kIssuer) {
     // ================================================================ products
     // One thread does all of it: what a product waits for is looked at in a few instructions.
@@ -1136,6 +1129,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         for (int i = 0; i < P.tries; ++i) {
           if (tc::bar_test(bar, parity)) {
             tc::fence_after();
+            if (!E4M3) tc::fence_smem();                      // threads' copies are not fenced where they are made
             return true;
           }
           if (*static_cast<volatile int*>(&notes.failed)) break;
