@@ -59,8 +59,7 @@ constexpr unsigned kLeast = kCosts[4]; // units to a block at the least
 constexpr int kWalks = 2 + kLoadWarps + 1;   // of the softmax slots, the loaders, the issuer
 constexpr int kKeep = 128;             // requests looked at together
 constexpr int kTries = 1 << 20;        // of a wait: more than one between warps of a block can need
-constexpr float kLazy = 8.0f;          // as in decode attention: a reference moves when a score passes it by 2^kLazy;
-constexpr float kLift = 7.0f;          // f16 weights reach 2^15, so that small ones are not lost
+constexpr float kLift = 7.0f;          // f16 weights begin at 2^7 and reach 2^15, so that small ones are not lost
 // One pair of scores in kShare / 2 is raised by multiplications (exp2_pair).
 #ifndef KSHARE
 #define KSHARE 8
@@ -94,7 +93,7 @@ struct Shape {
   static constexpr int kBlocks = (D + 63) / 64;            // of 64 elements
   static constexpr int kQ = 128 * kBlocks * 128;           // bytes of a slot's queries
   static constexpr int kTile = kKeys * kBlocks * 128;      // bytes of a tile
-  static constexpr int kScales = E4M3 ? kKeys * 12 : 0;    // of a tile: key scale, log2 and reciprocal of the value scale
+  static constexpr int kScales = E4M3 ? kKeys * 8 : 0;     // of a tile: key and value scales
   static constexpr int kRaw = E4M3 ? kKeys * (D + 8) : 0;  // of a tile as it is cached: codes, key and value scales
   static constexpr int kRaws = 3;
   static constexpr int kRoom = 227 * 1024 - 3072;          // beside the block's Notes
@@ -298,11 +297,6 @@ __device__ __forceinline__ void exp2_pair(float& a, float& b) {
 __device__ __forceinline__ float lg2(float x) {
   float r;
   asm("lg2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ float rcp(float x) {
-  float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 // A barrier of `threads` threads that tells all of them whether one said so.
@@ -578,9 +572,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         const float* sc = reinterpret_cast<const float*>(base_p + (s_scales - base) + ((before + j - jb) % S::kScaleRing) * S::kScales) + c0;
         const bool masked = (j + 1) * kKeys > least;
         const int left = lim - j * kKeys - c0;
-        // 32 scores in log2 units (16-bit rows: without their scale); an e4m3 value's scale goes
-        // into its weight through the exponent (weight 2^(s + log2 scale - m)), and the sum
-        // takes it back out.
+        // 32 scores; e4m3 rows: times their key's scale
         auto read = [&](uint32_t (&r)[32], int i) {
           tc::load32(r, s_at + c0 + 32 * i);
           tc::load_wait();
@@ -588,10 +580,12 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
           if (E4M3) {
 #pragma unroll
             for (int c = 0; c < 32; c += 4) {
-              const float4 kx = *reinterpret_cast<const float4*>(sc + 32 * i + c), lv = *reinterpret_cast<const float4*>(sc + kKeys + 32 * i + c);
-              const float x[4] = {kx.x, kx.y, kx.z, kx.w}, y[4] = {lv.x, lv.y, lv.z, lv.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) r[c + e] = __float_as_uint(fmaf(__uint_as_float(r[c + e]) * x[e], scale, y[e]));
+              const float4 k = *reinterpret_cast<const float4*>(sc + 32 * i + c);
+              float x, y;
+              tc::apart(tc::mul2(tc::two(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), tc::two(k.x, k.y)), x, y);
+              r[c] = __float_as_uint(x); r[c + 1] = __float_as_uint(y);
+              tc::apart(tc::mul2(tc::two(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), tc::two(k.z, k.w)), x, y);
+              r[c + 2] = __float_as_uint(x); r[c + 3] = __float_as_uint(y);
             }
           }
           if (masked) {
@@ -612,33 +606,32 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
           return max3(max_nan(t0, t1), t2, t3);
         };
         uint32_t w16[kC][16];
-        uint64_t sum0, sum1;                                  // four chains
+        uint64_t sum0, sum1, most;                            // of the weights; e4m3: most of their products with the scales
         auto weigh = [&](const uint32_t (&r)[32], int i, float ref) {
           // A weight is off by at most 2^-9 of itself in bf16 (2^-12 in f16), at random over the
-          // keys; the sum takes it as it was.
-          const uint64_t scale2 = tc::two(P.scale, P.scale), ref2 = tc::two(-ref, -ref);
+          // keys; the sum takes it as it was.  An e4m3 value's scale goes into its weight.
+          const uint64_t scale2 = tc::two(scale, scale), ref2 = tc::two(-ref, -ref);
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
-            const uint64_t a = tc::two(__uint_as_float(r[c]), __uint_as_float(r[c + 1]));
-            const uint64_t b = tc::two(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3]));
             float p[4];
-            tc::apart(E4M3 ? tc::add2(a, ref2) : tc::fma2(a, scale2, ref2), p[0], p[1]);
-            tc::apart(E4M3 ? tc::add2(b, ref2) : tc::fma2(b, scale2, ref2), p[2], p[3]);
+            tc::apart(tc::fma2(tc::two(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, ref2), p[0], p[1]);
+            tc::apart(tc::fma2(tc::two(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), scale2, ref2), p[2], p[3]);
             p[0] = ex2_approx(p[0]);
             p[1] = ex2_approx(p[1]);
-            if (c % kShare < 4) {                             // of some pairs by multiplications
+            if (c % kShare < 4 && !E4M3) {                    // of some pairs by multiplications
               exp2_pair(p[2], p[3]);
             } else {
               p[2] = ex2_approx(p[2]);
               p[3] = ex2_approx(p[3]);
             }
+            sum0 = tc::add2(tc::two(p[0], p[1]), sum0);
+            sum1 = tc::add2(tc::two(p[2], p[3]), sum1);
             if (E4M3) {
-              const float4 inv = *reinterpret_cast<const float4*>(sc + 2 * kKeys + 32 * i + c);
-              sum0 = tc::fma2(tc::two(p[0], p[1]), tc::two(inv.x, inv.y), sum0);
-              sum1 = tc::fma2(tc::two(p[2], p[3]), tc::two(inv.z, inv.w), sum1);
-            } else {
-              sum0 = tc::add2(tc::two(p[0], p[1]), sum0);
-              sum1 = tc::add2(tc::two(p[2], p[3]), sum1);
+              const float4 v = *reinterpret_cast<const float4*>(sc + kKeys + 32 * i + c);
+              const uint64_t a = tc::mul2(tc::two(p[0], p[1]), tc::two(v.x, v.y)), b = tc::mul2(tc::two(p[2], p[3]), tc::two(v.z, v.w));
+              most = tc::add2(most, tc::add2(a, b));
+              tc::apart(a, p[0], p[1]);
+              tc::apart(b, p[2], p[3]);
             }
             w16[i][c / 2] = pack2<HT>(p[0], p[1]);
             w16[i][c / 2 + 1] = pack2<HT>(p[2], p[3]);
@@ -646,37 +639,36 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         };
         // The reference of the tiles before nearly always serves (scores pass it by less than
         // 2^kLazy): weights are computed with it, and again with the largest score's where it did
-        // not.  A 16-bit row's sum of 64 weights tells; an e4m3 row's weights carry scales, so
-        // its largest score is found beside them.
+        // not, which the sum of a thread's 64 weights tells.
         float top = -INFINITY;
-        sum0 = sum1 = 0;
-        {
+        sum0 = sum1 = most = 0;
+        if (any) {
           const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
           for (int i = 0; i < kC; ++i) {
             uint32_t r[32];
-            if (!E4M3 && !any) break;
             read(r, i);
-            if (E4M3) top = largest(r, top);
-            if (any) weigh(r, i, ref);
+            weigh(r, i, ref);
           }
         }
-        bool passed = !any || !(top <= m + (kLazy + lift));
-        if (!E4M3) {
-          float l0, l1;
-          tc::apart(tc::add2(sum0, sum1), l0, l1);
-          passed = !any || !(l0 + l1 <= kMost);
+        bool passed = true;
+        {
+          float a, b;
+          tc::apart(E4M3 ? most : tc::add2(sum0, sum1), a, b);
+          passed = !any || !(a + b <= kMost);
         }
         if (any_of(pair, 64, passed)) {
-          if (!E4M3) {
 #pragma unroll
-            for (int i = 0; i < kC; ++i) {
-              uint32_t r[32];
-              read(r, i);
-              top = largest(r, top);
+          for (int i = 0; i < kC; ++i) {
+            uint32_t r[32];
+            read(r, i);
+            if (E4M3) {                                       // of the weights with their scales
+#pragma unroll
+              for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(fmaf(__uint_as_float(r[c]), scale, lg2(sc[kKeys + 32 * i + c])));
             }
-            top *= P.scale;
+            top = largest(r, top);
           }
+          if (!E4M3) top *= scale;
           notes.other[slot][half][row] = top;
           sync_some(pair, 64);
           top = max_nan(top, notes.other[slot][half ^ 1][row]);
@@ -698,7 +690,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
           }
           // a NaN or an infinite score makes the row NaN, whichever way its weight is computed
           const float ref = !(top < INFINITY) ? NAN : m == -INFINITY ? 0.0f : m;
-          sum0 = sum1 = 0;
+          sum0 = sum1 = most = 0;
 #pragma unroll
           for (int i = 0; i < kC; ++i) {
             uint32_t r[32];
@@ -802,78 +794,109 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         }
         tc::fence_before();
       } else {
-        if (live && speaks) P.part_ml[static_cast<long long>(part_slot(part)) * S::kRows + tile * 128 + row] = make_float2(m, l);
-        // [128 rows' part][D / 4][128][4]: neighbouring rows side by side
-        uint4* o = part_at(part_slot(part), tile) + my_first / 4 * 128 + row;
-#pragma unroll 1
-        for (int d = 0; d < my_columns && any; d += 8) {
-          uint32_t x[8];
-          tc::load8(x, my_at + d);
-          tc::load_wait();
-          tc::pin8(x);
-          if (live) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) o[(d / 4 + i) * 128] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-          }
-        }
-        tc::fence_before();
-        // the last part's block joins them all
+        // The block that arrives last joins the parts, in their order.  Where all others have
+        // arrived already (a part at the end of a share joins one from the start of the next) this
+        // one's sum is taken from where it is.
         const int parts = w.parts;
-        sync_some(9, 256 * kSlots);
+        unsigned* counter = P.counters + first_block;
         if (tid == 0) {
-          unsigned* counter = P.counters + first_block;
           unsigned n;
-          asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(n) : "l"(counter) : "memory");
-          const bool last = n + 1u == static_cast<unsigned>(parts);
-          if (last) *counter = 0u;
-          notes.flag = last;
+          asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(counter) : "memory");
+          notes.flag = n + 1u == static_cast<unsigned>(parts);
+          if (notes.flag) *counter = 0u;
         }
         sync_some(9, 256 * kSlots);
-        const bool mine = *static_cast<volatile int*>(&notes.flag) != 0;
-        if (mine) {
-          // several threads to a row, each with some of its columns
-          const int spread = two_sums ? 4 : 2;                // threads of a row (with one slot: 256 threads of 128 rows)
-          const int tile = own_rows ? tid >> 8 : 0, rr = tid & 127, nth = two_sums ? tid >> 7 : tid >> 7 & 1;
-          const int mine_row = tile * 128 + rr;
-          if (mine_row < w.rows) {
-            auto ml_at = [&](int x) { return __ldcg(P.part_ml + static_cast<long long>(part_slot(x)) * S::kRows + mine_row); };
-            float mm = -INFINITY, ll = 0.0f;
-            for (int x = 0; x < parts; ++x) mm = fmaxf(mm, ml_at(x).x);
-            for (int x = 0; x < parts; ++x) {
-              const float2 v = ml_at(x);
-              ll += v.x == -INFINITY ? (v.y != v.y ? v.y : 0.0f) : v.y * ex2_approx(v.x - mm);
-            }
-            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-            const int packed_r = w.row0 + mine_row, tok = packed_r / P.group, hd = w.head * P.group + packed_r - tok * P.group;
-            uint16_t* dst = static_cast<uint16_t*>(P.out) + (w.r.q0 + tok) * P.o_tok + hd * P.o_head;
-            if (P.lse && nth == 0) P.lse[static_cast<long long>(w.r.q0 + tok) * P.hq + hd] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * kLn2;
-            // 16 columns at a time
-            for (int d = nth * 16; d < D; d += spread * 16) {
-              float acc[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+        const bool here = *static_cast<volatile int*>(&notes.flag) != 0;
+        bool mine = here;
+        if (!here) {
+          if (live && speaks) P.part_ml[static_cast<long long>(part_slot(part)) * S::kRows + tile * 128 + row] = make_float2(m, l);
+          // [128 rows' part][D / 4][128][4]: neighbouring rows side by side
+          uint4* o = part_at(part_slot(part), tile) + my_first / 4 * 128 + row;
 #pragma unroll 2
-              for (int x = 0; x < parts; ++x) {
-                const float v = ml_at(x).x, f = v == -INFINITY ? 0.0f : ex2_approx(v - mm);
-                if (f == 0.0f) continue;                      // a sum of nothing was not written
-                const uint4* src = part_at(part_slot(x), tile) + d / 4 * 128 + rr;
+          for (int d = 0; d < my_columns && any; d += 8) {
+            uint32_t x[8];
+            tc::load8(x, my_at + d);
+            tc::load_wait();
+            tc::pin8(x);
+            if (live) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) o[(d / 4 + i) * 128] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            }
+          }
+          sync_some(9, 256 * kSlots);
+          if (tid == 0) {
+            unsigned n;
+            asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(n) : "l"(counter) : "memory");
+            notes.flag = n + 1u == static_cast<unsigned>(parts);
+            if (notes.flag) *counter = 0u;
+          }
+          sync_some(9, 256 * kSlots);
+          mine = *static_cast<volatile int*>(&notes.flag) != 0;
+        }
+        if (mine) {
+          auto ml_at = [&](int x) {
+            return here && x == part ? make_float2(m, l) : __ldcg(P.part_ml + static_cast<long long>(part_slot(x)) * S::kRows + tile * 128 + row);
+          };
+          constexpr int kKept = 4;                            // factors of so many parts are kept
+          float mm = -INFINITY, ll = 0.0f, kept[kKept] = {};
+          for (int x = 0; x < parts && live; ++x) mm = fmaxf(mm, ml_at(x).x);
+          auto factor = [&](float v) { return v == -INFINITY ? 0.0f : ex2_approx(v - mm); };
+          for (int x = 0; x < parts && live; ++x) {
+            const float2 v = ml_at(x);
+            const float f = factor(v.x);
+            ll += v.x == -INFINITY ? (v.y != v.y ? v.y : 0.0f) : v.y * f;
+#pragma unroll
+            for (int i = 0; i < kKept; ++i)
+              if (i == x) kept[i] = f;
+          }
+          const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+          uint16_t* dst = static_cast<uint16_t*>(P.out) + (w.r.q0 + token) * P.o_tok + head * P.o_head + my_first;
+          if (live && speaks && P.lse) P.lse[static_cast<long long>(w.r.q0 + token) * P.hq + head] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * kLn2;
+          for (int d = 0; d < my_columns; d += 16) {          // a multiple of 8: the last 8 may be none
+            const bool both = d + 8 < my_columns;
+            float acc[16] = {};
+            auto add = [&](int x, float f) {
+              uint32_t o[2][8] = {};
+              if (here && x == part) {
+                if (any) {
+                  tc::load8(o[0], my_at + d);
+                  if (both) tc::load8(o[1], my_at + d + 8);
+                  tc::load_wait();
+                  tc::pin8(o[0]);
+                  tc::pin8(o[1]);
+                }
+              } else if (f != 0.0f) {                         // a sum of nothing was not written
+                const uint4* src = part_at(part_slot(x), tile) + (my_first + d) / 4 * 128 + row;
+                uint4 v[4] = {};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (i < 2 || both) v[i] = __ldcg(src + i * 128);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                  const uint4 o = __ldcg(src + i * 128);
-                  acc[4 * i] = fmaf(f, __uint_as_float(o.x), acc[4 * i]);
-                  acc[4 * i + 1] = fmaf(f, __uint_as_float(o.y), acc[4 * i + 1]);
-                  acc[4 * i + 2] = fmaf(f, __uint_as_float(o.z), acc[4 * i + 2]);
-                  acc[4 * i + 3] = fmaf(f, __uint_as_float(o.w), acc[4 * i + 3]);
+                  o[i / 2][i % 2 * 4] = v[i].x; o[i / 2][i % 2 * 4 + 1] = v[i].y;
+                  o[i / 2][i % 2 * 4 + 2] = v[i].z; o[i / 2][i % 2 * 4 + 3] = v[i].w;
                 }
               }
+              if (f != 0.0f) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[i] = fmaf(f, __uint_as_float(o[i / 8][i % 8]), acc[i]);
+              }
+            };
+#pragma unroll
+            for (int x = 0; x < kKept; ++x)
+              if (x < parts) add(x, kept[x]);
+#pragma unroll 1
+            for (int x = kKept; x < parts; ++x) add(x, live ? factor(ml_at(x).x) : 0.0f);
+            if (live) {
               uint32_t h[8];
 #pragma unroll
               for (int i = 0; i < 8; ++i) h[i] = pack2<DT>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
               *reinterpret_cast<uint4*>(dst + d) = make_uint4(h[0], h[1], h[2], h[3]);
-              *reinterpret_cast<uint4*>(dst + d + 8) = make_uint4(h[4], h[5], h[6], h[7]);
+              if (both) *reinterpret_cast<uint4*>(dst + d + 8) = make_uint4(h[4], h[5], h[6], h[7]);
             }
           }
         }
+        tc::fence_before();
         sync_some(9, 256 * kSlots);                           // the flag and the part's room are free again
       }
       if (two_sums && !joined) sync_some(9, 512);             // and the first slot's sum, which four warps read
@@ -955,12 +978,14 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         for (int gi = 0; gi < (kGroups + kLoadWarps - 1) / kLoadWarps; ++gi) {
           const int g = wl + kLoadWarps * gi;
           if (g >= kGroups) break;
+          unsigned o[kEach];
+#pragma unroll
+          for (int x = 0; x < kEach; ++x) o[x] = __shfl_sync(0xFFFFFFFFu, p.off[gi >> 1], (gi & 1) * 16 + (x * 32 + lane) / kChunks);
 #pragma unroll
           for (int x = 0; x < kEach; ++x) {
-            const int c = x * 32 + lane, r = c / kChunks, col = c % kChunks, from = (gi & 1) * 16 + r;
-            const unsigned o = __shfl_sync(0xFFFFFFFFu, p.off[gi >> 1], from);
-            const bool there = (p.live[gi >> 1] >> from) & 1u;
-            cp16(to(g * 16 + r, col), side.base + (there ? o + col : 0u) * 16ull, there);
+            const int c = x * 32 + lane, r = c / kChunks, col = c % kChunks;
+            const bool there = (p.live[gi >> 1] >> ((gi & 1) * 16 + r)) & 1u;
+            cp16(to(g * 16 + r, col), side.base + (there ? o[x] + col : 0u) * 16ull, there);
           }
         }
       };
@@ -1072,10 +1097,16 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
           for (int gi = 0; gi < (kGroups + kLoadWarps - 1) / kLoadWarps; ++gi) {
             const int g = wl + kLoadWarps * gi;
             if (g >= kGroups) break;
+            uint4 codes[kEach];
+#pragma unroll
+            for (int x = 0; x < kEach; ++x) {
+              const int c = x * 32 + lane;
+              codes[x] = *reinterpret_cast<const uint4*>(raw + (g * 16 + c / kChunks) * D + c % kChunks * 16);
+            }
 #pragma unroll
             for (int x = 0; x < kEach; ++x) {
               const int c = x * 32 + lane, r = g * 16 + c / kChunks, col = c % kChunks;
-              const uint4 v = *reinterpret_cast<const uint4*>(raw + r * D + col * 16);
+              const uint4 v = codes[x];
               uint32_t h[8];
               e4m3x4(v.x, h[0], h[1]);
               e4m3x4(v.y, h[2], h[3]);
@@ -1094,10 +1125,8 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
             for (int x = 0; x < 2; ++x) {
               const int g = wl + kLoadWarps * (2 * x + (lane >> 4)), r = g * 16 + (lane & 15);
               if (g >= kGroups) continue;
-              const float v = max_nan(cached[kKeys + r], 8e-28f);   // 2^-90
               sc[r] = cached[r];
-              sc[kKeys + r] = lg2(v);
-              sc[2 * kKeys + r] = rcp(v);
+              sc[kKeys + r] = max_nan(cached[kKeys + r], 8e-28f);   // 2^-90
             }
             ++tiles;
           }
