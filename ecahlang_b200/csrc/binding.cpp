@@ -516,14 +516,14 @@ PyObject* copy_pages(PyObject*, PyObject* const* raw, Py_ssize_t n) {
     std::vector<float*> ks(layers), vs(layers);
     ecah_kv_cache first = {};
     for (Py_ssize_t i = 0; i < layers; ++i) {
-      const std::string who = "caches[" + std::to_string(i) + "]";
+      auto who = [&] { return "caches[" + std::to_string(i) + "]"; };
       PyObject* item = PySequence_Fast_GET_ITEM(seq.o, i);
       if (!(PyTuple_Check(item) || PyList_Check(item)) || PySequence_Fast_GET_SIZE(item) != 4)
-        refuse(who + ": expected (k_cache, v_cache, k_scale, v_scale)");
+        refuse(who() + ": expected (k_cache, v_cache, k_scale, v_scale)");
       const Args c{PySequence_Fast_ITEMS(item), 4};
       const at::Tensor &kc = *c.tensor(0, "k_cache"), &vc = *c.tensor(1, "v_cache");
       if (kc.scalar_type() != at::kHalf && kc.scalar_type() != at::kBFloat16 && kc.scalar_type() != at::kFloat8_e4m3fn)
-        refuse(who + ": unsupported cache dtype " + type_name(kc.scalar_type()));
+        refuse(who() + ": unsupported cache dtype " + type_name(kc.scalar_type()));
       need_apart(kc, "k_cache");
       need_apart(vc, "v_cache");
       ecah_kv_cache one = {};
@@ -534,7 +534,7 @@ PyObject* copy_pages(PyObject*, PyObject* const* raw, Py_ssize_t n) {
                  one.num_kv_heads != first.num_kv_heads || one.head_dim != first.head_dim || one.k_page_stride != first.k_page_stride ||
                  one.k_slot_stride != first.k_slot_stride || one.k_head_stride != first.k_head_stride ||
                  one.v_page_stride != first.v_page_stride || one.v_slot_stride != first.v_slot_stride || one.v_head_stride != first.v_head_stride) {
-        refuse(who + ": all layers must have one shape, dtype and set of strides");
+        refuse(who() + ": all layers must have one shape, dtype and set of strides");
       }
       k[i] = one.k_cache; v[i] = one.v_cache; ks[i] = one.k_scale; vs[i] = one.v_scale;
     }

@@ -21,6 +21,9 @@ namespace drafts {
 // dependent loads).  The block that arrives last takes the prefix sums of the warps'
 // sums in vocabulary order, and reads the one range again in which the target lies.
 
+#ifndef NBLK
+#define NBLK 4
+#endif
 constexpr int kT = 256;
 constexpr int kW = kT / 32;
 constexpr int kMaxChunks = 128;              // blocks to a request
@@ -50,8 +53,6 @@ template <int DT> struct Vec {               // 16 bytes of probabilities
   }
 };
 
-__device__ __forceinline__ bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 template <int DT>
 __device__ __forceinline__ float one(const void* row, long long i) {
   using Raw = typename DType<DT>::Raw;
@@ -70,35 +71,64 @@ template <int DT>
 struct Row {
   const void *p, *q;                         // q: subtracted, or NULL
   int out;                                   // entry left out (a certain draft that was refused), or -1
-  bool wide;                                 // both rows start on 16-byte boundaries
+  static constexpr int kN = Vec<DT>::kN, kSize = 16 / kN;
   __device__ __forceinline__ float mass(long long i) const {
     const float x = one<DT>(p, i);
     const float m = positive(q ? x - one<DT>(q, i) : x);
     return i == out ? 0.0f : m;
   }
-  // Sum of the warp's entries [lo, hi), in every lane.
+  // Sum of the warp's entries [lo, hi), in every lane: 16 bytes a load from the first
+  // 16-byte boundary on, where both rows have theirs at the same entries.
   __device__ __forceinline__ double sum(long long lo, long long hi) const {
-    constexpr int kN = Vec<DT>::kN;
     const int lane = threadIdx.x & 31;
-    double s = 0.0;
+    double s = 0.0, t = 0.0;                 // two chains
     long long i = lo;
-    if (wide) {                              // lo is a multiple of 8
+    const unsigned off = static_cast<unsigned>(reinterpret_cast<uintptr_t>(p) + lo * kSize) & 15u;
+    if (!q || ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(q)) & 15) == 0) {
+      const int head = static_cast<int>((16u - off) & 15u) / kSize;
+      if (lane < head && lo + lane < hi) s = mass(lo + lane);
+      i += head;
       const char *a = static_cast<const char*>(p), *b = static_cast<const char*>(q);
-#pragma unroll 2
-      for (; i + 32 * kN <= hi; i += 32 * kN) {
-        const long long at = i + lane * kN;
-        Vec<DT> x, y;
-        x.load(a + at * (16 / kN));
-        if (q) y.load(b + at * (16 / kN));
+      auto add = [&](const Vec<DT>& x, const Vec<DT>& y, long long at) {
 #pragma unroll
         for (int j = 0; j < kN; ++j) {
           const float m = positive(q ? x.x[j] - y.x[j] : x.x[j]);
-          s += at + j == out ? 0.0f : m;
+          (j & 1 ? t : s) += at + j == out ? 0.0f : m;
+        }
+      };
+      constexpr int kFlight = 4;             // loads of a row in flight
+      for (; i + 32 * kN * kFlight <= hi; i += 32 * kN * kFlight) {
+        Vec<DT> x[kFlight], y[kFlight];
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u) {
+          const long long at = i + (u * 32 + lane) * kN;
+          x[u].load(a + at * kSize);
+          if (q) y[u].load(b + at * kSize);
+        }
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u) add(x[u], y[u], i + (u * 32 + lane) * kN);
+      }
+      Vec<DT> x[kFlight], y[kFlight];
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u) {    // the rest, ended lane by lane
+        const long long at = i + (u * 32 + lane) * kN;
+        if (at + kN <= hi) {
+          x[u].load(a + at * kSize);
+          if (q) y[u].load(b + at * kSize);
         }
       }
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u) {
+        const long long at = i + (u * 32 + lane) * kN;
+        if (at + kN <= hi) add(x[u], y[u], at);
+      }
+      i = max(i, hi - (hi - min(i, hi)) % kN);               // what is no whole vector
+      if (i + lane < hi) t += mass(i + lane);
+    } else {
+#pragma unroll 8
+      for (i += lane; i < hi; i += 32) s += mass(i);
     }
-#pragma unroll 4
-    for (i += lane; i < hi; i += 32) s += mass(i);
+    s += t;
 #pragma unroll
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
     return s;
@@ -236,7 +266,6 @@ __global__ void __launch_bounds__(kT) verify_kernel(const Params P) {
   row.p = target + k * P.t_row;
   row.q = k < n && draft ? draft + k * P.d_row : nullptr;
   row.out = k < n && !draft ? ids[k] : -1;
-  row.wide = on16(row.p) && on16(row.q);
 
   unsigned char* record = P.workspace + static_cast<long long>(b) * kRecord;
   double* sums = reinterpret_cast<double*>(record + 256);
@@ -263,7 +292,6 @@ __global__ void __launch_bounds__(kT) verify_kernel(const Params P) {
     __syncthreads();
     row.q = nullptr;
     row.out = -1;
-    row.wide = on16(row.p);
     const long long range = (static_cast<long long>(P.V) + 8 * kW - 1) / (8 * kW) * 8;
     __shared__ double s_sum[kW];
     const double mine = row.sum(warp * range, min((warp + 1) * range, static_cast<long long>(P.V)));
@@ -308,9 +336,10 @@ int ecah_verify_drafts(const ecah_verify_args* a, void* stream) {
   P.tokens = a->tokens; P.accepted = a->accepted;
   P.workspace = static_cast<unsigned char*>(a->workspace);
   P.N = a->drafts; P.V = a->vocab;
-  // Blocks to a request: a few waves over the SMs, and ranges of kRange entries a warp at the least.
+  // Blocks to a request: about a wave over the SMs, and ranges of kRange entries a warp at the least.
+  const long long kBlocks = std::max<long long>(1, NBLK * static_cast<long long>(sms) / a->batch);
   const long long least = static_cast<long long>(drafts::kW) * drafts::kRange;
-  long long chunks = std::min<long long>((a->vocab + least - 1) / least, (8ll * sms + a->batch - 1) / a->batch);
+  long long chunks = std::min<long long>((a->vocab + least - 1) / least, kBlocks);
   chunks = std::max<long long>(1, std::min<long long>(chunks, drafts::kMaxChunks));
   const long long warps = chunks * drafts::kW;
   P.range = static_cast<int>((a->vocab + warps * 8 - 1) / (warps * 8) * 8);

@@ -48,7 +48,7 @@ __device__ __forceinline__ bool pair_of(const Params& P, int i, int* src, int* d
 __global__ void __launch_bounds__(kT) copy_kernel(const __grid_constant__ Params P) {
   grid_start();
   const int layer = blockIdx.y / P.sides, which = blockIdx.y - layer * P.sides;
-  const long long first = static_cast<long long>(blockIdx.x) * (kT * kUnroll) + threadIdx.x;
+  const unsigned first = blockIdx.x * (kT * kUnroll) + threadIdx.x;
   if (which < 2) {
     const Side& s = P.side[which];
     uint4* base = static_cast<uint4*>(P.base[layer][which]);
@@ -56,36 +56,37 @@ __global__ void __launch_bounds__(kT) copy_kernel(const __grid_constant__ Params
     uint4* to[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const long long g = first + u * kT;
-      const int pair = static_cast<int>(g / s.whole), c = static_cast<int>(g - static_cast<long long>(pair) * s.whole);
+      const unsigned g = first + u * kT, pair = g / s.whole, c = g - pair * s.whole;
       to[u] = nullptr;
       int src, dst, tokens;
-      if (g >= static_cast<long long>(P.pairs) * s.whole || !pair_of(P, pair, &src, &dst, &tokens)) continue;
-      const int run = s.slots_in_run ? s.run * tokens : s.run;
-      const int runs = s.slots_in_run ? s.heads : s.heads * tokens;
-      if (run == 0) continue;
-      const int o = c / run, i = c - o * run;
-      if (o >= runs) continue;
-      const int slot = s.slots_in_run ? 0 : o / s.heads, head = s.slots_in_run ? o : o - slot * s.heads;
+      if (pair >= static_cast<unsigned>(P.pairs) || !pair_of(P, pair, &src, &dst, &tokens)) continue;
+      const unsigned run = s.slots_in_run ? s.run * tokens : s.run, runs = s.slots_in_run ? s.heads : s.heads * tokens;
+      unsigned o = 0, i = c;
+      if (c >= run) {                        // not the first run
+        if (runs <= 1 || run == 0) continue;
+        o = c / run;
+        i = c - o * run;
+        if (o >= runs) continue;
+      }
+      const unsigned slot = s.slots_in_run ? 0 : o / s.heads, head = s.slots_in_run ? o : o - slot * s.heads;
       const long long at = slot * s.slot + head * s.head + i;
-      v[u] = base[src * s.page + at];
+      v[u] = __ldcs(base + src * s.page + at);
       to[u] = base + dst * s.page + at;
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-      if (to[u]) *to[u] = v[u];
+      if (to[u]) __stcs(to[u], v[u]);
   } else {
     float* base = static_cast<float*>(P.base[layer][which]);
-    const int whole = P.heads * P.page_size;
+    const unsigned whole = P.heads * P.page_size;
     float v[kUnroll];
     float* to[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const long long g = first + u * kT;
-      const int pair = static_cast<int>(g / whole), c = static_cast<int>(g - static_cast<long long>(pair) * whole);
+      const unsigned g = first + u * kT, pair = g / whole, c = g - pair * whole;
       to[u] = nullptr;
       int src, dst, tokens;
-      if (g >= static_cast<long long>(P.pairs) * whole || !pair_of(P, pair, &src, &dst, &tokens) || c % P.page_size >= tokens) continue;
+      if (pair >= static_cast<unsigned>(P.pairs) || !pair_of(P, pair, &src, &dst, &tokens) || c % P.page_size >= static_cast<unsigned>(tokens)) continue;
       v[u] = base[static_cast<long long>(src) * whole + c];
       to[u] = base + static_cast<long long>(dst) * whole + c;
     }
@@ -132,7 +133,8 @@ extern "C" int ecah_paged_copy(const ecah_copy_args* a, void* stream) {
   const int row = static_cast<int>(a->head_dim / unit);
   const double whole = static_cast<double>(a->page_size) * a->num_kv_heads * row;
   const double chunks = whole * a->pairs;
-  if (whole >= 2147483648.0 || chunks / (copy::kT * copy::kUnroll) >= 2147483647.0) return ECAH_ERR_SHAPE;
+  // chunks of a side are counted in 32 bits (64 GB of a layer's keys in one call)
+  if (whole >= 2147483648.0 || chunks >= 4294967296.0 - copy::kT * copy::kUnroll) return ECAH_ERR_SHAPE;
   copy::Params P;
   P.side[0] = copy::side_of(a->k_page_stride / unit, a->k_slot_stride / unit, a->k_head_stride / unit, a->page_size, a->num_kv_heads, row);
   P.side[1] = copy::side_of(a->v_page_stride / unit, a->v_slot_stride / unit, a->v_head_stride / unit, a->page_size, a->num_kv_heads, row);
