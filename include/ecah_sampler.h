@@ -513,6 +513,10 @@ ECAH_API int ecah_paged_decode_bounded(const ecah_decode_args* args, int32_t tri
  * entries are clamped into [0, tokens].  Sums, rounding and
  * clamped indices as in decode attention; results do not depend on which
  * block finishes last.
+ *
+ * A NaN or an infinity among a request's values may reach also its tokens
+ * that do not see the key (its weight is zero there, and zero times it is
+ * NaN); one among the keys reaches the tokens that see it alone.
  */
 typedef struct ecah_prefill_args {
   int32_t abi_version;

@@ -397,3 +397,58 @@ def test_a_wait_that_runs_out_gives_nan_and_ends(dtype, kv, D):
     assert bool((out[hi:] == 7.0).all()) and bool((lse[hi:] == 7.0).all())
     assert _abi.lib().ecah_paged_prefill_bounded(ctypes.byref(a), 1 << 20, stream) == 0
     compare(s, out, lse)
+
+
+@pytest.mark.parametrize("dtype,kv", KINDS)
+def test_scores_far_below_zero(dtype, kv):
+    """All scores near -600 (log2 units: -866): weights go by the largest, not by zero."""
+    s = setup([140], [150], 4, 2, 64, 16, dtype, kv, seed=15)
+    q = torch.zeros_like(s["q"])
+    q[..., 0] = -20.0
+    s["q"] = q
+    if kv:
+        s["k"].view(torch.uint8)[...] = torch.tensor(30.0, device=DEV).to(E4M3).view(torch.uint8)
+        s["ks"].fill_(1.0)
+    else:
+        s["k"][..., 0] = 30.0 + torch.rand(s["k"].shape[:-1], device=DEV).to(dtype)
+    pg, last = s["indices"].long(), int(s["last"][0])
+    if not kv:
+        s["k"][pg[-1], last:] = float("nan")
+    att = PagedAttention(4, 2, 64, 16, dtype, kv_dtype=kv, max_batch=1)
+    out, lse = call(att, s, return_lse=True, sm_scale=1.0)
+    compare(s, out, lse, sm_scale=1.0)
+    assert float(lse.max()) < -500
+
+
+@pytest.mark.parametrize("dtype,kv", KINDS)
+def test_first_keys_without_mass(dtype, kv):
+    """Scores of -inf through the first two tiles of keys: no reference yet where the others begin, at -200."""
+    s = setup([130], [300], 4, 2, 64, 16, dtype, kv, seed=16)
+    q = torch.zeros_like(s["q"])
+    q[..., 0] = 1.0
+    s["q"] = q
+    pg = s["indices"].long()
+    n, last = s["lengths"][0], int(s["last"][0])
+    if kv:
+        s["k"].view(torch.uint8)[...] = torch.tensor(-1.0, device=DEV).to(E4M3).view(torch.uint8)
+        s["ks"].fill_(200.0)
+        s["ks"][pg[:16]] = float("inf")
+        s["ks"].transpose(1, 2)[pg[-1], last:] = float("nan")
+    else:
+        s["k"][...] = -200.0
+        s["k"][pg[:16]] = 0.0
+        s["k"][pg[:16], :, :, 0] = float("-inf")
+        s["k"][pg[-1], last:] = float("nan")
+    att = PagedAttention(4, 2, 64, 16, dtype, kv_dtype=kv, max_batch=1)
+    out, lse = call(att, s, return_lse=True, sm_scale=1.0)
+    kk = -torch.full((n,), 200.0, dtype=torch.float64, device=DEV)
+    kk[:256] = -math.inf
+    rows = torch.arange(n - 130, n, device=DEV)
+    vv = values(s["v"].view(torch.uint8)[pg].view(E4M3) if kv else s["v"][pg], None if not kv else s["vs"][pg]).reshape(-1, 2, 64)[:n]
+    p = torch.softmax(kk[None, :].expand(130, n).masked_fill(torch.arange(n, device=DEV)[None, :] > rows[:, None], -math.inf), -1)
+    want = torch.einsum("tn,nhd->thd", p, vv).repeat_interleave(2, 1)
+    mass = torch.einsum("tn,nhd->thd", p, vv.abs()).repeat_interleave(2, 1)
+    u = HALF[dtype]
+    assert torch.isfinite(out).all()
+    assert ((out.double() - want).abs() <= u * want.abs() + (u + 2.0 ** -16) * mass + 1e-7).all()
+    assert float((lse.double() - (-200 + (rows - 255).double().log())[:, None]).abs().max()) < 1e-3
