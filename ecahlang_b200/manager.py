@@ -25,6 +25,8 @@ import numpy as np
 import torch
 
 from . import logprobs as token_logprobs
+from ._abi import check, lib
+from .drafts import DraftVerifier, VerifiedDrafts
 from .logprobs import RowLogprobs, TokenLogprobs
 from .sampler import PenaltyState, launch, new_philox_state, new_workspace, repetition_factor, resolve_device
 
@@ -280,6 +282,65 @@ class SamplingManager:
         if self._scorer is None:
             self._scorer = TokenLogprobs(self.vocab_size, self.dtype, self.device, self._logprob_workspace())
         return self._scorer(logits, ids, top_n=top_n, temperature=T, row_index=row_index)
+
+    def init_draft_buffers(self, max_batch: int, max_drafts: int) -> None:
+        """Buffers and workspaces of ``verify_drafts`` for up to ``max_batch``
+        requests of up to ``max_drafts`` drafts (the probabilities alone are
+        ``max_batch * (max_drafts + 1)`` rows of the vocabulary in float32).
+        Call it outside captures, after ``init_sampling_buffers``."""
+        self._outside_capture("verify_drafts")
+        rows, V, dev = max_batch * (max_drafts + 1), self.vocab_size, self.device
+        self._draft_temperature = torch.ones(rows, dtype=torch.float32, device=dev)
+        self._draft_top_k = torch.full((rows,), V, dtype=torch.int32, device=dev)
+        self._draft_top_p = torch.ones(rows, dtype=torch.float32, device=dev)
+        self._draft_uniforms = torch.zeros(rows, dtype=torch.float32, device=dev)
+        self._draft_ids = torch.zeros(rows, dtype=torch.int32, device=dev)
+        self._draft_probs = torch.zeros(rows, V, dtype=torch.float32, device=dev)
+        self._draft_workspace = new_workspace(rows, V, self.dtype, dev)
+        self._verifier = DraftVerifier(V, max_batch, dev)
+
+    def verify_drafts(self, logits: torch.Tensor, draft_ids: torch.Tensor, draft_probs: Optional[torch.Tensor] = None,
+                      num_drafts: Optional[torch.Tensor] = None, uniforms: Optional[torch.Tensor] = None,
+                      bucket_size: Optional[int] = None) -> VerifiedDrafts:
+        """Which of ``draft_ids`` int32 [B, N] are kept, and the token behind
+        them, for requests whose model ran over their last token and their
+        drafts at once: ``logits`` [B * (N + 1), V] (or [B, N + 1, V]), row j of
+        a request following its j-th draft.  The target's probabilities are the
+        sampler's under the filled temperatures, top-k and top-p, the same for
+        all of a request's rows; ``draft_probs``, ``num_drafts`` as
+        ``DraftVerifier`` takes them; ``uniforms`` float32 [B, N + 1] (None: from
+        the manager's Philox state, whose offset advances).  Enqueued on the
+        current stream; capturable.  Rows with penalties are refused: each draft
+        would change those of the rows after it."""
+        if not hasattr(self, "_verifier"):
+            raise RuntimeError("call init_draft_buffers before verify_drafts")
+        if draft_ids.dim() != 2:
+            raise RuntimeError("draft_ids must be [B, N]")
+        B, N = draft_ids.shape
+        rows = B * (N + 1)
+        if rows > self._draft_ids.numel():
+            raise RuntimeError(f"{B} requests of {N} drafts: more rows than init_draft_buffers was called for")
+        if logits.numel() != rows * self.vocab_size or logits.shape[-1] != self.vocab_size:
+            raise RuntimeError(f"logits must be [{rows}, {self.vocab_size}], got {tuple(logits.shape)}")
+        if bucket_size is not None and B != bucket_size:
+            raise RuntimeError(f"bucket {bucket_size} needs {bucket_size} requests, got {B}")
+        T, K, P, _, _, _, _, _, fp = self._buffers(B, bucket_size)
+        if fp or (not torch.cuda.is_current_stream_capturing() and bool(np.any(self.sampling_rep_np[:B] != 1.0))):
+            raise RuntimeError("verify_drafts takes no repetition, frequency or presence penalties")
+        t, k, p = self._draft_temperature[:rows], self._draft_top_k[:rows], self._draft_top_p[:rows]
+        for to, one in ((t, T), (k, K), (p, P)):
+            to.view(B, N + 1).copy_(one.view(B, 1).expand(B, N + 1))
+        u = self._draft_uniforms[:rows]
+        if uniforms is None:
+            with torch.cuda.device(self.device):
+                check(lib().ecah_philox_uniforms(self.philox_state.data_ptr(), rows, u.data_ptr(), 1,
+                                                 torch.cuda.current_stream(self.device).cuda_stream), "ecah_philox_uniforms")
+            uniforms = u.view(B, N + 1)
+        probs = self._draft_probs[:rows]
+        launch(logits.reshape(rows, self.vocab_size), t, k, p, self._draft_ids[:rows], self._draft_workspace,
+               uniforms=self._draft_uniforms[:rows], probs_out=probs)
+        return self._verifier(probs.view(B, N + 1, self.vocab_size), draft_ids, uniforms, draft_probs=draft_probs,
+                              num_drafts=num_drafts)
 
     def sample_async(self, logits: torch.Tensor, bucket_size: Optional[int] = None,
                      uniforms: Optional[torch.Tensor] = None, row_index=None) -> "PendingIds":
