@@ -643,58 +643,47 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
           }
         };
         // The reference of the tiles before nearly always serves (scores pass it by less than
-        // 2^kLazy): weights are computed with it, and again with the largest score's where it did
-        // not, which the sum of a thread's 64 weights tells.
-        float top = -INFINITY;
-        sum0 = sum1 = most = 0;
-        if (any) {
-          const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-          for (int i = 0; i < kC; ++i) {
-            uint32_t r[32];
-            read(r, i);
-            weigh(r, i, ref);
-          }
-        }
-        bool passed = true;
-        {
-          float a, b;
-          tc::apart(E4M3 ? most : tc::add2(sum0, sum1), a, b);
-          passed = !any || !(a + b <= kMost) || (m == -INFINITY && left > 0);   // the last: no reference yet
-        }
-        if (any_of(pair, 64, passed)) {
-#pragma unroll
-          for (int i = 0; i < kC; ++i) {
-            uint32_t r[32];
-            read(r, i);
-            if (E4M3) {                                       // of the weights with their scales
-#pragma unroll
-              for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(fmaf(__uint_as_float(r[c]), scale, lg2(sc[kKeys + 32 * i + c])));
-            }
-            top = largest(r, top);
-          }
-          if (!E4M3) top *= scale;
-          notes.other[slot][half][row] = top;
-          sync_some(pair, 64);
-          top = max_nan(top, notes.other[slot][half ^ 1][row]);
-          const float v = fmaxf(top - lift, m), f = m == v ? 1.0f : ex2_approx(m - v);
-          m = v;
-          l *= f;
-          if (any) {                                          // the row of O, once the product before is in it
-            wait_sum();
+        // 2^8): weights are computed with it, and again with the largest score's where it did
+        // not, which the sum of a thread's 64 weights tells.  A first tile begins with the latter.
+        float ref = m == -INFINITY ? 0.0f : m;
+        bool moved = !any;
 #pragma unroll 1
-            for (int d = 0; d < D / 2; d += 16) {
-              uint32_t o[16];
-              tc::load16(o, sum_at + d);
-              tc::load_wait();
-              tc::pin16(o);
+        while (true) {
+          if (moved) {
+            float top = -INFINITY;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tc::store16(sum_at + d, o);
+            for (int i = 0; i < kC; ++i) {
+              uint32_t r[32];
+              read(r, i);
+              if (E4M3) {                                     // of the weights with their scales
+#pragma unroll
+                for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(fmaf(__uint_as_float(r[c]), scale, lg2(sc[kKeys + 32 * i + c])));
+              }
+              top = largest(r, top);
             }
+            if (!E4M3) top *= scale;
+            notes.other[slot][half][row] = top;
+            sync_some(pair, 64);
+            top = max_nan(top, notes.other[slot][half ^ 1][row]);
+            const float v = fmaxf(top - lift, m), f = m == v ? 1.0f : ex2_approx(m - v);
+            m = v;
+            l *= f;
+            if (any) {                                        // the row of O, once the product before is in it
+              wait_sum();
+#pragma unroll 1
+              for (int d = 0; d < D / 2; d += 16) {
+                uint32_t o[16];
+                tc::load16(o, sum_at + d);
+                tc::load_wait();
+                tc::pin16(o);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tc::store16(sum_at + d, o);
+              }
+            }
+            // a NaN or an infinite score makes the row NaN, whichever way its weight is computed
+            ref = !(top < INFINITY) ? NAN : m == -INFINITY ? 0.0f : m;
           }
-          // a NaN or an infinite score makes the row NaN, whichever way its weight is computed
-          const float ref = !(top < INFINITY) ? NAN : m == -INFINITY ? 0.0f : m;
           sum0 = sum1 = most = 0;
 #pragma unroll
           for (int i = 0; i < kC; ++i) {
@@ -702,7 +691,15 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
             read(r, i);
             weigh(r, i, ref);
           }
-          sync_some(pair, 64);                                // both have read the scores that the weights lie over
+          // the weights lie over scores that the other half's thread reads: both are past that here
+          if (moved) {
+            sync_some(pair, 64);
+            break;
+          }
+          float a, b;
+          tc::apart(E4M3 ? most : tc::add2(sum0, sum1), a, b);
+          moved = any_of(pair, 64, !(a + b <= kMost) || (m == -INFINITY && left > 0));   // the last: no reference yet
+          if (!moved) break;
         }
 #pragma unroll
         for (int i = 0; i < kC; ++i) tc::store16(s_at + c0 / 2 + 16 * i, w16[i]);
