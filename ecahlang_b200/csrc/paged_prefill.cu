@@ -35,6 +35,7 @@ namespace prefill {
 // Warps: 8 of softmax to a slot, two threads to a row (a half of the columns each, so no
 // shuffles; they also rescale their row of O, which a lazily moved reference makes rare,
 // and write it out), 3 that bring keys and values, one thread that issues the products.
+// The softmax warps ask for the next item's queries before they write out this one's rows.
 // Whole tiles come by the copy engine, a box to a page; the last tile of a request (zeros
 // past its length), pages that no box fits and e4m3 rows by threads' 16-byte copies into
 // the swizzled tiles, e4m3 codes through a ring of their own and converted on the way.
@@ -101,12 +102,13 @@ struct Shape {
   static constexpr int kScales = E4M3 ? kKeys * 8 : 0;     // of a tile: key and value scales
   static constexpr int kRaw = E4M3 ? kKeys * (D + 8) : 0;  // of a tile as it is cached: codes, key and value scales
   static constexpr int kRaws = 3;
-  static constexpr int kRoom = 227 * 1024 - 3072;          // beside the block's Notes
+  static constexpr int kNotes = D == 64 ? 3584 : 3072;     // the block's Notes grow with its ring
+  static constexpr int kRoom = 227 * 1024 - kNotes;
   static constexpr int bytes(int n) { return kSlots * kQ + n * kTile + (n / 2 + 2) * kScales + kRaws * kRaw; }
   static constexpr int ring(int n) { return n == 3 || bytes(n) <= kRoom ? n : ring(n - 1); }
   static constexpr int kRing = ring(8);
   static constexpr int kScaleRing = kRing / 2 + 2;
-  static constexpr int kSmem = bytes(kRing) + 3072;
+  static constexpr int kSmem = bytes(kRing) + kNotes;
   static constexpr int kHalf = kKeys / 2;                  // columns of a thread
   static constexpr int kBuffer = kKeys;                    // tensor-memory columns of one of the two score buffers
   static constexpr int kSum = 2 * kKeys;                   // first column of the sums
@@ -328,7 +330,7 @@ struct Notes {
   Share share;
   uint32_t tmem;
   int failed, flag;
-  Walk<D, E4M3> walk[kWalks + 2];      // the softmax slots have two, in turn
+  Walk<D, E4M3> walk[kWalks + 4];      // the softmax slots have three each, in turn
   float other[2][2][128];                                     // between the threads of a row
 };
 
@@ -344,7 +346,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t base = tc::smem_u32(base_p);
   Notes<D, E4M3>& notes = *reinterpret_cast<Notes<D, E4M3>*>(base_p + S::bytes(kRing));
-  static_assert(sizeof(Notes<D, E4M3>) <= 3072 && S::bytes(kRing) % 16 == 0, "");
+  static_assert(sizeof(Notes<D, E4M3>) <= S::kNotes && S::bytes(kRing) % 16 == 0, "");
   Bars<D, E4M3>& s_bars = notes.bars;
   const uint32_t s_q = base, s_ring = base + kSlots * S::kQ, s_scales = s_ring + kRing * S::kTile,
                  s_raw = s_scales + S::kScaleRing * S::kScales;
@@ -355,7 +357,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
   // ---- barriers, tensor memory
   if (tid == 0) {
     auto init = [&](unsigned long long* b, int n) { tc::bar_init(tc::smem_u32(b), n); };
-    init(&s_bars.q_full, E4M3 ? 8 * kSlots : kLoadWarps);
+    init(&s_bars.q_full, 8 * kSlots);
     init(&s_bars.q_empty, 1);
     init(&s_bars.done, 1);
     for (int i = 0; i < kRing; ++i) { init(&s_bars.kv_full[i], kLoadWarps); init(&s_bars.kv_empty[i], 1); }
@@ -490,6 +492,14 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
     return ok;
   };
 
+  // An arrival of the warp once all its threads' copies so far are there; nobody waits here.
+  auto arrive_copied = [&](unsigned long long* b) {
+    const uint32_t bar = tc::smem_u32(b);
+    asm volatile("cp.async.mbarrier.arrive.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+    __syncwarp();
+    if (lane == 0) tc::bar_arrive(bar);
+  };
+
   // a slot's 8 warps share a walk
   Walk<D, E4M3>& w = notes.walk[warp < kLoaders ? warp >> 3 : warp - kLoaders + 2];
 
@@ -513,10 +523,36 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
       ok = ok && (kSlots == 2 ? wait(&s_bars.pv_done[slot], x & 1) : wait(&s_bars.pv_done[x & 1], x >> 1 & 1));
       tc::fence_after();
     };
+    // The 16-bit queries of an item, asked for while the item before it ends: a thread copies a
+    // half of its row (a quarter of one that four threads share).
+    auto ask = [&](const Walk<D, E4M3>& w, bool own_before) {
+      if (!w.found || w.jb >= w.je) return;
+      // Their place is free when the scores of the item before are computed; a slot with rows of
+      // its own has seen its last ones.
+      if (!(own_before && kSlots == 2 && !w.few)) ok = ok && wait(&s_bars.q_empty, q_phase ^ 1);
+      q_phase ^= 1;
+      if (ok) {
+        const bool own_rows = kSlots == 2 && !w.few, quarters = kSlots == 2 && !own_rows;
+        const int my = (own_rows ? slot * 128 : 0) + row, packed = w.row0 + my, token = packed / P.group;
+        const bool live = my < w.rows;
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.q) + (live ? (w.r.q0 + token) * P.q_tok +
+                               (w.head * P.group + packed - token * P.group) * P.q_head : 0));
+        const uint32_t dst = s_q + (own_rows ? slot : 0) * S::kQ + row * 128;
+        const int step = quarters ? 4 : 2;
+#pragma unroll 4
+        for (int c = quarters ? 2 * slot + half : half; c < D / 8; c += step)
+          cp16(dst + (c / 8) * (128 * 128) + ((c % 8) ^ (row & 7)) * 16, src + (live ? c : 0), live);
+      }
+      arrive_copied(&s_bars.q_full);
+    };
     if ((tid & 255) == 0) notes.walk[slot].found = notes.walk[slot].advance(P, notes.share);
-    for (int turn = 0;; turn ^= 1) {
-      sync_some(10 + slot, 256);                              // nobody looks at the item before any more
-      Walk<D, E4M3>& w = notes.walk[turn ? kWalks + slot : slot];
+    sync_some(10 + slot, 256);
+    if (!E4M3) ask(notes.walk[slot], false);
+    // Walks in turn: the one that is written while this item ends was read last two items ago,
+    // and every warp has passed the barrier since.
+    auto walk_at = [&](int turn) -> Walk<D, E4M3>& { return notes.walk[turn == 0 ? slot : kWalks + 2 * (turn - 1) + slot]; };
+    for (int turn = 0;; turn = turn == 2 ? 0 : turn + 1) {
+      Walk<D, E4M3>& w = walk_at(turn);
       if (!w.found) break;
       const bool own_rows = kSlots == 2 && !w.few;            // slots are halves of the rows
       const int my = (own_rows ? slot * 128 : 0) + row;       // row of the item
@@ -662,6 +698,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
               top = largest(r, top);
             }
             if (!E4M3) top *= scale;
+            if (!any) sync_some(pair, 64);                    // both have read what the item before left there
             notes.other[slot][half][row] = top;
             sync_some(pair, 64);
             top = max_nan(top, notes.other[slot][half ^ 1][row]);
@@ -717,12 +754,14 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         if (kSlots == 1) buf ^= 1;
       }
       before += max(w.je - jb, 0);
-      if ((tid & 255) == 0) {                                 // the item after this, while the last product runs
-        Walk<D, E4M3>& then = notes.walk[turn ? slot : kWalks + slot];
+      // the item after this, while the last product runs
+      Walk<D, E4M3>& then = walk_at(turn == 2 ? 0 : turn + 1);
+      if ((tid & 255) == 0) {
         then = w;
         then.found = then.advance(P, notes.share);
       }
-      __syncwarp();
+      sync_some(10 + slot, 256);
+      if (!E4M3) ask(then, own_rows && any);
       if (any) wait_sum();
       if (!ok) l = NAN;
       notes.other[slot][half][row] = l;
@@ -782,17 +821,24 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         if (live && speaks && P.lse)
           P.lse[static_cast<long long>(w.r.q0 + token) * P.hq + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 #pragma unroll 1
-        for (int d = 0; d < my_columns; d += 8) {
-          uint32_t x[8] = {};
+        for (int d = 0; d < my_columns; d += 32) {            // a multiple of 8: the last may be fewer
+          uint32_t x[4][8] = {};
           if (any) {
-            tc::load8(x, my_at + d);
-            tc::load_wait();
-            tc::pin8(x);
-          }
-          uint32_t h[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) h[i] = l == 0.0f ? 0u : pack2<DT>(__uint_as_float(x[2 * i]) * inv, __uint_as_float(x[2 * i + 1]) * inv);
-          if (live) *reinterpret_cast<uint4*>(o + d) = make_uint4(h[0], h[1], h[2], h[3]);
+            for (int i = 0; i < 4; ++i)
+              if (d + 8 * i < my_columns) tc::load8(x[i], my_at + d + 8 * i);
+            tc::load_wait();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tc::pin8(x[i]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t h[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              h[e] = l == 0.0f ? 0u : pack2<DT>(__uint_as_float(x[i][2 * e]) * inv, __uint_as_float(x[i][2 * e + 1]) * inv);
+            if (live && d + 8 * i < my_columns) *reinterpret_cast<uint4*>(o + d + 8 * i) = make_uint4(h[0], h[1], h[2], h[3]);
+          }
         }
         tc::fence_before();
       } else {
@@ -903,48 +949,17 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
       }
       if (two_sums && !joined) sync_some(9, 512);             // and the first slot's sum, which four warps read
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp >= kLoaders && warp < kLoaders + kLoadWarps) {
     // ================================================ keys and values to the ring
     const int wl = warp - kLoaders;
     unsigned n = 0, tiles = 0;                                // loads, key tiles so far
-    uint32_t q_phase = 0;
     bool ok = true;
-    // An arrival of the warp once all its threads' copies so far are there; nobody waits here.
-    auto arrive_copied = [&](unsigned long long* b) {
-      const uint32_t bar = tc::smem_u32(b);
-      asm volatile("cp.async.mbarrier.arrive.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-      __syncwarp();
-      if (lane == 0) tc::bar_arrive(bar);
-    };
     auto free_slot = [&]() { return wait(&s_bars.kv_empty[n % kRing], ((n / kRing) & 1) ^ 1); };
 
     while (ok && w.next(P, notes.share)) {
       if (w.jb >= w.je) continue;
       const bool shared = kSlots == 2 && !w.few;
-      auto queries = [&]() -> bool {
-        ok = wait(&s_bars.q_empty, q_phase ^ 1);
-        q_phase ^= 1;
-        if (!ok) return false;
-        for (int g = wl; g < (shared ? 8 : 4); g += kLoadWarps) {   // 32 rows at a time
-          const int my = 32 * g + lane;
-          long long off = -1;
-          if (my < w.rows) {
-            const int packed = w.row0 + my, token = packed / P.group;
-            off = (w.r.q0 + token) * P.q_tok + (w.head * P.group + packed - token * P.group) * P.q_head;
-          }
-          const uint32_t dst = s_q + (g >> 2) * S::kQ + (g & 3) * 32 * 128;
-          constexpr int kChunks = D / 8;
-#pragma unroll 8
-          for (int x = 0; x < kChunks; ++x) {
-            const int c = x * 32 + lane, r = c / kChunks, col = c % kChunks;
-            const long long o = __shfl_sync(0xFFFFFFFFu, off, r);
-            cp16(dst + (col / 8) * (128 * 128) + r * 128 + ((col % 8) ^ (r & 7)) * 16,
-                 static_cast<const uint16_t*>(P.q) + (o < 0 ? 0 : o + col * 8), o >= 0);
-          }
-        }
-        arrive_copied(&s_bars.q_full);
-        return true;
-      };
       const int* pages = C.indices + w.r.first;
       const int len = w.r.len, head = w.head, je = w.je;
       auto nth_page = [&](int key) { return P.page_shift >= 0 ? key >> P.page_shift : key / C.page_size; };
@@ -1002,8 +1017,6 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         };
         soon(jk);
         for (int i = 0; i < loads; ++i) {
-          // the item's queries behind its first two loads, which wait for nothing of this item
-          if (i == 2 && !queries()) break;
           bool is_v;
           const int j = turn(&is_v);
           const bool boxes_now = P.boxes && (j + 1) * kKeys <= len;
@@ -1045,7 +1058,6 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
           arrive_copied(&s_bars.kv_full[n % kRing]);
           ++n;
         }
-        if (ok && loads == 2) queries();
       } else {
         // Codes and scales as they are cached go to a ring of their own, kRaws - 1 tiles ahead; each
         // warp converts the rows that it copied.
