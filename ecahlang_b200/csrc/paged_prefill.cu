@@ -101,8 +101,8 @@ struct Shape {
   static constexpr int kTile = kKeys * kBlocks * 128;      // bytes of a tile
   static constexpr int kScales = E4M3 ? kKeys * 8 : 0;     // of a tile: key and value scales
   static constexpr int kRaw = E4M3 ? kKeys * (D + 8) : 0;  // of a tile as it is cached: codes, key and value scales
-  static constexpr int kRaws = 3;
-  static constexpr int kNotes = D == 64 ? 3584 : 3072;     // the block's Notes grow with its ring
+  static constexpr int kRaws = 3;                          // as many barriers in Bars
+  static constexpr int kNotes = D == 64 || D == 192 || E4M3 ? 3584 : 3072;     // the block's Notes grow with its ring
   static constexpr int kRoom = 227 * 1024 - kNotes;
   static constexpr int bytes(int n) { return kSlots * kQ + n * kTile + (n / 2 + 2) * kScales + kRaws * kRaw; }
   static constexpr int ring(int n) { return n == 3 || bytes(n) <= kRoom ? n : ring(n - 1); }
@@ -260,8 +260,6 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
 __device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void st16(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -321,6 +319,7 @@ struct Bars {
   unsigned long long q_full, q_empty, done;
   unsigned long long kv_full[Shape<D, E4M3>::kRing], kv_empty[Shape<D, E4M3>::kRing];
   unsigned long long s_full[2], p_full[2], pv_done[2];
+  unsigned long long raw_full[E4M3 ? 3 : 1], raw_empty[E4M3 ? 3 : 1];
 };
 
 // What the block keeps beside tiles.
@@ -361,6 +360,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
     init(&s_bars.q_empty, 1);
     init(&s_bars.done, 1);
     for (int i = 0; i < kRing; ++i) { init(&s_bars.kv_full[i], kLoadWarps); init(&s_bars.kv_empty[i], 1); }
+    for (int i = 0; E4M3 && i < S::kRaws; ++i) { init(&s_bars.raw_full[i], kLoadWarps); init(&s_bars.raw_empty[i], kLoadWarps); }
     for (int i = 0; i < 2; ++i) { init(&s_bars.s_full[i], 1); init(&s_bars.p_full[i], 8); init(&s_bars.pv_done[i], 1); }
     tc::fence_smem();
     notes.failed = 0;
@@ -1007,15 +1007,17 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         }
       };
       int page_next[2] = {page_of(jk, 0), page_of(jk, 1)};    // of the next keys: an L2 read away
+      // Whole tiles come as boxes by a page's slots: of 64 elements each, dealt to the warps, or of
+      // whole rows of codes.
+      const int in_tile = P.boxes ? max(1, kKeys >> P.page_shift) : 0, slots = kKeys / max(1, in_tile);
+      auto soon = [&](int j) {                                // its part of the page list into L1
+        if (lane == 0 && P.boxes && j < je && (j + 1) * kKeys <= len)
+          asm volatile("prefetch.global.L1 [%0];" ::"l"(pages + ((j * kKeys) >> P.page_shift)));
+      };
+      auto listed = [&](int j, int nth) { return min(max(pages[((j * kKeys) >> P.page_shift) + nth], 0), C.num_pages - 1); };
+      soon(jk);
       if (!E4M3) {
-        // whole tiles come as boxes of 64 elements by a page's slots, dealt to the warps
-        const int in_tile = P.boxes ? max(1, kKeys >> P.page_shift) : 0, slots = kKeys / max(1, in_tile);
         const int boxes = in_tile * S::kBlocks, mine = (boxes - wl + kLoadWarps - 1) / kLoadWarps;
-        auto soon = [&](int j) {                              // its part of the page list into L1
-          if (lane == 0 && P.boxes && j < je && (j + 1) * kKeys <= len)
-            asm volatile("prefetch.global.L1 [%0];" ::"l"(pages + ((j * kKeys) >> P.page_shift)));
-        };
-        soon(jk);
         for (int i = 0; i < loads; ++i) {
           bool is_v;
           const int j = turn(&is_v);
@@ -1037,13 +1039,11 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
               const uint32_t bar = tc::smem_u32(&s_bars.kv_full[n % kRing]);
               const void* map = is_v ? &P.v_map : &P.k_map;
               const int slot = (j * kKeys) & (C.page_size - 1);
-              const int* listed = pages + ((j * kKeys) >> P.page_shift);
               tc::bar_expect(bar, mine * slots * 128);
 #pragma unroll 4
               for (int x = wl; x < boxes; x += kLoadWarps) {
                 const int nth = x / S::kBlocks, block = x - nth * S::kBlocks;
-                tc::copy_box(dst + block * (kKeys * 128) + nth * slots * 128, map, block * 64, slot, head,
-                             min(max(listed[nth], 0), C.num_pages - 1), bar);
+                tc::copy_box(dst + block * (kKeys * 128) + nth * slots * 128, map, block * 64, slot, head, listed(j, nth), bar);
               }
             }
             __syncwarp();
@@ -1059,40 +1059,66 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
           ++n;
         }
       } else {
-        // Codes and scales as they are cached go to a ring of their own, kRaws - 1 tiles ahead; each
-        // warp converts the rows that it copied.
+        // Codes and scales as they are cached go to a ring of their own, kRaws - 1 tiles ahead, and
+        // are converted from there.
         int asked = 0;
         const unsigned n0 = n;
         auto ask = [&]() {
           if (asked < loads) {
+            const unsigned place_n = n0 + asked, at_n = place_n % S::kRaws;
             bool is_v;
             const int j = turn(&is_v);
+            const bool boxes_now = P.boxes && (j + 1) * kKeys <= len;
             int page[2] = {page_next[0], page_next[1]};
             if (is_v) {
               ++jv;
-              page[0] = page_of(j, 0); page[1] = page_of(j, 1);
+              if (!boxes_now) { page[0] = page_of(j, 0); page[1] = page_of(j, 1); }
             } else {
               ++jk;
-              page_next[0] = page_of(jk, 0); page_next[1] = page_of(jk, 1);
+              soon(jk + 1);
+              if (!P.boxes || (jk + 1) * kKeys > len) { page_next[0] = page_of(jk, 0); page_next[1] = page_of(jk, 1); }
             }
+            ok = ok && wait(&s_bars.raw_empty[at_n], ((place_n / S::kRaws) & 1) ^ 1);
             const kv::Side16& side = is_v ? P.v : P.k;
-            const uint32_t dst = s_raw + ((n0 + asked) % S::kRaws) * S::kRaw;
-            copy_rows(place(j, page, side), side, [&](int r, int col) { return dst + r * D + col * 16; });
-            if (!is_v) {
+            const uint32_t dst = s_raw + at_n * S::kRaw, bar = tc::smem_u32(&s_bars.raw_full[at_n]);
+            if (!ok) {
+            } else if (!boxes_now) {
+              copy_rows(place(j, page, side), side, [&](int r, int col) { return dst + r * D + col * 16; });
+              if (!is_v) {
 #pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const int g = wl + kLoadWarps * (2 * x + (lane >> 4));
-                if (g >= kGroups) continue;
-                const int key = j * kKeys + g * 16 + (lane & 15);
-                const long long at = page[x] < 0 ? 0 : (static_cast<long long>(page[x]) * C.heads + head) * C.page_size + key - nth_page(key) * C.page_size;
-                const uint32_t to = dst + kKeys * D + (g * 16 + (lane & 15)) * 4;
-                cp4(to, P.k.scale + at, page[x] >= 0);
-                cp4(to + kKeys * 4, P.v.scale + at, page[x] >= 0);
+                for (int x = 0; x < 2; ++x) {
+                  const int g = wl + kLoadWarps * (2 * x + (lane >> 4));
+                  if (g >= kGroups) continue;
+                  const int key = j * kKeys + g * 16 + (lane & 15);
+                  const long long at = page[x] < 0 ? 0 : (static_cast<long long>(page[x]) * C.heads + head) * C.page_size + key - nth_page(key) * C.page_size;
+                  const uint32_t to = dst + kKeys * D + (g * 16 + (lane & 15)) * 4;
+                  cp4(to, P.k.scale + at, page[x] >= 0);
+                  cp4(to + kKeys * 4, P.v.scale + at, page[x] >= 0);
+                }
               }
+              arrive_copied(&s_bars.raw_full[at_n]);
+            } else if (wl == 0) {                             // the first warp asks for the codes,
+              if (tc::elect()) {
+                const void* map = is_v ? &P.v_map : &P.k_map;
+                tc::bar_expect(bar, kKeys * D);
+#pragma unroll 4
+                for (int nth = 0; nth < in_tile; ++nth)
+                  tc::copy_box(dst + nth * slots * D, map, 0, (j * kKeys) & (C.page_size - 1), head, listed(j, nth), bar);
+              }
+              __syncwarp();
+            } else if (wl == 1 || is_v) {
+              if (lane == 0) tc::bar_arrive(bar);
+            } else {                                          // the last for the scales, four neighbours a copy
+#pragma unroll
+              for (int x = 0; x < kKeys / 64; ++x) {
+                const int c = x * 32 + lane, of = c / (kKeys / 4), at = c % (kKeys / 4) * 4, key = j * kKeys + at;
+                const long long from = (static_cast<long long>(listed(j, at >> P.page_shift)) * C.heads + head) * C.page_size + (key & (C.page_size - 1));
+                cp16(dst + kKeys * D + c * 16, (of ? P.v.scale : P.k.scale) + from, true);
+              }
+              arrive_copied(&s_bars.raw_full[at_n]);
             }
           }
           ++asked;
-          cp_commit();
         };
         int kk = w.jb, vv = w.jb;                             // the same order again, for what is converted
 #pragma unroll
@@ -1101,9 +1127,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
           const bool is_v = kk >= je || kk - vv >= ahead;
           if (is_v) ++vv; else ++kk;
           ask();
-          cp_wait<S::kRaws - 1>();
-          __syncwarp();
-          ok = free_slot();
+          ok = ok && wait(&s_bars.raw_full[n % S::kRaws], (n / S::kRaws) & 1) && free_slot();
           if (!ok) break;
           const uint32_t dst = s_ring + (n % kRing) * S::kTile;
           const unsigned char* raw = base_p + (s_raw - base) + (n % S::kRaws) * S::kRaw;
@@ -1146,7 +1170,10 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
           }
           tc::fence_smem();
           __syncwarp();
-          if (lane == 0) tc::bar_arrive(tc::smem_u32(&s_bars.kv_full[n % kRing]));
+          if (lane == 0) {
+            tc::bar_arrive(tc::smem_u32(&s_bars.kv_full[n % kRing]));
+            tc::bar_arrive(tc::smem_u32(&s_bars.raw_empty[n % S::kRaws]));
+          }
           ++n;
         }
       }
@@ -1301,17 +1328,19 @@ static bool box_map(CUtensorMap* map, const kv::Side& s, const ecah_kv_cache& c,
     return reinterpret_cast<Encode>(f);
   }();
   if (!encode) return false;
-  const cuuint64_t row = static_cast<cuuint64_t>(c.head_dim) * 2;
+  const bool e4m3 = c.kv_dtype == ECAH_KV_E4M3;
+  const cuuint64_t size = e4m3 ? 1 : 2, row = static_cast<cuuint64_t>(c.head_dim) * size;
   const cuuint64_t sizes[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.page_size), static_cast<cuuint64_t>(c.num_kv_heads),
                                static_cast<cuuint64_t>(c.num_pages)};
-  cuuint64_t strides[3] = {static_cast<cuuint64_t>(s.slot) * 2, static_cast<cuuint64_t>(s.head) * 2, static_cast<cuuint64_t>(s.page) * 2};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(s.slot) * size, static_cast<cuuint64_t>(s.head) * size, static_cast<cuuint64_t>(s.page) * size};
   for (int i = 0; i < 3; ++i) {
     if (sizes[i + 1] == 1) strides[i] = row;                  // of a dimension of one the stride may be anything
     if (strides[i] == 0 || strides[i] >= 1ull << 40) return false;
   }
-  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(slots), 1, 1}, steps[4] = {1, 1, 1, 1};
-  return encode(map, c.kv_dtype == ECAH_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, s.base, sizes, strides,
-                box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  // 16-bit rows into swizzled blocks of 64 elements; rows of codes as they are
+  const cuuint32_t box[4] = {e4m3 ? static_cast<cuuint32_t>(c.head_dim) : 64u, static_cast<cuuint32_t>(slots), 1, 1}, steps[4] = {1, 1, 1, 1};
+  return encode(map, e4m3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : c.kv_dtype == ECAH_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, s.base, sizes, strides,
+                box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, e4m3 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -1391,8 +1420,9 @@ int ecah_paged_prefill_bounded(const ecah_prefill_args* a, int32_t tries, void* 
       a->dtype == ECAH_DTYPE_F16 ? (e4m3 ? prefill::variant_for<ECAH_DTYPE_F16, true>(c.head_dim) : prefill::variant_for<ECAH_DTYPE_F16, false>(c.head_dim))
                                  : (e4m3 ? prefill::variant_for<ECAH_DTYPE_BF16, true>(c.head_dim) : prefill::variant_for<ECAH_DTYPE_BF16, false>(c.head_dim));
   // Whole tiles by the copy engine where a page is a power of two of 8 slots or more (the
-  // swizzle goes by 8 rows); smaller or odd pages and 8-bit rows go through threads.
-  P.boxes = !e4m3 && P.page_shift >= 3 && prefill::box_map(&P.k_map, P.cache.k, c, std::min(c.page_size, keys)) &&
+  // swizzle goes by 8 rows); smaller or odd pages go through threads (8192 tokens with pages
+  // of 1, 8 and 16 tokens: 731, 592 and 531 us).
+  P.boxes = P.page_shift >= 3 && (!e4m3 || (aligned16(c.k_scale) && aligned16(c.v_scale))) && prefill::box_map(&P.k_map, P.cache.k, c, std::min(c.page_size, keys)) &&
             prefill::box_map(&P.v_map, P.cache.v, c, std::min(c.page_size, keys));
   return launch_kernel(v.fn, dim3(sms), prefill::kT, v.smem, reinterpret_cast<cudaStream_t>(stream), P) ? ECAH_OK : ECAH_ERR_LAUNCH;
 }
