@@ -46,12 +46,13 @@ namespace prefill {
 // parts, so results do not depend on which that is.
 //
 // Measured on one B200, device time of graph replays: a prompt of 8192 tokens, 32/8 heads
-// of 128, bf16 490 to 540 us (1.0 to 1.1 PFLOP/s, 61 to 67 % of the measured GEMM rate; the
-// clock falls under it); 16 packed prompts of 100 to 1024 tokens, 16/2 heads, f16 62; 64
-// drafts of 5 tokens over contexts up to 8000, 32/8 heads, bf16 108 (3.3 TB/s); 7 chunks of
-// up to 333 tokens behind up to 6001 in an e4m3 cache 193; 2 prompts of heads of 256 74.
+// of 128, bf16 498 us (1.1 PFLOP/s, 66 % of the measured GEMM rate; 584 back to back, where
+// the power cap lowers the clock); 16 packed prompts of 100 to 1024 tokens, 16/2 heads, f16
+// 65; 64 drafts of 5 tokens over contexts up to 8000, 32/8 heads, bf16 104 (3.5 TB/s); 7
+// chunks of up to 333 tokens behind up to 6001 in an e4m3 cache 182; 2 prompts of heads of
+// 256 72; a prompt of 37 tokens 17.
 // What bounds the first: an iteration takes 3400 cycles, of which the products 2048 and the
-// exponentials' unit 1536, and a slot waits 1500 for its next scores.  An item takes about
+// exponentials' unit 1536, and a slot waits 1500 for its next scores.  An item takes 6 to
 // 9 us beside its iterations in a share of many small ones; the plan of the shares 1.5
 // (one request) to 4 us (64 requests).
 
@@ -102,7 +103,7 @@ struct Shape {
   static constexpr int kScales = E4M3 ? kKeys * 8 : 0;     // of a tile: key and value scales
   static constexpr int kRaw = E4M3 ? kKeys * (D + 8) : 0;  // of a tile as it is cached: codes, key and value scales
   static constexpr int kRaws = 3;                          // as many barriers in Bars
-  static constexpr int kNotes = D == 64 || D == 192 || E4M3 ? 3584 : 3072;     // the block's Notes grow with its ring
+  static constexpr int kNotes = D == 64 || D == 192 || E4M3 ? 3584 : 3 * 1024;     // the block's Notes grow with its ring
   static constexpr int kRoom = 227 * 1024 - kNotes;
   static constexpr int bytes(int n) { return kSlots * kQ + n * kTile + (n / 2 + 2) * kScales + kRaws * kRaw; }
   static constexpr int ring(int n) { return n == 3 || bytes(n) <= kRoom ? n : ring(n - 1); }
@@ -169,7 +170,7 @@ __device__ __forceinline__ int tiles_of(const Params& P, const Request& r) {
 struct Share {
   unsigned lo, hi, size, more;         // the first `more` blocks have size + 1, the others size
   __device__ __forceinline__ int block_of(unsigned x) const {
-    return static_cast<int>(x < more * (size + 1) ? x / (size + 1) : more + (x - more * (size + 1)) / size);
+    return static_cast<int>(min(x < more * (size + 1) ? x / (size + 1) : more + (x - more * (size + 1)) / size, gridDim.x - 1));
   }
 };
 
@@ -233,7 +234,7 @@ struct Walk {
         whole = i0 == 0 && i1 == t.iters;
         if (!whole) {
           first_block = share.block_of(begin);
-          parts = share.block_of(begin + (t.iters - 1) * unit) - first_block + 1;
+          parts = max(1, share.block_of(begin + (t.iters - 1) * unit) - first_block + 1);
         }
       }
       row0 = t.row0; rows = t.rows; keys = t.keys; few = t.few;
@@ -426,7 +427,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
       if (warp < 2 && x >= run && x < run + sum) {            // the item at an edge of the share
         unsigned p = run;
         int i = 0, t = 0;
-        for (int i0 = 0;; i0 += 32) {                         // its request,
+        for (int i0 = 0; i0 < kKeep; i0 += 32) {              // its request,
           const unsigned c = i0 + lane < min(kKeep, C.batch - b0) ? seen[i0 + lane].cost * C.heads : 0, at = p + before(c);
           const unsigned here = __ballot_sync(0xFFFFFFFFu, x >= at && x < at + c);
           if (here) {
@@ -437,11 +438,11 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
           p = __shfl_sync(0xFFFFFFFFu, at + c, 31);
         }
         const Request r = seen[i].r;
-        const int head = static_cast<int>((x - p) / seen[i].cost);
+        const int head = static_cast<int>((x - p) / max(1u, seen[i].cost));
         p += head * seen[i].cost;
         unsigned cost = 0;
         int iters = 0;
-        for (int t0 = 0;; t0 += 32) {                         // tile
+        for (int t0 = 0; t0 < seen[i].tiles; t0 += 32) {      // tile
           unsigned c = 0;
           if (t0 + lane < seen[i].tiles) {
             const Tile<D, E4M3> tile(P, r, t0 + lane);

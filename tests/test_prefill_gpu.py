@@ -452,3 +452,60 @@ def test_first_keys_without_mass(dtype, kv):
     assert torch.isfinite(out).all()
     assert ((out.double() - want).abs() <= u * want.abs() + (u + 2.0 ** -16) * mass + 1e-7).all()
     assert float((lse.double() - (-200 + (rows - 255).double().log())[:, None]).abs().max()) < 1e-3
+
+
+@pytest.mark.parametrize("dtype,kv", [(torch.float16, None), (torch.bfloat16, E4M3)])
+def test_a_cache_without_pages(dtype, kv):
+    """No key anywhere: zeros and -inf."""
+    att = PagedAttention(4, 2, 64, 16, dtype, kv_dtype=kv, max_batch=2)
+    k, v, ks, vs = att.new_cache(0)
+    q = torch.randn(9, 4, 64, device=DEV).to(dtype)
+    zero = torch.zeros(3, dtype=torch.int32, device=DEV)
+    out, lse = att.prefill(q, torch.tensor([0, 4, 9], dtype=torch.int32, device=DEV), zero, zero[:0], zero[:2], k, v, k_scale=ks,
+                           v_scale=vs, return_lse=True)
+    assert bool((out == 0).all()) and bool(torch.isneginf(lse).all())
+
+
+@pytest.mark.parametrize("kv", [None, E4M3])
+@pytest.mark.parametrize("page", [16, 3])
+def test_pages_past_2_to_the_31_elements(kv, page):
+    """Offsets beyond 32 bits in elements and bytes, by the copy engine and by threads."""
+    Hk, D = 8, 128
+    pages = (5 << 30) // (page * Hk * D)
+    g = torch.Generator(device=DEV).manual_seed(17)
+    raw = torch.uint8 if kv else torch.bfloat16
+    k, v = (torch.empty((pages, page, Hk, D), dtype=raw, device=DEV) for _ in range(2))
+    ks = vs = None
+    new, ctx = [40, 130], [300, 0]
+    lengths = [340, 130]
+    counts = [-(-n // page) for n in lengths]
+    indices = (pages - 1 - torch.randperm(sum(counts) * 2, generator=g, device=DEV)[:sum(counts)]).to(torch.int32)
+    at = indices.long()
+    if kv:
+        ks, vs = (torch.empty((pages, Hk, page), device=DEV) for _ in range(2))
+        for c, s in ((k, ks), (v, vs)):
+            c[at] = (torch.randn((len(at), page, Hk, D), generator=g, device=DEV) * 100).clamp(-448, 448).to(E4M3).view(torch.uint8)
+            s[at] = torch.rand((len(at), Hk, page), generator=g, device=DEV) * 0.02 + 1e-3
+        k, v = k.view(E4M3), v.view(E4M3)
+    else:
+        for c in (k, v):
+            c[at] = torch.randn((len(at), page, Hk, D), generator=g, device=DEV).to(raw)
+    s = dict(q=torch.randn(170, 16, D, generator=g, device=DEV).bfloat16(), ptr=[0, 40, 170], lengths=lengths,
+             qo_indptr=torch.tensor([0, 40, 170], dtype=torch.int32, device=DEV),
+             indptr=torch.tensor([0, counts[0], sum(counts)], dtype=torch.int32, device=DEV), indices=indices,
+             last=torch.tensor([(n - 1) % page + 1 for n in lengths], dtype=torch.int32, device=DEV), k=k, v=v, ks=ks, vs=vs)
+    att = PagedAttention(16, Hk, D, page, torch.bfloat16, kv_dtype=kv, max_batch=2)
+    out, lse = call(att, s, return_lse=True)
+    compare(s, out, lse)
+
+
+def test_requests_that_overlap_are_harmless():
+    """qo_indptr that decreases: not an order the contract allows, but nothing outside out is written and the
+    next launch is right."""
+    s = setup([50, 20], [0, 900], 8, 2, 128, 16, torch.bfloat16, seed=18)
+    att = PagedAttention(8, 2, 128, 16, torch.bfloat16, max_batch=2)
+    out = torch.full((72, 8, 128), 7.0, dtype=torch.bfloat16, device=DEV)
+    call(att, dict(s, qo_indptr=torch.tensor([60, 10, 70], dtype=torch.int32, device=DEV)), out=out[1:71])
+    assert bool((out[0] == 7.0).all()) and bool((out[71] == 7.0).all())
+    got, lse = call(att, s, return_lse=True)
+    compare(s, got, lse)
