@@ -904,9 +904,9 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
           for (int d = 0; d < my_columns; d += 16) {          // a multiple of 8: the last 8 may be none
             const bool both = d + 8 < my_columns;
             float acc[16] = {};
-            auto add = [&](int x, float f) {
-              uint32_t o[2][8] = {};
+            auto fetch = [&](int x, uint4 (&v)[4]) {
               if (here && x == part) {
+                uint32_t o[2][8] = {};
                 if (any) {
                   tc::load8(o[0], my_at + d);
                   if (both) tc::load8(o[1], my_at + d + 8);
@@ -914,28 +914,38 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
                   tc::pin8(o[0]);
                   tc::pin8(o[1]);
                 }
-              } else if (f != 0.0f) {                         // a sum of nothing was not written
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = make_uint4(o[i / 2][i % 2 * 4], o[i / 2][i % 2 * 4 + 1], o[i / 2][i % 2 * 4 + 2], o[i / 2][i % 2 * 4 + 3]);
+              } else {
                 const uint4* src = part_at(part_slot(x), tile) + (my_first + d) / 4 * 128 + row;
-                uint4 v[4] = {};
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                   if (i < 2 || both) v[i] = __ldcg(src + i * 128);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  o[i / 2][i % 2 * 4] = v[i].x; o[i / 2][i % 2 * 4 + 1] = v[i].y;
-                  o[i / 2][i % 2 * 4 + 2] = v[i].z; o[i / 2][i % 2 * 4 + 3] = v[i].w;
-                }
-              }
-              if (f != 0.0f) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[i] = fmaf(f, __uint_as_float(o[i / 8][i % 8]), acc[i]);
               }
             };
+            auto add = [&](float f, const uint4 (&v)[4]) {    // a sum of nothing was not written: its factor is 0
 #pragma unroll
-            for (int x = 0; x < kKept; ++x)
-              if (x < parts) add(x, kept[x]);
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t o[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[4 * i + e] = f == 0.0f ? acc[4 * i + e] : fmaf(f, __uint_as_float(o[e]), acc[4 * i + e]);
+              }
+            };
+            auto two_parts = [&](int x, float f, float g) {   // with their loads in flight together
+              uint4 v[4] = {}, u[4] = {};
+              fetch(x, v);
+              if (x + 1 < parts) fetch(x + 1, u);
+              add(f, v);
+              if (x + 1 < parts) add(g, u);
+            };
+#pragma unroll
+            for (int x = 0; x < kKept; x += 2)
+              if (x < parts) two_parts(x, kept[x], kept[x + 1]);
 #pragma unroll 1
-            for (int x = kKept; x < parts; ++x) add(x, live ? factor(ml_at(x).x) : 0.0f);
+            for (int x = kKept; x < parts; x += 2) {
+              const float2 v = ml_at(x), u = ml_at(min(x + 1, parts - 1));
+              two_parts(x, live ? factor(v.x) : 0.0f, live ? factor(u.x) : 0.0f);
+            }
             if (live) {
               uint32_t h[8];
 #pragma unroll
