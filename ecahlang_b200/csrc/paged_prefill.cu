@@ -75,7 +75,7 @@ constexpr int kShare = 8;
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct alignas(64) Params {
-  CUtensorMap k_map, v_map;            // [pages][heads][slots][head_dim], boxes of 64 elements by the slots of a page in a tile
+  CUtensorMap k_map, v_map;            // [pages][heads][slots][head_dim]; boxes of 64 elements (e4m3: rows) by the slots of a page in a tile
   int boxes;                           // whether the copy engine brings whole tiles
   const void* q;
   void* out;
@@ -279,15 +279,16 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// 2^a and 2^b for arguments below 128, -127 and less to zero, by multiplications: 2^n 2^f with
+// 2^a and 2^b by multiplications (-127 and less: zero; 127 and more, and NaN: 2^127, which no
+// sum of weights that is kept holds): 2^n 2^f with
 // n = round(x) and a polynomial of degree 4 for 2^f on [-1/2, 1/2] that is 1 at zero (its
 // relative error, minimised in the maximum, is at most 2.9e-6); n comes out of the sum x + 1.5 2^23
 // in its low bits, and goes into the exponent.  The exponential's unit does 16 a clock
 // on an SM, which is as long as the products take.
 __device__ __forceinline__ void exp2_pair(float& a, float& b) {
   constexpr float kMagic = 12582912.0f;
-  a = fmaxf(a, -127.0f);
-  b = fmaxf(b, -127.0f);
+  a = fmaxf(fminf(a, 127.0f), -127.0f);
+  b = fmaxf(fminf(b, 127.0f), -127.0f);
   const uint64_t x = tc::two(a, b), t = tc::add2(x, tc::two(kMagic, kMagic));
   const uint64_t f = tc::fma2(tc::add2(t, tc::two(-kMagic, -kMagic)), tc::two(-1.0f, -1.0f), x);
   uint64_t p = tc::fma2(f, tc::two(0x1.3a02ccp-7f, 0x1.3a02ccp-7f), tc::two(0x1.c9fc46p-5f, 0x1.c9fc46p-5f));

@@ -75,12 +75,6 @@ __device__ __forceinline__ void store8(uint32_t at, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), ECAH_I8(r, 0) : "memory");
 }
 __device__ __forceinline__ void pin16(uint32_t (&r)[16]) { asm volatile("" : ECAH_R8(r, 0), ECAH_R8(r, 8)); }
-__device__ __forceinline__ void store32(uint32_t at, const uint32_t (&r)[32]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-               "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-               "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-               ::"r"(at), ECAH_I8(r, 0), ECAH_I8(r, 8), ECAH_I8(r, 16), ECAH_I8(r, 24) : "memory");
-}
 __device__ __forceinline__ void store16(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
                "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"

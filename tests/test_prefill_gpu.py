@@ -509,3 +509,33 @@ def test_requests_that_overlap_are_harmless():
     assert bool((out[0] == 7.0).all()) and bool((out[71] == 7.0).all())
     got, lse = call(att, s, return_lse=True)
     compare(s, got, lse)
+
+
+@pytest.mark.parametrize("dtype,kv", KINDS)
+@pytest.mark.parametrize("jump", [100.0, 400.0, 30000.0, float("nan")])
+def test_one_key_that_outweighs_all_before_in_every_place(dtype, kv, jump):
+    """128 requests; request i's key 128 + i alone scores `jump` above the zeros before and behind it (a NaN:
+    makes its rows NaN), in a tile behind the first, in every column of it."""
+    B, D, page, n = 128, 64, 16, 384
+    k = torch.zeros(B * n // page, page, 1, D, device=DEV)
+    v = torch.zeros_like(k)
+    at = torch.arange(B, device=DEV) * n + 128 + torch.arange(B, device=DEV)
+    k.view(-1, D)[at, 0] = 1.0 if kv else jump
+    v.view(-1, D)[at] = 3.0
+    ks = vs = None
+    if kv:
+        ks, vs = (torch.ones(B * n // page, 1, page, device=DEV) for _ in range(2))
+        ks.view(-1)[at] = jump
+    q = torch.zeros(2 * B, 1, D, dtype=dtype, device=DEV)
+    q[:, 0, 0] = 1.0
+    att = PagedAttention(1, 1, D, page, dtype, kv_dtype=kv, max_batch=B)
+    out, lse = att.prefill(q, torch.arange(0, 2 * B + 1, 2, dtype=torch.int32, device=DEV),
+                           torch.arange(0, B * n // page + 1, n // page, dtype=torch.int32, device=DEV),
+                           torch.arange(B * n // page, dtype=torch.int32, device=DEV), torch.full((B,), page, dtype=torch.int32, device=DEV),
+                           k.to(kv or dtype), v.to(kv or dtype), k_scale=ks, v_scale=vs, sm_scale=1.0, return_lse=True)
+    if math.isnan(jump):
+        assert torch.isnan(out).all() and torch.isnan(lse).all()
+        return
+    assert bool((out == 3.0).all())
+    want = jump if kv else float(torch.tensor(jump).to(dtype))
+    assert float((lse - want).abs().max()) <= 2e-5 + 4e-6 * jump
