@@ -310,8 +310,9 @@ class SamplingManager:
         all of a request's rows; ``draft_probs``, ``num_drafts`` as
         ``DraftVerifier`` takes them; ``uniforms`` float32 [B, N + 1] (None: from
         the manager's Philox state, whose offset advances).  Enqueued on the
-        current stream; capturable.  Rows with penalties are refused: each draft
-        would change those of the rows after it."""
+        current stream; capturable.  Rows with penalties are refused, since each
+        draft would change those of the rows after it (a replayed capture does
+        not look again: do not fill any for its bucket)."""
         if not hasattr(self, "_verifier"):
             raise RuntimeError("call init_draft_buffers before verify_drafts")
         if draft_ids.dim() != 2:

@@ -539,3 +539,30 @@ def test_one_key_that_outweighs_all_before_in_every_place(dtype, kv, jump):
     assert bool((out == 3.0).all())
     want = jump if kv else float(torch.tensor(jump).to(dtype))
     assert float((lse - want).abs().max()) <= 2e-5 + 4e-6 * jump
+
+
+def test_two_handles_on_two_streams_at_once():
+    """Launches that overlap, of one kernel and of others, with a workspace each: the results of one after another."""
+    from ecahlang_b200.drafts import DraftVerifier
+    sets = [setup([400, 30, 7], [50, 3000, 900], 16, 2, 128, 16, torch.bfloat16, seed=20),
+            setup([90, 5, 5, 5], [0, 5000, 100, 2000], 32, 8, 64, 16, torch.float16, E4M3, seed=21)]
+    atts = [PagedAttention(16, 2, 128, 16, torch.bfloat16, max_batch=4), PagedAttention(32, 8, 64, 16, torch.float16, kv_dtype=E4M3, max_batch=4)]
+    g = torch.Generator(device=DEV).manual_seed(22)
+    p = torch.softmax(torch.randn(4, 3, 30000, generator=g, device=DEV), -1)
+    ids, u = p[:, :2].argmax(-1).int(), torch.rand(4, 3, generator=g, device=DEV)
+    vers = [DraftVerifier(30000, 4), DraftVerifier(30000, 4)]
+    want = [call(a, s, return_lse=True) for a, s in zip(atts, sets)]
+    drawn = vers[0](p, ids, u)
+    streams = [torch.cuda.Stream() for _ in atts]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(25):
+        for i, (a, s, st) in enumerate(zip(atts, sets, streams)):
+            with torch.cuda.stream(st):
+                got[i].append((*call(a, s, return_lse=True), *vers[i](p, ids, u)))
+    torch.cuda.synchronize()
+    for i, runs in enumerate(got):
+        lo, hi = sets[i]["ptr"][0], sets[i]["ptr"][-1]
+        for out, lse, tokens, accepted in runs:
+            assert torch.equal(out[lo:hi], want[i][0][lo:hi]) and torch.equal(lse[lo:hi], want[i][1][lo:hi])
+            assert torch.equal(tokens, drawn.tokens) and torch.equal(accepted, drawn.accepted)
