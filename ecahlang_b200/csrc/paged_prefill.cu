@@ -46,7 +46,7 @@ namespace prefill {
 // parts, so results do not depend on which that is.
 //
 // Measured on one B200, device time of graph replays: a prompt of 8192 tokens, 32/8 heads
-// of 128, bf16 500 us (1.1 PFLOP/s, 66 % of the measured GEMM rate; 584 back to back, where
+// of 128, bf16 500 us (1.1 PFLOP/s, 66 % of the measured GEMM rate; 584 to 600 back to back, as
 // the power cap lowers the clock); 16 packed prompts of 100 to 1024 tokens, 16/2 heads, f16
 // 65; 64 drafts of 5 tokens over contexts up to 8000, 32/8 heads, bf16 104 (3.5 TB/s); 7
 // chunks of up to 333 tokens behind up to 6001 in an e4m3 cache 182; 2 prompts of heads of
