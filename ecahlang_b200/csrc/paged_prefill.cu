@@ -530,8 +530,11 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
     auto ask = [&](const Walk<D, E4M3>& w, bool own_before) {
       if (!w.found || w.jb >= w.je) return;
       // Their place is free when the scores of the item before are computed; a slot with rows of
-      // its own has seen its last ones.
-      if (!(own_before && kSlots == 2 && !w.few)) ok = ok && wait(&s_bars.q_empty, q_phase ^ 1);
+      // its own has seen its last ones, and learns from the item's first scores that the phase has
+      // ended.  Where the item has none for it (a first half that sees no key) it looks here: its
+      // next look, two phases ahead of the barrier, would succeed at once.
+      const bool scored = slot != 0 || w.je0 > w.jb;
+      if (!(own_before && kSlots == 2 && !w.few && scored)) ok = ok && wait(&s_bars.q_empty, q_phase ^ 1);
       q_phase ^= 1;
       if (ok) {
         const bool own_rows = kSlots == 2 && !w.few, quarters = kSlots == 2 && !own_rows;

@@ -566,3 +566,16 @@ def test_two_handles_on_two_streams_at_once():
         for out, lse, tokens, accepted in runs:
             assert torch.equal(out[lo:hi], want[i][0][lo:hi]) and torch.equal(lse[lo:hi], want[i][1][lo:hi])
             assert torch.equal(tokens, drawn.tokens) and torch.equal(accepted, drawn.accepted)
+
+
+@pytest.mark.parametrize("dtype,kv", KINDS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("Hq,Hk,n,length", [(32, 32, 400, 250), (32, 8, 100, 60), (28, 4, 300, 275), (7, 7, 900, 700)])
+def test_first_halves_of_tiles_that_see_no_key(dtype, kv, D, Hq, Hk, n, length):
+    """More new tokens than cached ones, so that the first 128 rows of a tile see no key and the next 128 do, head
+    behind head in one block: the same bits every time, and right."""
+    att, s = check([n] * 4, [length - n] * 4, Hq, Hk, D, 16, dtype, kv, seed=n)
+    want = call(att, s, return_lse=True)
+    for _ in range(20):
+        for a, b in zip(call(att, s, return_lse=True), want):
+            assert torch.equal(a, b)
