@@ -331,6 +331,7 @@ struct Notes {
   Share share;
   uint32_t tmem;
   int failed, flag;
+  unsigned brought[kLoadWarps];        // tiles that a loader has announced on kv_full (e4m3: raw_full)
   Walk<D, E4M3> walk[kWalks + 4];      // the softmax slots have three each, in turn
   float other[2][2][128];                                     // between the threads of a row
 };
@@ -968,7 +969,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
   } else if (warp >= kLoaders && warp < kLoaders + kLoadWarps) {
     // ================================================ keys and values to the ring
     const int wl = warp - kLoaders;
-    unsigned n = 0, tiles = 0;                                // loads, key tiles so far
+    unsigned n = 0, raws = 0, tiles = 0;                      // loads; e4m3: those announced as they are cached; key tiles so far
     bool ok = true;
     auto free_slot = [&]() { return wait(&s_bars.kv_empty[n % kRing], ((n / kRing) & 1) ^ 1); };
 
@@ -1132,6 +1133,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
               }
               arrive_copied(&s_bars.raw_full[at_n]);
             }
+            if (ok) raws = place_n + 1;
           }
           ++asked;
         };
@@ -1193,6 +1195,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         }
       }
     }
+    if (lane == 0) notes.brought[wl] = E4M3 ? raws : n;
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == kIssuer) {
     // ================================================================ products
@@ -1309,6 +1312,19 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
   __syncthreads();
   tc::fence_after();
   if (warp == kIssuer) tc::tmem_free(tmem, S::kColumns);
+  // Where a wait ran out the copy engine may still be bringing tiles that nobody waited for: they
+  // land before the block ends and its shared memory is another's.  A loader that stopped first
+  // owes the tiles that another announced its arrival (one on a barrier at the most, since a place
+  // is used again only after all have arrived); nobody else looks at the barriers any more.
+  if (notes.failed && warp >= kLoaders && warp < kLoaders + kLoadWarps) {
+    constexpr unsigned ring = E4M3 ? S::kRaws : kRing;
+    unsigned long long* full = E4M3 ? s_bars.raw_full : s_bars.kv_full;
+    unsigned all = 0;
+    for (int i = 0; i < kLoadWarps; ++i) all = max(all, notes.brought[i]);
+    for (unsigned x = notes.brought[warp - kLoaders]; x < all && lane == 0; ++x) tc::bar_arrive(tc::smem_u32(&full[x % ring]));
+    for (unsigned x = all - min(all, ring); x < all; ++x)
+      for (int i = 0; i < kTries && !tc::bar_test(tc::smem_u32(&full[x % ring]), x / ring & 1); ++i) {}
+  }
 }
 
 using KernelFn = void (*)(const Params);

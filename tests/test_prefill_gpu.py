@@ -579,3 +579,38 @@ def test_first_halves_of_tiles_that_see_no_key(dtype, kv, D, Hq, Hk, n, length):
     for _ in range(20):
         for a, b in zip(call(att, s, return_lse=True), want):
             assert torch.equal(a, b)
+
+
+def bounded(att, s, out, lse, tries):
+    """``ecah_paged_prefill_bounded``, enqueued."""
+    ptr = lambda t: None if t is None else t.data_ptr()   # noqa: E731
+    q, k, v = s["q"], s["k"], s["v"]
+    half = 0 if q.dtype == torch.float16 else 1
+    a = _abi.PrefillArgs(abi_version=_abi.ABI_VERSION, dtype=half, tokens=q.shape[0], num_qo_heads=q.shape[1], sm_scale=q.shape[2] ** -0.5,
+                         causal=1, q=ptr(q), q_token_stride=q.stride(0), q_head_stride=q.stride(1), out=ptr(out),
+                         out_token_stride=out.stride(0), out_head_stride=out.stride(1), lse=ptr(lse), qo_indptr=ptr(s["qo_indptr"]),
+                         kv_last_page_len=ptr(s["last"]), workspace=ptr(att.prefill_workspace), workspace_bytes=att.prefill_workspace.numel())
+    a.cache = _abi.KVCache(kv_dtype=_abi.KV_E4M3 if k.dtype == E4M3 else half, num_pages=k.shape[0], page_size=k.shape[1],
+                           num_kv_heads=k.shape[2], head_dim=k.shape[3], batch=len(s["lengths"]), k_cache=ptr(k), v_cache=ptr(v),
+                           k_page_stride=k.stride(0), k_slot_stride=k.stride(1), k_head_stride=k.stride(2), v_page_stride=v.stride(0),
+                           v_slot_stride=v.stride(1), v_head_stride=v.stride(2), k_scale=ptr(s["ks"]), v_scale=ptr(s["vs"]),
+                           kv_indptr=ptr(s["indptr"]), kv_indices=ptr(s["indices"]), num_indices=s["indices"].numel())
+    assert _abi.lib().ecah_paged_prefill_bounded(ctypes.byref(a), tries, torch.cuda.current_stream().cuda_stream) == 0
+
+
+@pytest.mark.parametrize("dtype,kv", KINDS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_waits_of_a_few_tries_end_and_leave_the_next_launch_right(dtype, kv, D):
+    """Limits that run out in the middle, with tiles under way by the copy engine: the launch ends, writes no row
+    that is not the requests', and what follows on the same SMs and workspace is right."""
+    s = setup([300, 5, 40], [0, 6000, 2000], 8, 2, D, 16, dtype, kv, behind=3, seed=23)
+    att = PagedAttention(8, 2, D, 16, dtype, kv_dtype=kv, max_batch=3)
+    T, hi = s["q"].shape[0], s["ptr"][-1]
+    out, lse = torch.empty((T, 8, D), dtype=dtype, device=DEV), torch.empty((T, 8), device=DEV)
+    for tries in (1, 2, 3, 5, 9, 30, 100):
+        for limit in (tries, tries, 1 << 20):
+            out.fill_(7.0); lse.fill_(7.0)
+            bounded(att, s, out, lse, limit)
+            torch.cuda.synchronize()
+            assert bool((out[hi:] == 7.0).all()) and bool((lse[hi:] == 7.0).all())
+        compare(s, out, lse)
