@@ -769,7 +769,10 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
       sync_some(10 + slot, 256);
       if (!E4M3) ask(then, own_rows && any);
       if (any) wait_sum();
-      if (!ok) l = NAN;
+      // Warps whose wait ran out arrive without waiting, and so may have let products begin before
+      // others' weights or queries were there: the block's rows are NaN from here on.  (Those warps
+      // said so before they arrived, and this warp has waited for the products since.)
+      if (!ok || *static_cast<volatile int*>(&notes.failed)) l = NAN;
       notes.other[slot][half][row] = l;
       sync_some(pair, 64);
       l += notes.other[slot][half ^ 1][row];

@@ -614,3 +614,23 @@ def test_waits_of_a_few_tries_end_and_leave_the_next_launch_right(dtype, kv, D):
             torch.cuda.synchronize()
             assert bool((out[hi:] == 7.0).all()) and bool((lse[hi:] == 7.0).all())
         compare(s, out, lse)
+
+
+@pytest.mark.parametrize("dtype,kv", KINDS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_waits_that_run_out_for_some_give_nan_or_the_row(dtype, kv, D):
+    """Some warps of a block give up while others go on: no row may hold products of what was not there yet.  Both
+    many items of one tile of keys and few items of many."""
+    for new, ctx in (([300, 5, 40], [0, 6000, 2000]), ([257] * 24, [0] * 24), ([900], [3000])):
+        s = setup(new, ctx, 8, 2, D, 16, dtype, kv, seed=24)
+        att = PagedAttention(8, 2, D, 16, dtype, kv_dtype=kv, max_batch=len(new))
+        want, wlse, tol, ltol = reference(s["q"], s["ptr"], s["lengths"], s["indptr"], s["indices"], s["k"], s["v"], s["ks"], s["vs"],
+                                          D ** -0.5, True)
+        out, lse = torch.empty(want.shape, dtype=dtype, device=DEV), torch.empty(wlse.shape, device=DEV)
+        for tries in (1, 1, 2, 2, 3, 4, 6, 10, 20, 50):
+            out.fill_(7.0); lse.fill_(7.0)
+            bounded(att, s, out, lse, tries)
+            torch.cuda.synchronize()
+            lost = torch.isnan(lse)
+            assert bool(((out.double() - want).abs() <= tol)[~lost].all()) and bool(((lse.double() - wlse).abs() <= ltol)[~lost].all())
+            assert bool(torch.isnan(out).all(-1)[lost].all())
