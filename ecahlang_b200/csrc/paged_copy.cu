@@ -47,7 +47,7 @@ __device__ __forceinline__ bool pair_of(const Params& P, int i, int* src, int* d
   *src = P.src[i];
   *dst = P.dst[i];
   *tokens = P.tokens ? min(max(P.tokens[i], 0), P.page_size) : P.page_size;
-  return *src >= 0 && *dst >= 0 && *src < P.num_pages && *dst < P.num_pages && *src != *dst;
+  return *tokens > 0 && *src >= 0 && *dst >= 0 && *src < P.num_pages && *dst < P.num_pages && *src != *dst;
 }
 
 __global__ void __launch_bounds__(kT) copy_kernel(const __grid_constant__ Params P) {
@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kT) copy_kernel(const __grid_constant__ Params
       const unsigned run = s.slots_in_run ? s.run * tokens : s.run, runs = s.slots_in_run ? s.heads : s.heads * tokens;
       unsigned o = 0, i = c;
       if (c >= run) {                        // not the first run
-        if (runs <= 1 || run == 0) continue;
+        if (runs <= 1) continue;
         o = c / run;
         i = c - o * run;
         if (o >= runs) continue;

@@ -75,6 +75,23 @@ def test_strides_that_leave_gaps(dtype):
             assert torch.equal(now, old)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_no_tokens_of_pages_with_gaps(dtype):
+    """Zero tokens and fewer copy nothing, also where a slot does not follow its neighbour."""
+    g = torch.Generator(device=DEV).manual_seed(6)
+    big = [torch.zeros((9, 8, 4, 256), dtype=torch.uint8 if dtype == E4M3 else dtype, device=DEV).view(dtype) for _ in range(2)]
+    for b in big:
+        raw(b).copy_(torch.randint(0, 255, b.shape, generator=g, device=DEV).to(raw(b).dtype))
+    cuts = [lambda b: b[:, :, :3, :64], lambda b: b[:, :5, :, :], lambda b: b[:, 1:7:2, 1:2], lambda b: b[:, :, ::2, :128],
+            lambda b: b[:, :, 1::2, 64:128]]
+    for cut in cuts:
+        k, v = (cut(b) for b in big)
+        s = [None, None] if dtype != E4M3 else [torch.rand((9, k.shape[2], k.shape[1]), generator=g, device=DEV) for _ in range(2)]
+        src, dst, tokens = [0, 1, 2, 4], [7, 3, 5, 8], [0, -3, 0, 2]
+        t = [torch.tensor(x, dtype=torch.int32, device=DEV) for x in (src, dst, tokens)]
+        check([(k, v, *s)], lambda: paged.copy_pages(t[0], t[1], [(k, v, *s)], tokens=t[2]), src, dst, [max(n, 0) for n in tokens])
+
+
 def test_many_layers_and_pairs():
     g = torch.Generator(device=DEV).manual_seed(2)
     att = PagedAttention(8, 2, 64, 16, torch.float16, kv_dtype=E4M3)
