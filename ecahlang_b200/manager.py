@@ -58,6 +58,11 @@ class SamplingManager:
         # freq_pres_in_graphs=True captures every bucket with them.
         self.freq_pres_in_graphs = freq_pres_in_graphs
         self._cg_captured_fp: Dict[int, bool] = {}
+        # Which rows of each set of buffers (a bucket's, or None for the eager
+        # ones) hold penalties, and which sets verify_drafts was captured with:
+        # it takes none.
+        self._penalised: Dict[Optional[int], np.ndarray] = {}
+        self._captured_drafts: set = set()
         self._workspace: Optional[torch.Tensor] = None
         self._scorer: Optional[TokenLogprobs] = None
         self._scorer_workspace: Optional[torch.Tensor] = None
@@ -126,6 +131,7 @@ class SamplingManager:
         self.sampling_pres_gpu = torch.zeros(B, dtype=torch.float32, device=dev)
         self.sampling_slot_gpu = torch.full((B,), -1, dtype=torch.int32, device=dev)
         self.sampling_out = torch.zeros(B, dtype=torch.int32, device=dev)
+        self._forget_drafts(None, B)
         self._workspace = None
         if dev.type == "cuda":
             self._sample_workspace()
@@ -148,6 +154,22 @@ class SamplingManager:
             self._scorer_workspace = token_logprobs.new_workspace(self.device)
         return self._scorer_workspace
 
+    def _forget_drafts(self, buffers: Optional[int], rows: int) -> None:
+        """A set of buffers was made (again): no penalties, and no capture reads it."""
+        self._penalised[buffers] = np.zeros(rows, dtype=bool)
+        self._captured_drafts.discard(buffers)
+
+    def _note_penalties(self, buffers: Optional[int], n: int) -> None:
+        """Called between the write of n host rows and their copy to a set of device buffers."""
+        rows = (self.sampling_rep_np[:n] != 1) | (self.sampling_freq_np[:n] != 0) | (self.sampling_pres_np[:n] != 0)
+        if buffers in self._captured_drafts and rows.any():
+            raise RuntimeError(
+                f"{'the eager buffers were' if buffers is None else f'bucket {buffers} was'} captured into a CUDA graph "
+                "with verify_drafts, which takes no penalties: a replay would ignore them (fill another bucket)")
+        if buffers is not None:
+            self._penalised[buffers][:] = False              # the padding rows
+        self._penalised[buffers][:n] = rows
+
     def _write_host(self, n, temperatures, top_ks, top_ps, rep_pens, freq_pens, pres_pens, batch_ids) -> bool:
         self.sampling_temperature_np[:n, 0] = temperatures
         self.sampling_top_k_np[:n] = top_ks
@@ -164,7 +186,9 @@ class SamplingManager:
         """Writes the first n rows' parameters through the pinned buffers
         (manager.py:90-97).  rep_pens are the requests' repetition penalties
         (stored as the per-update factor), batch_ids select their slots."""
-        self._fp_eager = self._write_host(n, temperatures, top_ks, top_ps, rep_pens, freq_pens, pres_pens, batch_ids)
+        fp = self._write_host(n, temperatures, top_ks, top_ps, rep_pens, freq_pens, pres_pens, batch_ids)
+        self._note_penalties(None, n)
+        self._fp_eager = fp
         for g, c in ((self.sampling_temperature_gpu, self.sampling_temperature_cpu),
                      (self.sampling_top_k_gpu, self.sampling_top_k_cpu),
                      (self.sampling_top_p_gpu, self.sampling_top_p_cpu),
@@ -191,6 +215,7 @@ class SamplingManager:
             self._cg_slot[bs] = torch.full((bs,), -1, dtype=torch.int32, device=dev)
             self._cg_out[bs] = torch.zeros(bs, dtype=torch.int32, device=dev)
             self._fp_cg[bs] = False
+            self._forget_drafts(bs, bs)
 
     def fill_cuda_graph_sampling_params(self, bucket_size: int, n: int, temperatures, top_ks, top_ps,
                                         rep_pens=None, freq_pens=None, pres_pens=None,
@@ -210,6 +235,7 @@ class SamplingManager:
             raise RuntimeError(
                 f"bucket {bs} was captured into a CUDA graph without frequency/presence penalties; "
                 "a replay cannot apply them (construct the manager with freq_pres_in_graphs=True)")
+        self._note_penalties(bs, n)
         self._fp_cg[bs] = fp
         for g, c in ((self._cg_temperature[bs], self.sampling_temperature_cpu),
                      (self._cg_top_k[bs], self.sampling_top_k_cpu),
@@ -311,8 +337,9 @@ class SamplingManager:
         ``DraftVerifier`` takes them; ``uniforms`` float32 [B, N + 1] (None: from
         the manager's Philox state, whose offset advances).  Enqueued on the
         current stream; capturable.  Rows with penalties are refused, since each
-        draft would change those of the rows after it (a replayed capture does
-        not look again: do not fill any for its bucket)."""
+        draft would change those of the rows after it; so is a later fill with
+        penalties of a bucket (or of the eager buffers) that a capture of this
+        call reads."""
         if not hasattr(self, "_verifier"):
             raise RuntimeError("call init_draft_buffers before verify_drafts")
         if draft_ids.dim() != 2:
@@ -325,9 +352,11 @@ class SamplingManager:
             raise RuntimeError(f"logits must be [{rows}, {self.vocab_size}], got {tuple(logits.shape)}")
         if bucket_size is not None and B != bucket_size:
             raise RuntimeError(f"bucket {bucket_size} needs {bucket_size} requests, got {B}")
-        T, K, P, _, _, _, _, _, fp = self._buffers(B, bucket_size)
-        if fp or (not torch.cuda.is_current_stream_capturing() and bool(np.any(self.sampling_rep_np[:B] != 1.0))):
+        T, K, P = self._buffers(B, bucket_size)[:3]
+        if self._penalised[bucket_size][:B].any():
             raise RuntimeError("verify_drafts takes no repetition, frequency or presence penalties")
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            self._captured_drafts.add(bucket_size)
         t, k, p = self._draft_temperature[:rows], self._draft_top_k[:rows], self._draft_top_p[:rows]
         for to, one in ((t, T), (k, K), (p, P)):
             to.view(B, N + 1).copy_(one.view(B, 1).expand(B, N + 1))

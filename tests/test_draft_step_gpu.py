@@ -112,3 +112,34 @@ def test_example_runs():
         out = subprocess.run([sys.executable, os.path.join(ROOT, "examples", "draft_step.py"), "--steps", "3", *extra], check=True,
                              capture_output=True, text=True).stdout
         assert out.count("step ") == 3
+
+
+def test_a_captured_bucket_refuses_penalties_and_another_fill_does_not_hide_them():
+    from ecahlang_b200.manager import SamplingManager
+    V, B, N = 1000, 2, 3
+    m = SamplingManager(V, seq_lens=8, dtype=torch.float16, seed=5)
+    m.init_sampling_buffers(8)
+    m.init_cuda_graph_buffers([B, 4])
+    m.init_draft_buffers(8, N)
+    plain = ([1.0] * B, [V] * B, [1.0] * B)
+    best = torch.tensor([[7, 900, 7, 0], [999, 1, 2, 3]], device="cuda")
+    x = torch.zeros(B, N + 1, V, dtype=torch.float16, device="cuda").scatter_(2, best[..., None], 9.0)
+    ids = best[:, :N].int()
+    m.fill_cuda_graph_sampling_params(B, B, *plain, rep_pens=[1.5] * B)
+    m.fill_sampling_params(B, *plain)
+    with pytest.raises(RuntimeError, match="penalties"):
+        m.verify_drafts(x, ids, bucket_size=B)
+    m.fill_cuda_graph_sampling_params(B, B, *plain)
+    m.verify_drafts(x, ids, bucket_size=B)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = m.verify_drafts(x, ids, bucket_size=B)
+    for pens in (dict(rep_pens=[1.5] * B), dict(freq_pens=[0.5] * B), dict(pres_pens=[0.5] * B)):
+        with pytest.raises(RuntimeError, match="captured"):
+            m.fill_cuda_graph_sampling_params(B, B, *plain, **pens)
+        m.fill_cuda_graph_sampling_params(4, B, *plain, **pens)
+        m.fill_sampling_params(B, *plain, **pens)
+    m.fill_cuda_graph_sampling_params(B, B, [0.0] * B, [V] * B, [1.0] * B)
+    graph.replay()
+    assert out.accepted.tolist() == [N] * B and torch.equal(out.tokens, best.int())   # greedy

@@ -109,3 +109,56 @@ def test_full_penalty_history_is_reported():
     s2 = m.allocate("r2")
     assert s2 == s
     m.fill_sampling_params(1, [1.0], [V], [1.0], rep_pens=[1.1], batch_ids=["r2"])   # reset on allocate
+
+
+def _drafting():
+    m = _mgr()
+    m.init_cuda_graph_buffers([2, 4])
+    m.init_draft_buffers(8, 1)
+    return m
+
+
+def _verified(m, B, bucket=None):
+    """Whether verify_drafts takes the rows: it then reaches the launch, which has no CPU path."""
+    with pytest.raises(RuntimeError, match="CUDA|penalties") as e:
+        m.verify_drafts(torch.zeros(2 * B, V, dtype=torch.float16), torch.zeros(B, 1, dtype=torch.int32), uniforms=torch.zeros(B, 2),
+                        bucket_size=bucket)
+    return "penalties" not in str(e.value)
+
+
+@pytest.mark.parametrize("pens", [dict(rep_pens=[1.5, 1.5]), dict(freq_pens=[0.5, 0.0]), dict(pres_pens=[0.0, 0.5])])
+def test_verify_drafts_looks_at_the_penalties_of_its_own_buffers(pens):
+    """Not at those of whichever buffers were filled last, nor at rows that a fill did not write."""
+    m = _drafting()
+    plain = ([1.0, 1.0], [V, V], [1.0, 1.0])
+    m.fill_cuda_graph_sampling_params(2, 2, *plain, **pens)
+    m.fill_cuda_graph_sampling_params(4, 2, *plain)
+    m.fill_sampling_params(2, *plain)
+    assert not _verified(m, 2, 2) and _verified(m, 4, 4) and _verified(m, 2)
+    m.fill_cuda_graph_sampling_params(2, 2, *plain)
+    m.fill_sampling_params(2, *plain, **pens)
+    assert _verified(m, 2, 2) and _verified(m, 4, 4) and not _verified(m, 2)
+    m = _drafting()
+    m.fill_sampling_params(8, [1.0] * 8, [V] * 8, [1.0] * 8, **{k: v * 4 for k, v in pens.items()})
+    m.fill_cuda_graph_sampling_params(4, 2, *plain)
+    assert _verified(m, 4, 4)                                # its padding rows were reset
+    m.fill_sampling_params(2, *plain)
+    assert _verified(m, 2) and not _verified(m, 4)           # rows 2 and 3 still hold the first fill's
+
+
+@pytest.mark.parametrize("pens", [dict(rep_pens=[1.5]), dict(freq_pens=[0.5]), dict(pres_pens=[0.5])])
+@pytest.mark.parametrize("bucket", [2, None])
+def test_buffers_captured_by_verify_drafts_refuse_penalties(pens, bucket):
+    """A replay would ignore them."""
+    m = _drafting()
+    fill = lambda b, **kw: (m.fill_sampling_params(1, [1.0], [V], [1.0], **kw) if b is None else   # noqa: E731
+                            m.fill_cuda_graph_sampling_params(b, 1, [1.0], [V], [1.0], **kw))
+    m._captured_drafts.add(bucket)                           # what verify_drafts records while capturing
+    fill(bucket)
+    with pytest.raises(RuntimeError, match="captured"):
+        fill(bucket, **pens)
+    fill(4, **pens)                                          # other buffers take them
+    assert not _verified(m, 4, 4)
+    m.init_sampling_buffers(8)
+    m.init_cuda_graph_buffers([2, 4])                        # made again: no capture reads them
+    fill(bucket, **pens)
