@@ -63,6 +63,7 @@ class SamplingManager:
         # it takes none.
         self._penalised: Dict[Optional[int], np.ndarray] = {}
         self._captured_drafts: set = set()
+        self._draft_kept: list = []                             # buffers that captured verify_drafts may read
         self._workspace: Optional[torch.Tensor] = None
         self._scorer: Optional[TokenLogprobs] = None
         self._scorer_workspace: Optional[torch.Tensor] = None
@@ -313,9 +314,18 @@ class SamplingManager:
         """Buffers and workspaces of ``verify_drafts`` for up to ``max_batch``
         requests of up to ``max_drafts`` drafts (the probabilities alone are
         ``max_batch * (max_drafts + 1)`` rows of the vocabulary in float32).
-        Call it outside captures, after ``init_sampling_buffers``."""
-        self._outside_capture("verify_drafts")
+        Call it outside captures, after ``init_sampling_buffers``.  Called
+        again it keeps what is there if that is enough; else larger buffers are
+        made beside it, since captured calls go on reading the old ones."""
         rows, V, dev = max_batch * (max_drafts + 1), self.vocab_size, self.device
+        if hasattr(self, "_verifier"):
+            if rows <= self._draft_ids.numel() and max_batch <= self._verifier.max_batch:
+                return
+            rows, max_batch = max(rows, self._draft_ids.numel()), max(max_batch, self._verifier.max_batch)
+        self._outside_capture("verify_drafts")
+        if hasattr(self, "_verifier"):
+            self._draft_kept.append((self._draft_temperature, self._draft_top_k, self._draft_top_p, self._draft_uniforms,
+                                     self._draft_ids, self._draft_probs, self._draft_workspace, self._verifier))
         self._draft_temperature = torch.ones(rows, dtype=torch.float32, device=dev)
         self._draft_top_k = torch.full((rows,), V, dtype=torch.int32, device=dev)
         self._draft_top_p = torch.ones(rows, dtype=torch.float32, device=dev)

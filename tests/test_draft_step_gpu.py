@@ -143,3 +143,32 @@ def test_a_captured_bucket_refuses_penalties_and_another_fill_does_not_hide_them
     m.fill_cuda_graph_sampling_params(B, B, [0.0] * B, [V] * B, [1.0] * B)
     graph.replay()
     assert out.accepted.tolist() == [N] * B and torch.equal(out.tokens, best.int())   # greedy
+
+
+def test_a_capture_survives_draft_buffers_made_again():
+    from ecahlang_b200.manager import SamplingManager
+    V, B, N = 3000, 2, 3
+    m = SamplingManager(V, seq_lens=8, dtype=torch.float16, seed=6)
+    m.init_sampling_buffers(8)
+    m.init_cuda_graph_buffers([B])
+    m.init_draft_buffers(B, N)
+    m.fill_cuda_graph_sampling_params(B, B, [1.0] * B, [V] * B, [1.0] * B)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = (torch.randn(B, N + 1, V, generator=g, device="cuda") * 3).half()
+    ids, u = x[:, :N].float().argmax(-1).int(), torch.rand(B, N + 1, generator=g, device="cuda")
+    m.verify_drafts(x, ids, uniforms=u, bucket_size=B)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = m.verify_drafts(x, ids, uniforms=u, bucket_size=B)
+    for batch, drafts in ((B, N), (4, 5)):
+        m.init_draft_buffers(batch, drafts)
+        junk = [torch.full((B * (N + 1) * V,), float("nan"), device="cuda") for _ in range(4)] + \
+               [torch.full((n,), -7, dtype=torch.int32, device="cuda") for n in (8, 8, 2100, 4200, 8400)]
+        x.copy_((torch.randn(B, N + 1, V, generator=g, device="cuda") * 3).half())
+        u.copy_(torch.rand(B, N + 1, generator=g, device="cuda"))
+        for _ in range(2):
+            graph.replay()
+            want = m.verify_drafts(x, ids, uniforms=u, bucket_size=B)
+            assert torch.equal(out.tokens, want.tokens) and torch.equal(out.accepted, want.accepted)
+        assert all(bool(torch.isnan(t).all()) for t in junk[:4]) and all(bool((t == -7).all()) for t in junk[4:])   # nothing in their memory

@@ -162,3 +162,16 @@ def test_buffers_captured_by_verify_drafts_refuse_penalties(pens, bucket):
     m.init_sampling_buffers(8)
     m.init_cuda_graph_buffers([2, 4])                        # made again: no capture reads them
     fill(bucket, **pens)
+
+
+def test_draft_buffers_made_again_leave_those_of_captures():
+    m = _mgr()
+    m.init_draft_buffers(4, 3)
+    names = ("_draft_temperature", "_draft_top_k", "_draft_top_p", "_draft_uniforms", "_draft_ids", "_draft_probs", "_draft_workspace")
+    first = [getattr(m, n) for n in names] + [m._verifier]
+    m.init_draft_buffers(2, 7)                               # 16 rows of up to 4 requests are enough
+    assert all(getattr(m, n) is t for n, t in zip(names, first)) and m._verifier is first[-1] and not m._draft_kept
+    m.init_draft_buffers(2, 8)
+    assert len(m._draft_kept) == 1 and all(a is b for a, b in zip(m._draft_kept[0], first))
+    assert m._draft_ids.numel() == 18 and m._verifier.max_batch == 4     # no less than before
+    assert all(getattr(m, n) is not t for n, t in zip(names, first)) and m._verifier.workspace is not first[-1].workspace
