@@ -157,7 +157,8 @@ def copy_pages(src, dst, caches, *, tokens=None) -> None:
 
 class PagedAttention:
     """One model's paged attention on one stream: its head layout and the
-    workspaces, shared by all layers.
+    workspaces, shared by all layers (``prefill``'s is made by its first call,
+    which has to be outside a capture).
 
     ``kv_dtype`` is the model dtype (default) or ``torch.float8_e4m3fn``;
     ``max_batch`` bounds the requests of one ``decode`` or ``prefill``."""
@@ -180,12 +181,25 @@ class PagedAttention:
         self.device = resolve_device(device)
         with torch.cuda.device(self.device):
             n = decode_workspace_bytes(max_batch, num_qo_heads, num_kv_heads, head_dim)
-            m = prefill_workspace_bytes(head_dim)
         self.workspace = torch.zeros(n, dtype=torch.uint8, device=self.device)
-        self.prefill_workspace = torch.zeros(m, dtype=torch.uint8, device=self.device)
+        self._prefill_workspace: Optional[torch.Tensor] = None
         self._layout = (num_qo_heads, num_kv_heads, head_dim, page_size, int(kv_dtype == E4M3), max_batch,
                         _DTYPES[dtype])
         self._append, self._decode, self._prefill = binding().append, binding().decode, binding().prefill
+
+    @property
+    def prefill_workspace(self) -> torch.Tensor:
+        """``prefill``'s workspace (39 MB), made by the first ``prefill``, so that
+        a handle that only decodes holds none.  Not inside a CUDA-graph capture,
+        where it would be zero-filled by that graph's replays alone."""
+        if self._prefill_workspace is None:
+            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the workspace of prefill cannot be made inside a CUDA-graph capture: "
+                                   "call prefill once before it, or read prefill_workspace")
+            with torch.cuda.device(self.device):
+                n = prefill_workspace_bytes(self.head_dim)
+            self._prefill_workspace = torch.zeros(n, dtype=torch.uint8, device=self.device)
+        return self._prefill_workspace
 
     def new_cache(self, num_pages: int):
         """(k_cache, v_cache, k_scale, v_scale) of one layer, zero-filled; the
@@ -222,7 +236,7 @@ class PagedAttention:
         if lse is None and return_lse:
             lse = True
         got = self._prefill(q, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, k_cache, v_cache,
-                            self.prefill_workspace, k_scale, v_scale, causal, sm_scale, out, lse, self._layout)
+                            self._prefill_workspace if self._prefill_workspace is not None else self.prefill_workspace, k_scale, v_scale, causal, sm_scale, out, lse, self._layout)
         return got[0] if lse is not None and not return_lse else got
 
     def copy_pages(self, src, dst, caches, *, tokens=None) -> None:

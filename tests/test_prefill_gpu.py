@@ -634,3 +634,30 @@ def test_waits_that_run_out_for_some_give_nan_or_the_row(dtype, kv, D):
             lost = torch.isnan(lse)
             assert bool(((out.double() - want).abs() <= tol)[~lost].all()) and bool(((lse.double() - wlse).abs() <= ltol)[~lost].all())
             assert bool(torch.isnan(out).all(-1)[lost].all())
+
+
+def test_the_workspace_is_made_by_the_first_prefill(monkeypatch):
+    """A handle that only decodes holds none; a capture cannot make it; handles and captures after that share nothing."""
+    s = setup([40, 9], [3, 700], 8, 2, 128, 16, torch.float16, seed=25)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    att = PagedAttention(8, 2, 128, 16, torch.float16, max_batch=2)
+    dec = att.decode(s["q"][:2], s["indptr"], s["indices"], s["last"], s["k"], s["v"])
+    assert torch.cuda.memory_allocated() - before - att.workspace.numel() < 1 << 20
+    assert torch.isfinite(dec).all()
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="inside a CUDA-graph capture"):
+            call(att, s)
+    assert att._prefill_workspace is None
+    out, lse = call(att, s, return_lse=True)
+    compare(s, out, lse)
+    ws = att.prefill_workspace
+    assert ws.numel() == paged.prefill_workspace_bytes(128) and att.prefill_workspace is ws
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, l2 = call(att, s, return_lse=True)
+    graph.replay()
+    assert torch.equal(got, out) and torch.equal(l2, lse)
+    other = PagedAttention(8, 2, 128, 16, torch.float16, max_batch=2)
+    assert other.prefill_workspace.data_ptr() != ws.data_ptr()       # reading it makes it
