@@ -69,7 +69,8 @@ constexpr int kWalks = 2 + kLoadWarps + 1;   // of the softmax slots, the loader
 constexpr int kKeep = 128;             // requests looked at together
 constexpr int kTries = 1 << 20;        // of a wait: more than one between warps of a block can need
 constexpr float kLift = 7.0f;          // f16 weights begin at 2^7 and reach 2^15, so that small ones are not lost
-// Of four neighbouring scores the last two are raised by multiplications (exp2_pair) once
+// Of four neighbouring scores the last two are raised by multiplications (tc::exp2_pair), since
+// the exponentials' unit does 16 a clock on an SM, which is as long as the products take, once
 // in kShare scores (8192 tokens: 528 us with 8, 576 with 16 or none, 624 with 4).
 constexpr int kShare = 8;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -278,28 +279,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
-}
-// 2^a and 2^b by multiplications (-127 and less: zero; 127 and more, and NaN: 2^127, which no
-// sum of weights that is kept holds): 2^n 2^f with
-// n = round(x) and a polynomial of degree 4 for 2^f on [-1/2, 1/2] that is 1 at zero (its
-// relative error, minimised in the maximum, is at most 2.9e-6); n comes out of the sum x + 1.5 2^23
-// in its low bits, and goes into the exponent.  The exponential's unit does 16 a clock
-// on an SM, which is as long as the products take.
-__device__ __forceinline__ void exp2_pair(float& a, float& b) {
-  constexpr float kMagic = 12582912.0f;
-  a = fmaxf(fminf(a, 127.0f), -127.0f);
-  b = fmaxf(fminf(b, 127.0f), -127.0f);
-  const uint64_t x = tc::two(a, b), t = tc::add2(x, tc::two(kMagic, kMagic));
-  const uint64_t f = tc::fma2(tc::add2(t, tc::two(-kMagic, -kMagic)), tc::two(-1.0f, -1.0f), x);
-  uint64_t p = tc::fma2(f, tc::two(0x1.3a02ccp-7f, 0x1.3a02ccp-7f), tc::two(0x1.c9fc46p-5f, 0x1.c9fc46p-5f));
-  p = tc::fma2(f, p, tc::two(0x1.ec0378p-3f, 0x1.ec0378p-3f));
-  p = tc::fma2(f, p, tc::two(0x1.62e12cp-1f, 0x1.62e12cp-1f));
-  p = tc::fma2(f, p, tc::two(1.0f, 1.0f));
-  float pa, pb, ta, tb;
-  tc::apart(p, pa, pb);
-  tc::apart(t, ta, tb);
-  a = __uint_as_float(__float_as_uint(pa) + (__float_as_uint(ta) << 23));
-  b = __uint_as_float(__float_as_uint(pb) + (__float_as_uint(tb) << 23));
 }
 __device__ __forceinline__ float lg2(float x) {
   float r;
@@ -666,7 +645,7 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
             p[0] = ex2_approx(p[0]);
             p[1] = ex2_approx(p[1]);
             if (c % kShare < 4 && !E4M3) {                    // of some pairs by multiplications
-              exp2_pair(p[2], p[3]);
+              tc::exp2_pair(p[2], p[3]);
             } else {
               p[2] = ex2_approx(p[2]);
               p[3] = ex2_approx(p[3]);
