@@ -473,6 +473,9 @@ ECAH_API int ecah_paged_append(const ecah_append_args* args, void* stream);
  * length are never read.  Indices outside the cache are clamped into it.
  * The sums are float32; softmax weights are rounded to the 16-bit operand of
  * the tensor cores.  Results do not depend on which block finishes last.
+ * A score of NaN or +inf makes its row of o NaN, and its lse too (not +inf); a
+ * key of score -inf has no weight, and a row of nothing else gives o = 0 and
+ * lse = -inf.
  */
 typedef struct ecah_decode_args {
   int32_t abi_version;
@@ -518,8 +521,8 @@ ECAH_API int ecah_paged_decode_bounded(const ecah_decode_args* args, int32_t tri
  * A token that sees no key (len == 0, or n > len and i < n - len) gives o = 0
  * and lse = -inf.  Rows of q outside every request (padding rows behind the
  * last one) are neither read nor written.  qo_indptr must not decrease; its
- * entries are clamped into [0, tokens].  Sums, rounding and
- * clamped indices as in decode attention; results do not depend on which
+ * entries are clamped into [0, tokens].  Sums, rounding, clamped indices and
+ * infinite scores as in decode attention; results do not depend on which
  * block finishes last.
  *
  * A NaN or an infinity among a request's values may reach also its tokens

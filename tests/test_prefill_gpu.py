@@ -671,3 +671,63 @@ def test_exponentials_by_multiplications():
     assert int(bad) == 0
     assert 2.5e-6 < float(worst) <= 2.84e-6 + 1.2e-7
     assert _abi.lib().ecah_exp2_pair_check(None, bad.data_ptr(), stream) == 1
+
+
+def with_scores(new, ctx, D, dtype, kv, at, score):
+    """A batch of one request whose keys score 0, but key ``at`` as it says (scaled by 1); values random."""
+    s = setup([new], [ctx], 4, 2, D, 16, dtype, kv, seed=26)
+    q = torch.zeros_like(s["q"])
+    q[..., 0] = 1.0
+    s["q"] = q
+    pg = s["indices"].long()
+    (s["k"].view(torch.uint8) if kv else s["k"])[pg] = 0
+    where = (pg[at // 16], slice(None), at % 16) if kv else (pg[at // 16], at % 16)
+    if kv:
+        s["k"].view(torch.uint8)[pg[at // 16], at % 16, :, 0] = torch.tensor(1.0 if score > 0 or score != score else -1.0).to(E4M3).view(torch.uint8).item()
+        s["ks"][pg] = 1.0
+        s["ks"][where] = abs(score)
+    else:
+        s["k"][where + (slice(None), 0)] = score
+    return s
+
+
+@pytest.mark.parametrize("dtype,kv", KINDS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("score", [math.inf, math.nan, -math.inf])
+def test_infinite_scores_reach_the_rows_that_see_them_alone(dtype, kv, D, score):
+    """+inf and NaN: rows and log-sum-exp are NaN, in whole items and in ones joined of parts; -inf: no weight."""
+    att = PagedAttention(4, 2, D, 16, dtype, kv_dtype=kv, max_batch=1)
+    for new, ctx, at in ((200, 0, 150), (3, 9000, 40), (3, 9000, 8990), (300, 2000, 2100)):
+        s = with_scores(new, ctx, D, dtype, kv, at, score)
+        out, lse = call(att, s, return_lse=True, sm_scale=1.0)
+        sees = torch.arange(ctx, ctx + new, device=DEV) >= at
+        n = torch.arange(ctx + 1, ctx + new + 1, device=DEV).double()
+        if score == -math.inf:
+            n = n - sees.double()
+            sees = torch.zeros_like(sees)
+        assert torch.isnan(out[sees]).all() and torch.isnan(lse[sees]).all()
+        assert torch.isfinite(out[~sees]).all()
+        assert ((lse[~sees].double() - n[~sees].log()[:, None]).abs() <= 2e-5 + 4e-6 * 10).all()
+        if new == 3:                              # decode: the same rules for the last token
+            o, l = att.decode(s["q"][-1:], s["indptr"], s["indices"], s["last"], s["k"], s["v"], k_scale=s["ks"], v_scale=s["vs"],
+                              sm_scale=1.0, return_lse=True)
+            if score == -math.inf:
+                assert torch.isfinite(o).all() and ((l.double() - n[-1].log()).abs() <= 6e-5).all()
+            else:
+                assert torch.isnan(o).all() and torch.isnan(l).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_a_row_of_scores_without_mass(dtype, D):
+    """Every score -inf: zeros, and a log-sum-exp of -inf, in prefill and decode."""
+    s = setup([70], [200], 4, 2, D, 16, dtype, seed=27)
+    q = torch.zeros_like(s["q"])
+    q[..., 0] = 1.0
+    s["q"] = q
+    pg = s["indices"].long()
+    s["k"][pg] = 0.0
+    s["k"][pg, :, :, 0] = -math.inf
+    att = PagedAttention(4, 2, D, 16, dtype, max_batch=1)
+    for out, lse in (call(att, s, return_lse=True), att.decode(q[:1], s["indptr"], s["indices"], s["last"], s["k"], s["v"], return_lse=True)):
+        assert bool((out == 0).all()) and bool(torch.isneginf(lse).all())
