@@ -647,8 +647,9 @@ __global__ void __launch_bounds__(kT, Shape<D, E4M3, NT, BULK>::kBlocks) decode_
             l[x][1] += p1 + p3;
           }
           // Keys by heads to heads by keys: the products' second operand, in its 16 bits.  A
-          // weight is off by at most 2^-9 of itself in bf16 (2^-12 in f16), at random over the
-          // keys: in bf16 about 0.8 of the output's own rounding.
+          // weight is rounded by at most 2^-8 of itself in bf16 and 2^-11 in f16 (there, below
+          // 2^-14, by 2^-25), at random over the keys: in bf16 about 0.8 of the output's own
+          // rounding.
           pf[x][0] = transpose8x8(pack2<HT>(p0, p1));
           pf[x][1] = transpose8x8(pack2<HT>(p2, p3));
         }

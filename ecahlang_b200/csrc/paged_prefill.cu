@@ -550,7 +550,8 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
 
       if (E4M3 && w.jb < w.je) {
         // A row of queries, scaled by a power of two to a largest magnitude in [1, 2) so
-        // that bf16 queries fit f16's range; the power goes into the score scale.
+        // that bf16 queries fit f16's range; the power goes into the score scale.  bf16's bits
+        // fit f16's; entries below 2^-14 there are rounded by at most 2^-25.
         ok = ok && wait(&s_bars.q_empty, q_phase ^ 1);
         q_phase ^= 1;
         const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(P.q) + (w.r.q0 + token) * P.q_tok + head * P.q_head);
@@ -634,8 +635,9 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
         uint32_t w16[kC][16];
         uint64_t sum0, sum1, most;                            // of the weights; e4m3: most of their products with the scales
         auto weigh = [&](const uint32_t (&r)[32], int i, float ref) {
-          // A weight is off by at most 2^-9 of itself in bf16 (2^-12 in f16), at random over the
-          // keys; the sum takes it as it was.  An e4m3 value's scale goes into its weight.
+          // A weight is rounded by at most 2^-8 of itself in bf16 and 2^-11 in f16 (there, below
+          // 2^-14, by 2^-25: 2^-32 of the row's largest, which lies at 2^7 or above), at random over
+          // the keys; the sum takes it as it was.  An e4m3 value's scale goes into its weight.
           const uint64_t scale2 = tc::two(scale, scale), ref2 = tc::two(-ref, -ref);
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
