@@ -29,7 +29,7 @@ EXPORTS = ("ecah_sampler_abi_version", "ecah_status_string", "ecah_sampler_works
            "ecah_sampler_launch_noalloc", "ecah_sampler_noalloc_scratch_bytes",
            "ecah_vp_local", "ecah_vp_merge", "ecah_vp_exchange_bytes", "ecah_vp_step",
            "ecah_vp_ipc_alloc", "ecah_vp_ipc_open", "ecah_vp_ipc_close", "ecah_vp_ipc_free",
-           "ecah_quotient_mismatches", "ecah_exp2_pair_check", "ecah_vp_reset", "ecah_vp_dist_pass",
+           "ecah_quotient_mismatches", "ecah_vp_reset", "ecah_vp_dist_pass",
            "ecah_token_logprobs_workspace_bytes", "ecah_token_logprobs", "ecah_paged_append",
            "ecah_paged_decode_workspace_bytes", "ecah_paged_decode", "ecah_paged_decode_bounded",
            "ecah_paged_prefill_workspace_bytes", "ecah_paged_prefill",
@@ -213,8 +213,6 @@ def lib():
         L.ecah_vp_ipc_free.argtypes = [c_void_p]
         L.ecah_quotient_mismatches.restype = c_int32
         L.ecah_quotient_mismatches.argtypes = [c_int32, c_void_p, c_int32, c_void_p, c_void_p]
-        L.ecah_exp2_pair_check.restype = c_int32
-        L.ecah_exp2_pair_check.argtypes = [c_void_p, c_void_p, c_void_p]
         L.ecah_token_logprobs_workspace_bytes.restype = c_size_t
         L.ecah_token_logprobs_workspace_bytes.argtypes = []
         L.ecah_token_logprobs.restype = c_int32

@@ -1,16 +1,11 @@
-// Diagnostic entry points of libecah_sampler.so.
-//
-// The quotient the kernels use for softmax masses (quot_rn: reciprocal plus
-// one correction step) against the IEEE quotient __fdiv_rn, over every input
-// of a dtype and a list of temperatures.  The reference divides with torch
-// (`logits / temperature`, ecahlang/main.py:170), an IEEE float32 divide; the
-// kernels' masses are exact only where the two agree.
-//
-// The exponentials that prefill attention raises by multiplications
-// (tc::exp2_pair) against 2^x in float64, over every float32.
+// Diagnostic entry point of libecah_sampler.so: the quotient the kernels use
+// for softmax masses (quot_rn: reciprocal plus one correction step) against
+// the IEEE quotient __fdiv_rn, over every input of a dtype and a list of
+// temperatures.  The reference divides with torch (`logits / temperature`,
+// ecahlang/main.py:170), an IEEE float32 divide; the kernels' masses are
+// exact only where the two agree.
 
 #include "common.cuh"
-#include "tcgen05.cuh"
 
 namespace ecah {
 
@@ -55,35 +50,6 @@ __global__ void quotient_check_kernel(const float* T, int nT, unsigned long long
   }
 }
 
-// Every float32 x through both places of exp2_pair.  worst: the largest
-// relative error over -126 <= x < 127 (the bits of a double); bad: results
-// that break what exp2_pair says of the other x, or differ between its places.
-__global__ void exp2_pair_kernel(unsigned long long* worst, unsigned long long* bad) {
-  const unsigned long long stride = static_cast<unsigned long long>(gridDim.x) * blockDim.x;
-  double most = 0.0;
-  unsigned broken = 0;
-  for (unsigned long long i = static_cast<unsigned long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < 1ull << 32; i += stride) {
-    const float x = __uint_as_float(static_cast<uint32_t>(i));
-    float a = x, b = 0.0f, c = 1.0f, d = x;
-    tc::exp2_pair(a, b);
-    tc::exp2_pair(c, d);
-    bool ok = __float_as_uint(a) == __float_as_uint(d) && b == 1.0f;
-    if (x >= -126.0f && x < 127.0f) {
-      const double want = exp2(static_cast<double>(x));
-      most = fmax(most, fabs(static_cast<double>(a) - want) / want);
-    } else if (x <= -127.0f) {
-      ok = ok && a == 0.0f;
-    } else if (x < 0.0f) {
-      ok = ok && a >= 0.0f && a <= 0x1p-126f;
-    } else {                                  // 127 and more, NaN
-      ok = ok && a == 0x1p127f;
-    }
-    broken += !ok;
-  }
-  atomicMax(worst, static_cast<unsigned long long>(__double_as_longlong(most)));
-  if (broken) atomicAdd(bad, static_cast<unsigned long long>(broken));
-}
-
 }  // namespace ecah
 
 using namespace ecah;
@@ -102,14 +68,5 @@ extern "C" int ecah_quotient_mismatches(int32_t dtype, const float* temperature,
     case ECAH_DTYPE_F32: quotient_check_kernel<ECAH_DTYPE_F32><<<1184, 1024, 0, s>>>(temperature, n_temperature, counts); break;
     default: return ECAH_ERR_DTYPE;
   }
-  return cudaGetLastError() == cudaSuccess ? ECAH_OK : ECAH_ERR_LAUNCH;
-}
-
-extern "C" int ecah_exp2_pair_check(double* worst, unsigned long long* bad, void* stream) {
-  if (!worst || !bad) return ECAH_ERR_NULL;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (cudaMemsetAsync(worst, 0, sizeof(double), s) != cudaSuccess || cudaMemsetAsync(bad, 0, sizeof(unsigned long long), s) != cudaSuccess)
-    return ECAH_ERR_LAUNCH;
-  exp2_pair_kernel<<<1184, 1024, 0, s>>>(reinterpret_cast<unsigned long long*>(worst), bad);
   return cudaGetLastError() == cudaSuccess ? ECAH_OK : ECAH_ERR_LAUNCH;
 }

@@ -104,30 +104,6 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// 2^a and 2^b by multiplications: 2^n 2^f with n = round(x) and a polynomial of degree 4 for
-// 2^f on [-1/2, 1/2] that is 1 at zero.  The polynomial is off by at most 2.84e-6 of the value
-// (minimised in the maximum), its evaluation by less than 1.2e-7 more: the last of its roundings
-// is 2^-24 of a value of 0.7 or more, those before it come in through f.  n comes out of the sum
-// x + 1.5 2^23 in its low bits, and goes into the exponent.
-// x of -127 and less: zero; between that and -126: something of at most 2^-126; of 127 and more,
-// and NaN: 2^127, which no sum of weights that is kept holds.  ecah_exp2_pair_check goes through
-// all of float32.
-__device__ __forceinline__ void exp2_pair(float& a, float& b) {
-  constexpr float kMagic = 12582912.0f;
-  a = fmaxf(fminf(a, 127.0f), -127.0f);
-  b = fmaxf(fminf(b, 127.0f), -127.0f);
-  const uint64_t x = two(a, b), t = add2(x, two(kMagic, kMagic));
-  const uint64_t f = fma2(add2(t, two(-kMagic, -kMagic)), two(-1.0f, -1.0f), x);
-  uint64_t p = fma2(f, two(0x1.3a02ccp-7f, 0x1.3a02ccp-7f), two(0x1.c9fc46p-5f, 0x1.c9fc46p-5f));
-  p = fma2(f, p, two(0x1.ec0378p-3f, 0x1.ec0378p-3f));
-  p = fma2(f, p, two(0x1.62e12cp-1f, 0x1.62e12cp-1f));
-  p = fma2(f, p, two(1.0f, 1.0f));
-  float pa, pb, ta, tb;
-  apart(p, pa, pb);
-  apart(t, ta, tb);
-  a = __uint_as_float(__float_as_uint(pa) + (__float_as_uint(ta) << 23));
-  b = __uint_as_float(__float_as_uint(pb) + (__float_as_uint(tb) << 23));
-}
 
 // ----------------------------------------------------------------- products
 // A tile in shared memory in rows of 128 bytes whose 16-byte chunks are swizzled by

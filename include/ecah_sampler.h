@@ -192,14 +192,6 @@ ECAH_API size_t ecah_sampler_noalloc_scratch_bytes(void);
 ECAH_API int ecah_quotient_mismatches(int32_t dtype, const float* temperature, int32_t n_temperature,
                                       unsigned long long* counts, void* stream);
 
-/* Diagnostic; no counterpart in the reference.  Runs every float32 x through the
- * exponential that prefill attention computes by multiplications, and compares
- * with 2^x in float64: *worst (device) = the largest relative error over
- * -126 <= x < 127; *bad (device) = inputs outside that range whose result is
- * not what the kernel counts on (0 at -127 and less, at most 2^-126 up to -126,
- * 2^127 at 127 and more and for NaN).  Takes some tens of milliseconds. */
-ECAH_API int ecah_exp2_pair_check(double* worst, unsigned long long* bad, void* stream);
-
 /*
  * Vocab-parallel sampling (fp16/bf16 logits).  Each of `world` ranks holds
  * columns [vocab_offset, vocab_offset + vocab_local) of the [batch, vocab]

@@ -663,16 +663,6 @@ def test_the_workspace_is_made_by_the_first_prefill(monkeypatch):
     assert other.prefill_workspace.data_ptr() != ws.data_ptr()       # reading it makes it
 
 
-def test_exponentials_by_multiplications():
-    """Every float32: the polynomial's 2.84e-6 and its evaluation's roundings, 1.2e-7, where 2^x is normal."""
-    worst, bad = torch.full((1,), 7.0, dtype=torch.float64, device=DEV), torch.full((1,), 7, dtype=torch.int64, device=DEV)
-    stream = torch.cuda.current_stream().cuda_stream
-    assert _abi.lib().ecah_exp2_pair_check(worst.data_ptr(), bad.data_ptr(), stream) == 0
-    assert int(bad) == 0
-    assert 2.5e-6 < float(worst) <= 2.84e-6 + 1.2e-7
-    assert _abi.lib().ecah_exp2_pair_check(None, bad.data_ptr(), stream) == 1
-
-
 def with_scores(new, ctx, D, dtype, kv, at, score):
     """A batch of one request whose keys score 0, but key ``at`` as it says (scaled by 1); values random."""
     s = setup([new], [ctx], 4, 2, D, 16, dtype, kv, seed=26)
