@@ -65,6 +65,8 @@ class SamplingManager:
         self._captured_drafts: set = set()
         self._draft_kept: list = []                             # buffers that captured verify_drafts may read
         self._workspace: Optional[torch.Tensor] = None
+        self._workspace_rows = 0
+        self._kept_workspaces: list = []                        # smaller ones, which captured buckets use
         self._scorer: Optional[TokenLogprobs] = None
         self._scorer_workspace: Optional[torch.Tensor] = None
         # overflow flags of the slot histories, copied to the host after every
@@ -107,7 +109,8 @@ class SamplingManager:
         (manager.py:74-88), plus the penalty columns, the sampler's output and
         the workspaces of ``sample`` and ``logprobs``: made here, because one
         made inside a CUDA-graph capture would be zero-filled by that graph's
-        replays alone."""
+        replays alone.  Called again it leaves the workspaces that captured
+        buckets use."""
         B, V, dev = max_batch_size, self.vocab_size, self.device
         self.max_batch_size = B
         self.sampling_temperature_cpu = _pinned(torch.ones(B, 1, dtype=torch.float32))
@@ -133,7 +136,9 @@ class SamplingManager:
         self.sampling_slot_gpu = torch.full((B,), -1, dtype=torch.int32, device=dev)
         self.sampling_out = torch.zeros(B, dtype=torch.int32, device=dev)
         self._forget_drafts(None, B)
-        self._workspace = None
+        if self._workspace is not None and B > self._workspace_rows:
+            self._kept_workspaces.append(self._workspace)
+            self._workspace = None
         if dev.type == "cuda":
             self._sample_workspace()
             self._logprob_workspace()
@@ -147,6 +152,7 @@ class SamplingManager:
         if self._workspace is None:
             self._outside_capture("sample")
             self._workspace = new_workspace(self.max_batch_size, self.vocab_size, self.dtype, self.device)
+            self._workspace_rows = self.max_batch_size
         return self._workspace
 
     def _logprob_workspace(self) -> torch.Tensor:

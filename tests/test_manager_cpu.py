@@ -175,3 +175,13 @@ def test_draft_buffers_made_again_leave_those_of_captures():
     assert len(m._draft_kept) == 1 and all(a is b for a, b in zip(m._draft_kept[0], first))
     assert m._draft_ids.numel() == 18 and m._verifier.max_batch == 4     # no less than before
     assert all(getattr(m, n) is not t for n, t in zip(names, first)) and m._verifier.workspace is not first[-1].workspace
+
+
+def test_sampling_buffers_made_again_leave_the_workspace_of_captures():
+    m = _mgr()
+    ws = m._sample_workspace()
+    for rows in (8, 3, 8):
+        m.init_sampling_buffers(rows)
+        assert m._sample_workspace() is ws and not m._kept_workspaces
+    m.init_sampling_buffers(40)
+    assert m._sample_workspace() is not ws and m._kept_workspaces == [ws] and m._workspace_rows == 40
