@@ -23,10 +23,10 @@ namespace drafts {
 // result depends on which block that is.
 //
 // Measured on one B200, passes through the Python entry point one after another: 64
-// requests of 5 drafts over 151 936 float32 entries 18.6 us (4.2 TB/s; floor 11.9), 128
-// requests of up to 8 looked-up drafts over 32 003 bf16 entries 10.0, one request of 4
-// drafts 7.1 (host and launch).  What bounds them: about 8 us of dependent reads (drafts,
-// probabilities, the row, the sums, the range again), from cold rows.  With twice the
+// requests of 5 drafts over 151 936 float32 entries 19 us (4.1 TB/s; floor 11.9), 128
+// requests of up to 8 looked-up drafts over 32 003 bf16 entries 10.0 (9.8 on the device), one
+// request of 4 drafts 7.1 (6.0 on the device).  What bounds them: about 8 us of dependent reads
+// (drafts, probabilities, the row, the sums, the range again), from cold rows.  With twice the
 // blocks the batch took 2 us more, with half as many 6; without 4 loads a row in flight 10.
 
 constexpr int kT = 256;

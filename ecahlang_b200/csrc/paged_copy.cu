@@ -17,9 +17,10 @@ namespace copy {
 // with all loads in flight, so short pages fill blocks too.
 //
 // Measured on one B200, passes through the Python entry point one after another: 2000
-// pages of 16 tokens of 8 heads of 128 in 4 layers (bf16) 165 us (6.4 TB/s, 98 % of a
-// copy's rate), 127 pages of an e4m3 cache in 7 layers 7.3, a fork's 3 pages in 28
-// layers 7.0 (host and launch).
+// pages of 16 tokens of 8 heads of 128 in 4 layers (bf16) 162 to 171 us (6.1 to 6.5 TB/s, 94 to
+// 99 % of a copy's rate), 127 pages of an e4m3 cache in 7 layers 7.3 (7.1 on the device: the
+// lists are read, then the rows, then they are written), a fork's 3 pages in 28 layers 7.2 (2.6
+// on the device; the host checks 28 layers).
 
 constexpr int kT = 256;
 constexpr int kUnroll = 4;

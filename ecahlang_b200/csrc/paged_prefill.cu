@@ -45,16 +45,21 @@ namespace prefill {
 // that spans several blocks is joined by the block that arrives last, in the order of the
 // parts, so results do not depend on which that is.
 //
-// Measured on one B200, device time of graph replays: a prompt of 8192 tokens, 32/8 heads
-// of 128, bf16 500 us (1.1 PFLOP/s, 66 % of the measured GEMM rate; 584 to 600 back to back, as
-// the power cap lowers the clock); 16 packed prompts of 100 to 1024 tokens, 16/2 heads, f16
-// 65; 64 drafts of 5 tokens over contexts up to 8000, 32/8 heads, bf16 104 (3.5 TB/s); 7
-// chunks of up to 333 tokens behind up to 6001 in an e4m3 cache 182; 2 prompts of heads of
-// 256 72; a prompt of 37 tokens 17.
-// What bounds the first: an iteration takes 3400 cycles, of which the products 2048 and the
-// exponentials' unit 1536, and a slot waits 1500 for its next scores.  An item takes 6 to
-// 9 us beside its iterations in a share of many small ones; the plan of the shares 1.5
-// (one request) to 4 us (64 requests).
+// Measured on one B200, passes through the Python entry point one after another with
+// changing inputs: a prompt of 8192 tokens, 32/8 heads of 128, bf16 566 us (972 TFLOP/s, 69 %
+// of the sustained GEMM rate) under the power cap at 1.67 GHz, 490 in short runs at 1.97 GHz
+// (1.1 PFLOP/s, 67 % of the burst rate); 16 packed prompts of 100 to 1024 tokens, 16/2 heads,
+// f16 63; 64 drafts of 5 tokens over contexts up to 8000, 32/8 heads, bf16 97 (3.7 TB/s); 7
+// chunks of up to 333 tokens behind up to 6001, bf16 110, e4m3 179; 2 prompts of heads of 256
+// 70; a prompt of 37 tokens 15.
+// What bounds the first: an iteration (256 rows by 128 keys) takes 4000 cycles, of which the
+// products 2048 and the exponentials' unit 2048, since a slot's scores wait for its product
+// and its softmax for the scores.  An item takes 6 to 9 us beside its iterations in a share of
+// many small ones; the plan of the shares 1.5 (one request) to 4 us (64 requests).  Iterations
+// of e4m3 caches take 6700 cycles (converting codes), of heads of 256 (128 rows by 64 keys)
+// 3000 for products of 1024.
+// Registers: 96 a thread.  16-bit caches of heads of 64 to 128 spill 40 bytes, e4m3 caches 16
+// (heads of 256) to 80.
 
 constexpr int kLoaders = 16;           // first of the warps that bring keys and values, and how many
 constexpr int kLoadWarps = 3;
@@ -640,8 +645,8 @@ __global__ void __launch_bounds__(kT, 1) prefill_kernel(const __grid_constant__ 
             float p[4];
             tc::apart(tc::fma2(tc::two(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, ref2), p[0], p[1]);
             tc::apart(tc::fma2(tc::two(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), scale2, ref2), p[2], p[3]);
-            // All by the exponentials' unit.  A quarter of them by a polynomial (off by 2.9e-6) made
-            // 8192 tokens 506 us instead of 486: issue slots are as scarce as the unit.
+            // All by the exponentials' unit (51 % busy with 8192 tokens).  A quarter of them by a
+            // polynomial, off by 2.9e-6, took 506 us instead of 486: a slot's softmax gets longer.
 #pragma unroll
             for (int e = 0; e < 4; ++e) p[e] = ex2_approx(p[e]);
             sum0 = tc::add2(tc::two(p[0], p[1]), sum0);
@@ -1427,8 +1432,9 @@ int ecah_paged_prefill_bounded(const ecah_prefill_args* a, int32_t tries, void* 
       a->dtype == ECAH_DTYPE_F16 ? (e4m3 ? prefill::variant_for<ECAH_DTYPE_F16, true>(c.head_dim) : prefill::variant_for<ECAH_DTYPE_F16, false>(c.head_dim))
                                  : (e4m3 ? prefill::variant_for<ECAH_DTYPE_BF16, true>(c.head_dim) : prefill::variant_for<ECAH_DTYPE_BF16, false>(c.head_dim));
   // Whole tiles by the copy engine where a page is a power of two of 8 slots or more (the
-  // swizzle goes by 8 rows); smaller or odd pages go through threads (8192 tokens with pages
-  // of 1, 8 and 16 tokens: 731, 592 and 531 us).
+  // swizzle goes by 8 rows); smaller or odd pages go through threads (8192 tokens in short
+  // runs: by the engine with pages of 8 and 16 tokens 538 and 490 us, by threads with pages of
+  // 4, 12 and 24 tokens 678, 792 and 793 us).
   P.boxes = P.page_shift >= 3 && (!e4m3 || (aligned16(c.k_scale) && aligned16(c.v_scale))) && prefill::box_map(&P.k_map, P.cache.k, c, std::min(c.page_size, keys)) &&
             prefill::box_map(&P.v_map, P.cache.v, c, std::min(c.page_size, keys));
   return launch_kernel(v.fn, dim3(sms), prefill::kT, v.smem, reinterpret_cast<cudaStream_t>(stream), P) ? ECAH_OK : ECAH_ERR_LAUNCH;
